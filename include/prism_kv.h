@@ -345,6 +345,89 @@ int pkv_rope_qk(const void* qkv, int64_t qkv_sb, int64_t qkv_ss, const int32_t* 
                 int32_t* status, void* stream);
 
 /*
+ * Rotary positions in their general form, on tensors of tokens (batch and sequence in one axis): optional RMSNorm
+ * of every head, then the rotation.  For token t < tokens and every head x = q[t, h] (n_heads of them, q_norm_w)
+ * and k[t, h] (n_kv, k_norm_w; n_kv = 0: q alone):
+ *   y = x * rsqrt(mean(x^2) + eps) * w     (w NULL: y = x)
+ *   out[i] = y[i] c[i] - y[p] s[i],  out[p] = y[p] c[i] + y[i] s[i]      for i < rotary_dim / 2
+ * with c, s = row positions[t] of cos_tab / sin_tab (fp32 [n_pos, rotary_dim / 2]), p the partner of element i:
+ * i + rotary_dim / 2, or, interleaved, elements 2 i and 2 i + 1.  Elements from rotary_dim on are y as it is.  fp32
+ * throughout, one rounding to dtype (PKV_BF16, PKV_FP16, PKV_FP32: of q, k, the outputs and the norm weights
+ * alike).  The outputs may be the inputs.  A position outside the tables is clamped and flags
+ * PKV_STATUS_BAD_POSITION.  head_dim at most 1024, rotary_dim even; any strides.  16-byte aligned rows with
+ * head_dim and rotary_dim multiples of 16 run in 16-byte accesses, others element by element.  The rotation is
+ * what engine/executor.py:_apply_rope does for the half layout of a whole head, without its bf16 rounding after
+ * every operation (pkv_rope_qk keeps those).
+ */
+#define PKV_BF16 0
+#define PKV_FP16 1
+#define PKV_FP32 2
+
+int pkv_rotate_qk(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
+                  const int32_t* positions, const float* cos_tab, const float* sin_tab, int32_t n_pos,
+                  const void* q_norm_w, const void* k_norm_w, float eps,
+                  void* q_out, int64_t qo_st, int64_t qo_sh, void* k_out, int64_t ko_st, int64_t ko_sh,
+                  int64_t tokens, int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t rotary_dim,
+                  int32_t interleaved, int32_t dtype, int32_t* status, void* stream);
+
+/*
+ * pkv_rotate_qk from the fused QKV projection's output, with the paged append: token t's row qkv + t * qkv_st =
+ * [q (n_heads * head_dim) | k (n_kv * head_dim) | v (n_kv * head_dim)], bf16.  The rotated q goes to q_out, the
+ * rotated k and the unchanged v to slot slots[t] of the cache: page slots[t] / page_size, row slots[t] % page_size.
+ * Slots of one call must differ.  A slot outside the pool is skipped and flags PKV_STATUS_BAD_PAGE.  head_dim 64 or
+ * 128, rotary_dim a multiple of 16.  Replaces, for a batch of tokens of many sequences, the QKV split, rotation
+ * and append around engine/executor.py:108-120 and :143-153, which take one chunk length for the whole batch.
+ */
+int pkv_packed_rope_append(const void* qkv, int64_t qkv_st, const int32_t* positions, const int32_t* slots,
+                           const float* cos_tab, const float* sin_tab, int32_t n_pos,
+                           const void* q_norm_w, const void* k_norm_w, float eps,
+                           void* q_out, int64_t qo_st, int64_t qo_sh,
+                           void* k_cache, void* v_cache, int64_t cache_page_stride,
+                           int64_t tokens, int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t rotary_dim,
+                           int32_t interleaved, int32_t page_size, int32_t num_pages,
+                           int32_t* status, void* stream);
+
+/*
+ * The work list of a pkv_packed_attn call, on the host (every pointer here is host memory; nothing is launched).
+ * Sequence b brings new_lens[b] >= 0 tokens behind ctx_lens[b] cached ones.  Their query rows are cut into blocks of
+ * 128 per KV head, and blocks with many keys into ranges, for a device of compute_units CUs.  items receives
+ * 8 int32 words per item, merges 8 per block of several ranges; counts (4 words) the items, the merges, the
+ * partial results that the workspace must hold and merge_rows.  items NULL: the counts only.
+ * PKV_ENOSPC where max_items or max_merges is too few.
+ */
+int pkv_packed_plan(const int32_t* new_lens, const int32_t* ctx_lens, int32_t batch, int32_t n_heads, int32_t n_kv,
+                    int32_t head_dim, int32_t window, int32_t compute_units, int32_t* items, int32_t max_items,
+                    int32_t* merges, int32_t max_merges, int32_t* counts);
+
+/* Bytes of workspace a pkv_packed_attn call with so many partials needs.  Its contents need not be kept or cleared. */
+size_t pkv_packed_workspace_bytes(int32_t partials, int32_t n_kv, int32_t head_dim);
+
+/*
+ * Causal attention of a packed batch over the paged cache: q [tokens, n_heads, head_dim] holds the new tokens of
+ * sequence 0, then those of sequence 1, and so on; each sequence may bring any number, one (decode) or a prompt
+ * chunk.  Their keys and values are in the cache already (pkv_packed_rope_append).  Token j of sequence b is at
+ * position ctx_lens[b] + j and sees the keys up to itself, with window > 0 only the last `window` of them.
+ * out = sum_t exp(s_t) v_t / (sum_t exp(s_t) + exp(sinks[h])), s = softmax_scale q . k; sinks (fp32 [n_heads])
+ * NULL: without that term.  lse (fp32 [tokens, n_heads], NULL: not wanted): the logarithm of the denominator.
+ * items, merges (device memory, 16-byte aligned) and the counts come from pkv_packed_plan for the same lengths,
+ * heads and window; the lengths are in them, and the block table needs ceil((ctx + new) / page_size) columns of
+ * each sequence (with a window, only those that hold a visible key are read).  Rows of out from `tokens` on are
+ * not written.  Values of masked keys take part in the products with weight 0: a NaN or infinity in a V row that
+ * belongs to the sequence reaches rows of the same 32 (head_dim 64: 64) keys that do not see it; what lies behind
+ * the sequence's last key does not matter.  bf16 in and out, fp32 softmax and sums, the probabilities rounded to
+ * bf16 for the second product.  Replaces flash_attn_with_kvcache (engine/executor.py:119-120, :260-261) for
+ * batches whose sequences bring different numbers of tokens.
+ */
+int pkv_packed_attn(const void* q, int64_t q_st, int64_t q_sh, const void* k_cache, const void* v_cache,
+                    int64_t cache_page_stride, const int32_t* block_table, int64_t bt_stride,
+                    void* out, int64_t o_st, int64_t o_sh, float* lse, const float* sinks,
+                    const int32_t* items, int32_t n_items, const int32_t* merges, int32_t n_merges,
+                    int32_t partials, int32_t merge_rows, void* workspace, size_t workspace_bytes,
+                    int32_t tokens, int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim,
+                    int32_t page_size, int32_t num_pages, int32_t max_blocks, int32_t window, float softmax_scale,
+                    int32_t* status, void* stream);
+
+/*
  * RMSNorm over rows (engine/fused_kernels.py:31-65 fused_rms_norm; called at
  * engine/executor.py:106, :122, :131): out[r] = bf16(h * rsqrt(mean(h^2) + eps) * weight) in
  * fp32, h = x[r], or, when residual is non-NULL, h = bf16(x[r] + residual[r]) (the preceding

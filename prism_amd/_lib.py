@@ -27,6 +27,9 @@ PKV_DECODE_TWO_PASS = 1
 PKV_DECODE_FUSED_MERGE = 2
 PKV_DECODE_HEADS = 4
 PKV_DECODE_RESET_COUNTERS = 8
+PKV_BF16 = 0
+PKV_FP16 = 1
+PKV_FP32 = 2
 ABI_VERSION = 1
 
 _I64 = c_int64
@@ -136,6 +139,35 @@ _SIGNATURES = {
         _P, _I64, _P,                    # block table, seqlens
         _I32, _I32, _I32, _I32, _I32,    # batch, s_new, n_heads, n_kv, head_dim
         _I32, _I32, _I32,                # page_size, num_pages, max_blocks
+        _P, _P,                          # status, stream
+    ]),
+    "pkv_rotate_qk": (c_int32, [
+        _P, _I64, _I64, _P, _I64, _I64,  # q, k + strides
+        _P, _P, _P, _I32,                # positions, cos, sin, n_pos
+        _P, _P, c_float,                 # q_norm_w, k_norm_w, eps
+        _P, _I64, _I64, _P, _I64, _I64,  # q_out, k_out + strides
+        _I64, _I32, _I32, _I32, _I32,    # tokens, n_heads, n_kv, head_dim, rotary_dim
+        _I32, _I32, _P, _P,              # interleaved, dtype, status, stream
+    ]),
+    "pkv_packed_rope_append": (c_int32, [
+        _P, _I64, _P, _P,                # qkv + stride, positions, slots
+        _P, _P, _I32,                    # cos, sin, n_pos
+        _P, _P, c_float,                 # q_norm_w, k_norm_w, eps
+        _P, _I64, _I64,                  # q_out + strides
+        _P, _P, _I64,                    # caches
+        _I64, _I32, _I32, _I32, _I32,    # tokens, n_heads, n_kv, head_dim, rotary_dim
+        _I32, _I32, _I32, _P, _P,        # interleaved, page_size, num_pages, status, stream
+    ]),
+    "pkv_packed_plan": (c_int32, [_P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P, _I32, _P, _I32, _P]),
+    "pkv_packed_workspace_bytes": (c_size_t, [_I32] * 3),
+    "pkv_packed_attn": (c_int32, [
+        _P, _I64, _I64, _P, _P, _I64,    # q + strides, caches
+        _P, _I64, _P, _I64, _I64,        # block table, out + strides
+        _P, _P,                          # lse, sinks
+        _P, _I32, _P, _I32, _I32, _I32,  # items, merges, partials, merge_rows
+        _P, c_size_t,                    # workspace
+        _I32, _I32, _I32, _I32, _I32,    # tokens, batch, n_heads, n_kv, head_dim
+        _I32, _I32, _I32, _I32, c_float,  # page_size, num_pages, max_blocks, window, scale
         _P, _P,                          # status, stream
     ]),
     "pkv_rms_norm": (c_int32, [

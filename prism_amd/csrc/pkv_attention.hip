@@ -29,6 +29,7 @@
 #include <type_traits>
 
 #include "pkv_common.h"
+#include "pkv_packed.h"
 
 namespace pkv {
 
@@ -71,6 +72,14 @@ struct AttnParams {
   const uint16_t* rot_sin;
   int n_pos;
   float scale_log2;  // softmax_scale * log2(e)
+  // pkv_packed_attn: the work lists (PackedItem, PackedMerge) of a batch whose new tokens are the rows
+  // [0, tokens) of q and out, one behind the other; window keys per row (0: all); sink logits per query head
+  // and the rows' log-sum-exp [tokens, n_heads], either null
+  const PackedItem* items;
+  const PackedMerge* merges;
+  const float* sinks;
+  float* lse;
+  int tokens, window;
 };
 
 // Maxima of attention scores without IEEE-mode canonicalisation.  fmaxf on an MFMA result makes
@@ -3002,6 +3011,12 @@ static void fill_params(AttnParams& p, const void* q, int64_t q_sb, int64_t q_ss
   p.rot_cos = nullptr;
   p.rot_sin = nullptr;
   p.n_pos = 0;
+  p.items = nullptr;
+  p.merges = nullptr;
+  p.sinks = nullptr;
+  p.lse = nullptr;
+  p.tokens = 0;
+  p.window = 0;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
 }
 
@@ -3128,6 +3143,20 @@ static void launch_prefill_tiles(const AttnParams& p, int batch, hipStream_t str
     return;
   }
   prefill_tile_kernel<HD, pf::kDirect><<<dim3(nx, p.n_kv, batch), 64 * pf::kWaves, 0, stream>>>(p);
+}
+
+template <int HD>
+static void launch_packed(const AttnParams& p, int n_items, int n_merges, int merge_rows, int page_size, hipStream_t stream) {
+  const dim3 grid(unsigned(n_items) * unsigned(p.n_kv));
+  const bool small = page_size < pf::Geo<HD>::TOK;
+  auto* kernel = small ? (p.lse ? prefill_tile_kernel<HD, pf::kPacked, pf::kWaves, true, true>
+                                : prefill_tile_kernel<HD, pf::kPacked, pf::kWaves, true>)
+                       : (p.lse ? prefill_tile_kernel<HD, pf::kPacked, pf::kWaves, false, true>
+                                : prefill_tile_kernel<HD, pf::kPacked>);
+  kernel<<<grid, 64 * pf::kWaves, 0, stream>>>(p);
+  constexpr int kRowsPerGroup = 1024 / HD;
+  if (n_merges > 0)
+    packed_merge_kernel<HD><<<dim3((merge_rows + kRowsPerGroup - 1) / kRowsPerGroup, p.n_kv, n_merges), 256, 0, stream>>>(p);
 }
 
 template <int HD>
@@ -3605,6 +3634,64 @@ extern "C" int pkv_prefill_attn(const void* q, int64_t q_sb, int64_t q_ss, int64
                              v_cache, cache_page_stride, block_table, bt_stride, cache_seqlens, out, o_sb, o_ss, o_sh,
                              nullptr, 0, batch, s_q, n_heads, n_kv, head_dim, page_size, num_pages, max_blocks,
                              causal, softmax_scale, status, stream);
+}
+
+extern "C" size_t pkv_packed_workspace_bytes(int32_t partials, int32_t n_kv, int32_t head_dim) {
+  if (partials <= 0 || n_kv <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
+  return size_t(partials) * n_kv * pkv::kPackedRows * (head_dim + 4) * sizeof(float);
+}
+
+extern "C" int pkv_packed_attn(const void* q, int64_t q_st, int64_t q_sh, const void* k_cache, const void* v_cache,
+                               int64_t cache_page_stride, const int32_t* block_table, int64_t bt_stride, void* out,
+                               int64_t o_st, int64_t o_sh, float* lse, const float* sinks, const int32_t* items,
+                               int32_t n_items, const int32_t* merges, int32_t n_merges, int32_t partials,
+                               int32_t merge_rows, void* workspace, size_t workspace_bytes, int32_t tokens,
+                               int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t page_size,
+                               int32_t num_pages, int32_t max_blocks, int32_t window, float softmax_scale,
+                               int32_t* status, void* stream) {
+  using namespace pkv;
+  clear_error();
+  const char* fn = "pkv_packed_attn";
+  if (tokens < 0 || n_items < 0 || n_merges < 0 || partials < 0 || merge_rows < 0 || window < 0)
+    return fail(PKV_EINVAL, "%s: bad sizes tokens=%d n_items=%d n_merges=%d partials=%d merge_rows=%d window=%d", fn,
+                tokens, n_items, n_merges, partials, merge_rows, window);
+  // the lengths are the plan's: the block table stands in for the pointer that validation asks for
+  int rc = validate_attn(fn, q, 0, q_st, q_sh, nullptr, 0, 0, 0, nullptr, 0, 0, 0,
+                         const_cast<void*>(k_cache), const_cast<void*>(v_cache), cache_page_stride, block_table,
+                         bt_stride, block_table, out, 0, o_st, o_sh, batch, 1, n_heads,
+                         n_kv, head_dim, page_size, num_pages, max_blocks, softmax_scale);
+  if (rc) return rc;
+  if ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(sinks)) & 3u)
+    return fail(PKV_EINVAL, "%s: lse/sinks not 4-byte aligned", fn);
+  if (n_items == 0) return PKV_OK;
+  if (!items || (n_merges > 0 && !merges)) return fail(PKV_EINVAL, "%s: null work list", fn);
+  if (!aligned16(items) || !aligned16(merges)) return fail(PKV_EINVAL, "%s: work lists not 16-byte aligned", fn);
+  if (int64_t(n_items) * n_kv > 0x7fffffff || n_merges > 65535) return fail(PKV_EINVAL, "%s: too many work items", fn);
+  const size_t need = pkv_packed_workspace_bytes(partials, n_kv, head_dim);
+  if (need > 0 && (!workspace || !aligned16(workspace)))
+    return fail(PKV_EINVAL, "%s: workspace null or not 16-byte aligned", fn);
+  if (need > 0 && workspace_bytes < need)
+    return fail(PKV_ENOSPC, "%s: workspace %zu bytes < %zu needed", fn, workspace_bytes, need);
+  AttnParams p;
+  fill_params(p, q, 0, q_st, q_sh, nullptr, 0, 0, 0, nullptr, 0, 0, 0, const_cast<void*>(k_cache),
+              const_cast<void*>(v_cache), cache_page_stride, block_table, bt_stride, nullptr, out, 0, o_st, o_sh, 1,
+              n_heads, n_kv, page_size, num_pages, max_blocks, 1, softmax_scale, status);
+  p.items = reinterpret_cast<const PackedItem*>(items);
+  p.merges = reinterpret_cast<const PackedMerge*>(merges);
+  p.sinks = sinks;
+  p.lse = lse;
+  p.tokens = tokens;
+  p.window = window;
+  if (need > 0) {
+    p.ws_o = static_cast<float*>(workspace);
+    p.ws_ml = p.ws_o + size_t(partials) * n_kv * kPackedRows * head_dim;
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (head_dim == 128)
+    launch_packed<128>(p, n_items, n_merges, merge_rows, page_size, s);
+  else
+    launch_packed<64>(p, n_items, n_merges, merge_rows, page_size, s);
+  return check_launch(fn);
 }
 
 #ifdef PKV_TILE_STAMPS

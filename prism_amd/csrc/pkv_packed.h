@@ -1,0 +1,28 @@
+// Work lists of packed attention, laid out by pkv_packed_plan on the host and read by the kernels.
+#pragma once
+
+#include <stdint.h>
+
+namespace pkv {
+
+constexpr int kPackedRows = 128;  // query rows (token x head of the group) of a work item
+
+// One key range of one row block of one sequence, for every KV head.  32 bytes.
+struct PackedItem {
+  int32_t tok0;    // the sequence's first row of q and out
+  int32_t n_new;   // its new tokens
+  int32_t ctx;     // its keys before them
+  int32_t seq;     // its row of the block table
+  int32_t row0;    // the block's first query row, new token x group size + head in the group
+  int32_t stage0;  // the range's first stage (of 32 keys, head_dim 128, or 64)
+  int32_t stages;
+  int32_t slot;    // where its partial result goes, -1 for a block of one range
+};
+
+// A row block of several ranges: their partials are slots slot .. slot + count - 1.  32 bytes.
+struct PackedMerge {
+  int32_t tok0, n_new, row0, slot, count;
+  int32_t pad[3];
+};
+
+}  // namespace pkv

@@ -78,6 +78,7 @@ enum Dest {
   kDirect,   // the bf16 output rows
   kCascade,  // the shared-prefix pass of a cascade launch: fp16 O / l and the log-sum-exp of one key split
   kSplit,    // one of max_splits key ranges: fp32 O and (m, l) for prefill_merge_kernel
+  kPacked,   // rows of a packed batch: the bf16 output, or fp32 O and (m, l) of a key range for packed_merge_kernel
 };
 
 // Key ranges.  A call with few row blocks (150 tokens onto 3500 at the 7B shape: 36 items of 115 stages)
@@ -148,6 +149,25 @@ __device__ __forceinline__ float max_halves(float v) {
 __device__ __forceinline__ void pin(float& v) { asm volatile("" : "+v"(v)); }
 __device__ __forceinline__ void pin(uint32_t& v) { asm volatile("" : "+v"(v)); }
 
+// What a packed row's output is to be multiplied by, from its maximum m (log2 units) and row sum l (l_true: before
+// rounding), and its natural log-sum-exp.  A sink is one more term of the row sum, with nothing to add to the output.
+__device__ __forceinline__ float finish_row(const AttnParams& p, int hq, float m, float l, float l_true, float& lse) {
+  // sink - top below must be of the rounded product: fused, a sink of 1e30 would come out 2^76 above itself
+#pragma clang fp contract(off)
+  float keep = 1.f;
+  if (p.sinks) {
+    const float sink = p.sinks[hq] * 1.4426950408889634f;
+    const float top = fmaxf(m, sink);
+    keep = m == -INFINITY ? 0.f : fast_exp2(m - top);
+    const float term = sink == -INFINITY ? 0.f : fast_exp2(sink - top);
+    l = l * keep + term;
+    l_true = l_true * keep + term;
+    m = top;
+  }
+  lse = l_true > 0.f ? (m + __builtin_amdgcn_logf(l_true)) * 0.6931471805599453f : -INFINITY;
+  return l > 0.f ? keep / l : 0.f;
+}
+
 // Verify's ranges.  The stages of all sequences, sequence after sequence, are cut into ranges of one
 // length (`chunk`: about lean_grid ranges for each KV head, at least kMinVerifyStages stages each: 4 to 6
 // are level), each inside
@@ -190,8 +210,18 @@ __device__ __forceinline__ VerifyPlan verify_plan(const AttnParams& p) {
 // W waves own 32 W rows.  W = 2 (kSplit only) is speculative verify: one row block per (sequence, KV
 // head); each range appends the new rows it covers itself, before it copies them; P is a bf16 pair (two
 // PV products).
-template <int HD, int DEST, int W = pf::kWaves>
+//
+// PACKED form (DEST == kPacked): grid (items x KV heads), the heads of an item next to each other.  A PackedItem
+// names the sequence, the row block and the stages of its keys; the host cuts and orders them.  Row j of a sequence
+// sees its last `window` keys (0: all) up to itself.  A wave of which no row is real (decode tokens fill a few
+// of a block's 128 rows) copies its share of the tiles and computes nothing.  SMALL: pages of fewer tokens than
+// a stage, looked up copy by copy (a copy's rows are always of one page).
+// LSE: the rows' log-sum-exp is wanted.  The sum that divides the output is of the probabilities as rounded for the
+// product (their errors then cancel where V is level); the log-sum-exp, an fp32 result, has a sum of its own of
+// the unrounded ones.
+template <int HD, int DEST, int W = pf::kWaves, bool SMALL = false, bool LSE = false>
 __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParams p) {
+  static_assert((!SMALL && !LSE) || DEST == pf::kPacked, "packed rows only");
   using G = pf::Geo<HD>;
   constexpr int kRows = 32 * W;
   constexpr int kLead = W == pf::kWaves ? 3 : 2;  // iterations between a copy's issue and its use
@@ -200,6 +230,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
   constexpr int kCopies = 8 / W;                  // copies of a K (or V) stage per wave
   constexpr int TT = G::TT, DT = G::DT, KK = G::KK, TOK = G::TOK;
   constexpr bool CASCADE = DEST == pf::kCascade;
+  constexpr bool PACKED = DEST == pf::kPacked;
   constexpr bool PAIR = W != pf::kWaves;          // P as bf16 hi + lo
   constexpr int NP = PAIR ? 4 * TT : 2 * TT;      // PV operands of a stage: hi (then lo) of each key step
   __shared__ __attribute__((aligned(16))) char lds[2 * kRing * G::STAGE];
@@ -210,7 +241,8 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
   const int hi = lane >> 5;
   int b, h, xblk;
   int c, L;
-  const int R_all = CASCADE ? p.batch * p.R : p.R;  // query rows of the launch's row space
+  int R_all = CASCADE ? p.batch * p.R : p.R;        // query rows of the launch's (PACKED: the sequence's) row space
+  int tok0 = 0;                                     // PACKED: the sequence's first row of q and out
   int t_first = 0;                                  // first stage of this workgroup's key range
   int n;                                            // its stages
   int split = 0, count = 1, chunk = 0;              // kSplit: which range of the item, of how many, stages each
@@ -220,6 +252,20 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
     b = 0;
     c = 0;
     L = p.k0;
+  } else if constexpr (PACKED) {
+    const int i = int(blockIdx.x);
+    const int it = i / p.n_kv;
+    h = i - it * p.n_kv;
+    const PackedItem item = p.items[it];
+    b = item.seq;
+    c = item.ctx;
+    L = c + item.n_new;
+    tok0 = item.tok0;
+    R_all = item.n_new * p.g;
+    xblk = item.row0;  // the block's first row, here
+    t_first = item.stage0;
+    n = item.stages;
+    split = item.slot;  // the range's partial in the workspace, -1: the whole of the rows' keys
   } else {
     const int i = int(blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z));
     if constexpr (W != pf::kWaves) {
@@ -265,7 +311,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
   sv.t_end = L;
   sv.bt = p.block_table + int64_t(b) * p.bt_stride;
 
-  const int blk_row0 = xblk * kRows;
+  const int blk_row0 = PACKED ? xblk : xblk * kRows;
   if (blk_row0 >= R_all) return;
   const int row0 = blk_row0 + wave * 32;
   // the block's last row sees the most keys (rows increase with j)
@@ -276,7 +322,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
     const int chunk = (n_shared + int(gridDim.z) - 1) / int(gridDim.z);
     t_first = int(blockIdx.z) * chunk;
     n = max(min(chunk, n_shared - t_first), 0);
-  } else {
+  } else if constexpr (!PACKED) {
     n = pf::stages_of<TOK>(p, L, blk_last);
     if constexpr (DEST == pf::kSplit) {
       if constexpr (W == pf::kWaves) {
@@ -303,6 +349,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
   // Q rows (key step kk: elements 16 kk + 8 hi .. + 7 of row row0 + ln) and the row's last visible key
   bf16x8 qf[KK];
   int lim = kNoQueryRow;
+  int lo_key = 0, lo_max = 0;  // PACKED: the row's first visible key, and the largest of the wave's
   // row (and its sequence) of lane index l: real rows, sequence, row in it, query position, query head
   struct LaneRow {
     bool real;
@@ -320,10 +367,16 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
   };
   const LaneRow lr = lane_row(lane);
   if (lr.real) {
-    const uint16_t* src = p.q + lr.b * p.q_sb + lr.j * p.q_ss + lr.hq * p.q_sh + 8 * hi;
+    const uint16_t* src = p.q + (PACKED ? (tok0 + lr.j) * p.q_ss : lr.b * p.q_sb + lr.j * p.q_ss) + lr.hq * p.q_sh + 8 * hi;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) qf[kk] = __builtin_bit_cast(bf16x8, ld16(src + 16 * kk));
-    lim = CASCADE ? p.k0 - 1 : min(p.causal ? L - p.s_q + lr.j : L - 1, L - 1);
+    if constexpr (PACKED) {
+      lim = c + lr.j;
+      lo_key = p.window > 0 ? max(lim - p.window + 1, 0) : 0;
+      lo_max = lo_key;
+    } else {
+      lim = CASCADE ? p.k0 - 1 : min(p.causal ? L - p.s_q + lr.j : L - 1, L - 1);
+    }
   } else {
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) qf[kk] = __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
@@ -332,6 +385,11 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) lim_min = min(lim_min, __shfl_xor(lim_min, off, 64));
   lim_min = __builtin_amdgcn_readfirstlane(lim_min);
+  if constexpr (PACKED) {
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) lo_max = max(lo_max, __shfl_xor(lo_max, off, 64));
+    lo_max = __builtin_amdgcn_readfirstlane(lo_max);
+  }
 
   BtWindow btw;
   bt_window_load(p, sv, (t_first * TOK) >> p.log2_page, btw);
@@ -352,19 +410,35 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
   // the last, or the first of the next page.
   const int pmask = (1 << p.log2_page) - 1;
   const int stage_elems = TOK * p.n_kv * HD;
-  int64_t off_k = 0;
+  constexpr int kOff = SMALL ? kCopies : 1;  // page lookups of a stage
+  struct Offs {
+    int64_t at[kOff];
+  };
+  Offs off_k = {};
   int T_k = t_first * TOK;
   bool bad_page = false;
-  auto page_start = [&] {
-    const int col = T_k >> p.log2_page;
+  // first key that a row of the block sees
+  const int first_key = PACKED && p.window > 0 ? max(c + blk_row0 / p.g - p.window + 1, 0) : 0;
+  // offset of token row T (uniform) of head h
+  auto row_of = [&](int T) {
+    const int col = T >> p.log2_page;
     if (col - btw.col0 >= 64) {
       bt_window_load(p, sv, col, btw);
       __builtin_amdgcn_s_waitcnt(0x0F70);  // here, once per 64 pages: not at every use of the window
     }
     const int pid = __builtin_amdgcn_readlane(btw.ids, col - btw.col0);
     const bool ok = unsigned(pid) < unsigned(p.num_pages);
-    bad_page |= !ok && T_k < L;
-    off_k = int64_t(ok ? pid : 0) * p.page_stride + int64_t(T_k & pmask) * (p.n_kv * HD) + h * HD;
+    if constexpr (SMALL) {
+      // rows of a stage that lie before every row's window, or behind the last key, may have no page: they read as
+      // zeros
+      if (T + G::RPC <= first_key || T >= L) return int64_t(-1);
+    }
+    bad_page |= !ok && T < L;
+    return int64_t(ok ? pid : 0) * p.page_stride + int64_t(T & pmask) * (p.n_kv * HD) + h * HD;
+  };
+  auto page_start = [&] {
+#pragma unroll
+    for (int k = 0; k < kOff; ++k) off_k.at[k] = row_of(T_k + (SMALL ? (wave + W * k) * G::RPC : 0));
   };
   char* const ring_k = lds;
   char* const ring_v = lds + kRing * G::STAGE;
@@ -373,32 +447,37 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
   // empty buffer: they fetch nothing and write zeros to a free slot, and the loop has neither branches nor
   // other counts to wait for.  A stage's page lookup serves its K copies and, three iterations later,
   // its V copies: off1 .. off3 hold the offsets of the stages in between, oldest first.
-  int64_t off1 = 0, off2 = 0, off3 = 0;
+  Offs off1 = {}, off2 = {}, off3 = {};
   int slot_k = 0, slot_v = 0;    // ring slots the next copies go to
   int left_k = n, left_v = n;    // stages left to copy
   auto next_slot = [](int slot) { return slot == (kRing - 1) * G::STAGE ? 0 : slot + G::STAGE; };
   auto next_stage = [&] {
-    if (__builtin_expect((T_k & pmask) == 0 && left_k > 0, 0)) page_start();
+    if (__builtin_expect((SMALL || (T_k & pmask) == 0) && left_k > 0, SMALL)) page_start();
     off1 = off2;
     off2 = off3;
     off3 = off_k;
-    off_k += stage_elems;
+    if (!SMALL) off_k.at[0] += stage_elems;
     T_k += TOK;
   };
   auto copy_k = [&](int k) {
     const int i = wave + W * k;
-    pf::copy_1k(p.k_cache + off3, left_k > 0 ? TOK * row_bytes : 0, vk ^ uint32_t(G::swz_k(W * k * G::RPC) << 4),
-                i * G::RPC * row_bytes, ring_k + slot_k + i * 1024);
+    const int64_t off = off3.at[SMALL ? k : 0];
+    const bool some = left_k > 0 && !(SMALL && off < 0);
+    pf::copy_1k(p.k_cache + (SMALL && off < 0 ? 0 : off), some ? (SMALL ? G::RPC : TOK) * row_bytes : 0,
+                vk ^ uint32_t(G::swz_k(W * k * G::RPC) << 4), SMALL ? 0 : i * G::RPC * row_bytes,
+                ring_k + slot_k + i * 1024);
     if (k == kCopies - 1) {
       slot_k = next_slot(slot_k);
       --left_k;
     }
   };
   // off_v: off1 as it was before this iteration's next_stage()
-  auto copy_v = [&](int k, int64_t off_v) {
+  auto copy_v = [&](int k, const Offs& off_v) {
     const int i = wave + W * k;
-    pf::copy_1k(p.v_cache + off_v, left_v > 0 ? TOK * row_bytes : 0, vv, i * G::RPC * row_bytes,
-                ring_v + slot_v + i * 1024);
+    const int64_t off = off_v.at[SMALL ? k : 0];
+    const bool some = left_v > 0 && !(SMALL && off < 0);
+    pf::copy_1k(p.v_cache + (SMALL && off < 0 ? 0 : off), some ? (SMALL ? G::RPC : TOK) * row_bytes : 0, vv,
+                SMALL ? 0 : i * G::RPC * row_bytes, ring_v + slot_v + i * 1024);
     if (k == kCopies - 1) {
       slot_v = next_slot(slot_v);
       --left_v;
@@ -444,6 +523,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
   float m_run = -INFINITY, neg_m = 0.f, l_run = 0.f, lmax = -INFINITY;
+  float l_true = 0.f;  // LSE: the sum before rounding
 
   auto product_qk = [&](f32x16 (&s)[TT], int i) {
     const int kk = i / TT, u = i % TT;
@@ -481,6 +561,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
       } else {
         pair = pack_bf16x2(e_held, e1);
         l_run = pf::add_pair(pair, l_run);
+        if constexpr (LSE) l_true += e_held + e1;
       }
       pf::pin(pair);
       pk[pr >> 2][pr & 3] = pair;
@@ -502,12 +583,14 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
     pf::wait_vm<2 * kCopies * (kLead - 1), true>();
     raw_barrier();
     const int T0 = (t_first + t) * TOK;
-    if (__builtin_expect(T0 + TOK - 1 > lim_min, 0)) {
+    if (__builtin_expect(T0 + TOK - 1 > lim_min || (PACKED && T0 < lo_max), 0)) {
 #pragma unroll
       for (int u = 0; u < TT; ++u)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (T0 + 32 * u + 8 * (r >> 2) + 4 * hi + (r & 3) > lim) s[u][r] = -INFINITY;
+        for (int r = 0; r < 16; ++r) {
+          const int key = T0 + 32 * u + 8 * (r >> 2) + 4 * hi + (r & 3);
+          if (key > lim || (PACKED && key < lo_key)) s[u][r] = -INFINITY;
+        }
 #pragma unroll
       for (int i = 0; i < 8; ++i) max_step(s, lmax, i);
     }
@@ -519,10 +602,11 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
       const float m_new = mx > m_run + kRescaleSlack ? mx : m_run;
       alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);  // a row that has seen no key keeps -inf
       l_run *= alpha;
+      if constexpr (LSE) l_true *= alpha;
       m_run = m_new;
       neg_m = m_new == -INFINITY ? 0.f : -m_new;
     }
-    const int64_t off_v = off1;
+    const Offs off_v = off1;
     next_stage();
     // phase A
     __builtin_amdgcn_sched_barrier(0);
@@ -573,7 +657,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
       for (int i = 0; i < kCopies; ++i) *reinterpret_cast<u32x4*>(z + i * 1024 * W) = u32x4{0u, 0u, 0u, 0u};
     }
     page_start();
-    int64_t off_v = 0;
+    Offs off_v = {};
     for (int t = -kLead - 2; t < -1; ++t) {
       off_v = off1;
       next_stage();
@@ -587,6 +671,26 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
     pf::wait_vm<kCopies * (kLead - 1 + kLead - 2)>();
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the zeroed slot
     raw_barrier();
+    if (PACKED && row0 >= R_all) {
+      // no real row in this wave: the other waves' waits and barriers, and its share of the copies
+      raw_barrier();
+      for (int t = -1; t < n; ++t) {
+        if (t >= 0) {
+          pf::wait_vm<2 * kCopies * (kLead - 1)>();
+          raw_barrier();
+        }
+        off_v = off1;
+        next_stage();
+#pragma unroll
+        for (int k = 0; k < kCopies; ++k) copy_k(k);
+#pragma unroll
+        for (int k = 0; k < kCopies; ++k) copy_v(k, off_v);
+      }
+      pf::wait_vm<0>();
+      raw_barrier();
+      if (bad_page && lane == 0) flag_status(p.status, PKV_STATUS_BAD_PAGE);
+      return;
+    }
     // The scores and probabilities alternate between two register sets, so the iterations go in pairs;
     // an odd count does stage 0 by itself.
     f32x16 s0[TT], s1[TT];
@@ -651,6 +755,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
 
   const float lsum = pf::sum_halves(l_run);
   const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
+  const float lsum_true = LSE ? pf::sum_halves(l_true) : lsum;
   uint32_t l_end = threadIdx.x & 63;
   pf::pin(l_end);  // the row is worked out again: kept, it would hold registers through the loop
   const LaneRow lo = lane_row(int(l_end));
@@ -679,11 +784,11 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
     if (__any(ovf) && lane == 0) flag_status(p.status, PKV_STATUS_PARTIAL_RANGE);
     return;
   }
-  if constexpr (DEST == pf::kSplit) {
-    if (count > 1) {
+  if constexpr (DEST == pf::kSplit || PACKED) {
+    if (PACKED ? split >= 0 : count > 1) {
       if (lo.real) {
-        int64_t slot = int64_t(blockIdx.x);
-        if constexpr (W == pf::kWaves)
+        int64_t slot = PACKED ? int64_t(split) * p.n_kv + h : int64_t(blockIdx.x);
+        if constexpr (W == pf::kWaves && !PACKED)
           slot = int64_t((b * p.n_kv + h) * (int(gridDim.x) / p.max_splits) + xblk) * p.max_splits + split;
         const int64_t wrow = slot * kRows + lo.r - blk_row0;
         float* dst = p.ws_o + wrow * HD + 4 * hi;
@@ -693,19 +798,31 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
           for (int q = 0; q < 4; ++q)
             *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * q) =
                 f32x4{o[dt][4 * q], o[dt][4 * q + 1], o[dt][4 * q + 2], o[dt][4 * q + 3]};
-        if (hi == 0) *reinterpret_cast<f32x2*>(p.ws_ml + 2 * wrow) = f32x2{m_run, lsum};
+        if constexpr (PACKED) {
+          if (hi == 0) *reinterpret_cast<f32x4*>(p.ws_ml + 4 * wrow) = f32x4{m_run, lsum, lsum_true, 0.f};
+        } else {
+          if (hi == 0) *reinterpret_cast<f32x2*>(p.ws_ml + 2 * wrow) = f32x2{m_run, lsum};
+        }
       }
       return;
     }
   }
+  float scale = inv;
+  if constexpr (PACKED) {
+    if (lo.real) {
+      float lse;
+      scale = pf::finish_row(p, lo.hq, m_run, lsum, lsum_true, lse);
+      if (LSE && hi == 0) p.lse[int64_t(tok0 + lo.j) * (p.n_kv * p.g) + lo.hq] = lse;
+    }
+  }
   if (lo.real) {
-    uint16_t* dst = p.out + lo.b * p.o_sb + lo.j * p.o_ss + lo.hq * p.o_sh + 4 * hi;
+    uint16_t* dst = p.out + (PACKED ? (tok0 + lo.j) * p.o_ss : lo.b * p.o_sb + lo.j * p.o_ss) + lo.hq * p.o_sh + 4 * hi;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const u32x2 ov = {pack_bf16x2(o[dt][4 * q] * inv, o[dt][4 * q + 1] * inv),
-                          pack_bf16x2(o[dt][4 * q + 2] * inv, o[dt][4 * q + 3] * inv)};
+        const u32x2 ov = {pack_bf16x2(o[dt][4 * q] * scale, o[dt][4 * q + 1] * scale),
+                          pack_bf16x2(o[dt][4 * q + 2] * scale, o[dt][4 * q + 3] * scale)};
         *reinterpret_cast<u32x2*>(dst + 32 * dt + 8 * q) = ov;
       }
   }
@@ -768,4 +885,54 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(const AttnParams p, 
   const float inv = l > 0.f ? 1.f / l : 0.f;
   uint16_t* dst = p.out + b * p.o_sb + j * p.o_ss + (h * p.g + row - j * p.g) * p.o_sh + d;
   *reinterpret_cast<u32x2*>(dst) = u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
+}
+
+// Merge of a kPacked launch's split row blocks: grid (kRows / rows per workgroup, or fewer where no split block has
+// so many rows, KV head, split block).
+template <int HD>
+__global__ __launch_bounds__(256) void packed_merge_kernel(const AttnParams p) {
+  constexpr int TPR = HD / 4, RPW = 256 / TPR, B = 8;
+  const PackedMerge mg = p.merges[blockIdx.z];
+  const int h = blockIdx.y;
+  const int r = int(blockIdx.x) * RPW + int(threadIdx.x) / TPR;  // row in the block
+  const int row = mg.row0 + r;
+  if (r >= pf::kRows || row >= mg.n_new * p.g) return;
+  const int64_t w0 = (int64_t(mg.slot) * p.n_kv + h) * pf::kRows + r;
+  const int64_t w_step = int64_t(p.n_kv) * pf::kRows;
+  const int d = (int(threadIdx.x) % TPR) * 4;
+  float m = -INFINITY, l = 0.f, l_true = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < mg.count; s0 += B) {
+    f32x4 po[B];
+    f32x4 pm[B];
+#pragma unroll
+    for (int k = 0; k < B; ++k) {
+      const int64_t w = w0 + min(s0 + k, mg.count - 1) * w_step;
+      po[k] = *reinterpret_cast<const f32x4*>(p.ws_o + w * HD + d);
+      pm[k] = *reinterpret_cast<const f32x4*>(p.ws_ml + 4 * w);
+    }
+    float m_new = m;
+#pragma unroll
+    for (int k = 0; k < B; ++k) m_new = fmaxf(m_new, pm[k][0]);
+    const float keep = m_new == -INFINITY ? 1.f : fast_exp2(m - m_new);
+    l *= keep;
+    l_true *= keep;
+    o *= keep;
+#pragma unroll
+    for (int k = 0; k < B; ++k) {
+      // a range of which the row sees no key has l = 0 and m = -inf
+      const float wt = s0 + k < mg.count && pm[k][1] > 0.f ? fast_exp2(pm[k][0] - m_new) : 0.f;
+      l += wt * pm[k][1];
+      l_true += wt * pm[k][2];
+      o += wt * po[k];
+    }
+    m = m_new;
+  }
+  const int j = row / p.g;
+  const int hq = h * p.g + row - j * p.g;
+  float lse;
+  const float scale = pf::finish_row(p, hq, m, l, l_true, lse);
+  if (p.lse && d == 0) p.lse[int64_t(mg.tok0 + j) * (p.n_kv * p.g) + hq] = lse;
+  uint16_t* dst = p.out + (mg.tok0 + j) * p.o_ss + hq * p.o_sh + d;
+  *reinterpret_cast<u32x2*>(dst) = u32x2{pack_bf16x2(o[0] * scale, o[1] * scale), pack_bf16x2(o[2] * scale, o[3] * scale)};
 }

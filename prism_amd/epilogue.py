@@ -17,10 +17,13 @@ Every call is asynchronous on the current stream and has no CPU fallback.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib
 from .attention import _BF16, _require_gpu, _stream_ptr, status_tensor
+from .packed import _on
 
 
 def rope_tables(head_dim: int, n_pos: int, theta: float = 10000.0,
@@ -118,6 +121,166 @@ def rope_qk(qkv: torch.Tensor, positions: torch.Tensor | int, cos: torch.Tensor,
         *((k_out.stride(0), k_out.stride(1), k_out.stride(2)) if k_out is not None else (0, 0, 0)),
         *cache_args, batch, s_new, n_heads, n_kv, hd, *page_args, st.data_ptr(), _stream_ptr(device))
     _lib.check(rc, "pkv_rope_qk")
+    return q_out, k_out
+
+
+def _scaled_frequencies(rotary_dim: int, n_pos: int, theta: float, scaling: dict | None):
+    """fp64 angle per position of each pair, and what cos and sin are multiplied by."""
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+    freq = float(theta) ** (-i / rotary_dim)
+    kind = (scaling or {}).get("rope_type", (scaling or {}).get("type", "default"))
+    if kind == "default":
+        return freq, 1.0
+    if kind not in ("linear", "dynamic", "yarn"):
+        raise ValueError(f"rotary scaling type {kind!r} is not one of default, linear, dynamic, yarn")
+    missing = {"factor", "original_max_position_embeddings"} - set(scaling) - ({"original_max_position_embeddings"}
+                                                                               if kind == "linear" else set())
+    if missing:
+        raise ValueError(f"rotary scaling {kind!r} needs {', '.join(sorted(missing))}")
+    factor = float(scaling["factor"])
+    if not factor >= 1.0:
+        raise ValueError(f"rotary scaling factor {factor} must be >= 1")
+    if kind == "linear":
+        return freq / factor, 1.0
+    orig = int(scaling["original_max_position_embeddings"])
+    if orig <= 0:
+        raise ValueError("original_max_position_embeddings must be positive")
+    if kind == "dynamic":
+        # a larger base, so that the slowest pair turns over n_pos positions as it did over the original ones
+        if rotary_dim <= 2:
+            raise ValueError("dynamic rotary scaling needs a rotary_dim above 2")
+        grow = max(factor * max(n_pos, orig) / orig - (factor - 1.0), 1.0)
+        return (float(theta) * grow ** (rotary_dim / (rotary_dim - 2))) ** (-i / rotary_dim), 1.0
+    # pairs that turn beta_fast times or more over the original length keep their frequency, pairs of beta_slow
+    # turns or fewer are stretched by the factor, those between by a linear ramp over the pairs' numbers
+    fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+    if not fast > slow > 0.0:
+        raise ValueError("yarn scaling needs beta_fast > beta_slow > 0")
+
+    def pair_of(turns: float) -> float:
+        return rotary_dim * math.log(orig / (turns * 2.0 * math.pi)) / (2.0 * math.log(float(theta)))
+
+    low, high = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rotary_dim - 1)
+    ramp = ((i / 2 - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+    gain = scaling.get("attention_factor")
+    gain = 0.1 * math.log(factor) + 1.0 if gain is None else float(gain)
+    return freq * (1.0 - ramp) + freq / factor * ramp, gain
+
+
+def rotary_tables(rotary_dim: int, n_pos: int, theta: float = 10000.0, *, scaling: dict | None = None,
+                  inv_freq: torch.Tensor | None = None, gain: float = 1.0,
+                  device: torch.device | str = "cuda") -> tuple[torch.Tensor, torch.Tensor]:
+    """cos / sin tables fp32 [n_pos, rotary_dim / 2] of rotate_qk and packed_rope_append: entry [t, i] is the
+    angle t * theta ** (-2 i / rotary_dim), taken in 64 bits (in 32, position 100,000 is off by 0.004 rad) and
+    rounded once.
+
+    ``scaling`` is a model configuration's dict for contexts longer than the trained ones: ``rope_type`` "linear"
+    (all angles divided by ``factor``), "dynamic" (a base that grows with n_pos past
+    ``original_max_position_embeddings``) or "yarn" (slow pairs stretched, fast ones kept; ``beta_fast``,
+    ``beta_slow``, ``attention_factor``).  Or give any frequencies (``inv_freq`` [rotary_dim / 2]) and what cos and
+    sin are multiplied by (``gain``)."""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim {rotary_dim} must be even and positive")
+    if n_pos <= 0:
+        raise ValueError(f"n_pos {n_pos} must be positive")
+    if inv_freq is not None:
+        if scaling is not None or tuple(inv_freq.shape) != (rotary_dim // 2,):
+            raise ValueError(f"inv_freq must be [{rotary_dim // 2}], without scaling")
+        freq = inv_freq.double()
+    else:
+        if not theta > 1.0:
+            raise ValueError(f"theta {theta} must be above 1")
+        freq, factor = _scaled_frequencies(rotary_dim, n_pos, theta, scaling)
+        gain = gain * factor
+    freq = freq.to(device)
+    cos = torch.empty((n_pos, rotary_dim // 2), dtype=torch.float32, device=device)
+    sin = torch.empty_like(cos)
+    for t0 in range(0, n_pos, 1 << 16):   # 64-bit intermediates of at most 2^16 positions
+        t1 = min(t0 + (1 << 16), n_pos)
+        angle = torch.outer(torch.arange(t0, t1, dtype=torch.float64, device=device), freq)
+        cos[t0:t1] = angle.cos() * gain
+        sin[t0:t1] = angle.sin() * gain
+    return cos, sin
+
+
+_ROTARY_DTYPES = {torch.bfloat16: _lib.PKV_BF16, torch.float16: _lib.PKV_FP16, torch.float32: _lib.PKV_FP32}
+
+
+def _check_rotary_tables(cos: torch.Tensor, sin: torch.Tensor, head_dim: int, device) -> int:
+    """The tables' rotary_dim."""
+    for name, t in (("cos", cos), ("sin", sin)):
+        if t.dtype != torch.float32 or t.dim() != 2 or not t.is_contiguous() or t.device != device:
+            raise RuntimeError(f"{name} must be a contiguous float32 [n_pos, rotary_dim / 2] table on {device} "
+                               "(rotary_tables)")
+    if cos.shape != sin.shape or cos.shape[0] == 0 or cos.shape[1] == 0:
+        raise RuntimeError(f"cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must have one shape, not empty")
+    if 2 * cos.shape[1] > head_dim:
+        raise RuntimeError(f"tables for a rotary_dim of {2 * cos.shape[1]} do not fit head_dim {head_dim}")
+    return 2 * cos.shape[1]
+
+
+def _check_norms(q_norm_w, k_norm_w, head_dim: int, dtype, device) -> None:
+    for name, t in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
+        if t is not None and (t.dtype != dtype or tuple(t.shape) != (head_dim,) or not t.is_contiguous() or
+                              t.device != device):
+            raise RuntimeError(f"{name} must be a contiguous {dtype} [{head_dim}] vector on {device}")
+
+
+def rotate_qk(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, cos: torch.Tensor,
+              sin: torch.Tensor, *, interleaved: bool = False, q_norm_w: torch.Tensor | None = None,
+              k_norm_w: torch.Tensor | None = None, eps: float = 1e-6, q_out: torch.Tensor | None = None,
+              k_out: torch.Tensor | None = None, status: torch.Tensor | None = None):
+    """Optional RMSNorm of every query and key head, then the position rotation, in one launch: q [..., n_heads,
+    head_dim] and k [..., n_kv, head_dim] (or None) of one dtype (bf16, fp16 or fp32) with the same leading
+    dimensions, which must flatten to one token axis without a copy; views into the QKV projection are fine.
+    ``positions`` is int32, one per token, ``cos`` / ``sin`` rotary_tables of any rotary_dim up to head_dim:
+    element i turns with its partner i + rotary_dim / 2, or, ``interleaved``, elements 2 i and 2 i + 1.
+
+    fp32 arithmetic, one rounding.  The outputs may be the inputs (in place); k = None returns (q, None).  With
+    ``-sin`` the rotation turns back, which is also its gradient."""
+    _require_gpu(q, "q")
+    if q.dtype not in _ROTARY_DTYPES:
+        raise RuntimeError(f"q must be bfloat16, float16 or float32, got {q.dtype}")
+    if q.dim() < 3:
+        raise RuntimeError(f"q must be [..., n_heads, head_dim] with a token axis, got {tuple(q.shape)}")
+    device, hd, lead = q.device, q.shape[-1], q.shape[:-2]
+    if k is not None and (k.dtype != q.dtype or k.device != device or k.dim() != q.dim() or
+                          k.shape[:-2] != lead or k.shape[-1] != hd):
+        raise RuntimeError(f"k {k.dtype} {tuple(k.shape)} must match q {q.dtype} {tuple(q.shape)} but for the heads")
+    if k is None and (k_norm_w is not None or k_out is not None):
+        raise RuntimeError("k_norm_w and k_out need a k")
+    rotary = _check_rotary_tables(cos, sin, hd, device)
+    _check_norms(q_norm_w, k_norm_w, hd, q.dtype, device)
+    tokens = math.prod(lead)
+    if positions.dtype != torch.int32 or positions.device != device or positions.numel() != tokens or \
+            not positions.is_contiguous():
+        raise RuntimeError(f"positions must be contiguous int32, one for each of the {tokens} tokens, on {device}")
+
+    def rows(t, name, like):
+        if t.dtype != q.dtype or t.device != device or t.shape != like.shape:
+            raise RuntimeError(f"{name} must be {q.dtype} {tuple(like.shape)} on {device}")
+        if t.stride(-1) != 1 and hd > 1:
+            raise RuntimeError(f"{name} must be contiguous in head_dim")
+        try:
+            t3 = t.view(tokens, t.shape[-2], hd)
+        except RuntimeError:
+            raise RuntimeError(f"{name} must flatten to a token axis without a copy") from None
+        return t.data_ptr(), t3.stride(0), t3.stride(1)
+
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=device) if q_out is None else q_out
+    ki = ko = (0, 0, 0)
+    if k is not None:
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=device) if k_out is None else k_out
+        ki, ko = rows(k, "k", k), rows(k_out, "k_out", k)
+    qi, qo = rows(q, "q", q), rows(q_out, "q_out", q)
+    st = status if status is not None else status_tensor(device)
+    with _on(device):
+        rc = _lib.load().pkv_rotate_qk(
+            *qi, *ki, positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+            q_norm_w.data_ptr() if q_norm_w is not None else 0, k_norm_w.data_ptr() if k_norm_w is not None else 0,
+            float(eps), *qo, *ko, tokens, q.shape[-2], k.shape[-2] if k is not None else 0, hd, rotary,
+            int(interleaved), _ROTARY_DTYPES[q.dtype], st.data_ptr(), _stream_ptr(device))
+    _lib.check(rc, "pkv_rotate_qk")
     return q_out, k_out
 
 

@@ -38,6 +38,7 @@ import torch
 
 from . import _lib
 from .attention import poll_status, status_tensor
+from .packed import PackedBatch
 
 
 def shared_prefix_pages(bt_host: np.ndarray, sl_host: np.ndarray, page_size: int) -> int:
@@ -306,6 +307,33 @@ class FlashAttnKVCache:
         if pin:
             poll_status(self.device)   # raises PrismKVStatusError for bits an earlier call set
         return bt, sl
+
+    def build_packed_batch(self, seq_ids: list[int], num_new_tokens: int | list[int], n_heads: int,
+                           windows=(None,)) -> PackedBatch:
+        """The step's PackedBatch: num_new_tokens[i] tokens of seq_ids[i], to be written behind its seq_len tokens
+        (prepare_append first: the pages must be there and not shared).  ``windows`` lists the attention windows
+        that the model's layers use (None: every key)."""
+        counts = [num_new_tokens] * len(seq_ids) if isinstance(num_new_tokens, int) else list(num_new_tokens)
+        if len(counts) != len(seq_ids):
+            raise ValueError(f"{len(seq_ids)} sequences but {len(counts)} token counts")
+        if len(set(seq_ids)) != len(seq_ids):
+            raise ValueError("a sequence is in the batch twice")
+        P = self.page_size
+        for sid, n in zip(seq_ids, counts):
+            pages, start = self.seq_pages[sid], self.seq_len[sid]
+            if n > 0 and -(-(start + n) // P) > len(pages):
+                raise RuntimeError(f"sequence {sid} has {len(pages)} pages for {start} + {n} tokens: prepare_append first")
+            if n > 0 and any(self.is_shared(p) for p in pages[start // P:-(-(start + n) // P)]):
+                raise RuntimeError(f"sequence {sid} would write to a shared page: prepare_append first")
+        if seq_ids:
+            bt, sl = self.block_table_host(seq_ids)
+        else:
+            bt, sl = np.zeros((0, 1), np.int32), np.zeros(0, np.int32)
+        batch = PackedBatch(counts, sl, bt, page_size=P, num_pages=self.max_pages, n_heads=n_heads,
+                            n_kv=self.num_kv_heads, head_dim=self.head_dim, windows=windows, device=self.device)
+        if torch.device(self.device).type == "cuda":
+            poll_status(self.device)
+        return batch
 
     # ------------------------------------------------------------------ page movement
     def layer_bases(self) -> torch.Tensor:

@@ -1,0 +1,282 @@
+"""packed_attention on the device against fp64, and the packed step as a whole."""
+import numpy as np
+import pytest
+import torch
+
+import prism_amd
+from oracle import packed as op
+from prism_amd.attention import read_status
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+def _tol(ref, mag, keys):
+    """The probabilities are rounded to bf16 (half a step, 2^-8 of each), the sum that divides them is of the rounded
+    ones: at most 2^-8 (sum_t p_t |v_t| + |out|).  Scores of N(0, 1) inputs (sums of magnitudes below 16 over 128
+    products), exponentials and sums in fp32: below 2^-12 of the same, and 2^-24 per key summed.  The output is
+    rounded once: 2^-8 of it."""
+    return ref.abs() * 2.0 ** -8 + (mag + ref.abs()) * (2.0 ** -8 + max(2.0 ** -12, keys * 2.0 ** -24))
+
+
+def _check(out, lse, want, keys, what):
+    ref, ref_lse, mag = want
+    got = out.double().cpu()
+    assert torch.isfinite(got).all(), f"{what}: not finite"
+    err = (got - ref).abs()
+    bad = err > _tol(ref, mag, keys)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float(err[bad].max()):.3g}"
+    if lse is not None:
+        # fp32 scores (magnitudes below 16 over 128 products of 2^-24 each), their exponentials' sum, one logarithm
+        e = (lse.double().cpu() - ref_lse).abs()
+        tol = 2.0 ** -12 + keys * 2.0 ** -24 + ref_lse.abs() * 2.0 ** -22
+        assert (e <= tol).all(), f"{what}: lse off by {float(e.max()):.3g}"
+
+
+def _case(gpu, new, ctx, P, nh, nk, hd, seed, windows=(None,), extra=0):
+    g = torch.Generator().manual_seed(seed)
+    need = [-(-(n + c) // P) for n, c in zip(new, ctx)]
+    ids = torch.randperm(sum(need) + 3, generator=g)
+    bt = np.full((len(new), max(need + [1])), -1, np.int32)
+    off = 0
+    for b, n in enumerate(need):
+        bt[b, :n] = ids[off:off + n].numpy()
+        off += n
+    pages = sum(need) + 3
+    kc = torch.randn(pages, P, nk, hd, generator=g).to(BF16)
+    vc = torch.randn(pages, P, nk, hd, generator=g).to(BF16)
+    q = torch.randn(sum(new) + extra, nh, hd, generator=g).to(BF16)
+    batch = prism_amd.PackedBatch(new, ctx, bt, page_size=P, num_pages=pages, n_heads=nh, n_kv=nk, head_dim=hd, windows=windows,
+                                  device=gpu)
+    return batch, torch.from_numpy(bt), kc, vc, q
+
+
+LENGTHS = {
+    "one": ([1], [0]),
+    "short": ([1], [37]),
+    "decode": ([1] * 9, [0, 1, 31, 32, 63, 64, 500, 255, 256]),
+    "mixed": ([1, 65, 0, 1, 200, 3, 17], [700, 0, 50, 1, 129, 31, 64]),
+    "chunk": ([333], [100]),
+    "long": ([1, 2, 40], [5000, 3999, 2500]),
+}
+
+
+@pytest.mark.parametrize("lengths", list(LENGTHS))
+@pytest.mark.parametrize("nh,nk,hd", [(28, 4, 128), (14, 2, 64), (7, 1, 128), (8, 8, 128), (6, 3, 64), (200, 1, 64)])
+@pytest.mark.parametrize("P", [16, 32, 64, 256])
+def test_attention(gpu, lengths, nh, nk, hd, P):
+    new, ctx = LENGTHS[lengths]
+    window = 100 if (nh + P) % 3 == 0 else None
+    batch, bt, kc, vc, q = _case(gpu, new, ctx, P, nh, nk, hd, seed=nh + P, windows=(None, 100))
+    dk, dv, dq = kc.to(gpu), vc.to(gpu), q.to(gpu)
+    for w in {None, window}:
+        out, lse = prism_amd.packed_attention(dq, dk, dv, batch, window=w, return_lse=True)
+        want = op.packed_attention64(q, kc, vc, new, ctx, bt, window=w)
+        _check(out, lse, want, max(n + c for n, c in zip(new, ctx)), f"{lengths} window {w}")
+        plain = prism_amd.packed_attention(dq, dk, dv, batch, window=w)
+        assert torch.equal(plain, out)
+
+
+@pytest.mark.parametrize("window", [1, 2, 31, 32, 33, 64, 129, 5000])
+@pytest.mark.parametrize("P,nh,nk,hd", [(16, 14, 2, 64), (256, 28, 4, 128), (16, 7, 1, 128), (64, 14, 2, 64)])
+def test_windows_and_gone_pages(gpu, window, P, nh, nk, hd):
+    new, ctx = [1, 70, 5, 1, 300], [900, 500, 63, 0, 33]
+    batch, bt, kc, vc, q = _case(gpu, new, ctx, P, nh, nk, hd, seed=window, windows=(window,))
+    sinks = torch.randn(nh, generator=torch.Generator().manual_seed(1)) * 3
+    want = op.packed_attention64(q, kc, vc, new, ctx, bt, window=window, sinks=sinks)
+    # the pages wholly before the first row's window are gone, and what they held is NaN
+    gone = bt.clone()
+    for b in range(len(new)):
+        first = max(ctx[b] - window + 1, 0) // P
+        kc[bt[b, :first].long()] = float("nan")
+        vc[bt[b, :first].long()] = float("nan")
+        gone[b, :first] = -1
+    batch = prism_amd.PackedBatch(new, ctx, gone, page_size=P, num_pages=len(kc), n_heads=nh, n_kv=nk, head_dim=hd,
+                                  windows=(window,), device=gpu)
+    out, lse = prism_amd.packed_attention(q.to(gpu), kc.to(gpu), vc.to(gpu), batch, window=window, sinks=sinks.to(gpu),
+                                          return_lse=True)
+    _check(out, lse, want, 900, f"window {window}")
+    with pytest.raises(RuntimeError, match="laid out for"):
+        prism_amd.packed_attention(q.to(gpu), kc.to(gpu), vc.to(gpu), batch)
+
+
+@pytest.mark.parametrize("P", [16, 256])
+def test_stale_rows_behind_the_last_key_do_not_matter(gpu, P):
+    new, ctx = [1, 33, 7], [100, 0, 250]
+    batch, bt, kc, vc, q = _case(gpu, new, ctx, P, 14, 2, 64, seed=9)
+    want = op.packed_attention64(q, kc, vc, new, ctx, bt)
+    keep = torch.zeros(kc.shape[:2], dtype=torch.bool)
+    for b in range(3):
+        t = torch.arange(new[b] + ctx[b])
+        keep[bt[b].long()[t // P], t % P] = True
+    for bad in (float("nan"), float("inf"), torch.finfo(BF16).min):
+        k2, v2 = kc.clone(), vc.clone()
+        k2[~keep], v2[~keep] = bad, bad
+        _check(prism_amd.packed_attention(q.to(gpu), k2.to(gpu), v2.to(gpu), batch), None, want, 300, f"stale {bad}")
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_extreme_scores_and_sinks(gpu, hd):
+    """Scores of thousands: the softmax is a choice of one key, or of the sink."""
+    new, ctx = [40, 1], [60, 1999]
+    batch, bt, kc, vc, q = _case(gpu, new, ctx, 64, 8, 2, hd, seed=4)
+    q = q * 256
+    # scores are exact up to 2^-24 of the magnitudes summed (below 256 * 16): 2^-12 of a unit, like N(0, 1) inputs'
+    # 2^-12; rows whose two best keys are closer than that are still within the tolerance's p-weighted terms
+    for sinks in (None, torch.tensor([-1e30, -3000.0, 0.0, 500.0, 1000.0, 5000.0, float("-inf"), 1e30])):
+        want = op.packed_attention64(q, kc, vc, new, ctx, bt, sinks=sinks)
+        out, lse = prism_amd.packed_attention(q.to(gpu), kc.to(gpu), vc.to(gpu), batch, return_lse=True,
+                                              sinks=sinks.to(gpu) if sinks is not None else None)
+        assert torch.isfinite(out).all()
+        # a score error d of up to 2^-24 * 128 * 4096 = 2^-5 moves p by p (1 - p) d
+        # a weight below the smallest normal fp32 number (2^-126) may be lost: with fewer than 2^11 keys and |v| < 2^3
+        # that is less than 2^-112 of the output (rows that a sink leaves next to nothing of)
+        err = (out.double().cpu() - want[0]).abs()
+        tol = _tol(want[0], want[2], 2000) + 2.0 ** -4 * (want[2] + want[0].abs()) + 2.0 ** -112
+        assert (err <= tol).all(), f"{float((err / tol).max())} {float(want[0].flatten()[(err / tol).argmax()])}"
+        e = (lse.double().cpu() - want[1]).abs()
+        assert (e <= 2.0 ** -5 + want[1].abs() * 2.0 ** -22).all()
+
+
+def test_scale_strides_out_and_padding(gpu):
+    new, ctx = [3, 60, 1], [10, 70, 500]
+    nh, nk, hd, P, total = 14, 2, 64, 64, 64
+    batch, bt, kc, vc, q = _case(gpu, new, ctx, P, nh, nk, hd, seed=2, extra=6)
+    want = op.packed_attention64(q[:total], kc, vc, new, ctx, bt, scale=0.3)
+    # q a view into the fused projection, the caches views of one pool, out a view with a row of its own
+    wide = torch.randn(total + 6, (nh + 4) * hd).to(BF16)
+    wide[:, :nh * hd] = q.flatten(1)
+    pool = torch.stack([kc, vc], 1).to(gpu)
+    out = torch.full((total + 6, nh + 2, hd), 9.0, dtype=BF16, device=gpu)
+    got = prism_amd.packed_attention(wide.to(gpu)[:, :nh * hd].unflatten(1, (nh, hd)), pool[:, 0], pool[:, 1], batch,
+                                     softmax_scale=0.3, out=out[:, 1:-1])
+    assert got.data_ptr() == out[:, 1:-1].data_ptr()
+    _check(got[:total], None, want, 600, "views")
+    assert (out[:, 0] == 9).all() and (out[:, -1] == 9).all() and (out[total:] == 9).all()
+    own, lse = prism_amd.packed_attention(q.to(gpu), pool[:, 0], pool[:, 1], batch, softmax_scale=0.3, return_lse=True)
+    assert torch.equal(own[:total], got[:total]) and not own[total:].any() and not lse[total:].any()
+
+
+def test_nothing_new(gpu):
+    for new, ctx in (([], []), ([0, 0], [5, 0])):
+        batch, bt, kc, vc, q = _case(gpu, new, ctx, 16, 14, 2, 64, seed=2, extra=3)
+        out, lse = prism_amd.packed_attention(q.to(gpu), kc.to(gpu), vc.to(gpu), batch, return_lse=True)
+        assert out.shape == (3, 14, 64) and not out.any() and not lse.any()
+        cos, sin = prism_amd.rotary_tables(64, 4, device=gpu)
+        x = torch.zeros(3, 18 * 64, dtype=BF16, device=gpu)
+        assert not prism_amd.packed_rope_append(x, kc.to(gpu), vc.to(gpu), batch, cos, sin).any()
+
+
+def test_a_page_that_goes_bad_is_flagged(gpu):
+    for P in (16, 256):
+        batch, bt, kc, vc, q = _case(gpu, [1, 30], [400, 300], P, 14, 2, 64, seed=2)
+        batch.block_table[1, 0] = len(kc)
+        prism_amd.packed_attention(q.to(gpu), kc.to(gpu), vc.to(gpu), batch)
+        assert read_status(gpu) == prism_amd._lib.PKV_STATUS_BAD_PAGE
+
+
+def test_refusals(gpu):
+    batch, bt, kc, vc, q = _case(gpu, [3], [4], 16, 4, 2, 64, seed=2)
+    q, kc, vc = q.to(gpu), kc.to(gpu), vc.to(gpu)
+    f = prism_amd.packed_attention
+    for a, kw in [((q.float(), kc, vc, batch), {}), ((q[:2], kc, vc, batch), {}), ((q[:, :2], kc, vc, batch), {}),
+                  ((q.transpose(1, 2).contiguous().transpose(1, 2), kc, vc, batch), {}), ((q, kc.float(), vc.float(), batch), {}),
+                  ((q, kc[:, :8], vc[:, :8], batch), {}), ((q, kc[:2], vc[:2], batch), {}), ((q, kc, vc, batch), dict(window=3)),
+                  ((q, kc, vc, batch), dict(sinks=torch.zeros(4, dtype=BF16, device=gpu))),
+                  ((q, kc, vc, batch), dict(sinks=torch.zeros(3, device=gpu))), ((q, kc, vc, batch), dict(out=q[:, :2])),
+                  ((q, kc, vc, batch), dict(out=q.float())), ((q, kc, vc, batch), dict(softmax_scale=0.0))]:
+        with pytest.raises(RuntimeError):
+            f(*a, **kw)
+    with pytest.raises(RuntimeError, match="host"):
+        prism_amd.PackedBatch(torch.tensor([1], device=gpu), [0], [[0]], page_size=16, num_pages=1, n_heads=4, n_kv=2, head_dim=64)
+    with pytest.raises(RuntimeError, match="before the capture"):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            _case(gpu, [3], [4], 16, 4, 2, 64, seed=2)
+
+
+def test_captured_replayed_and_two_streams(gpu):
+    """Calls that split their keys, in two graphs and eagerly on two streams at once: each has partials of its own."""
+    new, ctx = [1, 1, 20], [3000, 6000, 2500]
+    batch, bt, kc, vc, q = _case(gpu, new, ctx, 64, 28, 4, 128, seed=8)
+    assert batch._plans[None][3] > 0
+    dk, dv = kc.to(gpu), vc.to(gpu)
+    qs = [q.to(gpu), (q * 0.5).to(gpu)]
+    graphs, outs = [], []
+    for x in qs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(prism_amd.packed_attention(x, dk, dv, batch, return_lse=True))
+        graphs.append(graph)
+    side = torch.cuda.Stream()
+    for i in range(4):
+        for x in qs:
+            x.normal_()
+        torch.cuda.synchronize()
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+            eager1 = prism_amd.packed_attention(qs[0], dk, dv, batch, return_lse=True)
+        eager0 = prism_amd.packed_attention(qs[1], dk, dv, batch, return_lse=True)
+        torch.cuda.synchronize()
+        for a, b in ((outs[0], eager1), (outs[1], eager0)):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]), i
+    want = op.packed_attention64(qs[0].cpu(), kc, vc, new, ctx, bt)
+    _check(*outs[0], want, 6001, "replayed")
+
+
+def test_same_bits_every_time(gpu):
+    batch, bt, kc, vc, q = _case(gpu, [1, 50, 1], [9000, 2000, 10], 256, 28, 4, 128, seed=8)
+    a = [prism_amd.packed_attention(q.to(gpu), kc.to(gpu), vc.to(gpu), batch, return_lse=True) for _ in range(5)]
+    assert all(torch.equal(a[0][0], b[0]) and torch.equal(a[0][1], b[1]) for b in a[1:])
+
+
+@pytest.mark.parametrize("nh,nk,hd,P,window", [(28, 4, 128, 256, None), (14, 2, 64, 16, 40), (7, 1, 128, 16, None)])
+def test_steps_of_a_served_batch(gpu, nh, nk, hd, P, window):
+    """Three steps (prompts; a mix with a forked sequence; decode) through the cache: every step's queries, cache and
+    attention against a history kept in fp64 from the inputs, and the pages that others share left alone."""
+    kv = prism_amd.FlashAttnKVCache(1, nk, hd, 64 if P == 256 else 200, P, gpu)
+    g = torch.Generator().manual_seed(nh)
+    cos, sin = prism_amd.rotary_tables(hd, 4096, 1e4, device=gpu)
+    freq = 1e4 ** (-torch.arange(0, hd, 2, dtype=torch.float64) / hd)
+    for s in (1, 2, 3):
+        kv.new_sequence(s)
+    hist = {s: [] for s in (1, 2, 3, 4)}
+    steps = [([1, 2, 3], [300, 45, 1]), ([3, 1, 2], [1, 70, 1]), ([4, 1, 3, 2], [5, 1, 1, 130]), ([1, 2, 3, 4], [1, 1, 1, 1])]
+    for ids, counts in steps:
+        if 4 in ids and 4 not in kv.seq_pages:
+            kv.fork_sequence(2, 4)
+            hist[4] = list(hist[2])
+        kv.prepare_append(ids, counts)
+        batch = kv.build_packed_batch(ids, counts, nh, windows=(window,))
+        x = torch.randn(sum(counts), (nh + 2 * nk) * hd, generator=g).to(BF16)
+        q = prism_amd.packed_rope_append(x.to(gpu), kv.k_caches[0], kv.v_caches[0], batch, cos, sin)
+        out, lse = prism_amd.packed_attention(q, kv.k_caches[0], kv.v_caches[0], batch, window=window, return_lse=True)
+        ctx = [kv.seq_len[s] for s in ids]
+        kv.update_seqlens(ids, counts)
+        pos = batch.positions.cpu()
+        want, mag = op.rotate64(x[:, :(nh + nk) * hd].unflatten(1, (nh + nk, hd)), pos, freq)
+        tol = want.abs() * 2.0 ** -8 + mag * 2.0 ** -20
+        assert ((q.double().cpu() - want[:, :nh]).abs() <= tol[:, :nh]).all()
+        first = 0
+        bt, _ = kv.block_table_host(ids)
+        for s, n in zip(ids, counts):
+            hist[s] += [(want[i, nh:], tol[i, nh:], x[i, (nh + nk) * hd:].unflatten(0, (nk, hd))) for i in range(first, first + n)]
+            first += n
+            at = torch.arange(len(hist[s]))
+            row = torch.tensor(kv.seq_pages[s])[at // P]
+            k, v = kv.k_caches[0].cpu()[row, at % P], kv.v_caches[0].cpu()[row, at % P]
+            assert ((k.double() - torch.stack([h[0] for h in hist[s]])).abs() <= torch.stack([h[1] for h in hist[s]])).all()
+            assert torch.equal(v, torch.stack([h[2] for h in hist[s]]))
+        ref = op.packed_attention64(q.cpu(), kv.k_caches[0].cpu(), kv.v_caches[0].cpu(), counts, ctx, torch.from_numpy(bt), window=window)
+        _check(out, lse, ref, 500, f"step {ids}")
+        if window is None:
+            # the framework's other attention, sequence by sequence over the same pages
+            first = 0
+            for i, (s, n) in enumerate(zip(ids, counts)):
+                o = prism_amd.flash_attn_with_kvcache(q[None, first:first + n], kv.k_caches[0], kv.v_caches[0],
+                                                      cache_seqlens=torch.tensor([kv.seq_len[s]], dtype=torch.int32, device=gpu),
+                                                      block_table=torch.from_numpy(bt[i:i + 1]).to(gpu), causal=True)
+                t = _tol(ref[0][first:first + n], ref[2][first:first + n], 500)
+                assert ((o[0].double().cpu() - ref[0][first:first + n]).abs() <= t).all()
+                first += n

@@ -1,0 +1,323 @@
+"""The packed step without a GPU: work lists, slots, tables, refusals."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import prism_amd
+from oracle import packed as op
+from prism_amd import _lib
+from prism_amd.kv_cache import FlashAttnKVCache
+
+A16 = 1 << 20
+
+
+def _plan(new, ctx, nh, nk, hd, window=0, cus=256):
+    lib = _lib.load()
+    new, ctx = np.asarray(new, np.int32), np.asarray(ctx, np.int32)
+    counts = np.zeros(4, np.int32)
+    args = (new.ctypes.data, ctx.ctypes.data, len(new), nh, nk, hd, window, cus)
+    assert lib.pkv_packed_plan(*args, 0, 0, 0, 0, counts.ctypes.data) == 0
+    items, merges = np.zeros((counts[0], 8), np.int32), np.zeros((max(counts[1], 1), 8), np.int32)
+    assert lib.pkv_packed_plan(*args, items.ctypes.data, counts[0], merges.ctypes.data, counts[1], counts.ctypes.data) == 0
+    return items, merges[:counts[1]], counts
+
+
+@pytest.mark.parametrize("nh,nk,hd", [(28, 4, 128), (14, 2, 64), (7, 1, 128), (40, 8, 128), (300, 2, 64), (64, 64, 128)])
+@pytest.mark.parametrize("window", [0, 1, 33, 1000])
+@pytest.mark.parametrize("cus", [256, 8, 1])
+def test_plan_covers_every_visible_key_once(nh, nk, hd, window, cus):
+    rng = np.random.default_rng(nh + window + cus)
+    for trial in range(6):
+        n = int(rng.integers(0, 40))
+        new = np.where(rng.random(n) < 0.6, 1, rng.integers(0, 700, n)) * (rng.random(n) < 0.9)
+        ctx = rng.integers(0, [1, 50, 3000, 60000][trial % 4], n) if n else new
+        items, merges, counts = _plan(new, ctx, nh, nk, hd, window, cus)
+        g, tok = nh // nk, 32 if hd == 128 else 64
+        tok0 = np.cumsum(new) - new
+        stages, slots = {}, []
+        for t0, s, c, b, row0, st0, ns, slot in items.tolist():
+            assert (t0, s, c) == (tok0[b], new[b], ctx[b]) and s > 0 and ns > 0 and row0 % 128 == 0 and row0 < s * g
+            stages.setdefault((b, row0), []).append((st0, ns, slot))
+            if slot >= 0:
+                slots.append(slot)
+        assert sorted(slots) == list(range(counts[2]))
+        assert set(stages) == {(b, r) for b in range(n) for r in range(0, int(new[b]) * g, 128)}
+        for (b, row0), parts in stages.items():
+            last = ctx[b] + (min(row0 + 128, new[b] * g) - 1) // g
+            first = max(ctx[b] + row0 // g - window + 1, 0) if window else 0
+            parts.sort()
+            at = first // tok
+            for st0, ns, slot in parts:
+                assert st0 == at and (slot >= 0) == (len(parts) > 1)
+                at += ns
+            assert at == last // tok + 1
+        split = {k: v for k, v in stages.items() if len(v) > 1}
+        assert len(merges) == len(split)
+        for t0, s, row0, slot, count, *_ in merges.tolist():
+            (b,) = [b for b in range(n) if tok0[b] == t0 and new[b] == s and (b, row0) in split]
+            assert sorted(p[2] for p in split[b, row0]) == list(range(slot, slot + count))
+            assert counts[3] >= min(128, s * g - row0)
+        assert counts[3] <= 128
+
+
+def test_plan_refusals():
+    lib = _lib.load()
+    c = np.zeros(4, np.int32)
+    one, neg, big = np.array([1], np.int32), np.array([-1], np.int32), np.array([1 << 27], np.int32)
+
+    def call(new=one, ctx=one, batch=1, nh=4, nk=2, hd=128, window=0, cus=256, counts=c.ctypes.data, mi=0, items=0):
+        return lib.pkv_packed_plan(new.ctypes.data if new is not None else 0, ctx.ctypes.data, batch, nh, nk, hd, window,
+                                   cus, items, mi, 0, 0, counts)
+    assert call() == 0
+    for bad in [dict(new=neg), dict(ctx=neg), dict(ctx=big), dict(nh=3), dict(nk=0), dict(hd=96), dict(window=-1),
+                dict(cus=0), dict(batch=-1), dict(counts=0), dict(new=None), dict(new=big, ctx=np.zeros(1, np.int32), nh=64)]:
+        assert call(**bad) == _lib.PKV_EINVAL, bad
+        assert "pkv_packed_plan" in lib.pkv_last_error().decode()
+    room = np.zeros(8, np.int32)
+    assert call(items=room.ctypes.data, mi=0) == _lib.PKV_ENOSPC
+
+
+def _batch(**over):
+    a = dict(new_lens=[1, 0, 300], cache_lens=[500, 3, 7], block_table=[[1, 2], [-1, -1], [4, 5]], page_size=256, num_pages=9,
+             n_heads=28, n_kv=4, head_dim=128, device="cpu")
+    a.update(over)
+    return prism_amd.PackedBatch(a.pop("new_lens"), a.pop("cache_lens"), a.pop("block_table"), **a)
+
+
+def test_batch_positions_and_slots():
+    b = _batch(windows=(None, 64, None))
+    assert b.total_tokens == 301 and list(b._plans) == [None, 64]
+    assert b.positions.tolist() == [500] + list(range(7, 307))
+    assert b.slots.tolist() == [2 * 256 + 244] + [(4 if t < 256 else 5) * 256 + t % 256 for t in range(7, 307)]
+    assert b.block_table.tolist() == [[1, 2], [-1, -1], [4, 5]]
+    empty = _batch(new_lens=[], cache_lens=[], block_table=np.zeros((0, 1), np.int32))
+    assert empty.total_tokens == 0 and empty.positions.numel() == 0
+    none = _batch(new_lens=[0, 0, 0])
+    assert none.total_tokens == 0 and none._plans[None][1] == 0
+    # pages wholly before the window may be gone
+    _batch(new_lens=[1, 0, 0], block_table=[[-1, 2], [-1, -1], [-1, -1]], windows=(100,))
+
+
+@pytest.mark.parametrize("over,msg", [
+    (dict(new_lens=[1, 0]), "block-table rows"),
+    (dict(new_lens=[1, 0, -3]), "negative"),
+    (dict(cache_lens=[500, 3, 1 << 27]), "2\\^27"),
+    (dict(new_lens=[1.0, 0.0, 3.0]), "integers"),
+    (dict(block_table=[[1, 2, 3, 4, 5, 6]]), "block-table rows"),
+    (dict(new_lens=[1, 0, 600]), "columns"),
+    (dict(block_table=[[1, 9], [-1, -1], [4, 5]]), "outside"),
+    (dict(block_table=[[-1, 2], [-1, -1], [4, 5]]), "outside"),
+    (dict(block_table=[[1, 2], [-1, -1], [4, 2]]), "one page"),
+    (dict(block_table=[[1, 2], [-1, -1], [4, 4]]), "one page"),
+    (dict(page_size=48), "power of two"),
+    (dict(page_size=8), "power of two"),
+    (dict(num_pages=0), "pool"),
+    (dict(num_pages=1 << 24), "pool"),
+    (dict(head_dim=96), "head_dim"),
+    (dict(n_heads=30), "multiple"),
+    (dict(windows=()), "at least one"),
+    (dict(windows=(0,)), "window"),
+    (dict(windows=(2.5,)), "window"),
+    (dict(windows=(True,)), "window"),
+])
+def test_batch_refusals(over, msg):
+    with pytest.raises(RuntimeError, match=msg):
+        _batch(**over)
+
+
+def test_ops_need_the_device():
+    b = _batch()
+    x = torch.zeros(301, 36 * 128, dtype=torch.bfloat16)
+    cache = torch.zeros(9, 256, 4, 128, dtype=torch.bfloat16)
+    cos, sin = prism_amd.rotary_tables(128, 4, device="cpu")
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        prism_amd.packed_rope_append(x, cache, cache, b, cos, sin)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        prism_amd.packed_attention(x[:, :3584].view(301, 28, 128), cache, cache, b)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        prism_amd.rotate_qk(x.view(301, 36, 128), None, torch.zeros(301, dtype=torch.int32), cos, sin)
+
+
+def test_cache_builds_the_batch():
+    kv = FlashAttnKVCache(1, 2, 64, 12, 16, "cpu")
+    kv.new_sequence(1)
+    kv.new_sequence(2)
+    kv.prepare_append([1, 2], [20, 1])
+    kv.update_seqlens([1, 2], [20, 1])
+    with pytest.raises(RuntimeError, match="prepare_append"):
+        kv.build_packed_batch([1, 2], [40, 1], 14)
+    with pytest.raises(ValueError, match="twice"):
+        kv.build_packed_batch([1, 1], 1, 14)
+    with pytest.raises(ValueError, match="counts"):
+        kv.build_packed_batch([1, 2], [1], 14)
+    kv.prepare_append([1, 2], [40, 1])
+    b = kv.build_packed_batch([2, 1], [1, 40], 14, windows=(None, 8))
+    pages = kv.seq_pages
+    assert b.positions.tolist() == [1] + list(range(20, 60))
+    assert b.slots.tolist() == [pages[2][0] * 16 + 1] + [pages[1][t // 16] * 16 + t % 16 for t in range(20, 60)]
+    kv.fork_sequence(2, 3)
+    with pytest.raises(RuntimeError, match="shared"):
+        kv.build_packed_batch([3], 1, 14)
+    assert kv.build_packed_batch([], [], 14).total_tokens == 0
+
+
+# ---------------------------------------------------------------------------------- tables
+def _yarn(rd, theta, f, orig, fast=32.0, slow=1.0):
+    """Pair by pair: turns over the original length decide between the plain and the stretched frequency."""
+    out = []
+    number = lambda turns: rd * math.log(orig / (turns * 2 * math.pi)) / (2 * math.log(theta))
+    lo, hi = max(math.floor(number(fast)), 0), min(math.ceil(number(slow)), rd - 1)
+    for i in range(rd // 2):
+        plain = theta ** (-2 * i / rd)
+        r = min(max((i - lo) / max(hi - lo, 1e-3), 0.0), 1.0)
+        out.append(plain * (1 - r) + plain / f * r)
+    return torch.tensor(out, dtype=torch.float64)
+
+
+@pytest.mark.parametrize("rd,theta,n_pos,scaling", [
+    (128, 1e6, 70000, None), (64, 1e4, 3, None), (2, 1e4, 5, None),
+    (64, 1e4, 900, dict(rope_type="linear", factor=8.0)),
+    (64, 1e4, 900, dict(rope_type="default")),
+    (32, 1e4, 9000, dict(type="dynamic", factor=2.0, original_max_position_embeddings=2048)),
+    (32, 1e4, 900, dict(type="dynamic", factor=2.0, original_max_position_embeddings=2048)),
+    (128, 1e6, 131072, dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=32768)),
+    (64, 1e4, 500, dict(rope_type="yarn", factor=16.0, original_max_position_embeddings=2048, beta_fast=20, beta_slow=2,
+                        attention_factor=1.0)),
+])
+def test_rotary_tables(rd, theta, n_pos, scaling):
+    cos, sin = prism_amd.rotary_tables(rd, n_pos, theta, scaling=scaling, device="cpu")
+    assert cos.shape == sin.shape == (n_pos, rd // 2) and cos.dtype == torch.float32
+    kind = (scaling or {}).get("rope_type", (scaling or {}).get("type"))
+    freq, gain = theta ** (-torch.arange(rd // 2, dtype=torch.float64) * 2 / rd), 1.0
+    if kind == "linear":
+        freq = freq / scaling["factor"]
+    elif kind == "dynamic":
+        orig, f = 2048, 2.0
+        base = theta * max(f * max(n_pos, orig) / orig - f + 1, 1.0) ** (rd / (rd - 2))
+        freq = base ** (-torch.arange(rd // 2, dtype=torch.float64) * 2 / rd)
+    elif kind == "yarn":
+        freq = _yarn(rd, theta, scaling["factor"], scaling["original_max_position_embeddings"],
+                     scaling.get("beta_fast", 32.0), scaling.get("beta_slow", 1.0))
+        gain = scaling.get("attention_factor", 0.1 * math.log(scaling["factor"]) + 1)
+    pos = torch.unique(torch.tensor([0, 1, n_pos // 2, n_pos - 1]).clamp(max=n_pos - 1))
+    angle = pos.double()[:, None] * freq
+    # the fp64 angle is off by a few 2^-53 of up to n_pos radians; then one rounding to 24 bits
+    tol = gain * (2.0 ** -24 + 8 * n_pos * 2.0 ** -53)
+    assert (cos[pos].double() - angle.cos() * gain).abs().max() <= tol
+    assert (sin[pos].double() - angle.sin() * gain).abs().max() <= tol
+
+
+def test_rotary_tables_frequencies_and_refusals():
+    f = torch.tensor([0.5, 0.25])
+    cos, sin = prism_amd.rotary_tables(4, 3, inv_freq=f, gain=2.0, device="cpu")
+    assert torch.allclose(cos[2], 2 * torch.cos(2 * f)) and torch.allclose(sin[1], 2 * torch.sin(f))
+    for kw in [dict(rotary_dim=3), dict(rotary_dim=0), dict(n_pos=0), dict(theta=1.0), dict(inv_freq=torch.ones(3)),
+               dict(inv_freq=torch.ones(2), scaling=dict(rope_type="linear", factor=2.0)),
+               dict(scaling=dict(rope_type="linear", factor=0.5)), dict(scaling=dict(rope_type="ntk", factor=2.0)),
+               dict(rotary_dim=2, scaling=dict(rope_type="dynamic", factor=2.0, original_max_position_embeddings=8)),
+               dict(scaling=dict(rope_type="yarn", factor=2.0, original_max_position_embeddings=8, beta_fast=1, beta_slow=2)),
+               dict(scaling=dict(rope_type="yarn", factor=2.0, original_max_position_embeddings=0))]:
+        a = dict(rotary_dim=4, n_pos=3, device="cpu")
+        a.update(kw)
+        with pytest.raises(ValueError):
+            prism_amd.rotary_tables(a.pop("rotary_dim"), a.pop("n_pos"), **a)
+
+
+def test_oracle_rotation_gradient():
+    """The rotation is linear in the head: its gradient is the rotation by the opposite angle."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(3, 2, 16, generator=g, dtype=torch.float64)
+    w = torch.randn(3, 2, 16, generator=g, dtype=torch.float64)
+    pos, f = torch.tensor([0, 5, 9]), torch.rand(4, generator=g, dtype=torch.float64)
+    for inter in (False, True):
+        back, _ = op.rotate64(w, -pos, f, interleaved=inter, gain=1.5)
+        for k in range(5):
+            d = torch.zeros_like(x)
+            d.view(-1)[k * 17] = 1.0
+            diff = ((op.rotate64(x + d, pos, f, interleaved=inter, gain=1.5)[0] -
+                     op.rotate64(x - d, pos, f, interleaved=inter, gain=1.5)[0]) / 2 * w).sum()
+            want = back.clone()
+            want[..., 8:] = w[..., 8:]
+            assert abs(diff - want.view(-1)[k * 17]) < 1e-12
+
+
+# ---------------------------------------------------------------------------------- the C entries' refusals
+def _rotate(lib, **over):
+    a = dict(q=A16, q_st=512, q_sh=128, k=A16, k_st=512, k_sh=128, pos=A16, cos=A16, sin=A16, n_pos=5, qw=0, kw=0, eps=1e-6,
+             qo=A16, qo_st=512, qo_sh=128, ko=A16, ko_st=512, ko_sh=128, tokens=3, nh=4, nk=4, hd=128, rd=128, inter=0, dtype=0)
+    a.update(over)
+    return lib.pkv_rotate_qk(*a.values(), None, None)
+
+
+@pytest.mark.parametrize("over,msg", [
+    (dict(tokens=-1), "bad sizes"), (dict(nh=0), "bad sizes"), (dict(n_pos=0), "bad sizes"), (dict(nk=-1), "bad sizes"),
+    (dict(hd=0), "head_dim"), (dict(hd=1025), "head_dim"), (dict(rd=0), "rotary_dim"), (dict(rd=130), "rotary_dim"),
+    (dict(rd=63), "rotary_dim"), (dict(cos=0), "null"), (dict(sin=A16 + 2), "aligned"), (dict(eps=-1.0), "eps"),
+    (dict(eps=math.nan), "eps"), (dict(dtype=3), "dtype"), (dict(q=0), "null"), (dict(k=0), "null"), (dict(ko=0), "null"),
+    (dict(pos=0), "null"), (dict(qo=A16 + 1), "aligned"), (dict(kw=A16 + 1), "aligned"), (dict(q=A16 + 2, dtype=2), "aligned"),
+    (dict(nh=70000), "heads"),
+])
+def test_rotate_argument_errors(over, msg):
+    lib = _lib.load()
+    assert _rotate(lib, **over) == _lib.PKV_EINVAL
+    err = lib.pkv_last_error().decode()
+    assert "pkv_rotate_qk" in err and msg in err, err
+
+
+def test_rotate_nothing_to_do():
+    assert _rotate(_lib.load(), tokens=0, q=0, k=0) == 0
+
+
+def _append(lib, **over):
+    a = dict(qkv=A16, st=36 * 128, pos=A16, slots=A16, cos=A16, sin=A16, n_pos=5, qw=0, kw=0, eps=1e-6, qo=A16, qo_st=28 * 128,
+             qo_sh=128, kc=A16, vc=A16, ps=256 * 512, tokens=3, nh=28, nk=4, hd=128, rd=128, inter=0, page=256, pages=9)
+    a.update(over)
+    return lib.pkv_packed_rope_append(*a.values(), None, None)
+
+
+@pytest.mark.parametrize("over,msg", [
+    (dict(hd=96, rd=96), "head_dim"), (dict(rd=24), "rotary_dim"), (dict(nk=0), "bad sizes"), (dict(pages=0), "bad sizes"),
+    (dict(page=24), "page_size"), (dict(page=8), "page_size"), (dict(pages=1 << 23), "slots"), (dict(slots=0), "null"),
+    (dict(kc=0), "null"), (dict(ps=100), "page stride"), (dict(ps=256 * 512 + 4), "page stride"), (dict(qkv=A16 + 8), "aligned"),
+    (dict(st=36 * 128 + 4), "aligned"), (dict(vc=A16 + 8), "aligned"), (dict(cos=A16 + 4), "aligned"),
+    (dict(qw=A16 + 4), "aligned"), (dict(qo=A16 + 4), "aligned"), (dict(qo_sh=132), "multiples of 8"), (dict(tokens=-1), "bad sizes"),
+])
+def test_append_argument_errors(over, msg):
+    lib = _lib.load()
+    assert _append(lib, **over) == _lib.PKV_EINVAL
+    err = lib.pkv_last_error().decode()
+    assert "pkv_packed_rope_append" in err and msg in err, err
+
+
+def _attn(lib, **over):
+    a = dict(q=A16, q_st=28 * 128, q_sh=128, kc=A16, vc=A16, ps=256 * 512, bt=A16, bts=4, out=A16, o_st=28 * 128, o_sh=128, lse=0,
+             sinks=0, items=A16, n_items=3, merges=A16, n_merges=1, partials=2, merge_rows=7, ws=A16, wsb=1 << 30, tokens=3,
+             batch=3, nh=28, nk=4, hd=128, page=256, pages=9, mb=4, window=0, scale=0.1)
+    a.update(over)
+    return lib.pkv_packed_attn(*a.values(), None, None)
+
+
+@pytest.mark.parametrize("over,msg", [
+    (dict(tokens=-1), "bad sizes"), (dict(n_items=-1), "bad sizes"), (dict(window=-1), "bad sizes"), (dict(hd=96), "head_dim"),
+    (dict(page=24), "page_size"), (dict(bts=3), "bt_stride"), (dict(nh=30), "multiple of n_kv"), (dict(q=A16 + 8), "aligned"),
+    (dict(o_st=28 * 128 + 4), "multiples of 8"), (dict(lse=A16 + 2), "aligned"), (dict(sinks=A16 + 1), "aligned"),
+    (dict(items=0), "null"), (dict(merges=0), "null"), (dict(items=A16 + 4), "aligned"), (dict(n_merges=65536), "too many"),
+    (dict(ws=0), "workspace"), (dict(ws=A16 + 8), "workspace"), (dict(scale=math.inf), "softmax_scale"), (dict(kc=0), "null"),
+    (dict(n_items=1 << 30), "too many"),
+])
+def test_attention_argument_errors(over, msg):
+    lib = _lib.load()
+    assert _attn(lib, **over) == _lib.PKV_EINVAL
+    err = lib.pkv_last_error().decode()
+    assert "pkv_packed_attn" in err and msg in err, err
+
+
+def test_attention_workspace():
+    lib = _lib.load()
+    need = lib.pkv_packed_workspace_bytes(2, 4, 128)
+    assert need == 2 * 4 * 128 * 132 * 4
+    assert lib.pkv_packed_workspace_bytes(0, 4, 128) == 0
+    assert _attn(lib, wsb=need - 1) == _lib.PKV_ENOSPC
+    assert _attn(lib, n_items=0, items=0, ws=0) == 0
