@@ -355,7 +355,7 @@ int pkv_rope_qk(const void* qkv, int64_t qkv_sb, int64_t qkv_ss, const int32_t* 
  * throughout, one rounding to dtype (PKV_BF16, PKV_FP16, PKV_FP32: of q, k, the outputs and the norm weights
  * alike).  The outputs may be the inputs.  A position outside the tables is clamped and flags
  * PKV_STATUS_BAD_POSITION.  head_dim at most 1024, rotary_dim even; any strides.  16-byte aligned rows with
- * head_dim and rotary_dim multiples of 16 run in 16-byte accesses, others element by element.  The rotation is
+ * head_dim and rotary_dim multiples of 16 (fp32: 8) run in 16-byte accesses, others element by element.  The rotation is
  * what engine/executor.py:_apply_rope does for the half layout of a whole head, without its bf16 rounding after
  * every operation (pkv_rope_qk keeps those).
  */

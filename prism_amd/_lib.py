@@ -6,6 +6,7 @@ package raises.  There is no CPU or PyTorch fallback.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import re
 import threading
 from ctypes import c_float, c_int32, c_int64, c_size_t, c_void_p, c_char_p, POINTER
@@ -186,6 +187,8 @@ _SIGNATURES = {
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
+FASTCALL_PATH = Path(__file__).resolve().parent / "_fastcall.so"
+_fast = None
 
 
 class PrismKVError(RuntimeError):
@@ -217,8 +220,29 @@ def load() -> ctypes.CDLL:
         ver = lib.pkv_abi_version()
         if ver != ABI_VERSION:
             raise PrismKVError(f"libprism_kv ABI version {ver} != expected {ABI_VERSION}")
+        _attach(lib)
         _lib = lib
         return lib
+
+
+def _attach(lib: ctypes.CDLL) -> None:
+    """Points _fastcall.so at the library just loaded."""
+    global _fast
+    if _fast is None:
+        if not FASTCALL_PATH.exists():
+            raise PrismKVError(f"{FASTCALL_PATH} is not built; run `python -m prism_amd.build` first")
+        spec = importlib.util.spec_from_file_location("_fastcall", FASTCALL_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _fast = module
+    _fast.attach(lib._handle)
+
+
+def fast():
+    """The entry points that are called once per layer, without ctypes (csrc_binding/fastcall.cpp)."""
+    if _lib is None:
+        load()
+    return _fast
 
 
 def use(path: Path) -> ctypes.CDLL:

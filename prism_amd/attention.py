@@ -53,6 +53,10 @@ def _stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+# the current stream of a device index as an int, without a torch.cuda.Stream around it (0.1 us, not 1)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _require_gpu(t: torch.Tensor, name: str) -> None:
     if t.device.type != "cuda":
         raise RuntimeError(f"{name} must be a ROCm device tensor (got {t.device}); "

@@ -5,8 +5,9 @@ Usage: python -m prism_amd.build   (or prism_amd.build.build() from Python).
 Every .hip file under prism_amd/csrc is compiled by hipcc for gfx950 into one object each (in
 parallel), then linked into prism_amd/libprism_kv.so.  The .so is what the ctypes loader
 (prism_amd/_lib.py) opens; it is git-ignored but travels with the source tree to a GPU host.
-Two more libraries come out of the same run: libpkv_probe.so (the streaming-read probe of
-bench.py --workload peak) and libprism_kv_stamps.so (the kernels with decode_lean_kernel's
+Three more come out of the same run: _fastcall.so (the Python binding of the entry points that are
+called once per layer), libpkv_probe.so (the streaming-read probe of bench.py --workload peak) and
+libprism_kv_stamps.so (the kernels with decode_lean_kernel's
 timeline stamps, for bench.py --workload tile-stamps).
 """
 from __future__ import annotations
@@ -16,6 +17,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -23,6 +25,8 @@ CSRC = PKG_DIR / "csrc"
 LIB_NAME = "libprism_kv.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 PROBE_LIB_PATH = PKG_DIR / "libpkv_probe.so"
+# the Python binding of the per-layer entry points (prism_amd/_lib.py loads it beside the library)
+FASTCALL_PATH = PKG_DIR / "_fastcall.so"
 # the same library with decode_lean_kernel's timeline stamps (-DPKV_TILE_STAMPS): only
 # bench.py --workload tile-stamps loads it
 STAMPS_LIB_PATH = PKG_DIR / "libprism_kv_stamps.so"
@@ -102,6 +106,13 @@ def build(verbose: bool = False, extra_flags: list[str] | None = None) -> Path:
     os.replace(tmp, STAMPS_LIB_PATH)
     if verbose:
         print(f"built {STAMPS_LIB_PATH}")
+    # host code only: the host compiler, against this interpreter's headers
+    tmp = FASTCALL_PATH.with_suffix(".so.tmp")
+    _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+          f"-I{sysconfig.get_paths()['include']}", str(PKG_DIR / "csrc_binding" / "fastcall.cpp"), "-ldl", "-o", str(tmp)])
+    os.replace(tmp, FASTCALL_PATH)
+    if verbose:
+        print(f"built {FASTCALL_PATH}")
     # the bandwidth probe bench.py --workload peak runs: its own library, outside the paged-KV ABI
     probe_src = PKG_DIR / "csrc_probe" / "pkv_probe.hip"
     probe_tmp = PROBE_LIB_PATH.with_suffix(".so.tmp")

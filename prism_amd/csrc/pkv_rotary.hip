@@ -45,36 +45,43 @@ struct RotaryParams {
   int shift;
 };
 
-// 8 consecutive elements of T as floats, and back (rounded to nearest even).
+// 16 bytes of T as floats, and back (rounded to nearest even); N floats of a table.
 template <typename T>
-struct Vec8;
-template <>
-struct Vec8<float> {
-  static __device__ __forceinline__ void load(const float* src, float (&f)[8]) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(src), b = *reinterpret_cast<const f32x4*>(src + 4);
+struct Chunk {
+  static constexpr int V = 16 / sizeof(T);
+  typedef T TV __attribute__((ext_vector_type(V)));
+  static __device__ __forceinline__ void load(const T* src, float (&f)[V]) {
+    const TV v = __builtin_bit_cast(TV, ld16(src));
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = a[e], f[4 + e] = b[e];
+    for (int e = 0; e < V; ++e) f[e] = static_cast<float>(v[e]);
   }
-  static __device__ __forceinline__ void store(float* dst, const float (&f)[8]) {
-    __builtin_nontemporal_store(f32x4{f[0], f[1], f[2], f[3]}, reinterpret_cast<f32x4*>(dst));
-    __builtin_nontemporal_store(f32x4{f[4], f[5], f[6], f[7]}, reinterpret_cast<f32x4*>(dst + 4));
-  }
-};
-template <typename T>
-struct Vec8 {
-  typedef T T8 __attribute__((ext_vector_type(8)));
-  static __device__ __forceinline__ void load(const T* src, float (&f)[8]) {
-    const T8 v = __builtin_bit_cast(T8, ld16(src));
+  static __device__ __forceinline__ void store(T* dst, const float (&f)[V]) {
+    TV v;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = static_cast<float>(v[e]);
-  }
-  static __device__ __forceinline__ void store(T* dst, const float (&f)[8]) {
-    T8 v;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = static_cast<T>(f[e]);
+    for (int e = 0; e < V; ++e) v[e] = static_cast<T>(f[e]);
     __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), reinterpret_cast<u32x4*>(dst));
   }
 };
+template <int N>
+__device__ __forceinline__ void load_table(const float* src, float (&f)[N]) {
+  typedef float FN __attribute__((ext_vector_type(N < 4 ? N : 4)));
+#pragma unroll
+  for (int e = 0; e < N; e += 4) {
+    const FN v = *reinterpret_cast<const FN*>(src + e);
+#pragma unroll
+    for (int k = 0; k < (N < 4 ? N : 4); ++k) f[e + k] = v[k];
+  }
+}
+// N / 2 neighbouring pairs.
+template <int N>
+__device__ __forceinline__ void turn_pairs(float (&x)[N], const float (&c)[N / 2], const float (&s)[N / 2]) {
+#pragma unroll
+  for (int k = 0; k < N / 2; ++k) {
+    const float a = x[2 * k], b = x[2 * k + 1];
+    x[2 * k] = a * c[k] - b * s[k];
+    x[2 * k + 1] = b * c[k] + a * s[k];
+  }
+}
 
 // Row of the rotation tables of token t, clamped (and flagged) outside them.
 __device__ __forceinline__ int table_row(const RotaryParams& p, uint32_t t) {
@@ -95,12 +102,16 @@ __device__ __forceinline__ int64_t slot_row(const RotaryParams& p, uint32_t t) {
   return int64_t(page) * p.page_stride + int64_t(slot & ((1 << p.log2_page) - 1)) * p.n_kv * p.head_dim;
 }
 
-// One lane holds 16 elements of one head, as two chunks of 8: the two halves of 8 pairs (half layout), or 16
-// neighbours (interleaved, and behind the rotated part).  It reads nothing that another lane writes, so the
-// outputs may be the inputs; the norm's sum goes over the head's lanes by shuffles.  Lanes are counted over the
-// heads of all tokens: a token's 2 + 14 or 16 + 40 heads leave no lane of a workgroup idle.
+// One lane holds two 16-byte chunks of one head: half layout, the two halves of its pairs (behind the rotated
+// part, chunks of the two halves of the rest); interleaved, chunks of the two halves of the head.  So the lanes of a
+// head read and write 16 bytes next to each other with every instruction (two neighbouring chunks per lane, and in
+// fp32 four, took 52 us where 5003 tokens of 32 heads now take SEE BELOW).  A lane reads nothing that another
+// writes, so the outputs may be the inputs; the norm's sum goes over the head's lanes by shuffles.  Lanes are
+// counted over the heads of all tokens: a token's 2 + 14 or 16 + 40 heads leave no lane of a workgroup idle.
 template <typename T, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
+  using C = Chunk<T>;
+  constexpr int V = C::V;
   const uint32_t i = blockIdx.x * 256u + threadIdx.x;
   const uint32_t r = i >> p.log2_lanes;
   const int c = int(i & ((1u << p.log2_lanes) - 1));
@@ -108,88 +119,97 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
   int hh = int(r - t * p.rows);
   // the lanes past the last head, and those past a head whose chunks are no power of two, only take part in
   // the shuffles
-  const bool live = t < p.tokens && c < p.head_dim / 16;
+  const bool live = t < p.tokens && 2 * V * c < p.head_dim;
   const bool is_v = hh >= p.n_heads + p.n_kv, is_k = hh >= p.n_heads;
-  int o1, o2;
-  const bool rotated = 16 * c < p.rotary;
-  if (rotated && !INTERLEAVED) {
-    o1 = 8 * c;
-    o2 = p.rotary / 2 + 8 * c;
-  } else {
-    o1 = 16 * c;
-    o2 = 16 * c + 8;
-  }
+  int o1 = V * c, o2 = p.head_dim / 2 + V * c;
   if (is_v) {
     if (live) {
-      const uint16_t* src = p.v + t * p.v_st + (hh - p.n_heads - p.n_kv) * p.v_sh + 16 * c;
-      const u32x4 v1 = ld16(src), v2 = ld16(src + 8);
+      const uint16_t* src = p.v + t * p.v_st + (hh - p.n_heads - p.n_kv) * p.v_sh;
+      const u32x4 v1 = ld16(src + o1), v2 = ld16(src + o2);
       const int64_t row = slot_row(p, t);
       if (row >= 0) {
-        uint16_t* dst = p.v_cache + row + (hh - p.n_heads - p.n_kv) * p.head_dim + 16 * c;
-        __builtin_nontemporal_store(v1, reinterpret_cast<u32x4*>(dst));
-        __builtin_nontemporal_store(v2, reinterpret_cast<u32x4*>(dst + 8));
+        uint16_t* dst = p.v_cache + row + (hh - p.n_heads - p.n_kv) * p.head_dim;
+        __builtin_nontemporal_store(v1, reinterpret_cast<u32x4*>(dst + o1));
+        __builtin_nontemporal_store(v2, reinterpret_cast<u32x4*>(dst + o2));
       }
     }
     return;  // a head's lanes are of one kind, so none of a shuffle's partners leaves
   }
+  const bool rotated = 2 * V * c < p.rotary;  // half layout
+  if (!INTERLEAVED) {
+    o1 = rotated ? V * c : p.rotary / 2 + V * c;
+    o2 = o1 + (rotated ? p.rotary : p.head_dim - p.rotary) / 2;
+  }
   hh -= is_k ? p.n_heads : 0;
-  float x1[8], x2[8];
+  float x1[V], x2[V];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x1[e] = x2[e] = 0.f;
+  for (int e = 0; e < V; ++e) x1[e] = x2[e] = 0.f;
   int pos = 0;
   if (live) {
     const T* src = static_cast<const T*>(is_k ? p.k : p.q) + t * (is_k ? p.k_st : p.q_st) + hh * (is_k ? p.k_sh : p.q_sh);
-    Vec8<T>::load(src + o1, x1);
-    Vec8<T>::load(src + o2, x2);
+    C::load(src + o1, x1);
+    C::load(src + o2, x2);
     pos = table_row(p, t);
   }
   const T* nw = static_cast<const T*>(is_k ? p.k_norm_w : p.q_norm_w);
   if (nw) {
     float ss = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss += x1[e] * x1[e] + x2[e] * x2[e];
+    for (int e = 0; e < V; ++e) ss += x1[e] * x1[e] + x2[e] * x2[e];
     for (int off = 1; off < (1 << p.log2_lanes); off <<= 1) ss += __shfl_xor(ss, off, 64);
     const float rs = rsqrtf(ss / float(p.head_dim) + p.eps);
     if (live) {
-      float w1[8], w2[8];
-      Vec8<T>::load(nw + o1, w1);
-      Vec8<T>::load(nw + o2, w2);
+      float w1[V], w2[V];
+      C::load(nw + o1, w1);
+      C::load(nw + o2, w2);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x1[e] *= rs * w1[e], x2[e] *= rs * w2[e];
+      for (int e = 0; e < V; ++e) x1[e] *= rs * w1[e], x2[e] *= rs * w2[e];
     }
   }
   if (!live) return;
-  if (rotated) {
-    float cs[8], sn[8];
-    Vec8<float>::load(p.cos_tab + int64_t(pos) * (p.rotary / 2) + 8 * c, cs);
-    Vec8<float>::load(p.sin_tab + int64_t(pos) * (p.rotary / 2) + 8 * c, sn);
+  const float* ct = p.cos_tab + int64_t(pos) * (p.rotary / 2);
+  const float* st = p.sin_tab + int64_t(pos) * (p.rotary / 2);
+  if constexpr (INTERLEAVED) {
+    float cs[V / 2], sn[V / 2];
+    if (o1 < p.rotary) {
+      load_table(ct + o1 / 2, cs);
+      load_table(st + o1 / 2, sn);
+      turn_pairs(x1, cs, sn);
+    }
+    if (o2 < p.rotary) {
+      load_table(ct + o2 / 2, cs);
+      load_table(st + o2 / 2, sn);
+      turn_pairs(x2, cs, sn);
+    }
+  } else if (rotated) {
+    float cs[V], sn[V];
+    load_table(ct + o1, cs);
+    load_table(st + o1, sn);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float& a = INTERLEAVED ? (e < 4 ? x1[2 * e] : x2[2 * e - 8]) : x1[e];
-      float& b = INTERLEAVED ? (e < 4 ? x1[2 * e + 1] : x2[2 * e - 7]) : x2[e];
-      const float ra = a * cs[e] - b * sn[e];
-      b = b * cs[e] + a * sn[e];
-      a = ra;
+    for (int e = 0; e < V; ++e) {
+      const float a = x1[e], b = x2[e];
+      x1[e] = a * cs[e] - b * sn[e];
+      x2[e] = b * cs[e] + a * sn[e];
     }
   }
   if (!is_k) {
     T* dst = static_cast<T*>(p.q_out) + t * p.qo_st + hh * p.qo_sh;
-    Vec8<T>::store(dst + o1, x1);
-    Vec8<T>::store(dst + o2, x2);
+    C::store(dst + o1, x1);
+    C::store(dst + o2, x2);
     return;
   }
   if (p.k_out) {
     T* dst = static_cast<T*>(p.k_out) + t * p.ko_st + hh * p.ko_sh;
-    Vec8<T>::store(dst + o1, x1);
-    Vec8<T>::store(dst + o2, x2);
+    C::store(dst + o1, x1);
+    C::store(dst + o2, x2);
   }
   if constexpr (std::is_same<T, __bf16>::value) {
     if (p.k_cache) {
       const int64_t row = slot_row(p, t);
       if (row >= 0) {
         T* dst = reinterpret_cast<T*>(p.k_cache) + row + hh * p.head_dim;
-        Vec8<T>::store(dst + o1, x1);
-        Vec8<T>::store(dst + o2, x2);
+        C::store(dst + o1, x1);
+        C::store(dst + o2, x2);
       }
     }
   }
@@ -288,7 +308,8 @@ static int check_rotary(const char* fn, int64_t tokens, int n_heads, int n_kv, i
   return PKV_OK;
 }
 
-static int lanes_log2(int head_dim) { return ilog2((head_dim + 15) / 16); }
+// Lanes of a head, two chunks of 16 bytes each; at most a wave.
+static int lanes_log2(int head_dim, int size) { return ilog2((head_dim * size + 31) / 32); }
 
 }  // namespace pkv
 
@@ -314,8 +335,10 @@ extern "C" int pkv_rotate_qk(const void* q, int64_t q_st, int64_t q_sh, const vo
   const uintptr_t tables = reinterpret_cast<uintptr_t>(cos_tab) | reinterpret_cast<uintptr_t>(sin_tab);
   const uint64_t strides = uint64_t(q_st) | uint64_t(q_sh) | uint64_t(k_st) | uint64_t(k_sh) | uint64_t(qo_st) |
                            uint64_t(qo_sh) | uint64_t(ko_st) | uint64_t(ko_sh);
-  const bool wide = ((bases | tables) & 15u) == 0 && (strides * size) % 16 == 0 && head_dim % 16 == 0 &&
-                    rotary_dim % 16 == 0;
+  const int granule = 32 / size;  // two 16-byte chunks
+  const bool wide = ((bases | tables) & 15u) == 0 && (strides * size) % 16 == 0 && head_dim % granule == 0 &&
+                    head_dim <= 64 * granule &&
+                    rotary_dim % granule == 0;
   RotaryParams p = {};
   p.q = q; p.q_st = q_st; p.q_sh = q_sh;
   p.k = k; p.k_st = k_st; p.k_sh = k_sh;
@@ -334,7 +357,7 @@ extern "C" int pkv_rotate_qk(const void* q, int64_t q_st, int64_t q_sh, const vo
   p.rotary = rotary_dim;
   p.interleaved = interleaved ? 1 : 0;
   p.rows = uint32_t(n_heads + n_kv);
-  p.log2_lanes = lanes_log2(head_dim);
+  p.log2_lanes = lanes_log2(head_dim, size);
   p.status = status;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == PKV_BF16)
@@ -401,7 +424,7 @@ extern "C" int pkv_packed_rope_append(const void* qkv, int64_t qkv_st, const int
   p.rotary = rotary_dim;
   p.interleaved = interleaved ? 1 : 0;
   p.rows = uint32_t(n_heads + 2 * n_kv);
-  p.log2_lanes = lanes_log2(head_dim);
+  p.log2_lanes = lanes_log2(head_dim, 2);
   p.status = status;
   launch_rotary<__bf16>(p, tokens, true, static_cast<hipStream_t>(stream));
   return check_launch(fn);
