@@ -1,6 +1,7 @@
 // Host side of packed attention: the step's work list, cut and ordered before the kernels run.
 #include <algorithm>
 #include <exception>
+#include <functional>
 #include <vector>
 
 #include "pkv_common.h"
@@ -9,80 +10,136 @@
 namespace pkv {
 namespace {
 
-// A range pays about two stages' time to start and one to end, and a launch that merges: see kMinStages in
-// pkv_prefill.h, whose walk this is.
-constexpr int kMinRange = 8;
+// Costs in stages (of 16 KB of K and V).  A range's start and end take about five stages' time: loads of the item,
+// then of Q and pages, then of the first tiles, one behind the other.  Below six stages a piece is not worth that: one
+// decode token on 27 stages takes 8.8 us in pieces of 7, 11.0 in pieces of 9, 20.7 whole.
+constexpr int kRangeCost = 5;
+constexpr int kPartialCost = 8;  // of 128 rows: 66 KB each way
+constexpr int kMinRange = 6;
 constexpr int kWorkgroupsPerCu = 2;
 
 struct Block {
   int seq, row0, stage0, stages;
+  int cut_cost;  // of each piece, where it is cut: its partial is written and read back
 };
 
-int range_count(int stages, int64_t chunk) {
-  return int(std::max<int64_t>(std::min<int64_t>((stages + chunk - 1) / chunk, stages / kMinRange), 1));
-}
-
-}  // namespace
-
 // Row blocks of kPackedRows query rows, each with the stages that its rows see: up to its last row's own key, from
-// its first row's window on.  `slots` ranges run at once per KV head.  With fewer blocks than slots the longest
-// are cut until the card is full in one round (a range count just past the slots would cost a second round: the
-// ranges are lengthened until they fit); with more, only blocks above the average slot's share are cut, so that
-// none of them is what the launch ends with.  The longest go first.
-static int plan_blocks(const int32_t* new_lens, const int32_t* ctx_lens, int batch, int g, int tok, int window,
-                       int slots, std::vector<PackedItem>& items, std::vector<PackedMerge>& merges, int32_t* partials,
-                       int32_t* merge_rows) {
+// its first row's window on.
+std::vector<Block> row_blocks(const int32_t* new_lens, const int32_t* ctx_lens, int batch, int g, int tok, int window) {
   std::vector<Block> blocks;
-  int64_t total = 0;
   for (int b = 0; b < batch; ++b) {
     const int rows = new_lens[b] * g, ctx = ctx_lens[b];
     for (int r0 = 0; r0 < rows; r0 += kPackedRows) {
       const int last = ctx + (std::min(r0 + kPackedRows, rows) - 1) / g;
       const int first = window > 0 ? std::max(ctx + r0 / g - window + 1, 0) : 0;
-      const int stage0 = first / tok;
-      blocks.push_back({b, r0, stage0, last / tok + 1 - stage0});
-      total += blocks.back().stages;
+      const int cost = (kPartialCost * std::min(kPackedRows, rows - r0) + kPackedRows - 1) / kPackedRows;
+      blocks.push_back({b, r0, first / tok, last / tok + 1 - first / tok, cost});
     }
   }
-  int64_t chunk = std::max<int64_t>((total + slots - 1) / slots, kMinRange);
-  if (int64_t(blocks.size()) <= slots) {
-    for (;;) {
+  return blocks;
+}
+
+struct Piece {
+  int block, stage0, stages;
+};
+
+// The launch as the card will run it: `slots` ranges at once per KV head, the next of the list where one ends.
+struct Schedule {
+  std::vector<int64_t> load;  // a heap: when each slot is free, the earliest in front
+  std::vector<Piece> list;
+  int64_t end = 0;  // of the last range
+  explicit Schedule(int slots) : load(slots, 0) {}
+  void add(const Block& b, int block, int stage0, int stages) {
+    std::pop_heap(load.begin(), load.end(), std::greater<int64_t>());
+    load.back() += stages + kRangeCost + (stages < b.stages ? b.cut_cost : 0);
+    end = std::max(end, load.back());
+    std::push_heap(load.begin(), load.end(), std::greater<int64_t>());
+    list.push_back({block, stage0, stages});
+  }
+};
+
+// The blocks longest first, in equal pieces of about `chunk` stages.
+Schedule in_chunks(const std::vector<Block>& blocks, int slots, int64_t chunk) {
+  Schedule s(slots);
+  for (int i = 0; i < int(blocks.size()); ++i) {
+    const int n = blocks[i].stages;
+    const int count = int(std::max<int64_t>(std::min<int64_t>((n + chunk - 1) / chunk, n / kMinRange), 1));
+    const int len = (n + count - 1) / count;
+    for (int at = 0; at < n; at += len) s.add(blocks[i], i, at, std::min(len, n - at));
+  }
+  return s;
+}
+
+// The blocks longest first, each whole where it ends by `target`, else in pieces that do.
+Schedule filled(const std::vector<Block>& blocks, int slots, int64_t target) {
+  Schedule s(slots);
+  for (int i = 0; i < int(blocks.size()); ++i) {
+    for (int at = 0, take; at < blocks[i].stages; at += take) {
+      const int left = blocks[i].stages - at;
+      const int64_t room = target - s.load[0] - kRangeCost;
+      take = left;
+      if (left > room + kMinRange / 2 && left >= 2 * kMinRange)
+        take = int(std::min<int64_t>(std::max<int64_t>(room, kMinRange), left - kMinRange));
+      s.add(blocks[i], i, at, take);
+    }
+  }
+  return s;
+}
+
+// Whole blocks can need a round more than their work does (129 blocks of 34 stages on 64 slots, a window's, take
+// three rounds for one block too many), and few blocks leave the card idle.  Two ways to cut them: pieces of one
+// length that fit one round, and, where that schedule would end a tenth earlier, pieces that fill every slot up to an
+// even share of the work.  (Less than that is lost again: pieces that wait for a slot start into a card that reads
+// as fast as it can.)  us a launch, one length / filled: 47 decode tokens and two chunks (7B) 46 / 60, 6 and 2 on
+// 40 k keys 106 / 132; 208 short chats (0.5B) 27 / 22, chunks in a window of 1024 (14B; whole blocks) 113 / 100.
+// Many rounds even out by themselves: above kRounds of them nothing is cut.
+constexpr int kRounds = 8;
+std::vector<Piece> cut(std::vector<Block>& blocks, int slots) {
+  std::stable_sort(blocks.begin(), blocks.end(), [](const Block& a, const Block& b) { return a.stages > b.stages; });
+  const int64_t n = int64_t(blocks.size());
+  if (n > int64_t(kRounds) * slots) return in_chunks(blocks, 1, INT64_MAX / 2).list;
+  int64_t total = 0;
+  for (const Block& b : blocks) total += b.stages;
+  const int64_t share = (total + kRangeCost * n + slots - 1) / slots;
+  Schedule best = filled(blocks, slots, share + kRangeCost);
+  if (n <= slots) {
+    int64_t chunk = std::max<int64_t>((total + slots - 1) / slots, kMinRange);
+    for (;; chunk += std::max<int64_t>(chunk / 16, 1)) {
       int64_t ranges = 0;
-      for (const Block& k : blocks) ranges += range_count(k.stages, chunk);
+      for (const Block& b : blocks)
+        ranges += std::max<int64_t>(std::min<int64_t>((b.stages + chunk - 1) / chunk, b.stages / kMinRange), 1);
       if (ranges <= slots) break;
-      chunk += std::max<int64_t>(chunk / 16, 1);
     }
+    Schedule even = in_chunks(blocks, slots, chunk);
+    if (9 * even.end <= 10 * best.end) best = std::move(even);
   }
+  return std::move(best.list);
+}
+
+}  // namespace
+
+static void plan(const int32_t* new_lens, const int32_t* ctx_lens, int batch, int g, int tok, int window, int slots,
+                 std::vector<PackedItem>& items, std::vector<PackedMerge>& merges, int32_t* partials,
+                 int32_t* merge_rows) {
+  std::vector<Block> blocks = row_blocks(new_lens, ctx_lens, batch, g, tok, window);
+  const std::vector<Piece> list = cut(blocks, slots);
   std::vector<int32_t> tok0(batch);
-  int32_t t = 0;
-  for (int b = 0; b < batch; ++b) {
-    tok0[b] = t;
-    t += new_lens[b];
-  }
-  *partials = 0;
-  *merge_rows = 0;
-  for (const Block& k : blocks) {
-    const int count = range_count(k.stages, chunk);
-    const int len = (k.stages + count - 1) / count;
-    PackedItem it = {tok0[k.seq], new_lens[k.seq], ctx_lens[k.seq], k.seq, k.row0, k.stage0, k.stages, -1};
-    if (count == 1) {
-      items.push_back(it);
-      continue;
+  for (int b = 1; b < batch; ++b) tok0[b] = tok0[b - 1] + new_lens[b - 1];
+  *partials = *merge_rows = 0;
+  for (size_t i = 0; i < list.size(); ++i) {  // the pieces of a block are next to each other
+    const Piece& k = list[i];
+    const Block& b = blocks[k.block];
+    const int n_new = new_lens[b.seq];
+    const bool whole = k.stages == b.stages;
+    items.push_back({tok0[b.seq], n_new, ctx_lens[b.seq], b.seq, b.row0, b.stage0 + k.stage0, k.stages,
+                     whole ? -1 : (*partials)++});
+    if (whole) continue;
+    if (k.stage0 == 0) {
+      merges.push_back({tok0[b.seq], n_new, b.row0, *partials - 1, 0, {0, 0, 0}});
+      *merge_rows = std::max(*merge_rows, std::min(kPackedRows, n_new * g - b.row0));
     }
-    int used = 0;
-    for (int s = 0; s < k.stages; s += len) {
-      it.stage0 = k.stage0 + s;
-      it.stages = std::min(len, k.stages - s);
-      it.slot = *partials + used++;
-      items.push_back(it);
-    }
-    merges.push_back({it.tok0, it.n_new, it.row0, *partials, used, {0, 0, 0}});
-    *partials += used;
-    *merge_rows = std::max(*merge_rows, std::min(kPackedRows, it.n_new * g - it.row0));
+    ++merges.back().count;
   }
-  std::stable_sort(items.begin(), items.end(),
-                   [](const PackedItem& a, const PackedItem& b) { return a.stages > b.stages; });
-  return PKV_OK;
 }
 
 }  // namespace pkv
@@ -111,7 +168,7 @@ extern "C" int pkv_packed_plan(const int32_t* new_lens, const int32_t* ctx_lens,
     std::vector<PackedItem> it;
     std::vector<PackedMerge> mg;
     const int slots = std::max(compute_units * kWorkgroupsPerCu / n_kv, 1);
-    plan_blocks(new_lens, ctx_lens, batch, g, head_dim == 128 ? 32 : 64, window, slots, it, mg, &counts[2], &counts[3]);
+    plan(new_lens, ctx_lens, batch, g, head_dim == 128 ? 32 : 64, window, slots, it, mg, &counts[2], &counts[3]);
     counts[0] = int32_t(it.size());
     counts[1] = int32_t(mg.size());
     if (!items) return PKV_OK;
