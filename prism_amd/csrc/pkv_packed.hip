@@ -20,7 +20,9 @@ constexpr int kWorkgroupsPerCu = 2;
 
 struct Block {
   int seq, row0, stage0, stages;
-  int cut_cost;  // of each piece, where it is cut: its partial is written and read back
+  int rows;
+  // of each piece, where it is cut: its partial is written and read back
+  int cut_cost() const { return (kPartialCost * rows + kPackedRows - 1) / kPackedRows; }
 };
 
 // Row blocks of kPackedRows query rows, each with the stages that its rows see: up to its last row's own key, from
@@ -32,8 +34,7 @@ std::vector<Block> row_blocks(const int32_t* new_lens, const int32_t* ctx_lens, 
     for (int r0 = 0; r0 < rows; r0 += kPackedRows) {
       const int last = ctx + (std::min(r0 + kPackedRows, rows) - 1) / g;
       const int first = window > 0 ? std::max(ctx + r0 / g - window + 1, 0) : 0;
-      const int cost = (kPartialCost * std::min(kPackedRows, rows - r0) + kPackedRows - 1) / kPackedRows;
-      blocks.push_back({b, r0, first / tok, last / tok + 1 - first / tok, cost});
+      blocks.push_back({b, r0, first / tok, last / tok + 1 - first / tok, std::min(kPackedRows, rows - r0)});
     }
   }
   return blocks;
@@ -51,19 +52,23 @@ struct Schedule {
   explicit Schedule(int slots) : load(slots, 0) {}
   void add(const Block& b, int block, int stage0, int stages) {
     std::pop_heap(load.begin(), load.end(), std::greater<int64_t>());
-    load.back() += stages + kRangeCost + (stages < b.stages ? b.cut_cost : 0);
+    load.back() += stages + kRangeCost + (stages < b.stages ? b.cut_cost() : 0);
     end = std::max(end, load.back());
     std::push_heap(load.begin(), load.end(), std::greater<int64_t>());
     list.push_back({block, stage0, stages});
   }
 };
 
+int pieces(int stages, int64_t chunk) {
+  return int(std::max<int64_t>(std::min<int64_t>((stages + chunk - 1) / chunk, stages / kMinRange), 1));
+}
+
 // The blocks longest first, in equal pieces of about `chunk` stages.
 Schedule in_chunks(const std::vector<Block>& blocks, int slots, int64_t chunk) {
   Schedule s(slots);
   for (int i = 0; i < int(blocks.size()); ++i) {
     const int n = blocks[i].stages;
-    const int count = int(std::max<int64_t>(std::min<int64_t>((n + chunk - 1) / chunk, n / kMinRange), 1));
+    const int count = pieces(n, chunk);
     const int len = (n + count - 1) / count;
     for (int at = 0; at < n; at += len) s.add(blocks[i], i, at, std::min(len, n - at));
   }
@@ -86,15 +91,50 @@ Schedule filled(const std::vector<Block>& blocks, int slots, int64_t target) {
   return s;
 }
 
+// Pieces of one length, for one workgroup per CU or for two, whichever ends sooner.  One per CU already reads as fast
+// as the card does (5.8 TB/s: all CUs together 370 stages a us, 0.6 us each); two even out what the blocks' lengths
+// leave uneven, at the price of more partials, 0.4 us per MB written and read, and 3.5 us for the launch that merges them.  Between the
+// two some CUs would have one and some two.  6 decode tokens and two chunks on 40 k keys: 102 + 5 us in 59 pieces per
+// KV head, 110 + 10 in 124; 47 decode tokens on 1500: 35 + 5 in 126 pieces, 41 + 5 in 77.
+Schedule even(const std::vector<Block>& blocks, int slots, int n_kv, int head_dim) {
+  int64_t total = 0;
+  for (const Block& b : blocks) total += b.stages;
+  int64_t best_chunk = 0;
+  double best = 0;
+  for (const int64_t room : {int64_t(std::max(slots / 2, 1)), int64_t(slots)}) {
+    if (int64_t(blocks.size()) > room) continue;
+    for (int64_t chunk = std::max<int64_t>((total + room - 1) / room, kMinRange);;
+         chunk += std::max<int64_t>(chunk / 16, 1)) {
+      int64_t ranges = 0, longest = 0, rows = 0;
+      for (const Block& b : blocks) {
+        const int count = pieces(b.stages, chunk);
+        ranges += count;
+        longest = std::max<int64_t>(longest, (b.stages + count - 1) / count);
+        if (count > 1) rows += int64_t(count) * b.rows;
+      }
+      if (ranges > room) continue;
+      const double at_once = std::min(370.0, 2.0 * ranges * n_kv);
+      const double us = std::max(total * n_kv / at_once, 0.58 * longest) +
+                        (rows ? 3.5 + 0.4e-6 * rows * n_kv * (head_dim + 4) * 4 : 0.0);
+      if (best_chunk == 0 || us < best) {
+        best = us;
+        best_chunk = chunk;
+      }
+      break;
+    }
+  }
+  return in_chunks(blocks, slots, best_chunk);
+}
+
 // Whole blocks can need a round more than their work does (129 blocks of 34 stages on 64 slots, a window's, take
 // three rounds for one block too many), and few blocks leave the card idle.  Two ways to cut them: pieces of one
 // length that fit one round, and, where that schedule would end a tenth earlier, pieces that fill every slot up to an
 // even share of the work.  (Less than that is lost again: pieces that wait for a slot start into a card that reads
-// as fast as it can.)  us a launch, one length / filled: 47 decode tokens and two chunks (7B) 46 / 60, 6 and 2 on
-// 40 k keys 106 / 132; 208 short chats (0.5B) 27 / 22, chunks in a window of 1024 (14B; whole blocks) 113 / 100.
+// as fast as it can.)  us a launch, one length / filled: 47 decode tokens and two chunks (7B) 46 / 60; 208 short
+// chats (0.5B) 27 / 22, chunks in a window of 1024 (14B; whole blocks) 113 / 100.
 // Many rounds even out by themselves: above kRounds of them nothing is cut.
 constexpr int kRounds = 8;
-std::vector<Piece> cut(std::vector<Block>& blocks, int slots) {
+std::vector<Piece> cut(std::vector<Block>& blocks, int slots, int n_kv, int head_dim) {
   std::stable_sort(blocks.begin(), blocks.end(), [](const Block& a, const Block& b) { return a.stages > b.stages; });
   const int64_t n = int64_t(blocks.size());
   if (n > int64_t(kRounds) * slots) return in_chunks(blocks, 1, INT64_MAX / 2).list;
@@ -103,26 +143,19 @@ std::vector<Piece> cut(std::vector<Block>& blocks, int slots) {
   const int64_t share = (total + kRangeCost * n + slots - 1) / slots;
   Schedule best = filled(blocks, slots, share + kRangeCost);
   if (n <= slots) {
-    int64_t chunk = std::max<int64_t>((total + slots - 1) / slots, kMinRange);
-    for (;; chunk += std::max<int64_t>(chunk / 16, 1)) {
-      int64_t ranges = 0;
-      for (const Block& b : blocks)
-        ranges += std::max<int64_t>(std::min<int64_t>((b.stages + chunk - 1) / chunk, b.stages / kMinRange), 1);
-      if (ranges <= slots) break;
-    }
-    Schedule even = in_chunks(blocks, slots, chunk);
-    if (9 * even.end <= 10 * best.end) best = std::move(even);
+    Schedule one = even(blocks, slots, n_kv, head_dim);
+    if (n <= slots / 2 || 9 * one.end <= 10 * best.end) best = std::move(one);
   }
   return std::move(best.list);
 }
 
 }  // namespace
 
-static void plan(const int32_t* new_lens, const int32_t* ctx_lens, int batch, int g, int tok, int window, int slots,
-                 std::vector<PackedItem>& items, std::vector<PackedMerge>& merges, int32_t* partials,
+static void plan(const int32_t* new_lens, const int32_t* ctx_lens, int batch, int g, int n_kv, int head_dim, int window,
+                 int slots, std::vector<PackedItem>& items, std::vector<PackedMerge>& merges, int32_t* partials,
                  int32_t* merge_rows) {
-  std::vector<Block> blocks = row_blocks(new_lens, ctx_lens, batch, g, tok, window);
-  const std::vector<Piece> list = cut(blocks, slots);
+  std::vector<Block> blocks = row_blocks(new_lens, ctx_lens, batch, g, head_dim == 128 ? 32 : 64, window);
+  const std::vector<Piece> list = cut(blocks, slots, n_kv, head_dim);
   std::vector<int32_t> tok0(batch);
   for (int b = 1; b < batch; ++b) tok0[b] = tok0[b - 1] + new_lens[b - 1];
   *partials = *merge_rows = 0;
@@ -168,7 +201,7 @@ extern "C" int pkv_packed_plan(const int32_t* new_lens, const int32_t* ctx_lens,
     std::vector<PackedItem> it;
     std::vector<PackedMerge> mg;
     const int slots = std::max(compute_units * kWorkgroupsPerCu / n_kv, 1);
-    plan(new_lens, ctx_lens, batch, g, head_dim == 128 ? 32 : 64, window, slots, it, mg, &counts[2], &counts[3]);
+    plan(new_lens, ctx_lens, batch, g, n_kv, head_dim, window, slots, it, mg, &counts[2], &counts[3]);
     counts[0] = int32_t(it.size());
     counts[1] = int32_t(mg.size());
     if (!items) return PKV_OK;

@@ -419,26 +419,41 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
   bool bad_page = false;
   // first key that a row of the block sees
   const int first_key = PACKED && p.window > 0 ? max(c + blk_row0 / p.g - p.window + 1, 0) : 0;
-  // offset of token row T (uniform) of head h
-  auto row_of = [&](int T) {
-    const int col = T >> p.log2_page;
-    if (col - btw.col0 >= 64) {
+  // SMALL: lane l holds the offset of page col0 + l, -1 for a page that lies wholly before every row's window or
+  // behind the last key (it may not exist: its rows read as zeros).  One multiplication per lane and 64 pages, two
+  // readlanes per copy; worked out stage by stage, a window's chunks (14B, pages of 16) took 106 us where pages of
+  // 256 take 91.
+  int64_t page_offs = -1;
+  auto load_offs = [&] {
+    const int key = (btw.col0 + lane) << p.log2_page;
+    const bool needed = key < L && key + pmask >= first_key;
+    const bool ok = unsigned(btw.ids) < unsigned(p.num_pages);
+    page_offs = needed ? int64_t(ok ? btw.ids : 0) * p.page_stride : -1;
+    bad_page |= __any(needed && !ok);
+  };
+  if constexpr (SMALL) load_offs();
+  auto page_start = [&] {
+    const int col = T_k >> p.log2_page;
+    if (col - btw.col0 > (SMALL ? 64 - TOK / 16 : 63)) {
       bt_window_load(p, sv, col, btw);
       __builtin_amdgcn_s_waitcnt(0x0F70);  // here, once per 64 pages: not at every use of the window
+      if constexpr (SMALL) load_offs();
     }
-    const int pid = __builtin_amdgcn_readlane(btw.ids, col - btw.col0);
-    const bool ok = unsigned(pid) < unsigned(p.num_pages);
     if constexpr (SMALL) {
-      // rows of a stage that lie before every row's window, or behind the last key, may have no page: they read as
-      // zeros
-      if (T + G::RPC <= first_key || T >= L) return int64_t(-1);
-    }
-    bad_page |= !ok && T < L;
-    return int64_t(ok ? pid : 0) * p.page_stride + int64_t(T & pmask) * (p.n_kv * HD) + h * HD;
-  };
-  auto page_start = [&] {
 #pragma unroll
-    for (int k = 0; k < kOff; ++k) off_k.at[k] = row_of(T_k + (SMALL ? (wave + W * k) * G::RPC : 0));
+      for (int k = 0; k < kOff; ++k) {
+        const int row = (wave + W * k) * G::RPC;
+        const int at = col - btw.col0 + (row >> p.log2_page);
+        const uint32_t lo = __builtin_amdgcn_readlane(uint32_t(page_offs), at);
+        const int32_t hi32 = __builtin_amdgcn_readlane(int32_t(page_offs >> 32), at);
+        off_k.at[k] = hi32 < 0 ? -1 : int64_t((uint64_t(uint32_t(hi32)) << 32) | lo) + (row & pmask) * (p.n_kv * HD) + h * HD;
+      }
+    } else {
+      const int pid = __builtin_amdgcn_readlane(btw.ids, col - btw.col0);
+      const bool ok = unsigned(pid) < unsigned(p.num_pages);
+      bad_page |= !ok && T_k < L;
+      off_k.at[0] = int64_t(ok ? pid : 0) * p.page_stride + int64_t(T_k & pmask) * (p.n_kv * HD) + h * HD;
+    }
   };
   char* const ring_k = lds;
   char* const ring_v = lds + kRing * G::STAGE;
