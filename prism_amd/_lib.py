@@ -226,20 +226,22 @@ def load() -> ctypes.CDLL:
 
 
 def _attach(lib: ctypes.CDLL) -> None:
-    """Points _fastcall.so at the library just loaded."""
+    """Points _fastcall.so (which needs torch loaded) at the library just loaded."""
     global _fast
     if _fast is None:
         if not FASTCALL_PATH.exists():
             raise PrismKVError(f"{FASTCALL_PATH} is not built; run `python -m prism_amd.build` first")
+        import torch  # noqa: F401  its libraries are what the module's symbols are found in
+
         spec = importlib.util.spec_from_file_location("_fastcall", FASTCALL_PATH)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
         _fast = module
-    _fast.attach(lib._handle)
+    _fast.attach(lib._handle, PrismKVError)
 
 
 def fast():
-    """The entry points that are called once per layer, without ctypes (csrc_binding/fastcall.cpp)."""
+    """The calls that are made once per layer, without Python's checks and ctypes (csrc_binding/fastcall.cpp)."""
     if _lib is None:
         load()
     return _fast

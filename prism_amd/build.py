@@ -106,10 +106,15 @@ def build(verbose: bool = False, extra_flags: list[str] | None = None) -> Path:
     os.replace(tmp, STAMPS_LIB_PATH)
     if verbose:
         print(f"built {STAMPS_LIB_PATH}")
-    # host code only: the host compiler, against this interpreter's headers
+    # host code only: the host compiler, against this interpreter's and torch's headers
+    from torch.utils import cpp_extension
+
     tmp = FASTCALL_PATH.with_suffix(".so.tmp")
-    _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
-          f"-I{sysconfig.get_paths()['include']}", str(PKG_DIR / "csrc_binding" / "fastcall.cpp"), "-ldl", "-o", str(tmp)])
+    torch_lib = cpp_extension.TORCH_LIB_PATH
+    _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden",
+          f"-I{sysconfig.get_paths()['include']}", *(f"-isystem{d}" for d in cpp_extension.include_paths()),
+          str(PKG_DIR / "csrc_binding" / "fastcall.cpp"), "-o", str(tmp),
+          f"-L{torch_lib}", f"-Wl,-rpath,{torch_lib}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-ldl"])
     os.replace(tmp, FASTCALL_PATH)
     if verbose:
         print(f"built {FASTCALL_PATH}")

@@ -203,30 +203,6 @@ def rotary_tables(rotary_dim: int, n_pos: int, theta: float = 10000.0, *, scalin
     return cos, sin
 
 
-_ROTARY_DTYPES = {torch.bfloat16: _lib.PKV_BF16, torch.float16: _lib.PKV_FP16, torch.float32: _lib.PKV_FP32}
-
-
-def _check_rotary_tables(cos: torch.Tensor, sin: torch.Tensor, head_dim: int, device) -> int:
-    """The tables' rotary_dim."""
-    shape = cos.shape
-    for name, t in (("cos", cos), ("sin", sin)):
-        if t.dtype is not torch.float32 or len(shape) != 2 or not t.is_contiguous() or t.device != device:
-            raise RuntimeError(f"{name} must be a contiguous float32 [n_pos, rotary_dim / 2] table on {device} "
-                               "(rotary_tables)")
-    if shape != sin.shape or shape[0] == 0 or shape[1] == 0:
-        raise RuntimeError(f"cos {tuple(shape)} and sin {tuple(sin.shape)} must have one shape, not empty")
-    if 2 * shape[1] > head_dim:
-        raise RuntimeError(f"tables for a rotary_dim of {2 * shape[1]} do not fit head_dim {head_dim}")
-    return 2 * shape[1]
-
-
-def _check_norms(q_norm_w, k_norm_w, head_dim: int, dtype, device) -> None:
-    for name, t in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
-        if t is not None and (t.dtype != dtype or tuple(t.shape) != (head_dim,) or not t.is_contiguous() or
-                              t.device != device):
-            raise RuntimeError(f"{name} must be a contiguous {dtype} [{head_dim}] vector on {device}")
-
-
 def rotate_qk(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, cos: torch.Tensor,
               sin: torch.Tensor, *, interleaved: bool = False, q_norm_w: torch.Tensor | None = None,
               k_norm_w: torch.Tensor | None = None, eps: float = 1e-6, q_out: torch.Tensor | None = None,
@@ -239,62 +215,11 @@ def rotate_qk(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, 
 
     fp32 arithmetic, one rounding.  The outputs may be the inputs (in place); k = None returns (q, None).  With
     ``-sin`` the rotation turns back, which is also its gradient."""
+    dev = q.device
     _require_gpu(q, "q")
-    dtype, device, shape = q.dtype, q.device, q.shape
-    code = _ROTARY_DTYPES.get(dtype)
-    if code is None:
-        raise RuntimeError(f"q must be bfloat16, float16 or float32, got {dtype}")
-    if len(shape) < 3:
-        raise RuntimeError(f"q must be [..., n_heads, head_dim] with a token axis, got {tuple(shape)}")
-    hd, nh, nk, tokens = shape[-1], shape[-2], 0, math.prod(shape[:-2])
-    rotary = _check_rotary_tables(cos, sin, hd, device)
-    if q_norm_w is not None or k_norm_w is not None:
-        _check_norms(q_norm_w, k_norm_w, hd, dtype, device)
-    if positions.dtype is not torch.int32 or positions.device != device or positions.numel() != tokens or \
-            not positions.is_contiguous():
-        raise RuntimeError(f"positions must be contiguous int32, one for each of the {tokens} tokens, on {device}")
-    if q_out is None:
-        q_out = torch.empty(shape, dtype=dtype, device=device)
-    elif q_out.dtype != dtype or q_out.device != device or q_out.shape != shape:
-        raise RuntimeError(f"q_out must be {dtype} {tuple(shape)} on {device}")
-    qi, qo = _token_rows(q, "q", tokens), _token_rows(q_out, "q_out", tokens)
-    ki = ko = (0, 0)
-    if k is not None:
-        kshape = k.shape
-        if k.dtype != dtype or k.device != device or kshape[:-2] != shape[:-2] or kshape[-1] != hd:
-            raise RuntimeError(f"k {k.dtype} {tuple(kshape)} must match q {dtype} {tuple(shape)} but for the heads")
-        nk = kshape[-2]
-        if k_out is None:
-            k_out = torch.empty(kshape, dtype=dtype, device=device)
-        elif k_out.dtype != dtype or k_out.device != device or k_out.shape != kshape:
-            raise RuntimeError(f"k_out must be {dtype} {tuple(kshape)} on {device}")
-        ki, ko = _token_rows(k, "k", tokens), _token_rows(k_out, "k_out", tokens)
-    elif k_norm_w is not None or k_out is not None:
-        raise RuntimeError("k_norm_w and k_out need a k")
-    st = status if status is not None else status_tensor(device)
-    with _on(device):
-        rc = _lib.fast().pkv_rotate_qk(
-            q.data_ptr(), qi[0], qi[1], k.data_ptr() if nk else 0, ki[0], ki[1], positions.data_ptr(), cos.data_ptr(),
-            sin.data_ptr(), cos.shape[0], q_norm_w.data_ptr() if q_norm_w is not None else 0,
-            k_norm_w.data_ptr() if k_norm_w is not None else 0, float(eps), q_out.data_ptr(), qo[0], qo[1],
-            k_out.data_ptr() if nk else 0, ko[0], ko[1], tokens, nh, nk, hd, rotary, int(interleaved), code,
-            st.data_ptr(), _raw_stream(device.index))
-    if rc:
-        _lib.check(rc, "pkv_rotate_qk")
-    return q_out, k_out
-
-
-def _token_rows(t: torch.Tensor, name: str, tokens: int) -> tuple[int, int]:
-    """Token and head strides of [..., heads, head_dim] as [tokens, heads, head_dim]."""
-    strides = t.stride()
-    if len(strides) != 3:
-        try:
-            strides = t.view(tokens, *t.shape[-2:]).stride()
-        except RuntimeError:
-            raise RuntimeError(f"{name} must flatten to a token axis without a copy") from None
-    if strides[2] != 1 and t.shape[-1] > 1:
-        raise RuntimeError(f"{name} must be contiguous in head_dim")
-    return strides[0], strides[1]
+    with _on(dev):
+        return _lib.fast().rotate_qk(q, k, positions, cos, sin, interleaved, q_norm_w, k_norm_w, eps, q_out, k_out,
+                                     status if status is not None else status_tensor(dev), _raw_stream(dev.index))
 
 
 def _rows2d(t: torch.Tensor, name: str) -> torch.Tensor:

@@ -18,23 +18,23 @@ replays then work on that very batch: its lengths are in the work list).
 from __future__ import annotations
 
 import contextlib
-import math
 from typing import Sequence
 
 import numpy as np
 import torch
 
 from . import _lib
-from .attention import _BF16, _check_cache, _raw_stream, _require_gpu, status_tensor
+from .attention import _raw_stream, _require_gpu, status_tensor
 
 _MAX_KEYS = 1 << 27
 
 
+_here = contextlib.nullcontext()
+
+
 def _on(device: torch.device):
     """Makes `device` current where it is not: kernels are launched on the current device."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    return _here if device.type != "cuda" or device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _host_ints(x, name: str, ndim: int) -> np.ndarray:
@@ -95,8 +95,6 @@ class PackedBatch:
         self.batch, self.total_tokens = len(new), total
         self.page_size, self.num_pages = page_size, num_pages
         self.n_heads, self.n_kv, self.head_dim, self.device = n_heads, n_kv, head_dim, device
-        self._page_shape = (page_size, n_kv, head_dim)
-        self._page_strides = (n_kv * head_dim, head_dim, 1)
         self.max_blocks = max(bt.shape[1], 1)
         widest = _MAX_KEYS if any(w is None for w in windows) else max(windows)
         self._check_pages(new, ctx, bt, widest)
@@ -112,14 +110,19 @@ class PackedBatch:
         host = staged.numpy()
         for p, at in zip(parts, starts):
             host[at:at + p.size] = p
-        with _on(device) if device.type == "cuda" else contextlib.nullcontext():
+        with _on(device):
             self._buf = staged.to(device, non_blocking=True)
         view = [self._buf[at:at + p.size] for p, at in zip(parts, starts)]
         self.positions, self.slots = view[0], view[1]
         self.block_table = view[2].view(self.batch, bt.shape[1])
-        self._plans = {}
-        for i, (w, (items, merges, counts)) in enumerate(plans.items()):
-            self._plans[w] = (view[3 + 2 * i], len(items), view[4 + 2 * i], len(merges), int(counts[2]), int(counts[3]))
+        # per window: the kernels' arguments (window, items, their number, merges, their number, partials, merge rows)
+        base = self._buf.data_ptr()
+        self._plans = {w: (int(w or 0), base + 4 * int(starts[3 + 2 * i]), len(items), base + 4 * int(starts[4 + 2 * i]),
+                           len(merges), int(counts[2]), int(counts[3]))
+                       for i, (w, (items, merges, counts)) in enumerate(plans.items())}
+        self._native = _lib.fast().new_batch(self._buf, total, self.batch, n_heads, n_kv, head_dim, page_size, num_pages,
+                                             self.max_blocks, self.positions.data_ptr(), self.slots.data_ptr(),
+                                             base + 4 * int(starts[2]))
 
     def _check_pages(self, new, ctx, bt, widest) -> None:
         P, busy = self.page_size, new > 0
@@ -155,33 +158,6 @@ class PackedBatch:
         _lib.check(rc, "pkv_packed_plan")
         return items[:counts[0]], merges[:counts[1]], counts
 
-    def _check_cache(self, k_cache, v_cache) -> int:
-        """The caches' page stride."""
-        shape, strides = k_cache.shape, k_cache.stride()
-        if k_cache.dtype is _BF16 and v_cache.dtype is _BF16 and shape == v_cache.shape and strides == v_cache.stride() \
-                and len(shape) == 4 and shape[0] >= self.num_pages and shape[1:] == self._page_shape and \
-                strides[1:] == self._page_strides and k_cache.device == self.device and v_cache.device == self.device:
-            return strides[0]
-        num_pages, page_size, n_kv, hd = _check_cache(k_cache, v_cache)   # says what is wrong, where it is the cache's own
-        if (page_size, n_kv, hd) != self._page_shape or num_pages < self.num_pages:
-            raise RuntimeError(f"cache of {num_pages} pages x {page_size} x {n_kv} heads x {hd} does not fit a batch laid "
-                               f"out for {self.num_pages} x {self.page_size} x {self.n_kv} x {self.head_dim}")
-        raise RuntimeError(f"the cache must be on the batch's device {self.device}")
-
-
-def _rows3(t: torch.Tensor, name: str, batch: PackedBatch) -> tuple[int, int]:
-    shape, strides = t.shape, t.stride()
-    if t.dtype is not _BF16:
-        raise RuntimeError(f"{name} must be {_BF16}, got {t.dtype}")
-    if len(shape) != 3 or shape[0] < batch.total_tokens or shape[1] != batch.n_heads or shape[2] != batch.head_dim:
-        raise RuntimeError(f"{name} has shape {tuple(shape)}, expected [>= {batch.total_tokens}, {batch.n_heads}, "
-                           f"{batch.head_dim}]")
-    if strides[2] != 1:
-        raise RuntimeError(f"{name} must be contiguous in head_dim")
-    if t.device != batch.device:
-        raise RuntimeError(f"{name} must be on the batch's device {batch.device}")
-    return strides[0], strides[1]
-
 
 def packed_rope_append(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, batch: PackedBatch,
                        cos: torch.Tensor, sin: torch.Tensor, *, interleaved: bool = False,
@@ -195,44 +171,12 @@ def packed_rope_append(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     ``cos`` / ``sin`` are fp32 [n_pos, rotary_dim / 2] (rotary_tables); rotary_dim, a multiple of 16, may be less
     than the head.  A token turns by its place in its sequence, or by ``positions`` (int32 [tokens]) where they
     differ.  Rows of ``qkv`` and ``q_out`` behind the batch's tokens are not touched (zero in a result made here)."""
-    from .epilogue import _check_norms, _check_rotary_tables
+    dev = batch.device
     _require_gpu(qkv, "qkv")
-    page_stride = batch._check_cache(k_cache, v_cache)
-    nh, nk, hd, total, dev = batch.n_heads, batch.n_kv, batch.head_dim, batch.total_tokens, batch.device
-    shape, strides = qkv.shape, qkv.stride()
-    if qkv.dtype is not _BF16 or len(shape) != 2 or shape[0] < total or shape[1] != (nh + 2 * nk) * hd or strides[1] != 1:
-        raise RuntimeError(f"qkv must be bfloat16 [>= {total}, {(nh + 2 * nk) * hd}], contiguous in its last dimension, "
-                           f"got {qkv.dtype} {tuple(shape)}")
-    if qkv.device != dev:
-        raise RuntimeError(f"qkv must be on the batch's device {dev}")
-    rotary = _check_rotary_tables(cos, sin, hd, dev)
-    if q_norm_w is not None or k_norm_w is not None:
-        _check_norms(q_norm_w, k_norm_w, hd, _BF16, dev)
-    if positions is None:
-        positions = batch.positions
-    elif positions.dtype != torch.int32 or positions.dim() != 1 or positions.shape[0] < total or \
-            positions.device != dev or (total > 1 and positions.stride(0) != 1):
-        raise RuntimeError(f"positions must be contiguous int32 [>= {total}] on the batch's device")
-    if q_out is None:
-        q_out = torch.empty((shape[0], nh, hd), dtype=_BF16, device=dev)
-        if shape[0] > total:
-            q_out[total:].zero_()
-        qo = nh * hd, hd
-    else:
-        qo = _rows3(q_out, "q_out", batch)
-    if total == 0:
-        return q_out
-    st = status if status is not None else status_tensor(dev)
     with _on(dev):
-        rc = _lib.fast().pkv_packed_rope_append(
-            qkv.data_ptr(), strides[0], positions.data_ptr(), batch.slots.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-            cos.shape[0], q_norm_w.data_ptr() if q_norm_w is not None else 0,
-            k_norm_w.data_ptr() if k_norm_w is not None else 0, float(eps), q_out.data_ptr(), qo[0], qo[1],
-            k_cache.data_ptr(), v_cache.data_ptr(), page_stride, total, nh, nk, hd, rotary, int(interleaved),
-            batch.page_size, batch.num_pages, st.data_ptr(), _raw_stream(dev.index))
-    if rc:
-        _lib.check(rc, "pkv_packed_rope_append")
-    return q_out
+        return _lib.fast().packed_rope_append(qkv, k_cache, v_cache, batch._native, cos, sin, interleaved, q_norm_w,
+                                              k_norm_w, eps, positions, q_out,
+                                              status if status is not None else status_tensor(dev), _raw_stream(dev.index))
 
 
 def packed_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, batch: PackedBatch, *,
@@ -246,47 +190,12 @@ def packed_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     ``softmax_scale`` defaults to 1/sqrt(head_dim).  With ``return_lse`` also the natural logarithm of the
     denominators, fp32 [tokens, n_heads].  Rows of ``q`` and ``out`` behind the batch's tokens are not touched
     (zero in results made here)."""
+    dev = batch.device
     _require_gpu(q, "q")
-    qs = _rows3(q, "q", batch)
-    page_stride = batch._check_cache(k_cache, v_cache)
     plan = batch._plans.get(window)
     if plan is None:
         raise RuntimeError(f"the batch was laid out for the windows {list(batch._plans)}, not {window}")
-    dev, total, nh, hd = batch.device, batch.total_tokens, batch.n_heads, batch.head_dim
-    if sinks is not None and (sinks.dtype != torch.float32 or tuple(sinks.shape) != (nh,) or sinks.stride(0) != 1 or
-                              sinks.device != dev):
-        raise RuntimeError(f"sinks must be a contiguous float32 [{nh}] vector on the batch's device")
-    scale = 1.0 / math.sqrt(hd) if softmax_scale is None else float(softmax_scale)
-    items, n_items, merges, n_merges, partials, merge_rows = plan
     with _on(dev):
-        if out is None:
-            rows = q.shape[0]
-            out = torch.empty((rows, nh, hd), dtype=_BF16, device=dev)
-            if rows > total:
-                out[total:].zero_()
-            os_ = nh * hd, hd
-        else:
-            os_ = _rows3(out, "out", batch)
-        lse = None
-        if return_lse:
-            lse = torch.empty((q.shape[0], nh), dtype=torch.float32, device=dev)
-            if q.shape[0] > total:
-                lse[total:].zero_()
-        if total == 0:
-            return (out, lse) if return_lse else out
-        # the partials of this call alone, from torch's allocator: of the current stream, or of the graph it captures
-        nbytes, ws = 0, None
-        if partials:
-            nbytes = _lib.load().pkv_packed_workspace_bytes(partials, batch.n_kv, hd)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        st = status if status is not None else status_tensor(dev)
-        rc = _lib.fast().pkv_packed_attn(
-            q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), page_stride,
-            batch.block_table.data_ptr(), batch.max_blocks, out.data_ptr(), os_[0], os_[1],
-            lse.data_ptr() if lse is not None else 0, sinks.data_ptr() if sinks is not None else 0,
-            items.data_ptr(), n_items, merges.data_ptr() if n_merges else 0, n_merges, partials, merge_rows,
-            ws.data_ptr() if ws is not None else 0, nbytes, total, batch.batch, nh, batch.n_kv, hd, batch.page_size,
-            batch.num_pages, batch.max_blocks, int(window or 0), scale, st.data_ptr(), _raw_stream(dev.index))
-    if rc:
-        _lib.check(rc, "pkv_packed_attn")
-    return (out, lse) if return_lse else out
+        return _lib.fast().packed_attention(q, k_cache, v_cache, batch._native, plan, sinks, softmax_scale, return_lse,
+                                            out, status if status is not None else status_tensor(dev),
+                                            _raw_stream(dev.index))

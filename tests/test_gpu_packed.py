@@ -199,7 +199,7 @@ def test_captured_replayed_and_two_streams(gpu):
     """Calls that split their keys, in two graphs and eagerly on two streams at once: each has partials of its own."""
     new, ctx = [1, 1, 20], [3000, 6000, 2500]
     batch, bt, kc, vc, q = _case(gpu, new, ctx, 64, 28, 4, 128, seed=8)
-    assert batch._plans[None][3] > 0
+    assert batch._plans[None][4] > 0
     dk, dv = kc.to(gpu), vc.to(gpu)
     qs = [q.to(gpu), (q * 0.5).to(gpu)]
     graphs, outs = [], []

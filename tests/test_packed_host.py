@@ -95,7 +95,7 @@ def test_batch_positions_and_slots():
     empty = _batch(new_lens=[], cache_lens=[], block_table=np.zeros((0, 1), np.int32))
     assert empty.total_tokens == 0 and empty.positions.numel() == 0
     none = _batch(new_lens=[0, 0, 0])
-    assert none.total_tokens == 0 and none._plans[None][1] == 0
+    assert none.total_tokens == 0 and none._plans[None][2] == 0
     # pages wholly before the window may be gone
     _batch(new_lens=[1, 0, 0], block_table=[[-1, 2], [-1, -1], [-1, -1]], windows=(100,))
 
