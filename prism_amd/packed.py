@@ -27,6 +27,7 @@ from . import _lib
 from .attention import _raw_stream, _require_gpu, status_tensor
 
 _MAX_KEYS = 1 << 27
+_captured: list[torch.Tensor] = []   # work lists that a captured graph reads
 
 
 _here = contextlib.nullcontext()
@@ -56,8 +57,10 @@ class PackedBatch:
 
     Holds on the device, from one upload on the current stream: ``positions`` and ``slots`` (int32 [tokens]: each
     token's position and place in the cache, page * page_size + row), ``block_table`` (int32 [batch, max_blocks])
-    and, for each of ``windows`` (None: every key; w: the last w keys), the attention's work list.  Use it on
-    other streams, and free it while they run, as any tensor made on the current one.
+    and, for each of ``windows`` (None: every key; w: the last w keys), the attention's work list.  On another
+    stream, use it behind this one, as any tensor made here; calls there keep its memory until they have run, and a
+    call that a graph captures keeps it for the rest of the process (a replay reads it, whether the batch lives or
+    not).
 
     A page that a new token is written to must belong to one sequence alone, and every page that a token is written
     to or sees must be one of the pool's; columns behind them, or out of every window, may hold anything."""
@@ -110,6 +113,7 @@ class PackedBatch:
         host = staged.numpy()
         for p, at in zip(parts, starts):
             host[at:at + p.size] = p
+        self._stream = _raw_stream(device.index) if device.type == "cuda" else 0
         with _on(device):
             self._buf = staged.to(device, non_blocking=True)
         view = [self._buf[at:at + p.size] for p, at in zip(parts, starts)]
@@ -120,9 +124,19 @@ class PackedBatch:
         self._plans = {w: (int(w or 0), base + 4 * int(starts[3 + 2 * i]), len(items), base + 4 * int(starts[4 + 2 * i]),
                            len(merges), int(counts[2]), int(counts[3]))
                        for i, (w, (items, merges, counts)) in enumerate(plans.items())}
+        self._captured = False
         self._native = _lib.fast().new_batch(self._buf, total, self.batch, n_heads, n_kv, head_dim, page_size, num_pages,
                                              self.max_blocks, self.positions.data_ptr(), self.slots.data_ptr(),
                                              base + 4 * int(starts[2]))
+
+    def _used_on(self, stream: int) -> None:
+        """A call on `stream` will read the batch's memory."""
+        if torch._C._cuda_isCurrentStreamCapturing():
+            if not self._captured:
+                _captured.append(self._buf)
+                self._captured = True
+        elif stream != self._stream:
+            self._buf.record_stream(torch.cuda.current_stream(self.device))
 
     def _check_pages(self, new, ctx, bt, widest) -> None:
         P, busy = self.page_size, new > 0
@@ -173,10 +187,12 @@ def packed_rope_append(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     differ.  Rows of ``qkv`` and ``q_out`` behind the batch's tokens are not touched (zero in a result made here)."""
     dev = batch.device
     _require_gpu(qkv, "qkv")
+    stream = _raw_stream(dev.index)
     with _on(dev):
+        batch._used_on(stream)
         return _lib.fast().packed_rope_append(qkv, k_cache, v_cache, batch._native, cos, sin, interleaved, q_norm_w,
                                               k_norm_w, eps, positions, q_out,
-                                              status if status is not None else status_tensor(dev), _raw_stream(dev.index))
+                                              status if status is not None else status_tensor(dev), stream)
 
 
 def packed_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, batch: PackedBatch, *,
@@ -195,7 +211,8 @@ def packed_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     plan = batch._plans.get(window)
     if plan is None:
         raise RuntimeError(f"the batch was laid out for the windows {list(batch._plans)}, not {window}")
+    stream = _raw_stream(dev.index)
     with _on(dev):
+        batch._used_on(stream)
         return _lib.fast().packed_attention(q, k_cache, v_cache, batch._native, plan, sinks, softmax_scale, return_lse,
-                                            out, status if status is not None else status_tensor(dev),
-                                            _raw_stream(dev.index))
+                                            out, status if status is not None else status_tensor(dev), stream)

@@ -280,3 +280,65 @@ def test_steps_of_a_served_batch(gpu, nh, nk, hd, P, window):
                 t = _tol(ref[0][first:first + n], ref[2][first:first + n], 500)
                 assert ((o[0].double().cpu() - ref[0][first:first + n]).abs() <= t).all()
                 first += n
+
+
+def test_pages_past_32_bits(gpu):
+    """A pool of 2.4e9 elements: pages whose offset does not fit 32 bits, of bytes or of elements."""
+    P, nk, hd, nh = 256, 8, 128, 40
+    pages = 9200
+    kc = torch.zeros(pages, P, nk, hd, dtype=BF16, device=gpu)
+    vc = torch.zeros_like(kc)
+    bt = np.array([[9199, 9100], [4097, 8193]], np.int32)
+    new, ctx = [3, 200], [300, 100]
+    batch = prism_amd.PackedBatch(new, ctx, bt, page_size=P, num_pages=pages, n_heads=nh, n_kv=nk, head_dim=hd, device=gpu)
+    g = torch.Generator(device=gpu).manual_seed(1)
+    for p in bt.ravel().tolist():
+        kc[p].normal_(generator=g)
+        vc[p].normal_(generator=g)
+    cos, sin = prism_amd.rotary_tables(hd, 400, device=gpu)
+    x = torch.empty(203, (nh + 2 * nk) * hd, dtype=BF16, device=gpu).normal_(generator=g)
+    q = prism_amd.packed_rope_append(x, kc, vc, batch, cos, sin)
+    assert torch.equal(vc[9100, 44:47], x[:3, (nh + nk) * hd:].unflatten(1, (nk, hd)))
+    assert torch.equal(vc[4097, 100:], x[3:159, (nh + nk) * hd:].unflatten(1, (nk, hd)))
+    out, lse = prism_amd.packed_attention(q, kc, vc, batch, return_lse=True)
+    ids = sorted(set(bt.ravel().tolist()))
+    mini = torch.tensor([[ids.index(p) for p in row] for row in bt.tolist()])
+    at = torch.tensor(ids, device=gpu)
+    want = op.packed_attention64(q.cpu(), kc[at].cpu(), vc[at].cpu(), new, ctx, mini)
+    _check(out, lse, want, 303, "far pages")
+    del kc, vc
+    torch.cuda.empty_cache()
+
+
+def test_a_graph_outlives_the_batch_and_a_stream_its_use(gpu):
+    new, ctx = [1, 40], [700, 300]
+    batch, bt, kc, vc, q = _case(gpu, new, ctx, 64, 14, 2, 64, seed=3)
+    dq, dk, dv = q.to(gpu), kc.to(gpu), vc.to(gpu)
+    want = prism_amd.packed_attention(dq, dk, dv, batch)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = prism_amd.packed_attention(dq, dk, dv, batch)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = prism_amd.packed_attention(dq, dk, dv, batch)
+    size = batch._buf.numel()
+    del batch
+    for i in range(3):
+        junk = [torch.full((size,), -7 - i, dtype=torch.int32, device=gpu) for _ in range(50)]   # would land in freed memory
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+        del junk
+    assert torch.equal(other, want)
+
+
+@pytest.mark.parametrize("nh,nk,hd,P", [(28, 4, 128, 256), (14, 2, 64, 16)])
+def test_many_ranges_of_one_block(gpu, nh, nk, hd, P):
+    """One decode token and one short chunk on 20,000 keys: some twenty partials of a row to merge."""
+    new, ctx = [1, 30], [20000, 9000]
+    batch, bt, kc, vc, q = _case(gpu, new, ctx, P, nh, nk, hd, seed=5, windows=(None, 7000))
+    for w in (None, 7000):
+        out, lse = prism_amd.packed_attention(q.to(gpu), kc.to(gpu), vc.to(gpu), batch, window=w, return_lse=True)
+        _check(out, lse, op.packed_attention64(q, kc, vc, new, ctx, bt, window=w), 20001, f"window {w}")
