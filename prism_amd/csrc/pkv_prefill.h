@@ -410,6 +410,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
   // the last, or the first of the next page.
   const int pmask = (1 << p.log2_page) - 1;
   const int stage_elems = TOK * p.n_kv * HD;
+  int left_k = n, left_v = n;    // stages left to copy
   constexpr int kOff = SMALL ? kCopies : 1;  // page lookups of a stage
   struct Offs {
     int64_t at[kOff];
@@ -419,34 +420,36 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
   bool bad_page = false;
   // first key that a row of the block sees
   const int first_key = PACKED && p.window > 0 ? max(c + blk_row0 / p.g - p.window + 1, 0) : 0;
-  // SMALL: lane l holds the offset of page col0 + l, -1 for a page that lies wholly before every row's window or
-  // behind the last key (it may not exist: its rows read as zeros).  One multiplication per lane and 64 pages, two
-  // readlanes per copy; worked out stage by stage, a window's chunks (14B, pages of 16) took 106 us where pages of
-  // 256 take 91.
-  int64_t page_offs = -1;
+  // SMALL: lane l holds the byte offset of head h in page col0 + l, far below zero for a page that lies wholly before
+  // every row's window or behind the last key (it may not exist: copies of a negative offset fetch nothing and write
+  // zeros).  One multiplication per lane and 64 pages, two readlanes per copy; worked out stage by stage, a window's
+  // chunks (14B, pages of 16) took 106 us where pages of 256 take 91.
+  int64_t page_offs = 0;
   auto load_offs = [&] {
     const int key = (btw.col0 + lane) << p.log2_page;
     const bool needed = key < L && key + pmask >= first_key;
     const bool ok = unsigned(btw.ids) < unsigned(p.num_pages);
-    page_offs = needed ? int64_t(ok ? btw.ids : 0) * p.page_stride : -1;
+    page_offs = needed ? 2 * (int64_t(ok ? btw.ids : 0) * p.page_stride + h * HD) : INT64_MIN / 2;
     bad_page |= __any(needed && !ok);
   };
   if constexpr (SMALL) load_offs();
   auto page_start = [&] {
     const int col = T_k >> p.log2_page;
-    if (col - btw.col0 > (SMALL ? 64 - TOK / 16 : 63)) {
+    if (__builtin_expect(col - btw.col0 > (SMALL ? 64 - TOK / 16 : 63) && (!SMALL || left_k > 0), 0)) {
       bt_window_load(p, sv, col, btw);
       __builtin_amdgcn_s_waitcnt(0x0F70);  // here, once per 64 pages: not at every use of the window
       if constexpr (SMALL) load_offs();
     }
     if constexpr (SMALL) {
+      // (also for stages past the last, whose copies fetch nothing: no branch in the loop, and a lane number past
+      // 63 is taken modulo 64)
 #pragma unroll
       for (int k = 0; k < kOff; ++k) {
         const int row = (wave + W * k) * G::RPC;
         const int at = col - btw.col0 + (row >> p.log2_page);
         const uint32_t lo = __builtin_amdgcn_readlane(uint32_t(page_offs), at);
-        const int32_t hi32 = __builtin_amdgcn_readlane(int32_t(page_offs >> 32), at);
-        off_k.at[k] = hi32 < 0 ? -1 : int64_t((uint64_t(uint32_t(hi32)) << 32) | lo) + (row & pmask) * (p.n_kv * HD) + h * HD;
+        const uint32_t up = __builtin_amdgcn_readlane(uint32_t(page_offs >> 32), at);
+        off_k.at[k] = int64_t((uint64_t(up) << 32) | lo) + (row & pmask) * row_bytes;
       }
     } else {
       const int pid = __builtin_amdgcn_readlane(btw.ids, col - btw.col0);
@@ -464,21 +467,27 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
   // its V copies: off1 .. off3 hold the offsets of the stages in between, oldest first.
   Offs off1 = {}, off2 = {}, off3 = {};
   int slot_k = 0, slot_v = 0;    // ring slots the next copies go to
-  int left_k = n, left_v = n;    // stages left to copy
   auto next_slot = [](int slot) { return slot == (kRing - 1) * G::STAGE ? 0 : slot + G::STAGE; };
   auto next_stage = [&] {
-    if (__builtin_expect((SMALL || (T_k & pmask) == 0) && left_k > 0, SMALL)) page_start();
+    if constexpr (SMALL) {
+      page_start();
+    } else {
+      if (__builtin_expect((T_k & pmask) == 0 && left_k > 0, 0)) page_start();
+    }
     off1 = off2;
     off2 = off3;
     off3 = off_k;
     if (!SMALL) off_k.at[0] += stage_elems;
     T_k += TOK;
   };
+  auto byte_at = [](const uint16_t* base, int64_t bytes) {
+    return reinterpret_cast<const uint16_t*>(reinterpret_cast<uintptr_t>(base) + uintptr_t(bytes));
+  };
   auto copy_k = [&](int k) {
     const int i = wave + W * k;
     const int64_t off = off3.at[SMALL ? k : 0];
     const bool some = left_k > 0 && !(SMALL && off < 0);
-    pf::copy_1k(p.k_cache + (SMALL && off < 0 ? 0 : off), some ? (SMALL ? G::RPC : TOK) * row_bytes : 0,
+    pf::copy_1k(SMALL ? byte_at(p.k_cache, off) : p.k_cache + off, some ? (SMALL ? G::RPC : TOK) * row_bytes : 0,
                 vk ^ uint32_t(G::swz_k(W * k * G::RPC) << 4), SMALL ? 0 : i * G::RPC * row_bytes,
                 ring_k + slot_k + i * 1024);
     if (k == kCopies - 1) {
@@ -491,7 +500,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
     const int i = wave + W * k;
     const int64_t off = off_v.at[SMALL ? k : 0];
     const bool some = left_v > 0 && !(SMALL && off < 0);
-    pf::copy_1k(p.v_cache + (SMALL && off < 0 ? 0 : off), some ? (SMALL ? G::RPC : TOK) * row_bytes : 0, vv,
+    pf::copy_1k(SMALL ? byte_at(p.v_cache, off) : p.v_cache + off, some ? (SMALL ? G::RPC : TOK) * row_bytes : 0, vv,
                 SMALL ? 0 : i * G::RPC * row_bytes, ring_v + slot_v + i * 1024);
     if (k == kCopies - 1) {
       slot_v = next_slot(slot_v);

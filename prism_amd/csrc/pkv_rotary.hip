@@ -105,7 +105,7 @@ __device__ __forceinline__ int64_t slot_row(const RotaryParams& p, uint32_t t) {
 // One lane holds two 16-byte chunks of one head: half layout, the two halves of its pairs (behind the rotated
 // part, chunks of the two halves of the rest); interleaved, chunks of the two halves of the head.  So the lanes of a
 // head read and write 16 bytes next to each other with every instruction (two neighbouring chunks per lane, and in
-// fp32 four, took 52 us where 5003 tokens of 32 heads now take SEE BELOW).  A lane reads nothing that another
+// fp32 four, took 52 us where 5003 tokens of 32 heads now take 25).  A lane reads nothing that another
 // writes, so the outputs may be the inputs; the norm's sum goes over the head's lanes by shuffles.  Lanes are
 // counted over the heads of all tokens: a token's 2 + 14 or 16 + 40 heads leave no lane of a workgroup idle.
 template <typename T, bool INTERLEAVED>
