@@ -388,6 +388,17 @@ int pkv_packed_rope_append(const void* qkv, int64_t qkv_st, const int32_t* posit
                            int32_t* status, void* stream);
 
 /*
+ * Where a packed batch's new tokens go, on the host (every pointer here is host memory; nothing is launched): for
+ * token j of sequence b, one sequence behind the other, positions = ctx_lens[b] + j and slots = the place that row b
+ * of block_table gives that position, page * page_size + row.  Refused, with nothing to be relied on in the
+ * outputs: a page outside [0, num_pages) among those that a sequence's new tokens see (window 0: all its keys, else
+ * from its first row's window on) or are written to, and a page that two places of the batch write to.
+ */
+int pkv_packed_layout(const int32_t* new_lens, const int32_t* ctx_lens, int32_t batch, const int32_t* block_table,
+                      int64_t bt_stride, int32_t max_blocks, int32_t page_size, int32_t num_pages, int32_t window,
+                      int32_t* positions, int32_t* slots);
+
+/*
  * The work list of a pkv_packed_attn call, on the host (every pointer here is host memory; nothing is launched).
  * Sequence b brings new_lens[b] >= 0 tokens behind ctx_lens[b] cached ones.  Their query rows are cut into blocks of
  * 128 per KV head, and blocks with many keys into ranges, for a device of compute_units CUs.  items receives

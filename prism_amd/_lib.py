@@ -159,6 +159,7 @@ _SIGNATURES = {
         _I64, _I32, _I32, _I32, _I32,    # tokens, n_heads, n_kv, head_dim, rotary_dim
         _I32, _I32, _I32, _P, _P,        # interleaved, page_size, num_pages, status, stream
     ]),
+    "pkv_packed_layout": (c_int32, [_P, _P, _I32, _P, _I64, _I32, _I32, _I32, _I32, _P, _P]),
     "pkv_packed_plan": (c_int32, [_P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P, _I32, _P, _I32, _P]),
     "pkv_packed_workspace_bytes": (c_size_t, [_I32] * 3),
     "pkv_packed_attn": (c_int32, [

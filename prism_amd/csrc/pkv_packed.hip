@@ -177,6 +177,72 @@ static void plan(const int32_t* new_lens, const int32_t* ctx_lens, int batch, in
 
 }  // namespace pkv
 
+namespace pkv {
+// Sequence lengths as every entry here takes them; the tokens in all, -1 where one does not fit (recorded).
+static int64_t check_lengths(const char* fn, const int32_t* new_lens, const int32_t* ctx_lens, int batch) {
+  int64_t tokens = 0;
+  for (int b = 0; b < batch; ++b) {
+    if (new_lens[b] < 0 || ctx_lens[b] < 0 || int64_t(new_lens[b]) + ctx_lens[b] > (int64_t(1) << 27)) {
+      fail(PKV_EINVAL, "%s: sequence %d has %d new and %d cached tokens: not negative, and at most 2^27 together", fn, b,
+           new_lens[b], ctx_lens[b]);
+      return -1;
+    }
+    tokens += new_lens[b];
+  }
+  return tokens;
+}
+}  // namespace pkv
+
+extern "C" int pkv_packed_layout(const int32_t* new_lens, const int32_t* ctx_lens, int32_t batch,
+                                 const int32_t* block_table, int64_t bt_stride, int32_t max_blocks, int32_t page_size,
+                                 int32_t num_pages, int32_t window, int32_t* positions, int32_t* slots) {
+  using namespace pkv;
+  clear_error();
+  const char* fn = "pkv_packed_layout";
+  if (batch < 0 || max_blocks < 0 || bt_stride < max_blocks || window < 0)
+    return fail(PKV_EINVAL, "%s: bad sizes batch=%d max_blocks=%d bt_stride=%lld window=%d", fn, batch, max_blocks,
+                (long long)bt_stride, window);
+  if (!is_pow2(page_size) || page_size < 16)
+    return fail(PKV_EINVAL, "%s: page_size %d must be a power of two >= 16", fn, page_size);
+  if (num_pages <= 0 || int64_t(num_pages) * page_size > 0x7fffffff)
+    return fail(PKV_EINVAL, "%s: %d pages of %d tokens: the pool must have 1 to 2^31 - 1 slots", fn, num_pages, page_size);
+  if (batch > 0 && (!new_lens || !ctx_lens || (max_blocks > 0 && !block_table)))
+    return fail(PKV_EINVAL, "%s: null argument", fn);
+  const int64_t tokens = check_lengths(fn, new_lens, ctx_lens, batch);
+  if (tokens < 0) return PKV_EINVAL;
+  if (tokens > 0 && (!positions || !slots)) return fail(PKV_EINVAL, "%s: null argument", fn);
+  const int log2_page = ilog2(page_size);
+  try {
+    std::vector<bool> written(num_pages, false);
+    int64_t t = 0;
+    for (int b = 0; b < batch; ++b) {
+      const int n = new_lens[b], c = ctx_lens[b];
+      if (n == 0) continue;
+      const int32_t* row = block_table + b * bt_stride;
+      const int last = (c + n - 1) >> log2_page;
+      if (last >= max_blocks)
+        return fail(PKV_EINVAL, "%s: sequence %d needs %d pages, the block table has %d columns", fn, b, last + 1, max_blocks);
+      for (int col = (window > 0 ? std::max(c - window + 1, 0) : 0) >> log2_page; col <= last; ++col)
+        if (unsigned(row[col]) >= unsigned(num_pages))
+          return fail(PKV_EINVAL, "%s: sequence %d needs block-table column %d, which lists page %d, outside [0, %d)", fn, b,
+                      col, row[col], num_pages);
+      for (int col = c >> log2_page; col <= last; ++col) {
+        if (written[row[col]])
+          return fail(PKV_EINVAL, "%s: two places of the batch write to one page, %d, sequence %d the second (the same "
+                      "sequence twice, or a shared page that was not copied before the write)", fn, row[col], b);
+        written[row[col]] = true;
+      }
+      for (int pos = c; pos < c + n; ++pos, ++t) {
+        positions[t] = pos;
+        slots[t] = row[pos >> log2_page] * page_size + (pos & (page_size - 1));
+      }
+    }
+  } catch (const std::exception& e) {  // no memory: no C++ exception leaves a C entry
+    return fail(PKV_EINVAL, "%s: %s", fn, e.what());
+  }
+  return PKV_OK;
+}
+
 extern "C" int pkv_packed_plan(const int32_t* new_lens, const int32_t* ctx_lens, int32_t batch, int32_t n_heads,
                                int32_t n_kv, int32_t head_dim, int32_t window, int32_t compute_units, int32_t* items,
                                int32_t max_items, int32_t* merges, int32_t max_merges, int32_t* counts) {
@@ -189,13 +255,8 @@ extern "C" int pkv_packed_plan(const int32_t* new_lens, const int32_t* ctx_lens,
   if (head_dim != 64 && head_dim != 128) return fail(PKV_EINVAL, "%s: head_dim %d unsupported (64 or 128)", fn, head_dim);
   if ((batch > 0 && (!new_lens || !ctx_lens)) || !counts) return fail(PKV_EINVAL, "%s: null argument", fn);
   const int g = n_heads / n_kv;
-  int64_t tokens = 0;
-  for (int b = 0; b < batch; ++b) {
-    if (new_lens[b] < 0 || ctx_lens[b] < 0 || int64_t(new_lens[b]) + ctx_lens[b] > (int64_t(1) << 27))
-      return fail(PKV_EINVAL, "%s: sequence %d has %d new and %d cached tokens (0 to 2^27 in all)", fn, b, new_lens[b],
-                  ctx_lens[b]);
-    tokens += new_lens[b];
-  }
+  const int64_t tokens = check_lengths(fn, new_lens, ctx_lens, batch);
+  if (tokens < 0) return PKV_EINVAL;
   if (tokens * n_heads > (int64_t(1) << 30)) return fail(PKV_EINVAL, "%s: more than 2^30 query rows", fn);
   try {
     std::vector<PackedItem> it;

@@ -44,11 +44,13 @@ def _host_ints(x, name: str, ndim: int) -> np.ndarray:
             raise RuntimeError(f"{name} must be on the host: the step's work is laid out there")
         x = x.numpy()
     a = np.asarray(x)
-    if a.size == 0:
-        a = a.astype(np.int64)
-    if a.ndim != ndim or a.dtype.kind not in "iu":
+    if a.size and a.dtype.kind not in "iu" or a.ndim != ndim:
         raise RuntimeError(f"{name} must be {ndim}-dimensional integers, got {a.dtype} {a.shape}")
-    return a.astype(np.int64)
+    if a.dtype != np.int32:
+        if a.size and (a.min() < -1 << 31 or a.max() > (1 << 31) - 1):
+            raise RuntimeError(f"{name} must fit int32")
+        a = a.astype(np.int32)
+    return np.ascontiguousarray(a)
 
 
 class PackedBatch:
@@ -77,37 +79,32 @@ class PackedBatch:
         bt = _host_ints(block_table, "block_table", 2)
         if len(new) != len(ctx) or len(new) != bt.shape[0]:
             raise RuntimeError(f"{len(new)} new lengths, {len(ctx)} cached lengths and {bt.shape[0]} block-table rows")
-        if page_size < 16 or page_size & (page_size - 1):
-            raise RuntimeError(f"page_size {page_size} must be a power of two >= 16")
-        if num_pages <= 0 or num_pages * page_size > 0x7FFFFFFF:
-            raise RuntimeError(f"{num_pages} pages of {page_size} tokens: the pool must have 1 to 2^31 - 1 slots")
+        if not 0 < page_size <= _MAX_KEYS or not 0 < num_pages < 1 << 31:
+            raise RuntimeError(f"{num_pages} pages of {page_size} tokens: no pool of that size")
         if head_dim not in (64, 128):
             raise RuntimeError(f"head_dim {head_dim} unsupported (64 or 128)")
-        if n_kv <= 0 or n_heads <= 0 or n_heads % n_kv:
+        if n_kv <= 0 or n_heads <= 0 or n_heads % n_kv or n_heads > 1 << 20:
             raise RuntimeError(f"n_heads {n_heads} must be a multiple of n_kv {n_kv}")
         if not windows:
             raise RuntimeError("windows must name at least one window (None: every key)")
         for w in windows:
             if w is not None and (isinstance(w, bool) or not isinstance(w, (int, np.integer)) or not 1 <= w <= _MAX_KEYS):
                 raise RuntimeError(f"window {w!r} must be None or 1 to 2^27 keys")
-        if (new < 0).any() or (ctx < 0).any() or (new + ctx > _MAX_KEYS).any():
-            raise RuntimeError("lengths must not be negative, nor 2^27 keys be passed")
-        total = int(new.sum())
-        if total * n_heads > 1 << 30:
-            raise RuntimeError(f"{total} tokens of {n_heads} heads: more than 2^30 query rows")
-        self.batch, self.total_tokens = len(new), total
+        self.batch, self.total_tokens = len(new), int(new.sum(dtype=np.int64))
         self.page_size, self.num_pages = page_size, num_pages
         self.n_heads, self.n_kv, self.head_dim, self.device = n_heads, n_kv, head_dim, device
         self.max_blocks = max(bt.shape[1], 1)
-        widest = _MAX_KEYS if any(w is None for w in windows) else max(windows)
-        self._check_pages(new, ctx, bt, widest)
-        seq = np.repeat(np.arange(self.batch), new)
-        pos = np.arange(total) - np.repeat(np.cumsum(new) - new, new) + ctx[seq]
-        slots = bt[seq, pos // page_size] * page_size + pos % page_size if total else pos
-
+        lib, total = _lib.load(), self.total_tokens
+        lengths = (new.ctypes.data, ctx.ctypes.data, self.batch)
+        if total * n_heads > 1 << 30:
+            raise RuntimeError(f"{total} tokens of {n_heads} heads: more than 2^30 query rows")
+        where = np.empty((2, max(total, 0)), np.int32)
+        widest = 0 if any(w is None for w in windows) else max(windows)
+        _lib.check(lib.pkv_packed_layout(*lengths, bt.ctypes.data, bt.shape[1], bt.shape[1], page_size, num_pages, widest,
+                                         where[0].ctypes.data, where[1].ctypes.data), "pkv_packed_layout")
         cus = torch.cuda.get_device_properties(device).multi_processor_count if device.type == "cuda" else 256
-        plans = {w: self._plan(new, ctx, w, cus) for w in dict.fromkeys(windows)}
-        parts = [pos, slots, bt.ravel()] + [a.ravel() for items, merges, _ in plans.values() for a in (items, merges)]
+        plans = {w: self._plan(lengths, w, cus) for w in dict.fromkeys(windows)}
+        parts = [where[0], where[1], bt.ravel()] + [a.ravel() for items, merges, _ in plans.values() for a in (items, merges)]
         starts = np.cumsum([0] + [-(-p.size // 4) * 4 for p in parts])     # 16-byte aligned
         staged = torch.empty(int(starts[-1]) + 4, dtype=torch.int32, pin_memory=device.type == "cuda")
         host = staged.numpy()
@@ -138,28 +135,10 @@ class PackedBatch:
         elif stream != self._stream:
             self._buf.record_stream(torch.cuda.current_stream(self.device))
 
-    def _check_pages(self, new, ctx, bt, widest) -> None:
-        P, busy = self.page_size, new > 0
-        end = -(-(ctx + new) // P)
-        if (end[busy] > bt.shape[1]).any():
-            raise RuntimeError(f"a sequence needs {int(end[busy].max())} pages, the block table has {bt.shape[1]} columns")
-        cols = np.arange(bt.shape[1])[None]
-        first = np.maximum(ctx - widest + 1, 0) // P
-        used = busy[:, None] & (cols >= first[:, None]) & (cols < end[:, None])
-        if ((bt < 0) | (bt >= self.num_pages))[used].any():
-            raise RuntimeError(f"the block table lists a page outside [0, {self.num_pages}) that a sequence needs")
-        written = bt[busy[:, None] & (cols >= (ctx // P)[:, None]) & (cols < end[:, None])]
-        if np.unique(written).size != written.size:
-            raise RuntimeError("two places of the batch write to one page (the same sequence twice, or a shared page "
-                               "that was not copied before the write)")
-        if np.abs(bt).max(initial=0) > 0x7FFFFFFF:
-            raise RuntimeError("block_table must fit int32")
-
-    def _plan(self, new, ctx, window, cus):
+    def _plan(self, lengths, window, cus):
         lib = _lib.load()
-        n32, c32 = np.ascontiguousarray(new, np.int32), np.ascontiguousarray(ctx, np.int32)
         counts = np.zeros(4, np.int32)
-        sizes = (n32.ctypes.data, c32.ctypes.data, self.batch, self.n_heads, self.n_kv, self.head_dim, int(window or 0), cus)
+        sizes = (*lengths, self.n_heads, self.n_kv, self.head_dim, int(window or 0), cus)
         # enough for a block per 128 query rows and sequence and two ranges per workgroup; asked for where it is not
         g = self.n_heads // self.n_kv
         room = self.total_tokens * g // 128 + self.batch + 4 * max(2 * cus // self.n_kv, 1)

@@ -62,6 +62,21 @@ def test_plan_covers_every_visible_key_once(nh, nk, hd, window, cus):
         assert counts[3] <= 128
 
 
+def test_layout_refusals():
+    lib = _lib.load()
+    one, bt, out = np.array([1], np.int32), np.array([[3]], np.int32), np.zeros(4, np.int32)
+
+    def call(new=one, ctx=one, batch=1, bt=bt, bts=1, mb=1, page=16, pages=4, window=0, pos=out.ctypes.data):
+        return lib.pkv_packed_layout(new.ctypes.data, ctx.ctypes.data, batch, bt.ctypes.data, bts, mb, page, pages, window,
+                                     pos, out.ctypes.data)
+    assert call() == 0 and out[0] == 3 * 16 + 1
+    for bad in [dict(page=8), dict(page=24), dict(pages=3), dict(pages=0), dict(pages=1 << 30), dict(mb=2), dict(batch=-1),
+                dict(window=-1), dict(pos=0), dict(new=np.array([16], np.int32)), dict(bt=np.array([[-1]], np.int32)),
+                dict(ctx=np.array([-1], np.int32)), dict(ctx=np.array([1 << 27], np.int32))]:
+        assert call(**bad) == _lib.PKV_EINVAL, bad
+        assert "pkv_packed_layout" in lib.pkv_last_error().decode()
+
+
 def test_plan_refusals():
     lib = _lib.load()
     c = np.zeros(4, np.int32)
@@ -115,6 +130,11 @@ def test_batch_positions_and_slots():
     (dict(page_size=8), "power of two"),
     (dict(num_pages=0), "pool"),
     (dict(num_pages=1 << 24), "pool"),
+    (dict(num_pages=1 << 32), "pool"),
+    (dict(page_size=(1 << 32) + 16), "pool"),
+    (dict(new_lens=[1 << 26, 0, 1]), "2\\^30"),
+    (dict(new_lens=[1 << 33, 0, 1]), "int32"),
+    (dict(new_lens=[-(1 << 30), 1 << 20, 1]), "negative"),
     (dict(head_dim=96), "head_dim"),
     (dict(n_heads=30), "multiple"),
     (dict(windows=()), "at least one"),
