@@ -402,8 +402,9 @@ int pkv_packed_layout(const int32_t* new_lens, const int32_t* ctx_lens, int32_t 
  * The work list of a pkv_packed_attn call, on the host (every pointer here is host memory; nothing is launched).
  * Sequence b brings new_lens[b] >= 0 tokens behind ctx_lens[b] cached ones.  Their query rows are cut into blocks of
  * 128 per KV head, and blocks with many keys into ranges, for a device of compute_units CUs.  items receives
- * 8 int32 words per item, merges 8 per block of several ranges; counts (4 words) the items, the merges, the
- * partial results that the workspace must hold and merge_rows.  items NULL: the counts only.
+ * 12 int32 words per item, merges 8 per block of several ranges that the launch itself does not merge (blocks of
+ * more than 32 rows or 64 ranges); counts (4 words) the items, the merges, the partial results that the workspace
+ * must hold and merge_rows.  items NULL: the counts only.
  * PKV_ENOSPC where max_items or max_merges is too few.
  */
 int pkv_packed_plan(const int32_t* new_lens, const int32_t* ctx_lens, int32_t batch, int32_t n_heads, int32_t n_kv,

@@ -25,7 +25,9 @@
 // Every K/V byte of a (sequence, KV head) is fetched once per query-row tile.
 #include <math.h>
 
+#include <atomic>
 #include <mutex>
+#include <random>
 #include <type_traits>
 
 #include "pkv_common.h"
@@ -79,6 +81,8 @@ struct AttnParams {
   const PackedMerge* merges;
   const float* sinks;
   float* lse;
+  uint64_t* tags;  // [partials, n_kv]: which ranges' partials are stored (pf::merge_last)
+  uint64_t tag;    // this call's
   int tokens, window;
 };
 
@@ -3015,6 +3019,8 @@ static void fill_params(AttnParams& p, const void* q, int64_t q_sb, int64_t q_ss
   p.merges = nullptr;
   p.sinks = nullptr;
   p.lse = nullptr;
+  p.tags = nullptr;
+  p.tag = 0;
   p.tokens = 0;
   p.window = 0;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
@@ -3636,9 +3642,24 @@ extern "C" int pkv_prefill_attn(const void* q, int64_t q_sb, int64_t q_ss, int64
                              causal, softmax_scale, status, stream);
 }
 
+namespace pkv {
+// 64 bits that no other call of this process has had, nor likely any memory by chance: a counter from a random start,
+// mixed (a bijection).  Never 0, which is a cleared tag.
+static uint64_t next_tag() {
+  static std::atomic<uint64_t> counter{(uint64_t(std::random_device{}()) << 32) | std::random_device{}()};
+  for (;;) {
+    uint64_t x = counter.fetch_add(1, std::memory_order_relaxed);
+    x = (x ^ (x >> 30)) * 0xbf58476d1ce4e5b9ull;
+    x = (x ^ (x >> 27)) * 0x94d049bb133111ebull;
+    x ^= x >> 31;
+    if (x != 0) return x;
+  }
+}
+}  // namespace pkv
+
 extern "C" size_t pkv_packed_workspace_bytes(int32_t partials, int32_t n_kv, int32_t head_dim) {
   if (partials <= 0 || n_kv <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
-  return size_t(partials) * n_kv * pkv::kPackedRows * (head_dim + 4) * sizeof(float);
+  return size_t(partials) * n_kv * (pkv::kPackedRows * (head_dim + 4) * sizeof(float) + sizeof(uint64_t));
 }
 
 extern "C" int pkv_packed_attn(const void* q, int64_t q_st, int64_t q_sh, const void* k_cache, const void* v_cache,
@@ -3668,6 +3689,7 @@ extern "C" int pkv_packed_attn(const void* q, int64_t q_st, int64_t q_sh, const 
   if (!aligned16(items) || !aligned16(merges)) return fail(PKV_EINVAL, "%s: work lists not 16-byte aligned", fn);
   if (int64_t(n_items) * n_kv > 0x7fffffff || n_merges > 65535) return fail(PKV_EINVAL, "%s: too many work items", fn);
   const size_t need = pkv_packed_workspace_bytes(partials, n_kv, head_dim);
+  if (need > 0x7fffffff) return fail(PKV_EINVAL, "%s: %d partials need more than 2^31 bytes", fn, partials);
   if (need > 0 && (!workspace || !aligned16(workspace)))
     return fail(PKV_EINVAL, "%s: workspace null or not 16-byte aligned", fn);
   if (need > 0 && workspace_bytes < need)
@@ -3685,6 +3707,8 @@ extern "C" int pkv_packed_attn(const void* q, int64_t q_st, int64_t q_sh, const 
   if (need > 0) {
     p.ws_o = static_cast<float*>(workspace);
     p.ws_ml = p.ws_o + size_t(partials) * n_kv * kPackedRows * head_dim;
+    p.tags = reinterpret_cast<uint64_t*>(p.ws_ml + size_t(partials) * n_kv * kPackedRows * 4);
+    p.tag = next_tag();
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (head_dim == 128)

@@ -6,8 +6,10 @@
 namespace pkv {
 
 constexpr int kPackedRows = 128;  // query rows (token x head of the group) of a work item
+// Blocks of at most so many rows (one wave's) and ranges merge in the launch: the last range to end does it.
+constexpr int kPackedLastRows = 32, kPackedLastRanges = 64;
 
-// One key range of one row block of one sequence, for every KV head.  32 bytes.
+// One key range of one row block of one sequence, for every KV head.  48 bytes.
 struct PackedItem {
   int32_t tok0;    // the sequence's first row of q and out
   int32_t n_new;   // its new tokens
@@ -17,9 +19,11 @@ struct PackedItem {
   int32_t stage0;  // the range's first stage (of 32 keys, head_dim 128, or 64)
   int32_t stages;
   int32_t slot;    // where its partial result goes, -1 for a block of one range
+  int32_t first, count;  // the block's slots, where its ranges merge in the launch (count 0: a PackedMerge does)
+  int32_t pad[2];
 };
 
-// A row block of several ranges: their partials are slots slot .. slot + count - 1.  32 bytes.
+// Any other row block of several ranges: their partials are slots slot .. slot + count - 1.  32 bytes.
 struct PackedMerge {
   int32_t tok0, n_new, row0, slot, count;
   int32_t pad[3];

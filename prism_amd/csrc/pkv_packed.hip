@@ -91,31 +91,33 @@ Schedule filled(const std::vector<Block>& blocks, int slots, int64_t target) {
   return s;
 }
 
-// Pieces of one length, for one workgroup per CU or for two, whichever ends sooner.  One per CU already reads as fast
-// as the card does (5.8 TB/s: all CUs together 370 stages a us, 0.6 us each); two even out what the blocks' lengths
-// leave uneven, at the price of more partials, 0.4 us per MB written and read, and 3.5 us for the launch that merges them.  Between the
-// two some CUs would have one and some two.  6 decode tokens and two chunks on 40 k keys: 102 + 5 us in 59 pieces per
-// KV head, 110 + 10 in 124; 47 decode tokens on 1500: 35 + 5 in 126 pieces, 41 + 5 in 77.
+// Pieces of one length, for two workgroups per CU, for one or for fewer, whichever ends soonest.  One per CU already
+// reads as fast as the card does (5.8 TB/s: all CUs together 370 stages a us, 0.6 us each); two even out what the
+// blocks' lengths leave uneven (in between some CUs would have one and some two), at the price of more partials: 0.4
+// us per MB written and read, and 2.7 us and 0.1 per range of a block to merge them.  6 decode tokens and two chunks
+// on 40 k keys: 102 + 5 us in 59 pieces per KV head, 110 + 10 in 124; 47 decode tokens on 1500: 35 + 5 in 126
+// pieces, 41 + 5 in 77 (each with a launch that merges).
 Schedule even(const std::vector<Block>& blocks, int slots, int n_kv, int head_dim) {
   int64_t total = 0;
   for (const Block& b : blocks) total += b.stages;
   int64_t best_chunk = 0;
   double best = 0;
-  for (const int64_t room : {int64_t(std::max(slots / 2, 1)), int64_t(slots)}) {
-    if (int64_t(blocks.size()) > room) continue;
+  for (const int64_t room : {slots, slots / 2, slots / 4, slots / 8}) {
+    if (room < 1 || int64_t(blocks.size()) > room) continue;
     for (int64_t chunk = std::max<int64_t>((total + room - 1) / room, kMinRange);;
          chunk += std::max<int64_t>(chunk / 16, 1)) {
-      int64_t ranges = 0, longest = 0, rows = 0;
+      int64_t ranges = 0, longest = 0, rows = 0, most = 0;
       for (const Block& b : blocks) {
         const int count = pieces(b.stages, chunk);
         ranges += count;
         longest = std::max<int64_t>(longest, (b.stages + count - 1) / count);
         if (count > 1) rows += int64_t(count) * b.rows;
+        most = std::max<int64_t>(most, count);
       }
       if (ranges > room) continue;
       const double at_once = std::min(370.0, 2.0 * ranges * n_kv);
       const double us = std::max(total * n_kv / at_once, 0.58 * longest) +
-                        (rows ? 3.5 + 0.4e-6 * rows * n_kv * (head_dim + 4) * 4 : 0.0);
+                        (rows ? 2.7 + 0.1 * most + 0.4e-6 * rows * n_kv * (head_dim + 4) * 4 : 0.0);
       if (best_chunk == 0 || us < best) {
         best = us;
         best_chunk = chunk;
@@ -137,6 +139,7 @@ constexpr int kRounds = 8;
 std::vector<Piece> cut(std::vector<Block>& blocks, int slots, int n_kv, int head_dim) {
   std::stable_sort(blocks.begin(), blocks.end(), [](const Block& a, const Block& b) { return a.stages > b.stages; });
   const int64_t n = int64_t(blocks.size());
+  if (n == 0) return {};
   if (n > int64_t(kRounds) * slots) return in_chunks(blocks, 1, INT64_MAX / 2).list;
   int64_t total = 0;
   for (const Block& b : blocks) total += b.stages;
@@ -165,13 +168,21 @@ static void plan(const int32_t* new_lens, const int32_t* ctx_lens, int batch, in
     const int n_new = new_lens[b.seq];
     const bool whole = k.stages == b.stages;
     items.push_back({tok0[b.seq], n_new, ctx_lens[b.seq], b.seq, b.row0, b.stage0 + k.stage0, k.stages,
-                     whole ? -1 : (*partials)++});
-    if (whole) continue;
-    if (k.stage0 == 0) {
-      merges.push_back({tok0[b.seq], n_new, b.row0, *partials - 1, 0, {0, 0, 0}});
-      *merge_rows = std::max(*merge_rows, std::min(kPackedRows, n_new * g - b.row0));
+                     whole ? -1 : (*partials)++, 0, 0, {0, 0}});
+    if (whole || k.stage0 + k.stages < b.stages) continue;
+    // the block's last piece: its first is as many items back
+    size_t first = i;
+    while (list[first].stage0 > 0) --first;
+    const int count = int(i - first) + 1, slot = *partials - count;
+    if (b.rows <= kPackedLastRows && count <= kPackedLastRanges) {
+      for (size_t j = first; j <= i; ++j) {
+        items[j].first = slot;
+        items[j].count = count;
+      }
+      continue;
     }
-    ++merges.back().count;
+    merges.push_back({tok0[b.seq], n_new, b.row0, slot, count, {0, 0, 0}});
+    *merge_rows = std::max(*merge_rows, b.rows);
   }
 }
 

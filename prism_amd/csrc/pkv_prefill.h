@@ -70,6 +70,8 @@ __device__ __forceinline__ void wait_vm() {
   __builtin_amdgcn_s_waitcnt((LGKM ? 0x0070 : 0x0F70) | (N & 15) | ((N >> 4) << 14));
 }
 
+constexpr int kCoherentAccess = 16;  // cache policy sc1: memory that every XCD sees
+
 // The larger of the lane's scores (never NaN unless the inputs are, and then the row is NaN anyway).
 __device__ __forceinline__ float max2(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
@@ -164,8 +166,119 @@ __device__ __forceinline__ float finish_row(const AttnParams& p, int hq, float m
     l_true = l_true * keep + term;
     m = top;
   }
-  lse = l_true > 0.f ? (m + __builtin_amdgcn_logf(l_true)) * 0.6931471805599453f : -INFINITY;
-  return l > 0.f ? keep / l : 0.f;
+  lse = l_true == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l_true)) * 0.6931471805599453f;
+  return l == 0.f ? 0.f : keep / l;
+}
+
+// One range's partial of a packed block, rows of slot_row on: O, and (m, l, l before rounding) in 16 bytes.  POLICY:
+// the cache policy of the stores (device-coherent where another workgroup of the launch reads them).
+template <int HD, int POLICY>
+__device__ __forceinline__ void store_partial(const AttnParams& p, int64_t slot_row, int r, int hi, bool real,
+                                              const f32x16 (&o)[HD / 32], float m, float l, float l_true) {
+  const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(p.ws_o + slot_row * HD, 0, kRows * HD * 4, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rm = __builtin_amdgcn_make_buffer_rsrc(p.ws_ml + slot_row * 4, 0, kRows * 16, 0x00020000);
+  if (!real) return;
+#pragma unroll
+  for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 v = {o[dt][4 * q], o[dt][4 * q + 1], o[dt][4 * q + 2], o[dt][4 * q + 3]};
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), ro, ((r * HD) + 32 * dt + 8 * q + 4 * hi) * 4, 0,
+                                             POLICY);
+    }
+  if (hi == 0)
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{m, l, l_true, 0.f}), rm, r * 16, 0, POLICY);
+}
+
+// The merge of a packed block of one wave's rows by the last of its ranges to end, in place of a launch (9 us a call
+// where 20 decode tokens of 47 are cut).  Every range stores its partial, then the call's tag at its slot, then
+// reads the block's tags: each store is waited for before what follows it, and all of them go to and come from
+// memory that every XCD sees (sc1), so whichever range stores its tag last sees them all.  Two that see them all
+// both merge, to the same bits.  Tags are 64 bits that no other call has: what the workspace held before does not
+// matter, and the merge clears them for a replay of the same call.  Nothing waits for another workgroup.
+template <int HD>
+__device__ __forceinline__ void merge_last(const AttnParams& p, int h, int slot, int first, int count, int blk_row0,
+                                           int n_rows, int tok0) {
+  const int lane = threadIdx.x & 63;
+  uint64_t* tags = p.tags + h;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if (lane == 0) __hip_atomic_store(tags + int64_t(slot) * p.n_kv, p.tag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  uint64_t seen = p.tag;
+  if (lane < count)
+    seen = __hip_atomic_load(tags + int64_t(first + lane) * p.n_kv, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (!__all(seen == p.tag)) return;
+  asm volatile("" ::: "memory");
+  // Eight rows and eight ranges at a time.  Lane 8 k + r has the statistics of row r in range k of the eight (and, of
+  // what is merged so far, those of its row r); the output's lanes hold 16 bytes of a row, HD / 32 of them.
+  constexpr int TPR = HD / 4, NC = HD / 32;
+  const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(p.ws_o, 0, 0x7fffffff, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rm = __builtin_amdgcn_make_buffer_rsrc(p.ws_ml, 0, 0x7fffffff, 0x00020000);
+  const int row_step = p.n_kv * kRows;
+  const int base = (first * p.n_kv + h) * kRows;
+#pragma nounroll
+  for (int g0 = 0; g0 < n_rows; g0 += 8) {
+    float m = -INFINITY, l = 0.f, l_true = 0.f;
+    f32x4 acc[NC];
+#pragma unroll
+    for (int j = 0; j < NC; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma nounroll
+    for (int s = 0; s < count; s += 8) {
+      const int mine = s + (lane >> 3);
+      const f32x4 ml = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+          rm, (base + min(mine, count - 1) * row_step + g0 + (lane & 7)) * 16, 0, kCoherentAccess));
+      f32x4 v[8][NC];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+          v[k][j] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+              ro, ((base + min(s + k, count - 1) * row_step + g0 + lane / TPR + j * (64 / TPR)) * HD + (lane % TPR) * 4) * 4, 0,
+              kCoherentAccess));
+      // a range of which the row sees no key has l = 0 and m = -inf (a NaN is kept); ranges past the last count for
+      // nothing
+      const bool some = mine < count && ml[1] != 0.f;
+      float m_new = fmaxf(m, some ? ml[0] : -INFINITY);
+#pragma unroll
+      for (int off = 8; off < 64; off <<= 1) m_new = fmaxf(m_new, __shfl_xor(m_new, off, 64));
+      const float keep = m_new == -INFINITY ? 1.f : fast_exp2(m - m_new);
+      const float w = some ? fast_exp2(ml[0] - m_new) : 0.f;
+      float dl = some ? w * ml[1] : 0.f, dt = some ? w * ml[2] : 0.f;
+#pragma unroll
+      for (int off = 8; off < 64; off <<= 1) {
+        dl += __shfl_xor(dl, off, 64);
+        dt += __shfl_xor(dt, off, 64);
+      }
+      l = l * keep + dl;
+      l_true = l_true * keep + dt;
+      m = m_new;
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        const int in_group = lane / TPR + j * (64 / TPR);
+        acc[j] *= __shfl(keep, in_group, 64);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float wt = __shfl(w, 8 * k + in_group, 64);
+          if (s + k < count) acc[j] += wt * v[k][j];
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const int in_group = lane / TPR + j * (64 / TPR), r = g0 + in_group;
+      const float mj = __shfl(m, in_group, 64), lj = __shfl(l, in_group, 64), tj = __shfl(l_true, in_group, 64);
+      if (r < n_rows) {
+        const int row = blk_row0 + r, jq = row / p.g, hq = h * p.g + row - jq * p.g, d = (lane % TPR) * 4;
+        float lse;
+        const float scale = finish_row(p, hq, mj, lj, tj, lse);
+        if (p.lse && d == 0) p.lse[int64_t(tok0 + jq) * (p.n_kv * p.g) + hq] = lse;
+        *reinterpret_cast<u32x2*>(p.out + (tok0 + jq) * p.o_ss + hq * p.o_sh + d) =
+            u32x2{pack_bf16x2(acc[j][0] * scale, acc[j][1] * scale), pack_bf16x2(acc[j][2] * scale, acc[j][3] * scale)};
+      }
+    }
+  }
+  if (lane < count)
+    __hip_atomic_store(tags + int64_t(first + lane) * p.n_kv, uint64_t(0), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // Verify's ranges.  The stages of all sequences, sequence after sequence, are cut into ranges of one
@@ -808,11 +921,26 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
     if (__any(ovf) && lane == 0) flag_status(p.status, PKV_STATUS_PARTIAL_RANGE);
     return;
   }
-  if constexpr (DEST == pf::kSplit || PACKED) {
-    if (PACKED ? split >= 0 : count > 1) {
+  if constexpr (PACKED) {
+    if (split >= 0) {
+      // (read again: kept, these would hold registers through the loop)
+      const PackedItem* item = p.items + int(blockIdx.x) / p.n_kv;
+      const int ranges = item->count;
+      const int64_t slot = (int64_t(split) * p.n_kv + h) * kRows;
+      if (ranges > 0) {
+        pf::store_partial<HD, pf::kCoherentAccess>(p, slot, lo.r - blk_row0, hi, lo.real, o, m_run, lsum, lsum_true);
+        pf::merge_last<HD>(p, h, split, item->first, ranges, blk_row0, min(R_all - blk_row0, kPackedLastRows), tok0);
+      } else {
+        pf::store_partial<HD, 0>(p, slot, lo.r - blk_row0, hi, lo.real, o, m_run, lsum, lsum_true);
+      }
+      return;
+    }
+  }
+  if constexpr (DEST == pf::kSplit) {
+    if (count > 1) {
       if (lo.real) {
-        int64_t slot = PACKED ? int64_t(split) * p.n_kv + h : int64_t(blockIdx.x);
-        if constexpr (W == pf::kWaves && !PACKED)
+        int64_t slot = int64_t(blockIdx.x);
+        if constexpr (W == pf::kWaves)
           slot = int64_t((b * p.n_kv + h) * (int(gridDim.x) / p.max_splits) + xblk) * p.max_splits + split;
         const int64_t wrow = slot * kRows + lo.r - blk_row0;
         float* dst = p.ws_o + wrow * HD + 4 * hi;
@@ -822,11 +950,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
           for (int q = 0; q < 4; ++q)
             *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * q) =
                 f32x4{o[dt][4 * q], o[dt][4 * q + 1], o[dt][4 * q + 2], o[dt][4 * q + 3]};
-        if constexpr (PACKED) {
-          if (hi == 0) *reinterpret_cast<f32x4*>(p.ws_ml + 4 * wrow) = f32x4{m_run, lsum, lsum_true, 0.f};
-        } else {
-          if (hi == 0) *reinterpret_cast<f32x2*>(p.ws_ml + 2 * wrow) = f32x2{m_run, lsum};
-        }
+        if (hi == 0) *reinterpret_cast<f32x2*>(p.ws_ml + 2 * wrow) = f32x2{m_run, lsum};
       }
       return;
     }
@@ -944,8 +1068,8 @@ __global__ __launch_bounds__(256) void packed_merge_kernel(const AttnParams p) {
     o *= keep;
 #pragma unroll
     for (int k = 0; k < B; ++k) {
-      // a range of which the row sees no key has l = 0 and m = -inf
-      const float wt = s0 + k < mg.count && pm[k][1] > 0.f ? fast_exp2(pm[k][0] - m_new) : 0.f;
+      // a range of which the row sees no key has l = 0 and m = -inf (a NaN is kept)
+      const float wt = s0 + k < mg.count && pm[k][1] != 0.f ? fast_exp2(pm[k][0] - m_new) : 0.f;
       l += wt * pm[k][1];
       l_true += wt * pm[k][2];
       o += wt * po[k];

@@ -143,7 +143,7 @@ class PackedBatch:
         g = self.n_heads // self.n_kv
         room = self.total_tokens * g // 128 + self.batch + 4 * max(2 * cus // self.n_kv, 1)
         while True:
-            items, merges = np.empty((room, 8), np.int32), np.empty((room, 8), np.int32)
+            items, merges = np.empty((room, 12), np.int32), np.empty((room, 8), np.int32)
             rc = lib.pkv_packed_plan(*sizes, items.ctypes.data, room, merges.ctypes.data, room, counts.ctypes.data)
             if rc != _lib.PKV_ENOSPC:
                 break

@@ -342,3 +342,60 @@ def test_many_ranges_of_one_block(gpu, nh, nk, hd, P):
     for w in (None, 7000):
         out, lse = prism_amd.packed_attention(q.to(gpu), kc.to(gpu), vc.to(gpu), batch, window=w, return_lse=True)
         _check(out, lse, op.packed_attention64(q, kc, vc, new, ctx, bt, window=w), 20001, f"window {w}")
+
+
+@pytest.mark.parametrize("new,ctx", [([1, 1], [5000, 40]), ([300, 1], [900, 2]), ([40, 6], [3000, 2900])])
+def test_nan_stays_where_it_is_seen(gpu, new, ctx):
+    """A NaN query spoils its head's row, a NaN key the rows that see it, whatever the ranges; nothing else."""
+    batch, bt, kc, vc, q = _case(gpu, new, ctx, 64, 14, 2, 64, seed=6)
+    clean, clean_lse = prism_amd.packed_attention(q.to(gpu), kc.to(gpu), vc.to(gpu), batch, return_lse=True)
+    bad_q = q.clone()
+    bad_q[0, 5, 9] = float("nan")
+    out, lse = prism_amd.packed_attention(bad_q.to(gpu), kc.to(gpu), vc.to(gpu), batch, return_lse=True)
+    hit = torch.zeros(out.shape[:2], dtype=torch.bool, device=gpu)
+    hit[0, 5] = True
+    assert torch.isnan(out[hit]).all() and torch.isnan(lse[hit]).all()
+    assert torch.equal(out[~hit], clean[~hit]) and torch.equal(lse[~hit], clean_lse[~hit])
+    # key t of sequence 0, KV head 1: seen from position t on, by the second half of the heads
+    for t in (3, ctx[0], ctx[0] + new[0] - 1):
+        bad_k = kc.clone()
+        bad_k[int(bt[0, t // 64]), t % 64, 1, 17] = float("nan")
+        out, lse = prism_amd.packed_attention(q.to(gpu), bad_k.to(gpu), vc.to(gpu), batch, return_lse=True)
+        hit = torch.zeros(out.shape[:2], dtype=torch.bool, device=gpu)
+        hit[max(t - ctx[0], 0):new[0], 7:] = True
+        assert torch.isnan(out[hit]).all() and torch.isnan(lse[hit]).all(), t
+        assert torch.equal(out[~hit], clean[~hit]) and torch.equal(lse[~hit], clean_lse[~hit]), t
+
+
+def test_ranges_merge_in_the_launch_and_behind_it(gpu):
+    """Row blocks of 1 to 128 rows around the 32 that one wave holds, one to 70 ranges, replayed: the merge's two ways
+    and its tags."""
+    new, ctx = [1, 2, 4, 5, 18, 19, 1], [30000, 4000, 4000, 4000, 4000, 4000, 300]
+    batch, bt, kc, vc, q = _case(gpu, new, ctx, 256, 28, 4, 128, seed=12)
+    dk, dv, dq = kc.to(gpu), vc.to(gpu), q.to(gpu)
+    sinks = torch.randn(28, generator=torch.Generator().manual_seed(2))
+    want = op.packed_attention64(q, kc, vc, new, ctx, bt, sinks=sinks)
+    graph = torch.cuda.CUDAGraph()
+    first = prism_amd.packed_attention(dq, dk, dv, batch, sinks=sinks.to(gpu), return_lse=True)
+    sk = sinks.to(gpu)
+    with torch.cuda.graph(graph):
+        out, lse = prism_amd.packed_attention(dq, dk, dv, batch, sinks=sk, return_lse=True)
+    for i in range(20):
+        out.zero_()
+        lse.zero_()
+        graph.replay()
+        if i % 5 == 0:
+            torch.cuda.synchronize()
+            eager = prism_amd.packed_attention(dq, dk, dv, batch, sinks=sk, return_lse=True)
+            assert torch.equal(eager[0], out) and torch.equal(eager[1], lse), i
+    assert torch.equal(first[0], out) and torch.equal(first[1], lse)
+    _check(out, lse, want, 30001, "merged")
+
+
+def test_one_sequence_in_more_than_64_ranges(gpu):
+    """One row block on a card of its own: its ranges are more than a wave's lanes, and merge in a launch behind."""
+    new, ctx = [1], [70000]
+    batch, bt, kc, vc, q = _case(gpu, new, ctx, 256, 7, 1, 128, seed=13)
+    assert batch._plans[None][4] == 1 and batch._plans[None][5] > 64
+    out, lse = prism_amd.packed_attention(q.to(gpu), kc.to(gpu), vc.to(gpu), batch, return_lse=True)
+    _check(out, lse, op.packed_attention64(q, kc, vc, new, ctx, bt), 70001, "many ranges")

@@ -19,7 +19,7 @@ def _plan(new, ctx, nh, nk, hd, window=0, cus=256):
     counts = np.zeros(4, np.int32)
     args = (new.ctypes.data, ctx.ctypes.data, len(new), nh, nk, hd, window, cus)
     assert lib.pkv_packed_plan(*args, 0, 0, 0, 0, counts.ctypes.data) == 0
-    items, merges = np.zeros((counts[0], 8), np.int32), np.zeros((max(counts[1], 1), 8), np.int32)
+    items, merges = np.zeros((counts[0], 12), np.int32), np.zeros((max(counts[1], 1), 8), np.int32)
     assert lib.pkv_packed_plan(*args, items.ctypes.data, counts[0], merges.ctypes.data, counts[1], counts.ctypes.data) == 0
     return items, merges[:counts[1]], counts
 
@@ -37,7 +37,9 @@ def test_plan_covers_every_visible_key_once(nh, nk, hd, window, cus):
         g, tok = nh // nk, 32 if hd == 128 else 64
         tok0 = np.cumsum(new) - new
         stages, slots = {}, []
-        for t0, s, c, b, row0, st0, ns, slot in items.tolist():
+        marks = {}
+        for t0, s, c, b, row0, st0, ns, slot, first, count, *_ in items.tolist():
+            marks.setdefault((b, row0), set()).add((first, count))
             assert (t0, s, c) == (tok0[b], new[b], ctx[b]) and s > 0 and ns > 0 and row0 % 128 == 0 and row0 < s * g
             stages.setdefault((b, row0), []).append((st0, ns, slot))
             if slot >= 0:
@@ -53,7 +55,17 @@ def test_plan_covers_every_visible_key_once(nh, nk, hd, window, cus):
                 assert st0 == at and (slot >= 0) == (len(parts) > 1)
                 at += ns
             assert at == last // tok + 1
-        split = {k: v for k, v in stages.items() if len(v) > 1}
+        split = {}
+        for (b, row0), parts in stages.items():
+            rows = min(128, new[b] * g - row0)
+            if len(parts) == 1:
+                assert marks[b, row0] == {(0, 0)}
+            elif rows <= 32 and len(parts) <= 64:   # merged by the last range to end
+                ((first, count),) = marks[b, row0]
+                assert sorted(p[2] for p in parts) == list(range(first, first + count))
+            else:
+                assert marks[b, row0] == {(0, 0)}
+                split[b, row0] = parts
         assert len(merges) == len(split)
         for t0, s, row0, slot, count, *_ in merges.tolist():
             (b,) = [b for b in range(n) if tok0[b] == t0 and new[b] == s and (b, row0) in split]
@@ -90,7 +102,7 @@ def test_plan_refusals():
                 dict(cus=0), dict(batch=-1), dict(counts=0), dict(new=None), dict(new=big, ctx=np.zeros(1, np.int32), nh=64)]:
         assert call(**bad) == _lib.PKV_EINVAL, bad
         assert "pkv_packed_plan" in lib.pkv_last_error().decode()
-    room = np.zeros(8, np.int32)
+    room = np.zeros(12, np.int32)
     assert call(items=room.ctypes.data, mi=0) == _lib.PKV_ENOSPC
 
 
@@ -337,7 +349,7 @@ def test_attention_argument_errors(over, msg):
 def test_attention_workspace():
     lib = _lib.load()
     need = lib.pkv_packed_workspace_bytes(2, 4, 128)
-    assert need == 2 * 4 * 128 * 132 * 4
+    assert need == 2 * 4 * (128 * 132 * 4 + 8)
     assert lib.pkv_packed_workspace_bytes(0, 4, 128) == 0
     assert _attn(lib, wsb=need - 1) == _lib.PKV_ENOSPC
     assert _attn(lib, n_items=0, items=0, ws=0) == 0
