@@ -345,6 +345,14 @@ int pkv_rope_qk(const void* qkv, int64_t qkv_sb, int64_t qkv_ss, const int32_t* 
                 int32_t* status, void* stream);
 
 /*
+ * Tables of pkv_rotate_qk and pkv_packed_rope_append: cos_tab, sin_tab (device, fp32 [n_pos, half]) entry (t, i) =
+ * gain * cos, sin (t * freq[i]), the angle in 64 bits (in 32, position 100,000 is off by 0.004 rad), rounded once.
+ * freq_gain is host memory: the half frequencies, then gain.  Generalises engine/executor.py:45-57 (_build_rope: fp32 angles, 4096 positions).
+ */
+int pkv_rotary_tables(const double* freq_gain, int32_t half, int64_t n_pos, float* cos_tab, float* sin_tab,
+                      void* stream);
+
+/*
  * Rotary positions in their general form, on tensors of tokens (batch and sequence in one axis): optional RMSNorm
  * of every head, then the rotation.  For token t < tokens and every head x = q[t, h] (n_heads of them, q_norm_w)
  * and k[t, h] (n_kv, k_norm_w; n_kv = 0: q alone):

@@ -142,6 +142,7 @@ _SIGNATURES = {
         _I32, _I32, _I32,                # page_size, num_pages, max_blocks
         _P, _P,                          # status, stream
     ]),
+    "pkv_rotary_tables": (c_int32, [_P, _I32, _I64, _P, _P, _P]),
     "pkv_rotate_qk": (c_int32, [
         _P, _I64, _I64, _P, _I64, _I64,  # q, k + strides
         _P, _P, _P, _I32,                # positions, cos, sin, n_pos

@@ -258,6 +258,28 @@ __global__ __launch_bounds__(256) void rotary_any_kernel(const RotaryParams p) {
   }
 }
 
+// Entry (t, i) of the tables: cos and sin of t freq[i] in 64 bits, times gain, rounded once.
+constexpr int kTableFreqs = 128;  // frequencies of a launch: 1 KiB of its arguments
+struct TableParams {
+  double freq[kTableFreqs];
+  double gain;
+  float* cos_tab;
+  float* sin_tab;
+  int64_t entries;  // n_pos * count
+  int count, half;
+};
+__global__ __launch_bounds__(256) void rotary_tables_kernel(const TableParams p) {
+  const int64_t stride = int64_t(gridDim.x) * 256;
+  for (int64_t e = int64_t(blockIdx.x) * 256 + threadIdx.x; e < p.entries; e += stride) {
+    const int64_t t = e / p.count;
+    const int i = int(e - t * p.count);
+    double s, c;
+    sincos(double(t) * p.freq[i], &s, &c);
+    p.cos_tab[t * p.half + i] = float(c * p.gain);
+    p.sin_tab[t * p.half + i] = float(s * p.gain);
+  }
+}
+
 // Tokens go out in launches of fewer than 2^31 lanes, and pointers move on between them.
 template <typename T>
 static void launch_rotary(RotaryParams p, int64_t tokens, bool wide, hipStream_t stream) {
@@ -312,6 +334,31 @@ static int check_rotary(const char* fn, int64_t tokens, int n_heads, int n_kv, i
 static int lanes_log2(int head_dim, int size) { return ilog2((head_dim * size + 31) / 32); }
 
 }  // namespace pkv
+
+extern "C" int pkv_rotary_tables(const double* freq_gain, int32_t half, int64_t n_pos, float* cos_tab, float* sin_tab,
+                                 void* stream) {
+  using namespace pkv;
+  clear_error();
+  const char* fn = "pkv_rotary_tables";
+  if (half <= 0 || n_pos <= 0 || n_pos > 0x7fffffff)
+    return fail(PKV_EINVAL, "%s: bad sizes half=%d n_pos=%lld", fn, half, (long long)n_pos);
+  if (!freq_gain || !cos_tab || !sin_tab) return fail(PKV_EINVAL, "%s: null argument", fn);
+  if ((reinterpret_cast<uintptr_t>(cos_tab) | reinterpret_cast<uintptr_t>(sin_tab)) & 3u)
+    return fail(PKV_EINVAL, "%s: cos/sin tables not 4-byte aligned", fn);
+  for (int i0 = 0; i0 < half; i0 += kTableFreqs) {
+    TableParams p;
+    p.count = half - i0 < kTableFreqs ? half - i0 : kTableFreqs;
+    for (int i = 0; i < kTableFreqs; ++i) p.freq[i] = i < p.count ? freq_gain[i0 + i] : 0.0;
+    p.gain = freq_gain[half];
+    p.cos_tab = cos_tab + i0;
+    p.sin_tab = sin_tab + i0;
+    p.entries = n_pos * p.count;
+    p.half = half;
+    const int64_t blocks = (p.entries + 255) / 256;
+    rotary_tables_kernel<<<unsigned(blocks < 16384 ? blocks : 16384), 256, 0, static_cast<hipStream_t>(stream)>>>(p);
+  }
+  return check_launch(fn);
+}
 
 extern "C" int pkv_rotate_qk(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
                              const int32_t* positions, const float* cos_tab, const float* sin_tab, int32_t n_pos,

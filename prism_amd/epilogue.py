@@ -17,6 +17,7 @@ Every call is asynchronous on the current stream and has no CPU fallback.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -181,8 +182,8 @@ def rotary_tables(rotary_dim: int, n_pos: int, theta: float = 10000.0, *, scalin
     sin are multiplied by (``gain``)."""
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim {rotary_dim} must be even and positive")
-    if n_pos <= 0:
-        raise ValueError(f"n_pos {n_pos} must be positive")
+    if not 0 < n_pos < 1 << 31:
+        raise ValueError(f"n_pos {n_pos} must be positive and below 2^31")
     if inv_freq is not None:
         if scaling is not None or tuple(inv_freq.shape) != (rotary_dim // 2,):
             raise ValueError(f"inv_freq must be [{rotary_dim // 2}], without scaling")
@@ -192,12 +193,18 @@ def rotary_tables(rotary_dim: int, n_pos: int, theta: float = 10000.0, *, scalin
             raise ValueError(f"theta {theta} must be above 1")
         freq, factor = _scaled_frequencies(rotary_dim, n_pos, theta, scaling)
         gain = gain * factor
-    freq = freq.to(device)
+    device = torch.device(device)
     cos = torch.empty((n_pos, rotary_dim // 2), dtype=torch.float32, device=device)
     sin = torch.empty_like(cos)
+    if device.type == "cuda":
+        freq_gain = (ctypes.c_double * (rotary_dim // 2 + 1))(*freq.tolist(), float(gain))
+        with _on(cos.device):
+            _lib.check(_lib.load().pkv_rotary_tables(ctypes.addressof(freq_gain), rotary_dim // 2, n_pos, cos.data_ptr(),
+                                                     sin.data_ptr(), _raw_stream(cos.device.index)), "pkv_rotary_tables")
+        return cos, sin
     for t0 in range(0, n_pos, 1 << 16):   # 64-bit intermediates of at most 2^16 positions
         t1 = min(t0 + (1 << 16), n_pos)
-        angle = torch.outer(torch.arange(t0, t1, dtype=torch.float64, device=device), freq)
+        angle = torch.outer(torch.arange(t0, t1, dtype=torch.float64), freq.cpu())
         cos[t0:t1] = angle.cos() * gain
         sin[t0:t1] = angle.sin() * gain
     return cos, sin

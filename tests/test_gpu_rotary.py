@@ -33,6 +33,24 @@ def _tables(gpu, rd, n_pos, theta=1e4, scaling=None):
     return freq, gain, cos, sin
 
 
+@pytest.mark.parametrize("rd,n_pos,theta,scaling", [
+    (128, 131072, 1e6, None), (2, 1, 1e4, None), (6, 77, 1e4, dict(rope_type="linear", factor=3.0)), (1024, 900, 5e5, None),
+    (64, 40000, 1e4, dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=8192)),
+])
+def test_rotary_tables_on_the_device(gpu, rd, n_pos, theta, scaling):
+    """fp64 angles; cos and sin of the device's and the host's libraries are each within a few 2^-53 of the truth, and
+    the rounding to fp32 is half a step of the value, 2^-24, of what is at most gain."""
+    freq, gain, cos, sin = _tables(gpu, rd, n_pos, theta, scaling)
+    angle = torch.arange(n_pos, dtype=torch.float64, device=gpu)[:, None] * freq.to(gpu)
+    for got, want in ((cos, angle.cos() * gain), (sin, angle.sin() * gain)):
+        assert got.shape == (n_pos, rd // 2) and got.dtype == torch.float32
+        assert (got.double() - want).abs().max() <= gain * (2.0 ** -24 + 2.0 ** -45)
+    f = torch.rand(rd // 2, generator=torch.Generator().manual_seed(1))
+    c, s = prism_amd.rotary_tables(rd, 5, inv_freq=f.to(gpu), gain=0.5, device=gpu)
+    a = torch.arange(5, dtype=torch.float64)[:, None] * f.double()
+    assert (c.cpu().double() - a.cos() / 2).abs().max() <= 2.0 ** -24 and (s.cpu().double() - a.sin() / 2).abs().max() <= 2.0 ** -24
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
 @pytest.mark.parametrize("inter", [False, True])
 @pytest.mark.parametrize("hd,rd", [(128, 128), (64, 64), (128, 32), (64, 16), (96, 96), (80, 48), (256, 64), (1024, 1024),

@@ -257,6 +257,15 @@ def test_rotary_tables_frequencies_and_refusals():
             prism_amd.rotary_tables(a.pop("rotary_dim"), a.pop("n_pos"), **a)
 
 
+def test_tables_argument_errors():
+    lib = _lib.load()
+    f = np.ones(4)
+    ok = dict(freq=f.ctypes.data, half=3, n_pos=3, cos=A16, sin=A16)
+    for bad in [dict(freq=0), dict(half=0), dict(n_pos=0), dict(n_pos=1 << 31), dict(cos=0), dict(sin=A16 + 2)]:
+        assert lib.pkv_rotary_tables(*{**ok, **bad}.values(), None) == _lib.PKV_EINVAL, bad
+        assert "pkv_rotary_tables" in lib.pkv_last_error().decode()
+
+
 def test_oracle_rotation_gradient():
     """The rotation is linear in the head: its gradient is the rotation by the opposite angle."""
     g = torch.Generator().manual_seed(0)
