@@ -430,7 +430,8 @@ size_t pkv_packed_workspace_bytes(int32_t partials, int32_t n_kv, int32_t head_d
  * out = sum_t exp(s_t) v_t / (sum_t exp(s_t) + exp(sinks[h])), s = softmax_scale q . k; sinks (fp32 [n_heads])
  * NULL: without that term.  lse (fp32 [tokens, n_heads], NULL: not wanted): the logarithm of the denominator.
  * items, merges (device memory, 16-byte aligned) and the counts come from pkv_packed_plan for the same lengths,
- * heads and window; the lengths are in them, and the block table needs ceil((ctx + new) / page_size) columns of
+ * heads and window (items that do not fit tokens, batch and partials are skipped and flag PKV_STATUS_BAD_PAGE); the
+ * lengths are in them, and the block table needs ceil((ctx + new) / page_size) columns of
  * each sequence (with a window, only those that hold a visible key are read).  Rows of out from `tokens` on are
  * not written.  Values of masked keys take part in the products with weight 0: a NaN or infinity in a V row that
  * belongs to the sequence reaches rows of the same 32 (head_dim 64: 64) keys that do not see it; what lies behind

@@ -3704,6 +3704,8 @@ extern "C" int pkv_packed_attn(const void* q, int64_t q_st, int64_t q_sh, const 
   p.lse = lse;
   p.tokens = tokens;
   p.window = window;
+  p.batch = batch;
+  p.max_splits = partials;
   if (need > 0) {
     p.ws_o = static_cast<float*>(workspace);
     p.ws_ml = p.ws_o + size_t(partials) * n_kv * kPackedRows * head_dim;

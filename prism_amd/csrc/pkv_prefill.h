@@ -370,6 +370,12 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
     const int it = i / p.n_kv;
     h = i - it * p.n_kv;
     const PackedItem item = p.items[it];
+    // a list of another batch: nothing outside this call's tensors is touched
+    if (unsigned(item.seq) >= unsigned(p.batch) || item.tok0 < 0 || item.n_new <= 0 || item.n_new > p.tokens - item.tok0 ||
+        item.ctx < 0 || item.row0 < 0 || item.stage0 < 0 || item.stages <= 0 || item.slot >= p.max_splits) {
+      if (threadIdx.x == 0) flag_status(p.status, PKV_STATUS_BAD_PAGE);
+      return;
+    }
     b = item.seq;
     c = item.ctx;
     L = c + item.n_new;

@@ -175,6 +175,24 @@ def test_a_page_that_goes_bad_is_flagged(gpu):
         assert read_status(gpu) == prism_amd._lib.PKV_STATUS_BAD_PAGE
 
 
+def test_a_list_of_another_batch_is_flagged(gpu):
+    """The C entry with the work list of a larger batch: rows outside the call's tensors are not touched."""
+    big, bt, kc, vc, q = _case(gpu, [5, 60, 1], [10, 0, 30], 64, 14, 2, 64, seed=2)
+    dq, dk, dv = q.to(gpu), kc.to(gpu), vc.to(gpu)
+    lib, st = prism_amd._lib.load(), prism_amd.attention.status_tensor(gpu)
+    window, items, n_items, merges, n_merges, partials, merge_rows = big._plans[None]
+    assert partials == 0
+    want = prism_amd.packed_attention(dq, dk, dv, big)
+    for tokens, batch in ((65, 3), (66, 2)):     # the last sequence's token, or its block-table row, is not there
+        out = torch.full((66, 14, 64), 3.0, dtype=BF16, device=gpu)
+        rc = lib.pkv_packed_attn(dq.data_ptr(), 14 * 64, 64, dk.data_ptr(), dv.data_ptr(), dk.stride(0), big.block_table.data_ptr(),
+                                 big.max_blocks, out.data_ptr(), 14 * 64, 64, 0, 0, items, n_items, merges, n_merges, partials,
+                                 merge_rows, 0, 0, tokens, batch, 14, 2, 64, 64, big.num_pages, big.max_blocks, 0, 0.125,
+                                 st.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and read_status(gpu) == prism_amd._lib.PKV_STATUS_BAD_PAGE
+        assert torch.equal(out[:65], want[:65]) and (out[65] == 3.0).all()
+
+
 def test_refusals(gpu):
     batch, bt, kc, vc, q = _case(gpu, [3], [4], 16, 4, 2, 64, seed=2)
     q, kc, vc = q.to(gpu), kc.to(gpu), vc.to(gpu)
