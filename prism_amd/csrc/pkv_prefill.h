@@ -281,6 +281,90 @@ __device__ __forceinline__ void merge_last(const AttnParams& p, int h, int slot,
     __hip_atomic_store(tags + int64_t(first + lane) * p.n_kv, uint64_t(0), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// A packed block of at most 16 rows (decode tokens) without a window: its range's 32-token tiles go round the four
+// waves, each with tiles of its own in registers, and the waves' results meet in LDS.  The walk below would give the
+// rows to one wave of the four.  P is a bf16 pair, as elsewhere in decode: the rows' errors are their outputs'
+// rounding alone.
+constexpr int kFewRows = 16;
+template <int HD>
+__device__ __forceinline__ void few_rows(const AttnParams& p, const PackedItem& item, int h, char* lds) {
+  constexpr int KK = HD / 32, DPL = HD / 16, TOK = Geo<HD>::TOK, CPR = HD / 4;
+  struct Shared {
+    float o[kWaves][kFewRows][HD + 4], m[kWaves][kFewRows], l[kWaves][kFewRows];
+  };
+  static_assert(sizeof(Shared) <= 8 * Geo<HD>::STAGE, "the tile walk's rings hold it");
+  Shared& sm = *reinterpret_cast<Shared*>(lds);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int li = lane & 15, lq = lane >> 4;
+  const int n_rows = min(item.n_new * p.g - item.row0, kFewRows);
+  SeqView sv;
+  sv.b = item.seq;
+  sv.h = h;
+  sv.c = item.ctx;
+  sv.t_end = min((item.stage0 + item.stages) * TOK, item.ctx + item.n_new);
+  sv.bt = p.block_table + int64_t(item.seq) * p.bt_stride;
+  bf16x8 qf[1][KK];
+  int lim[1] = {kNoQueryRow};
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) qf[0][kk] = __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
+  if (li < n_rows) {
+    const int row = item.row0 + li, j = row / p.g;
+    const uint16_t* src = p.q + (item.tok0 + j) * p.q_ss + (h * p.g + row - j * p.g) * p.q_sh + 8 * lq;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) qf[0][kk] = __builtin_bit_cast(bf16x8, ld16(src + 32 * kk));
+    lim[0] = min(item.ctx + j, sv.t_end - 1);
+  }
+  float m_run[1] = {-INFINITY}, l_run[1] = {0.f};
+  f32x4 acc[1][DPL];
+#pragma unroll
+  for (int n = 0; n < DPL; ++n) acc[0][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  wave_attend<HD, 1, true, 2>(p, sv, qf, lim, item.stage0 * TOK + 32 * wave, sv.t_end, 32 * kWaves, m_run, l_run, acc);
+  const float l_wave = sum_over_quads(l_run[0]);
+  if (lq == 0) {
+    sm.m[wave][li] = m_run[0];
+    sm.l[wave][li] = l_wave;
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int n = 0; n < DPL; ++n) sm.o[wave][li][DPL * (4 * lq + r) + n] = acc[0][n][r];
+  __syncthreads();
+  const int64_t slot_row = (int64_t(item.slot) * p.n_kv + h) * kRows;
+  for (int i = threadIdx.x; i < n_rows * CPR; i += 64 * kWaves) {
+    const int r = i / CPR, d = (i - r * CPR) * 4;
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, sm.m[w][r]);
+    const float m_use = m == -INFINITY ? 0.f : m;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = fast_exp2(sm.m[w][r] - m_use);
+      l += f * sm.l[w][r];
+      o += f * *reinterpret_cast<const f32x4*>(&sm.o[w][r][d]);
+    }
+    if (item.slot >= 0) {
+      const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(p.ws_o + slot_row * HD, 0, kRows * HD * 4, 0x00020000);
+      const __amdgpu_buffer_rsrc_t rm = __builtin_amdgcn_make_buffer_rsrc(p.ws_ml + slot_row * 4, 0, kRows * 16, 0x00020000);
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), ro, (r * HD + d) * 4, 0, kCoherentAccess);
+      if (d == 0)
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{m, l, l, 0.f}), rm, r * 16, 0, kCoherentAccess);
+    } else {
+      const int row = item.row0 + r, j = row / p.g, hq = h * p.g + row - j * p.g;
+      float lse;
+      const float scale = finish_row(p, hq, m, l, l, lse);
+      if (p.lse && d == 0) p.lse[int64_t(item.tok0 + j) * (p.n_kv * p.g) + hq] = lse;
+      *reinterpret_cast<u32x2*>(p.out + (item.tok0 + j) * p.o_ss + hq * p.o_sh + d) =
+          u32x2{pack_bf16x2(o[0] * scale, o[1] * scale), pack_bf16x2(o[2] * scale, o[3] * scale)};
+    }
+  }
+  if (item.slot < 0 || item.count == 0) return;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every wave's share of the partial is stored
+  __syncthreads();
+  if (wave == 0) merge_last<HD>(p, h, item.slot, item.first, item.count, item.row0, n_rows, item.tok0);
+}
+
 // Verify's ranges.  The stages of all sequences, sequence after sequence, are cut into ranges of one
 // length (`chunk`: about lean_grid ranges for each KV head, at least kMinVerifyStages stages each: 4 to 6
 // are level), each inside
@@ -374,6 +458,10 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
     if (unsigned(item.seq) >= unsigned(p.batch) || item.tok0 < 0 || item.n_new <= 0 || item.n_new > p.tokens - item.tok0 ||
         item.ctx < 0 || item.row0 < 0 || item.stage0 < 0 || item.stages <= 0 || item.slot >= p.max_splits) {
       if (threadIdx.x == 0) flag_status(p.status, PKV_STATUS_BAD_PAGE);
+      return;
+    }
+    if (p.window == 0 && item.n_new * p.g - item.row0 <= pf::kFewRows) {
+      pf::few_rows<HD>(p, item, h, lds);
       return;
     }
     b = item.seq;
