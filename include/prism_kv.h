@@ -435,8 +435,9 @@ size_t pkv_packed_workspace_bytes(int32_t partials, int32_t n_kv, int32_t head_d
  * each sequence (with a window, only those that hold a visible key are read).  Rows of out from `tokens` on are
  * not written.  Values of masked keys take part in the products with weight 0: a NaN or infinity in a V row that
  * belongs to the sequence reaches rows of the same 32 (head_dim 64: 64) keys that do not see it; what lies behind
- * the sequence's last key does not matter.  bf16 in and out, fp32 softmax and sums, the probabilities rounded to
- * bf16 for the second product.  Replaces flash_attn_with_kvcache (engine/executor.py:119-120, :260-261) for
+ * the sequence's last key does not matter; an infinite V makes infinities or NaN of the rows that see it.  bf16 in
+ * and out, fp32 softmax and sums, the probabilities rounded to bf16 for the second product (a bf16 pair for blocks of
+ * at most 16 rows without a window).  Replaces flash_attn_with_kvcache (engine/executor.py:119-120, :260-261) for
  * batches whose sequences bring different numbers of tokens.
  */
 int pkv_packed_attn(const void* q, int64_t q_st, int64_t q_sh, const void* k_cache, const void* v_cache,
