@@ -12,7 +12,7 @@ namespace {
 
 // Costs in stages (of 16 KB of K and V).  A range's start and end take about five stages' time: loads of the item,
 // then of Q and pages, then of the first tiles, one behind the other.  Below six stages a piece is not worth that: one
-// decode token on 27 stages takes 8.8 us in pieces of 7, 11.0 in pieces of 9, 20.7 whole.
+// decode token on 27 stages takes 9.4 us a call in four pieces, 11.5 in two, 14.0 whole.
 constexpr int kRangeCost = 5;
 constexpr int kPartialCost = 8;  // of 128 rows: 66 KB each way
 constexpr int kMinRange = 6;
@@ -95,8 +95,7 @@ Schedule filled(const std::vector<Block>& blocks, int slots, int64_t target) {
 // reads as fast as the card does (5.8 TB/s: all CUs together 370 stages a us, 0.6 us each); two even out what the
 // blocks' lengths leave uneven (in between some CUs would have one and some two), at the price of more partials: 0.4
 // us per MB written and read, and 2.7 us and 0.1 per range of a block to merge them.  6 decode tokens and two chunks
-// on 40 k keys: 102 + 5 us in 59 pieces per KV head, 110 + 10 in 124; 47 decode tokens on 1500: 35 + 5 in 126
-// pieces, 41 + 5 in 77 (each with a launch that merges).
+// on 40 k keys: 112 us a call in 59 pieces per KV head, 124 in 124.
 Schedule even(const std::vector<Block>& blocks, int slots, int n_kv, int head_dim) {
   int64_t total = 0;
   for (const Block& b : blocks) total += b.stages;
@@ -132,9 +131,9 @@ Schedule even(const std::vector<Block>& blocks, int slots, int n_kv, int head_di
 // three rounds for one block too many), and few blocks leave the card idle.  Two ways to cut them: pieces of one
 // length that fit one round, and, where that schedule would end a tenth earlier, pieces that fill every slot up to an
 // even share of the work.  (Less than that is lost again: pieces that wait for a slot start into a card that reads
-// as fast as it can.)  us a launch, one length / filled: 47 decode tokens and two chunks (7B) 46 / 60; 208 short
-// chats (0.5B) 27 / 22, chunks in a window of 1024 (14B; whole blocks) 113 / 100.
-// Many rounds even out by themselves: above kRounds of them nothing is cut.
+// as fast as it can.)  us a call, uncut / one length / filled: 47 decode tokens and two chunks (7B) 111 / 56 / 70; 6
+// and two on 40 k keys 1063 / 112 / 137; 208 short chats (0.5B) 28 / 22 / 19; chunks in a window of 1024 (14B, more
+// blocks than slots) 107 / - / 97.  Many rounds even out by themselves: above kRounds of them nothing is cut.
 constexpr int kRounds = 8;
 std::vector<Piece> cut(std::vector<Block>& blocks, int slots, int n_kv, int head_dim) {
   std::stable_sort(blocks.begin(), blocks.end(), [](const Block& a, const Block& b) { return a.stages > b.stages; });

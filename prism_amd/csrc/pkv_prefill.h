@@ -190,8 +190,8 @@ __device__ __forceinline__ void store_partial(const AttnParams& p, int64_t slot_
     __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{m, l, l_true, 0.f}), rm, r * 16, 0, POLICY);
 }
 
-// The merge of a packed block of one wave's rows by the last of its ranges to end, in place of a launch (9 us a call
-// where 20 decode tokens of 47 are cut).  Every range stores its partial, then the call's tag at its slot, then
+// The merge of a packed block of one wave's rows by the last of its ranges to end, in place of a launch (208 short
+// chats 25.3 -> 22.8 us a call).  Every range stores its partial, then the call's tag at its slot, then
 // reads the block's tags: each store is waited for before what follows it, and all of them go to and come from
 // memory that every XCD sees (sc1), so whichever range stores its tag last sees them all.  Two that see them all
 // both merge, to the same bits.  Tags are 64 bits that no other call has: what the workspace held before does not
@@ -283,8 +283,10 @@ __device__ __forceinline__ void merge_last(const AttnParams& p, int h, int slot,
 
 // A packed block of at most 16 rows (decode tokens) without a window: its range's 32-token tiles go round the four
 // waves, each with tiles of its own in registers, and the waves' results meet in LDS.  The walk below would give the
-// rows to one wave of the four.  P is a bf16 pair, as elsewhere in decode: the rows' errors are their outputs'
-// rounding alone.
+// rows to one wave of the four: 208 short chats 23.2 -> 19.3 us a call, one token 11.5 -> 9.4, 30 tokens over pages of
+// 16 29.6 -> 25.4; ranges of 170 stages read 3% faster there (6 tokens and two chunks on 40 k keys 108 -> 112), for
+// which it is not kept.  P is a bf16 pair, as elsewhere in decode: the rows' errors are their outputs' rounding alone
+// (1.6e-3 of 64 bits, 2.3e-3 with P rounded once).
 constexpr int kFewRows = 16;
 template <int HD>
 __device__ __forceinline__ void few_rows(const AttnParams& p, const PackedItem& item, int h, char* lds) {
