@@ -13,6 +13,9 @@ Modules
                    from engine/kv_cache.py and engine/prefix_cache.py without tensors.
   epilogue         the elementwise steps around attention: rotary tables, QKV split + QK-norm +
                    RoPE, RMSNorm with the residual add, SiLU(gate) * up.
+  packed           the packed step: the rotation in general form (with each element's magnitudes, for
+                   tolerances) and attention with a length of its own for every sequence, a
+                   window, sinks and the log-sum-exp.
 
 How each function is pinned (tests/test_oracle.py; the epilogue in tests/test_epilogue_oracle.py):
   slot_mapping / append_kv     docs/architecture.md:140-147 worked example, hand-computed slots,
@@ -32,4 +35,9 @@ How each function is pinned (tests/test_oracle.py; the epilogue in tests/test_ep
   epilogue.rms_norm_f64        torch.nn.functional.rms_norm (fp64), constant rows (closed form),
                                scale invariance.
   epilogue.silu_mul_ref        torch.nn.functional.silu (fp64), silu(0) = 0 and the large-|g| limits.
+  packed.rotate64              epilogue.rope_f64 (half layout), its own half layout under the pairs'
+                               permutation (interleaved), torch's rms_norm, its gradient by differences
+                               (tests/test_packed_host.py, as the next).
+  packed.packed_attention64    attention_fp64 where every sequence brings the same tokens; row by row
+                               sums over the visible keys, sink term included.
 """

@@ -26,6 +26,8 @@
 #include <math.h>
 
 #include <atomic>
+#include <chrono>
+#include <exception>
 #include <mutex>
 #include <random>
 #include <type_traits>
@@ -3645,8 +3647,17 @@ extern "C" int pkv_prefill_attn(const void* q, int64_t q_sb, int64_t q_ss, int64
 namespace pkv {
 // 64 bits that no other call of this process has had, nor likely any memory by chance: a counter from a random start,
 // mixed (a bijection).  Never 0, which is a cleared tag.
+static uint64_t random_start() {
+  const uint64_t now = uint64_t(std::chrono::steady_clock::now().time_since_epoch().count());
+  try {
+    std::random_device d;
+    return now ^ (uint64_t(d()) << 32) ^ d();
+  } catch (const std::exception&) {  // no source of randomness: the clock and where the process was loaded
+    return now ^ uint64_t(reinterpret_cast<uintptr_t>(&random_start));
+  }
+}
 static uint64_t next_tag() {
-  static std::atomic<uint64_t> counter{(uint64_t(std::random_device{}()) << 32) | std::random_device{}()};
+  static std::atomic<uint64_t> counter{random_start()};
   for (;;) {
     uint64_t x = counter.fetch_add(1, std::memory_order_relaxed);
     x = (x ^ (x >> 30)) * 0xbf58476d1ce4e5b9ull;

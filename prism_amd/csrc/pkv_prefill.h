@@ -458,7 +458,8 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
     const PackedItem item = p.items[it];
     // a list of another batch: nothing outside this call's tensors is touched
     if (unsigned(item.seq) >= unsigned(p.batch) || item.tok0 < 0 || item.n_new <= 0 || item.n_new > p.tokens - item.tok0 ||
-        item.ctx < 0 || item.row0 < 0 || item.stage0 < 0 || item.stages <= 0 || item.slot >= p.max_splits) {
+        item.ctx < 0 || item.row0 < 0 || item.stage0 < 0 || item.stages <= 0 || item.slot >= p.max_splits ||
+        item.first < 0 || item.count < 0 || item.count > min(p.max_splits - item.first, kPackedLastRanges)) {
       if (threadIdx.x == 0) flag_status(p.status, PKV_STATUS_BAD_PAGE);
       return;
     }
@@ -1141,6 +1142,9 @@ template <int HD>
 __global__ __launch_bounds__(256) void packed_merge_kernel(const AttnParams p) {
   constexpr int TPR = HD / 4, RPW = 256 / TPR, B = 8;
   const PackedMerge mg = p.merges[blockIdx.z];
+  if (mg.tok0 < 0 || mg.n_new > p.tokens - mg.tok0 || mg.row0 < 0 || mg.slot < 0 || mg.count <= 0 ||
+      mg.count > p.max_splits - mg.slot)
+    return;  // a list of another batch, flagged by the items
   const int h = blockIdx.y;
   const int r = int(blockIdx.x) * RPW + int(threadIdx.x) / TPR;  // row in the block
   const int row = mg.row0 + r;

@@ -6,7 +6,9 @@ import pytest
 import torch
 
 import prism_amd
+from oracle import epilogue
 from oracle import packed as op
+from oracle import paged_attention as pa
 from prism_amd import _lib
 from prism_amd.kv_cache import FlashAttnKVCache
 
@@ -264,6 +266,46 @@ def test_tables_argument_errors():
     for bad in [dict(freq=0), dict(half=0), dict(n_pos=0), dict(n_pos=1 << 31), dict(cos=0), dict(sin=A16 + 2)]:
         assert lib.pkv_rotary_tables(*{**ok, **bad}.values(), None) == _lib.PKV_EINVAL, bad
         assert "pkv_rotary_tables" in lib.pkv_last_error().decode()
+
+
+def test_oracle_rotation_is_the_others():
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(5, 3, 64, generator=g, dtype=torch.float64)
+    pos = torch.tensor([0, 1, 77, 4095, 100000])
+    f = 1e4 ** (-torch.arange(0, 64, 2, dtype=torch.float64) / 64)
+    half, mag = op.rotate64(x, pos, f)
+    want = epilogue.rope_f64(x.numpy(), pos.numpy()[:, None], 64)
+    assert np.abs(half.numpy() - want).max() < 1e-9      # the angles of 100000 agree to 2^-53 of it
+    assert (mag >= half.abs() - 1e-12).all()
+    order = torch.arange(64).view(2, 32).t().flatten()   # pairs side by side
+    inter, _ = op.rotate64(x[..., order], pos, f, interleaved=True)
+    assert torch.equal(inter, half[..., order])
+    w = torch.rand(64, generator=g, dtype=torch.float64)
+    norm, _ = op.rotate64(x, torch.zeros(5), f, norm_w=w, eps=1e-3)
+    assert (norm - torch.nn.functional.rms_norm(x, (64,), w, 1e-3)).abs().max() < 1e-12
+    part, _ = op.rotate64(x, pos, f[:8])
+    assert torch.equal(part[..., 16:], x[..., 16:])
+
+
+def test_oracle_attention_is_the_other():
+    g = torch.Generator().manual_seed(4)
+    kc, vc = (torch.randn(9, 16, 2, 64, generator=g).to(torch.bfloat16) for _ in range(2))
+    q = torch.randn(3, 4, 6, 64, generator=g).to(torch.bfloat16)
+    ctx, bt = [20, 0, 33], torch.tensor([[3, 1, 8], [5, 0, 0], [2, 7, 4]])
+    out, lse, mag = op.packed_attention64(q.flatten(0, 1), kc, vc, [4] * 3, ctx, bt)
+    want = pa.attention_fp64(pa.bf16_bits(q), pa.bf16_bits(kc), pa.bf16_bits(vc), bt.numpy(), np.array(ctx) + 4, True)
+    assert np.abs(out.view(3, 4, 6, 64).numpy() - want).max() < 1e-12 and (mag >= out.abs() - 1e-12).all()
+    # row by row, with a window and sinks
+    sinks = torch.tensor([-1e30, 0.0, 3.0, 50.0, -2.0, 1.0])
+    out, lse, _ = op.packed_attention64(q.flatten(0, 1)[:7], kc, vc, [2, 0, 5], ctx, bt, window=6, sinks=sinks, scale=0.2)
+    for row, (b, p) in enumerate([(0, 20), (0, 21), (2, 33), (2, 34), (2, 35), (2, 36), (2, 37)]):
+        for h in range(6):
+            e, num = math.exp(sinks[h].double()), torch.zeros(64, dtype=torch.float64)
+            for t in range(max(p - 5, 0), p + 1):
+                page, r = int(bt[b, t // 16]), t % 16
+                x = math.exp(0.2 * float(q.flatten(0, 1)[row, h].double() @ kc[page, r, h // 3].double()))
+                e, num = e + x, num + x * vc[page, r, h // 3].double()
+            assert (out[row, h] - num / e).abs().max() < 1e-12 and abs(float(lse[row, h]) - math.log(e)) < 1e-12
 
 
 def test_oracle_rotation_gradient():
