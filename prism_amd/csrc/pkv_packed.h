@@ -6,6 +6,8 @@
 namespace pkv {
 
 constexpr int kPackedRows = 128;  // query rows (token x head of the group) of a work item
+// Blocks of at most so many rows, without a window, share their keys over the workgroup's four waves.
+constexpr int kPackedFewRows = 16;
 // Blocks of at most so many rows (one wave's) and ranges merge in the launch: the last range to end does it.
 constexpr int kPackedLastRows = 32, kPackedLastRanges = 64;
 

@@ -21,6 +21,7 @@ constexpr int kWorkgroupsPerCu = 2;
 struct Block {
   int seq, row0, stage0, stages;
   int rows;
+  bool few;  // its keys go round four waves
   // of each piece, where it is cut: its partial is written and read back
   int cut_cost() const { return (kPartialCost * rows + kPackedRows - 1) / kPackedRows; }
 };
@@ -34,7 +35,8 @@ std::vector<Block> row_blocks(const int32_t* new_lens, const int32_t* ctx_lens, 
     for (int r0 = 0; r0 < rows; r0 += kPackedRows) {
       const int last = ctx + (std::min(r0 + kPackedRows, rows) - 1) / g;
       const int first = window > 0 ? std::max(ctx + r0 / g - window + 1, 0) : 0;
-      blocks.push_back({b, r0, first / tok, last / tok + 1 - first / tok, std::min(kPackedRows, rows - r0)});
+      blocks.push_back({b, r0, first / tok, last / tok + 1 - first / tok, std::min(kPackedRows, rows - r0),
+                        window == 0 && rows - r0 <= kPackedFewRows});
     }
   }
   return blocks;
@@ -94,29 +96,32 @@ Schedule filled(const std::vector<Block>& blocks, int slots, int64_t target) {
 // Pieces of one length, for two workgroups per CU, for one or for fewer, whichever ends soonest.  One per CU already
 // reads as fast as the card does (5.8 TB/s: all CUs together 370 stages a us, 0.6 us each); two even out what the
 // blocks' lengths leave uneven (in between some CUs would have one and some two), at the price of more partials: 0.4
-// us per MB written and read, and 2.7 us and 0.1 per range of a block to merge them.  6 decode tokens and two chunks
-// on 40 k keys: 112 us a call in 59 pieces per KV head, 124 in 124.
+// us per MB written and read, and 2.7 us and 0.2 per range of a block to merge them (half of that at 64 a head).
+// Decode rows' stages take 0.3 us where few workgroups read, 0.45 at 128 of them.  us a call, two per CU always / so:
+// 6 decode tokens and two chunks on 40 k keys (7B) 124 / 112; one decode token on 20 k keys 24 / 19, 4 on 3000 each
+// 12.9 / 11.7, 8 on 500 each (not cut) 10.3 / 8.9; one KV head, two on 70 k each 37 / 28.
 Schedule even(const std::vector<Block>& blocks, int slots, int n_kv, int head_dim) {
   int64_t total = 0;
   for (const Block& b : blocks) total += b.stages;
   int64_t best_chunk = 0;
   double best = 0;
-  for (const int64_t room : {slots, slots / 2, slots / 4, slots / 8}) {
-    if (room < 1 || int64_t(blocks.size()) > room) continue;
+  for (int64_t room = slots; room > 0; room /= 2) {
+    if (int64_t(blocks.size()) > room) break;
     for (int64_t chunk = std::max<int64_t>((total + room - 1) / room, kMinRange);;
          chunk += std::max<int64_t>(chunk / 16, 1)) {
-      int64_t ranges = 0, longest = 0, rows = 0, most = 0;
+      int64_t ranges = 0, rows = 0, most = 0, longest_few = 0, longest = 0;
       for (const Block& b : blocks) {
         const int count = pieces(b.stages, chunk);
         ranges += count;
-        longest = std::max<int64_t>(longest, (b.stages + count - 1) / count);
+        int64_t& length = b.few ? longest_few : longest;
+        length = std::max<int64_t>(length, (b.stages + count - 1) / count);
         if (count > 1) rows += int64_t(count) * b.rows;
         most = std::max<int64_t>(most, count);
       }
       if (ranges > room) continue;
-      const double at_once = std::min(370.0, 2.0 * ranges * n_kv);
-      const double us = std::max(total * n_kv / at_once, 0.58 * longest) +
-                        (rows ? 2.7 + 0.1 * most + 0.4e-6 * rows * n_kv * (head_dim + 4) * 4 : 0.0);
+      const double few_us = std::min(std::max(0.32, (head_dim == 128 ? 0.2 : 0.37) + ranges * n_kv / 512.0), 0.58);
+      const double us = std::max({total * n_kv / 370.0, 0.58 * longest, few_us * longest_few}) +
+                        (rows ? 2.7 + 0.0016 * head_dim * most + 0.4e-6 * rows * n_kv * (head_dim + 4) * 4 : 0.0);
       if (best_chunk == 0 || us < best) {
         best = us;
         best_chunk = chunk;

@@ -287,7 +287,7 @@ __device__ __forceinline__ void merge_last(const AttnParams& p, int h, int slot,
 // 16 29.6 -> 25.4; ranges of 170 stages read 3% faster there (6 tokens and two chunks on 40 k keys 108 -> 112), for
 // which it is not kept.  P is a bf16 pair, as elsewhere in decode: the rows' errors are their outputs' rounding alone
 // (1.6e-3 of 64 bits, 2.3e-3 with P rounded once).
-constexpr int kFewRows = 16;
+constexpr int kFewRows = kPackedFewRows;
 template <int HD>
 __device__ __forceinline__ void few_rows(const AttnParams& p, const PackedItem& item, int h, char* lds) {
   constexpr int KK = HD / 32, DPL = HD / 16, TOK = Geo<HD>::TOK, CPR = HD / 4;

@@ -410,10 +410,13 @@ def test_ranges_merge_in_the_launch_and_behind_it(gpu):
     _check(out, lse, want, 30001, "merged")
 
 
-def test_one_sequence_in_more_than_64_ranges(gpu):
-    """One row block on a card of its own: its ranges are more than a wave's lanes, and merge in a launch behind."""
-    new, ctx = [1], [70000]
+@pytest.mark.parametrize("keys", [70001, 300001])
+def test_one_sequence_in_more_than_64_ranges(gpu, keys):
+    """One row block on a card of its own: its ranges merge in the launch, or, where they are more than a wave's
+    lanes, in a launch behind."""
+    new, ctx = [1], [keys - 1]
     batch, bt, kc, vc, q = _case(gpu, new, ctx, 256, 7, 1, 128, seed=13)
-    assert batch._plans[None][4] == 1 and batch._plans[None][5] > 64
+    merges, ranges = batch._plans[None][4:6]
+    assert (merges, ranges > 64) == ((0, False) if keys < 100000 else (1, True)) and ranges > 32
     out, lse = prism_amd.packed_attention(q.to(gpu), kc.to(gpu), vc.to(gpu), batch, return_lse=True)
-    _check(out, lse, op.packed_attention64(q, kc, vc, new, ctx, bt), 70001, "many ranges")
+    _check(out, lse, op.packed_attention64(q, kc, vc, new, ctx, bt), keys, "many ranges")
