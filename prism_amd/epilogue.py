@@ -125,19 +125,36 @@ def rope_qk(qkv: torch.Tensor, positions: torch.Tensor | int, cos: torch.Tensor,
     return q_out, k_out
 
 
+# the keys that each kind of rotary scaling understands, beside the kind itself
+_SCALING_KEYS = {
+    "default": set(),
+    "linear": {"factor", "original_max_position_embeddings"},
+    "dynamic": {"factor", "original_max_position_embeddings"},
+    "yarn": {"factor", "original_max_position_embeddings", "beta_fast", "beta_slow", "attention_factor", "truncate", "mscale",
+             "mscale_all_dim"},
+}
+
+
 def _scaled_frequencies(rotary_dim: int, n_pos: int, theta: float, scaling: dict | None):
     """fp64 angle per position of each pair, and what cos and sin are multiplied by."""
     i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
     freq = float(theta) ** (-i / rotary_dim)
-    kind = (scaling or {}).get("rope_type", (scaling or {}).get("type", "default"))
+    scaling = {key: value for key, value in (scaling or {}).items() if value is not None}
+    kinds = {scaling.pop(key) for key in ("rope_type", "type") if key in scaling}
+    if len(kinds) > 1:
+        raise ValueError(f"rotary scaling has two types, {' and '.join(sorted(map(repr, kinds)))}")
+    kind = kinds.pop() if kinds else "default"
+    if kind not in _SCALING_KEYS:
+        raise ValueError(f"rotary scaling type {kind!r} is not one of {', '.join(_SCALING_KEYS)}")
+    # a key that is passed over would give other tables than the configuration's
+    unknown = set(scaling) - _SCALING_KEYS[kind]
+    if unknown:
+        raise ValueError(f"rotary scaling {kind!r} does not take {', '.join(sorted(map(str, unknown)))}")
     if kind == "default":
         return freq, 1.0
-    if kind not in ("linear", "dynamic", "yarn"):
-        raise ValueError(f"rotary scaling type {kind!r} is not one of default, linear, dynamic, yarn")
-    missing = {"factor", "original_max_position_embeddings"} - set(scaling) - ({"original_max_position_embeddings"}
-                                                                               if kind == "linear" else set())
-    if missing:
-        raise ValueError(f"rotary scaling {kind!r} needs {', '.join(sorted(missing))}")
+    needed = {"factor"} if kind == "linear" else {"factor", "original_max_position_embeddings"}
+    if needed - set(scaling):
+        raise ValueError(f"rotary scaling {kind!r} needs {', '.join(sorted(needed - set(scaling)))}")
     factor = float(scaling["factor"])
     if not factor >= 1.0:
         raise ValueError(f"rotary scaling factor {factor} must be >= 1")
@@ -153,18 +170,36 @@ def _scaled_frequencies(rotary_dim: int, n_pos: int, theta: float, scaling: dict
         grow = max(factor * max(n_pos, orig) / orig - (factor - 1.0), 1.0)
         return (float(theta) * grow ** (rotary_dim / (rotary_dim - 2))) ** (-i / rotary_dim), 1.0
     # pairs that turn beta_fast times or more over the original length keep their frequency, pairs of beta_slow
-    # turns or fewer are stretched by the factor, those between by a linear ramp over the pairs' numbers
+    # turns or fewer are stretched by the factor, those between by a linear ramp over the pairs' numbers, from
+    # whole pair to whole pair unless truncate is false
     fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
     if not fast > slow > 0.0:
         raise ValueError("yarn scaling needs beta_fast > beta_slow > 0")
+    truncate = scaling.get("truncate", True)
+    if not isinstance(truncate, bool):
+        raise ValueError(f"yarn scaling's truncate must be true or false, not {truncate!r}")
 
     def pair_of(turns: float) -> float:
         return rotary_dim * math.log(orig / (turns * 2.0 * math.pi)) / (2.0 * math.log(float(theta)))
 
-    low, high = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rotary_dim - 1)
-    ramp = ((i / 2 - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
-    gain = scaling.get("attention_factor")
-    gain = 0.1 * math.log(factor) + 1.0 if gain is None else float(gain)
+    low, high = pair_of(fast), pair_of(slow)
+    if truncate:
+        low, high = math.floor(low), math.ceil(high)
+    low, high = max(low, 0), min(high, rotary_dim - 1)
+    ramp = ((i / 2 - low) / (high - low if high > low else 1e-3)).clamp(0.0, 1.0)
+
+    def gain_of(mscale: float) -> float:
+        return 0.1 * mscale * math.log(factor) + 1.0
+
+    # mscale and mscale_all_dim: the attention's scale takes the second, the tables the ratio.  One of them alone is
+    # read in two ways, so it is refused.
+    scales = [scaling[key] for key in ("mscale", "mscale_all_dim") if key in scaling]
+    if scales and not (len(scales) == 2 and scales[0] > 0.0 and scales[1] > 0.0):
+        raise ValueError("yarn scaling takes mscale and mscale_all_dim together, both above 0")
+    if "attention_factor" in scaling:
+        gain = float(scaling["attention_factor"])
+    else:
+        gain = gain_of(scales[0]) / gain_of(scales[1]) if scales else gain_of(1.0)
     return freq * (1.0 - ramp) + freq / factor * ramp, gain
 
 
@@ -177,9 +212,11 @@ def rotary_tables(rotary_dim: int, n_pos: int, theta: float = 10000.0, *, scalin
 
     ``scaling`` is a model configuration's dict for contexts longer than the trained ones: ``rope_type`` "linear"
     (all angles divided by ``factor``), "dynamic" (a base that grows with n_pos past
-    ``original_max_position_embeddings``) or "yarn" (slow pairs stretched, fast ones kept; ``beta_fast``,
-    ``beta_slow``, ``attention_factor``).  Or give any frequencies (``inv_freq`` [rotary_dim / 2]) and what cos and
-    sin are multiplied by (``gain``)."""
+    ``original_max_position_embeddings``: one table for the longest sequence turns shorter ones by the longest's
+    base too) or "yarn" (slow pairs stretched, fast ones kept; ``beta_fast``, ``beta_slow``, ``truncate``,
+    ``attention_factor``, ``mscale`` with ``mscale_all_dim``).  "dynamic" and "yarn" need ``factor`` and
+    ``original_max_position_embeddings``; None counts as absent, and any other type or key is refused.  Or give any
+    frequencies (``inv_freq`` [rotary_dim / 2]) and what cos and sin are multiplied by (``gain``)."""
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim {rotary_dim} must be even and positive")
     if not 0 < n_pos < 1 << 31:

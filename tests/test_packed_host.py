@@ -259,6 +259,67 @@ def test_rotary_tables_frequencies_and_refusals():
             prism_amd.rotary_tables(a.pop("rotary_dim"), a.pop("n_pos"), **a)
 
 
+def _yarn_dict(**over):
+    return dict(rope_type="yarn", factor=32.0, original_max_position_embeddings=4096, **over)
+
+
+def _yarn_ends(rd, theta, orig, fast=32.0, slow=1.0):
+    """The pairs that turn `fast` and `slow` times over the original length, not rounded to whole pairs."""
+    return [rd * math.log(orig / (turns * 2 * math.pi)) / (2 * math.log(theta)) for turns in (fast, slow)]
+
+
+@pytest.mark.parametrize("rd,theta", [(64, 150000.0), (128, 1e6), (32, 1e4)])
+def test_yarn_ramp_not_rounded(rd, theta):
+    """truncate: false keeps the ramp's ends where they fall between two pairs."""
+    lo, hi = _yarn_ends(rd, theta, 4096)
+    if rd == 64:
+        assert abs(lo - 8.09) < 0.01 and abs(hi - 17.40) < 0.01
+    freq, gain = prism_amd.epilogue._scaled_frequencies(rd, 9, theta, _yarn_dict(truncate=False))
+    for i in range(rd // 2):
+        plain, r = theta ** (-2 * i / rd), min(max((i - lo) / (hi - lo), 0.0), 1.0)
+        want = plain * (1 - r) + plain / 32.0 * r
+        assert abs(float(freq[i]) - want) <= 1e-12 * plain, i      # a few 2^-53 per power, quotient and product
+    assert abs(gain - (0.1 * math.log(32.0) + 1)) < 1e-15
+    whole, _ = prism_amd.epilogue._scaled_frequencies(rd, 9, theta, _yarn_dict())
+    same, _ = prism_amd.epilogue._scaled_frequencies(rd, 9, theta, _yarn_dict(truncate=True))
+    assert torch.equal(whole, same) and not torch.equal(whole, freq)
+
+
+@pytest.mark.parametrize("a,b", [(1.0, 1.0), (0.707, 0.707), (1.0, 0.5), (0.5, 2)])
+def test_yarn_gain_of_two_scales(a, b):
+    """mscale and mscale_all_dim: cos and sin take the ratio of their two gains, the attention's scale the rest."""
+    _, gain = prism_amd.epilogue._scaled_frequencies(64, 9, 1e4, _yarn_dict(mscale=a, mscale_all_dim=b))
+    assert abs(gain - (0.1 * a * math.log(32.0) + 1) / (0.1 * b * math.log(32.0) + 1)) < 1e-15
+    _, gain = prism_amd.epilogue._scaled_frequencies(64, 9, 1e4, _yarn_dict(mscale=a, mscale_all_dim=b, attention_factor=1.25))
+    assert gain == 1.25
+
+
+def test_scaling_none_is_absent():
+    full = _yarn_dict(beta_fast=None, beta_slow=None, attention_factor=None, truncate=None, mscale=None, mscale_all_dim=None,
+                      type="yarn", low_freq_factor=None)
+    a, b = (prism_amd.epilogue._scaled_frequencies(64, 9, 1e4, s) for s in (full, _yarn_dict()))
+    assert torch.equal(a[0], b[0]) and a[1] == b[1]
+    for s in ({}, dict(rope_type=None), dict(rope_type="default", factor=None)):
+        f, gain = prism_amd.epilogue._scaled_frequencies(8, 9, 1e4, s)
+        assert torch.equal(f, 1e4 ** (-torch.arange(0, 8, 2, dtype=torch.float64) / 8)) and gain == 1.0
+
+
+@pytest.mark.parametrize("scaling", [
+    dict(factor=4.0), dict(rope_type="default", factor=4.0), dict(type="linear", factor=4.0, original=8),
+    dict(rope_type="yarn", type="linear", factor=4.0, original_max_position_embeddings=8),
+    dict(rope_type="linear", factor=4.0, beta_fast=32.0), dict(rope_type="linear", factor=None),
+    dict(rope_type="dynamic", factor=2.0, original_max_position_embeddings=8, attention_factor=1.0),
+    _yarn_dict(mscale=1.0), _yarn_dict(mscale_all_dim=1.0), _yarn_dict(mscale=0.0, mscale_all_dim=1.0),
+    _yarn_dict(mscale=1.0, mscale_all_dim=-1.0), _yarn_dict(mscale=1.0, mscale_all_dim=math.nan), _yarn_dict(truncate=0.5), _yarn_dict(short_factor=[1.0]),
+    _yarn_dict(rope_theta=1e4), _yarn_dict(partial_rotary_factor=0.5), _yarn_dict(finetuned=True),
+    _yarn_dict(beta_fast=float("nan")), dict(rope_type="llama3", factor=8.0, original_max_position_embeddings=8192),
+])
+def test_scaling_keys_that_are_not_understood(scaling):
+    """Nothing that would change the tables is passed over."""
+    with pytest.raises(ValueError):
+        prism_amd.rotary_tables(64, 3, scaling=scaling, device="cpu")
+
+
 def test_tables_argument_errors():
     lib = _lib.load()
     f = np.ones(4)
