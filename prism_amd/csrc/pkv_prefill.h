@@ -156,17 +156,22 @@ __device__ __forceinline__ void pin(uint32_t& v) { asm volatile("" : "+v"(v)); }
 __device__ __forceinline__ float finish_row(const AttnParams& p, int hq, float m, float l, float l_true, float& lse) {
   // sink - top below must be of the rounded product: fused, a sink of 1e30 would come out 2^76 above itself
 #pragma clang fp contract(off)
-  float keep = 1.f;
+  float keep = 1.f, sink_ln = 0.f;
+  bool sink_tops = false;
   if (p.sinks) {
-    const float sink = p.sinks[hq] * 1.4426950408889634f;
+    sink_ln = p.sinks[hq];
+    const float sink = sink_ln * 1.4426950408889634f;
     const float top = fmaxf(m, sink);
     keep = m == -INFINITY ? 0.f : fast_exp2(m - top);
-    const float term = sink == -INFINITY ? 0.f : fast_exp2(sink - top);
+    // (a sink of +inf, or one that the product takes there, is all of the sum: not inf - inf)
+    const float term = sink == -INFINITY ? 0.f : sink == top ? 1.f : fast_exp2(sink - top);
     l = l * keep + term;
     l_true = l_true * keep + term;
+    sink_tops = sink == top;
     m = top;
   }
-  lse = l_true == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l_true)) * 0.6931471805599453f;
+  const float log2_l = __builtin_amdgcn_logf(l_true);
+  lse = l_true == 0.f ? -INFINITY : sink_tops ? sink_ln + log2_l * 0.6931471805599453f : (m + log2_l) * 0.6931471805599453f;
   return l == 0.f ? 0.f : keep / l;
 }
 

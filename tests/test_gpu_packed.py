@@ -420,3 +420,22 @@ def test_one_sequence_in_more_than_64_ranges(gpu, keys):
     assert (merges, ranges > 64) == ((0, False) if keys < 100000 else (1, True)) and ranges > 32
     out, lse = prism_amd.packed_attention(q.to(gpu), kc.to(gpu), vc.to(gpu), batch, return_lse=True)
     _check(out, lse, op.packed_attention64(q, kc, vc, new, ctx, bt), keys, "many ranges")
+
+
+@pytest.mark.parametrize("nh,nk,hd", [(8, 2, 128), (8, 2, 64)])
+def test_sinks_past_every_score(gpu, nh, nk, hd):
+    """A sink of +inf, or one whose product with log2 e overflows, takes all of the weight: the row is 0 and its
+    log-sum-exp the sink, decode rows and chunk rows alike, in one range or several."""
+    new, ctx = [1, 40, 1, 9], [5, 60, 6000, 3000]
+    batch, bt, kc, vc, q = _case(gpu, new, ctx, 64, nh, nk, hd, seed=4, windows=(None, 50))
+    top = torch.finfo(torch.float32).max
+    sinks = torch.tensor([float("inf"), top, 0.5, float("inf"), -top, 2.5e38, float("-inf"), 1.0])
+    for window in (None, 50):
+        out, lse = prism_amd.packed_attention(q.to(gpu), kc.to(gpu), vc.to(gpu), batch, window=window, sinks=sinks.to(gpu),
+                                              return_lse=True)
+        all_of_it = [0, 1, 3, 5]
+        assert not out[:, all_of_it].any()
+        assert torch.equal(lse[:, all_of_it].cpu(), sinks[all_of_it].expand(sum(new), 4))
+        rest = [2, 4, 6, 7]
+        want = op.packed_attention64(q, kc, vc, new, ctx, bt, window=window, sinks=sinks)
+        _check(out[:, rest], lse[:, rest], [x[:, rest] for x in want], 6001, f"window {window}")
