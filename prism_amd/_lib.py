@@ -222,30 +222,29 @@ def load() -> ctypes.CDLL:
         ver = lib.pkv_abi_version()
         if ver != ABI_VERSION:
             raise PrismKVError(f"libprism_kv ABI version {ver} != expected {ABI_VERSION}")
-        _attach(lib)
+        if _fast is not None:
+            _fast.attach(lib._handle, PrismKVError)
         _lib = lib
         return lib
 
 
-def _attach(lib: ctypes.CDLL) -> None:
-    """Points _fastcall.so (which needs torch loaded) at the library just loaded."""
-    global _fast
-    if _fast is None:
-        if not FASTCALL_PATH.exists():
-            raise PrismKVError(f"{FASTCALL_PATH} is not built; run `python -m prism_amd.build` first")
-        import torch  # noqa: F401  its libraries are what the module's symbols are found in
-
-        spec = importlib.util.spec_from_file_location("_fastcall", FASTCALL_PATH)
-        module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(module)
-        _fast = module
-    _fast.attach(lib._handle, PrismKVError)
-
-
 def fast():
-    """The calls that are made once per layer, without Python's checks and ctypes (csrc_binding/fastcall.cpp)."""
-    if _lib is None:
-        load()
+    """The calls that are made once per layer, without Python's checks and ctypes (csrc_binding/fastcall.cpp).  Only
+    they need _fastcall.so, a module built against the installed torch: the other calls do without it."""
+    global _fast
+    if _fast is None or _lib is None:
+        lib = load()
+        with _lock:
+            if _fast is None:
+                if not FASTCALL_PATH.exists():
+                    raise PrismKVError(f"{FASTCALL_PATH} is not built; run `python -m prism_amd.build` first")
+                import torch  # noqa: F401  its libraries are what the module's symbols are found in
+
+                spec = importlib.util.spec_from_file_location("_fastcall", FASTCALL_PATH)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                module.attach((_lib or lib)._handle, PrismKVError)
+                _fast = module
     return _fast
 
 

@@ -465,3 +465,53 @@ def test_attention_workspace():
     assert lib.pkv_packed_workspace_bytes(0, 4, 128) == 0
     assert _attn(lib, wsb=need - 1) == _lib.PKV_ENOSPC
     assert _attn(lib, n_items=0, items=0, ws=0) == 0
+
+
+# ---------------------------------------------------------------------------------- the binding
+def _in_a_process(code):
+    import subprocess
+    import sys
+
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       cwd=str(_lib.FASTCALL_PATH.parents[1]))
+    assert r.returncode == 0, r.stderr
+    return r.stdout
+
+
+def test_only_the_packed_step_needs_the_binding():
+    """Without _fastcall.so the library loads and its calls go through ctypes, as they do where that module was built
+    against another torch; a packed call names what is missing."""
+    out = _in_a_process("""
+import pathlib
+from prism_amd import _lib
+_lib.FASTCALL_PATH = pathlib.Path("/nowhere/_fastcall.so")
+print(_lib.load().pkv_abi_version())
+import prism_amd
+kv = prism_amd.FlashAttnKVCache(1, 2, 64, 4, 16, "cpu")
+kv.new_sequence(1)
+kv.prepare_append([1], 3)
+try:
+    kv.build_packed_batch([1], 3, 14)
+except _lib.PrismKVError as e:
+    print(e)
+""")
+    assert "_fastcall.so is not built" in out and out.startswith("1\n")
+
+
+def test_the_binding_follows_the_library_in_use():
+    """_lib.use after the first packed call: the binding's calls go to the library that is loaded then."""
+    stamps = _lib.LIB_PATH.with_name("libprism_kv_stamps.so")
+    out = _in_a_process(f"""
+import pathlib
+from prism_amd import _lib
+seen = []
+class Fake:
+    attach = staticmethod(lambda handle, error: seen.append(handle))
+first = _lib.load()
+_lib.fast()
+_lib._fast = Fake
+second = _lib.use(pathlib.Path({str(stamps)!r}))
+assert _lib.fast() is Fake
+print(seen == [second._handle] and second._handle != first._handle)
+""")
+    assert out == "True\n"
