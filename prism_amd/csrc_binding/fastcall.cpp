@@ -73,6 +73,14 @@ void on_device(const at::Tensor& t, const char* name, c10::Device d) {
   if (t.device() != d) refuse(c10::str(name, " must be on ", d, ", not ", t.device()));
 }
 
+// The word that a kernel sets its error bits in.
+int32_t* status_word(PyObject* o, c10::Device d) {
+  const at::Tensor& t = tensor(o, "status");
+  if (t.scalar_type() != at::kInt || t.numel() < 1 || t.device() != d)
+    refuse(c10::str("status must be an int32 word on ", d, ", got ", shape_of(t), " on ", t.device()));
+  return t.data_ptr<int32_t>();
+}
+
 // The tables' rotary_dim.
 int rotary_dim(const at::Tensor& cos, const at::Tensor& sin, int64_t head_dim, c10::Device d) {
   const at::Tensor* tables[] = {&cos, &sin};
@@ -128,6 +136,7 @@ PyObject* rotate_qk(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const auto dtype = q.scalar_type();
     const int code = dtype == at::kBFloat16 ? PKV_BF16 : dtype == at::kHalf ? PKV_FP16 : dtype == at::kFloat ? PKV_FP32 : -1;
     if (code < 0) refuse(c10::str("q must be bfloat16, float16 or float32, got ", dtype));
+    int32_t* const status = status_word(a[11], q.device());
     const int64_t dims = q.dim();
     if (dims < 3) refuse(c10::str("q must be [..., n_heads, head_dim] with a token axis, got ", q.sizes()));
     const c10::Device dev = q.device();
@@ -175,7 +184,7 @@ PyObject* rotate_qk(PyObject*, PyObject* const* a, Py_ssize_t n) {
                               cos.data_ptr<float>(), sin.data_ptr<float>(), int32_t(cos.size(0)), qw, kw,
                               float(real(a[8])), q_out.data_ptr(), qo.token, qo.head, ko_ptr, ko.token, ko.head, tokens,
                               int32_t(nh), int32_t(nk), int32_t(hd), rd, truth(a[5]) ? 1 : 0, code,
-                              tensor(a[11], "status").data_ptr<int32_t>(), address(a[12])),
+                              status, address(a[12])),
             "pkv_rotate_qk");
     PyObject* kobj = has_k ? THPVariable_Wrap(k_out) : (Py_INCREF(Py_None), Py_None);
     return Py_BuildValue("(NN)", THPVariable_Wrap(q_out), kobj);
@@ -261,6 +270,7 @@ PyObject* packed_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor &qkv = tensor(a[0], "qkv"), &kc = tensor(a[1], "k_cache"), &vc = tensor(a[2], "v_cache");
     const Batch& b = batch_of(a[3]);
     on_gpu(qkv, "qkv");
+    int32_t* const status = status_word(a[12], b.device);
     const int64_t page_stride = check_cache(kc, vc, b);
     const int64_t width = (b.n_heads + 2 * b.n_kv) * b.head_dim;
     if (qkv.scalar_type() != at::kBFloat16 || qkv.dim() != 2 || qkv.size(0) < b.tokens || qkv.size(1) != width ||
@@ -295,7 +305,7 @@ PyObject* packed_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 int32_t(cos.size(0)), qw, kw, float(real(a[9])), q_out.data_ptr(), qo.token, qo.head, kc.data_ptr(),
                 vc.data_ptr(), page_stride, b.tokens, int32_t(b.n_heads), int32_t(b.n_kv), int32_t(b.head_dim), rd,
                 truth(a[6]) ? 1 : 0, int32_t(b.page_size), int32_t(b.num_pages),
-                tensor(a[12], "status").data_ptr<int32_t>(), address(a[13])),
+                status, address(a[13])),
             "pkv_packed_rope_append");
     return THPVariable_Wrap(q_out);
   } catch (const Failed&) {
@@ -313,6 +323,7 @@ PyObject* packed_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor &q = tensor(a[0], "q"), &kc = tensor(a[1], "k_cache"), &vc = tensor(a[2], "v_cache");
     const Batch& b = batch_of(a[3]);
     const Rows qr = check_rows(q, "q", b);
+    int32_t* const status = status_word(a[9], b.device);
     const int64_t page_stride = check_cache(kc, vc, b);
     if (!PyTuple_Check(a[4]) || PyTuple_GET_SIZE(a[4]) != 7) refuse("a plan has 7 entries");
     int64_t plan[7];
@@ -348,7 +359,7 @@ PyObject* packed_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 int32_t(plan[4]), int32_t(plan[5]), int32_t(plan[6]), bytes ? ws.data_ptr() : nullptr, bytes,
                 int32_t(b.tokens), int32_t(b.batch), int32_t(b.n_heads), int32_t(b.n_kv), int32_t(b.head_dim),
                 int32_t(b.page_size), int32_t(b.num_pages), int32_t(b.max_blocks), int32_t(plan[0]), float(scale),
-                tensor(a[9], "status").data_ptr<int32_t>(), address(a[10])),
+                status, address(a[10])),
             "pkv_packed_attn");
     }
     if (!want_lse) return THPVariable_Wrap(out);

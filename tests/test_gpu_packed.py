@@ -439,3 +439,22 @@ def test_sinks_past_every_score(gpu, nh, nk, hd):
         rest = [2, 4, 6, 7]
         want = op.packed_attention64(q, kc, vc, new, ctx, bt, window=window, sinks=sinks)
         _check(out[:, rest], lse[:, rest], [x[:, rest] for x in want], 6001, f"window {window}")
+
+
+def test_a_status_word_elsewhere_is_refused(gpu):
+    """The kernels write to the status word: one that is not the device's, or none, never reaches them."""
+    batch, bt, kc, vc, q = _case(gpu, [3], [4], 16, 4, 2, 64, seed=2)
+    q, kc, vc = q.to(gpu), kc.to(gpu), vc.to(gpu)
+    cos, sin = prism_amd.rotary_tables(64, 8, device=gpu)
+    x = torch.zeros(3, 8 * 64, dtype=BF16, device=gpu)
+    for status in (torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int64, device=gpu),
+                   torch.zeros(0, dtype=torch.int32, device=gpu)):
+        for call in (lambda: prism_amd.packed_attention(q, kc, vc, batch, status=status),
+                     lambda: prism_amd.packed_rope_append(x, kc, vc, batch, cos, sin, status=status),
+                     lambda: prism_amd.rotate_qk(q, None, batch.positions, cos, sin, status=status)):
+            with pytest.raises(RuntimeError, match="status"):
+                call()
+    own = torch.zeros(1, dtype=torch.int32, device=gpu)
+    batch.block_table[0, 0] = -1
+    prism_amd.packed_attention(q, kc, vc, batch, status=own)
+    assert own.item() == prism_amd._lib.PKV_STATUS_BAD_PAGE and read_status(gpu) == 0
