@@ -27,7 +27,7 @@ from . import _lib
 from .attention import _raw_stream, _require_gpu, status_tensor
 
 _MAX_KEYS = 1 << 27
-_captured: list[torch.Tensor] = []   # work lists that a captured graph reads
+_captured: list[torch.Tensor] = []   # work lists that a captured graph reads (PackedBatch.release takes them out)
 
 
 _here = contextlib.nullcontext()
@@ -61,8 +61,7 @@ class PackedBatch:
     token's position and place in the cache, page * page_size + row), ``block_table`` (int32 [batch, max_blocks])
     and, for each of ``windows`` (None: every key; w: the last w keys), the attention's work list.  On another
     stream, use it behind this one, as any tensor made here; calls there keep its memory until they have run, and a
-    call that a graph captures keeps it for the rest of the process (a replay reads it, whether the batch lives or
-    not).
+    call that a graph captures keeps it (a replay reads it, whether the batch lives or not) until ``release``.
 
     A page that a new token is written to must belong to one sequence alone, and every page that a token is written
     to or sees must be one of the pool's; columns behind them, or out of every window, may hold anything."""
@@ -134,6 +133,12 @@ class PackedBatch:
                 self._captured = True
         elif stream != self._stream:
             self._buf.record_stream(torch.cuda.current_stream(self.device))
+
+    def release(self) -> None:
+        """Lets go of the memory that captured calls kept, which then lives as long as the batch.  For a batch whose
+        graphs are gone, or were captured again with another: none of their replays may run now or later."""
+        _captured[:] = [buf for buf in _captured if buf is not self._buf]
+        self._captured = False
 
     def _plan(self, lengths, window, cus):
         lib = _lib.load()

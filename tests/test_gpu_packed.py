@@ -458,3 +458,25 @@ def test_a_status_word_elsewhere_is_refused(gpu):
     batch.block_table[0, 0] = -1
     prism_amd.packed_attention(q, kc, vc, batch, status=own)
     assert own.item() == prism_amd._lib.PKV_STATUS_BAD_PAGE and read_status(gpu) == 0
+
+
+def test_captures_again_and_again_do_not_grow(gpu):
+    """A graph captured anew for every batch, the old one released: the lists' memory comes back."""
+    def step(seed):
+        batch, bt, kc, vc, q = _case(gpu, [1, 40], [700, 300], 64, 14, 2, 64, seed=seed)
+        dq, dk, dv = q.to(gpu), kc.to(gpu), vc.to(gpu)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = prism_amd.packed_attention(dq, dk, dv, batch)
+        for _ in range(2):
+            out.zero_()
+            graph.replay()
+            assert torch.equal(out, prism_amd.packed_attention(dq, dk, dv, batch))
+        torch.cuda.synchronize()
+        del graph
+        batch.release()
+    step(0)
+    held, memory = len(prism_amd.packed._captured), torch.cuda.memory_allocated()
+    for seed in range(1, 5):
+        step(seed)
+        assert len(prism_amd.packed._captured) == held and torch.cuda.memory_allocated() <= memory

@@ -515,3 +515,27 @@ assert _lib.fast() is Fake
 print(seen == [second._handle] and second._handle != first._handle)
 """)
     assert out == "True\n"
+
+
+def test_a_released_batch_keeps_nothing(monkeypatch):
+    """A captured call keeps the batch's memory, once; release gives it up, and a later capture keeps it again."""
+    import gc
+    import weakref
+
+    from prism_amd import packed
+
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: True)
+    a, b = _batch(), _batch()
+    held = len(packed._captured)
+    for _ in range(2):
+        for x in (a, b, a):
+            x._used_on(0)
+        assert len(packed._captured) == held + 2
+        a.release()
+        a.release()
+        assert len(packed._captured) == held + 1 and any(t is b._buf for t in packed._captured)
+    gone, kept = weakref.ref(a._buf), weakref.ref(b._buf)
+    del a, b, x
+    gc.collect()
+    assert gone() is None and kept() is not None
+    packed._captured[:] = [t for t in packed._captured if t is not kept()]
