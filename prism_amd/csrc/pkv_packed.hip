@@ -134,12 +134,21 @@ Schedule even(const std::vector<Block>& blocks, int slots, int n_kv, int head_di
 
 // Whole blocks can need a round more than their work does (129 blocks of 34 stages on 64 slots, a window's, take
 // three rounds for one block too many), and few blocks leave the card idle.  Two ways to cut them: pieces of one
-// length that fit one round, and, where that schedule would end a tenth earlier, pieces that fill every slot up to an
-// even share of the work.  (Less than that is lost again: pieces that wait for a slot start into a card that reads
-// as fast as it can.)  us a call, uncut / one length / filled: 47 decode tokens and two chunks (7B) 111 / 56 / 70; 6
-// and two on 40 k keys 1063 / 112 / 137; 208 short chats (0.5B) 28 / 22 / 19; chunks in a window of 1024 (14B, more
-// blocks than slots) 107 / - / 97.  Many rounds even out by themselves: above kRounds of them nothing is cut.
+// length that fit one round, and pieces that fill every slot up to an even share of the work.
+// Up to one block per slot: one length, or, with more than half as many blocks as slots and where that schedule would
+// end a tenth earlier, filled.  (Less than that is lost again: pieces that wait for a slot start into a card that reads
+// as fast as it can.)  us a call, uncut / one length / filled: 47 decode tokens and two chunks (7B) 111 / 56 / 70; 6 and
+// two on 40 k keys 1063 / 112 / 137; 208 short chats (0.5B) 28 / 22 / 19.
+// More blocks than slots: filled or whole.  Filling goes on past the share by the price of its own cuts, in ever shorter
+// pieces, and a cut costs the launch more than its slot, as the others read no faster meanwhile: about kCutWait stages of
+// one slot each.  us a call, whole / filled, and what the schedules' ends alone would promise: six chunks of 1000 in a
+// window of 512 (7B) 76 / 92 (1.31 of whole), four of 2048 in 2048 (0.5B) 85 / 106 (1.33), four of 700 in 1024 (14B)
+// 80 / 104 (1.31); 300 decode tokens on 900 keys (7B) 107 / 114 (0.95), 64 on 2000 and three chunks (14B) 147 / 161
+// (0.92); 140 decode tokens on 3000 (7B) 179 / 164 (0.58), three chunks of 700 on 8000 (14B) 424 / 382 (0.74), chunks and
+// decode tokens in a window of 1024 (14B, three cuts) 107 / 96 (0.93).  Many rounds even out by themselves: above
+// kRounds of them nothing is cut.
 constexpr int kRounds = 8;
+constexpr int kCutWait = 20;
 std::vector<Piece> cut(std::vector<Block>& blocks, int slots, int n_kv, int head_dim) {
   std::stable_sort(blocks.begin(), blocks.end(), [](const Block& a, const Block& b) { return a.stages > b.stages; });
   const int64_t n = int64_t(blocks.size());
@@ -152,6 +161,9 @@ std::vector<Piece> cut(std::vector<Block>& blocks, int slots, int n_kv, int head
   if (n <= slots) {
     Schedule one = even(blocks, slots, n_kv, head_dim);
     if (n <= slots / 2 || 9 * one.end <= 10 * best.end) best = std::move(one);
+  } else {
+    Schedule whole = in_chunks(blocks, slots, INT64_MAX / 2);
+    if ((whole.end - best.end) * slots <= kCutWait * (int64_t(best.list.size()) - n)) best = std::move(whole);
   }
   return std::move(best.list);
 }

@@ -76,6 +76,53 @@ def test_plan_covers_every_visible_key_once(nh, nk, hd, window, cus):
         assert counts[3] <= 128
 
 
+def _ends(new, ctx, nh, nk, hd, window=0, cus=256):
+    """The planner's schedule, replayed: when its list ends, when the blocks would end whole, an even share of the work,
+    and blocks per slot.  A range costs its stages and five, a piece of a block up to eight more, by its rows."""
+    import heapq
+    g, tok, slots = nh // nk, 32 if hd == 128 else 64, max(2 * cus // nk, 1)
+    blocks = {}
+    for b, (n, c) in enumerate(zip(new, ctx)):
+        for r0 in range(0, n * g, 128):
+            rows = min(128, n * g - r0)
+            first = max(c + r0 // g - window + 1, 0) if window else 0
+            blocks[b, r0] = ((c + (r0 + rows - 1) // g) // tok + 1 - first // tok, rows)
+
+    def end(costs):
+        load = [0] * slots
+        for cost in costs:
+            heapq.heapreplace(load, load[0] + cost)
+        return max(load)
+    listed = []
+    for it in _plan(new, ctx, nh, nk, hd, window, cus)[0].tolist():
+        stages, rows = blocks[it[3], it[4]]
+        listed.append(it[6] + 5 + (-(-8 * rows // 128) if it[6] < stages else 0))
+    whole = [stages + 5 for stages, _ in sorted(blocks.values(), key=lambda x: -x[0])]
+    return end(listed), end(whole), sum(whole) / slots, len(blocks) / slots
+
+
+SHAPES = [(28, 4, 128), (14, 2, 64), (40, 8, 128), (7, 1, 128)]
+
+
+def test_plan_is_not_worse_than_whole_blocks():
+    """Where the blocks are more than the slots, cutting them never ends later than leaving them whole."""
+    seen = 0
+    for chunks, n, c, w, s in [(6, 1000, 4000, 512, 0), (4, 2048, 8000, 2048, 1), (4, 700, 4000, 1024, 2), (3, 3500, 0, 2048, 3),
+                               (2, 2048, 1000, 1024, 0), (8, 500, 4000, 1024, 0), (5, 500, 1000, 0, 2), (2, 1500, 1000, 0, 0)]:
+        listed, whole, _, per_slot = _ends([n] * chunks, [c] * chunks, *SHAPES[s], w)
+        assert per_slot > 1 and listed <= whole, (chunks, n, c, w, s)
+    rng = np.random.default_rng(5)
+    for trial in range(300):
+        n = int(rng.integers(1, 300))
+        new = np.where(rng.random(n) < rng.random(), 1, rng.integers(1, 900, n)).tolist()
+        ctx = rng.integers(0, int(rng.choice([1, 600, 5000, 30000])), n).tolist()
+        listed, whole, _, per_slot = _ends(new, ctx, *SHAPES[trial % 4], int(rng.choice([0, 0, 100, 1024])))
+        if per_slot > 1:
+            seen += 1
+            assert listed <= whole, trial
+    assert seen > 100
+
+
 def test_layout_refusals():
     lib = _lib.load()
     one, bt, out = np.array([1], np.int32), np.array([[3]], np.int32), np.zeros(4, np.int32)
