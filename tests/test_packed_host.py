@@ -123,6 +123,19 @@ def test_plan_is_not_worse_than_whole_blocks():
     assert seen > 100
 
 
+def test_plan_cuts_a_long_block_among_many():
+    """Rounds of short blocks even out by themselves, one long block beside them does not: a document of 100,000 keys
+    among 1100 chats, a chunk on 30,000 keys among them, one document among 9000 sequences."""
+    for new, ctx, s in [([1] * 1101, [400] * 1100 + [100000], 0), ([1] * 1100 + [600], [400] * 1100 + [30000], 0),
+                        ([1] * 9001, [16] * 4500 + [120000] + [16] * 4500, 2)]:
+        listed, whole, share, per_slot = _ends(new, ctx, *SHAPES[s])
+        assert per_slot > 8 and whole > 2 * share
+        assert listed <= 1.1 * share + 20, (listed, whole, share)     # 20: a piece's start, cut and end
+    # and equal blocks stay whole, however many
+    items, merges, counts = _plan([1] * 9000, [100] * 9000, *SHAPES[2])
+    assert counts[0] == 9000 and counts[2] == 0
+
+
 def test_layout_refusals():
     lib = _lib.load()
     one, bt, out = np.array([1], np.int32), np.array([[3]], np.int32), np.zeros(4, np.int32)
