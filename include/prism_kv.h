@@ -428,14 +428,16 @@ size_t pkv_packed_workspace_bytes(int32_t partials, int32_t n_kv, int32_t head_d
  * chunk.  Their keys and values are in the cache already (pkv_packed_rope_append).  Token j of sequence b is at
  * position ctx_lens[b] + j and sees the keys up to itself, with window > 0 only the last `window` of them.
  * out = sum_t exp(s_t) v_t / (sum_t exp(s_t) + exp(sinks[h])), s = softmax_scale q . k; sinks (fp32 [n_heads])
- * NULL: without that term.  lse (fp32 [tokens, n_heads], NULL: not wanted): the logarithm of the denominator.
- * items, merges (device memory, 16-byte aligned) and the counts come from pkv_packed_plan for the same lengths,
+ * NULL: without that term (so too -inf; +inf: rows of zeros).  lse (fp32 [tokens, n_heads], NULL: not wanted): the
+ * logarithm of the denominator.  items, merges (device memory, 16-byte aligned) and the counts come from pkv_packed_plan for the same lengths,
  * heads and window (items that do not fit tokens, batch and partials are skipped and flag PKV_STATUS_BAD_PAGE); the
  * lengths are in them, and the block table needs ceil((ctx + new) / page_size) columns of
  * each sequence (with a window, only those that hold a visible key are read).  Rows of out from `tokens` on are
- * not written.  Values of masked keys take part in the products with weight 0: a NaN or infinity in a V row that
- * belongs to the sequence reaches rows of the same 32 (head_dim 64: 64) keys that do not see it; what lies behind
- * the sequence's last key does not matter; an infinite V makes infinities or NaN of the rows that see it.  bf16 in
+ * not written.  Values of masked keys take part in the products with weight 0, in blocks of 128 query rows (row = new
+ * token * group size + head in the group, of one sequence and KV head): a NaN or infinity in a V row of the sequence
+ * reaches that element of every row of each block that sees any of the same 32 (head_dim 64: 64) keys, of rows that do
+ * not see the key among them; other blocks, sequences and heads keep their bits.  What lies behind the
+ * sequence's last key does not matter; an infinite V makes infinities or NaN of the rows that see it.  bf16 in
  * and out, fp32 softmax and sums, the probabilities rounded to bf16 for the second product (a bf16 pair for blocks of
  * at most 16 rows without a window).  Replaces flash_attn_with_kvcache (engine/executor.py:119-120, :260-261) for
  * batches whose sequences bring different numbers of tokens.

@@ -480,3 +480,34 @@ def test_captures_again_and_again_do_not_grow(gpu):
     for seed in range(1, 5):
         step(seed)
         assert len(prism_amd.packed._captured) == held and torch.cuda.memory_allocated() <= memory
+
+
+@pytest.mark.parametrize("window", [None, 90])
+@pytest.mark.parametrize("nh,nk,hd", [(4, 4, 128), (4, 4, 64), (4, 2, 128), (14, 2, 64)])
+def test_a_bad_value_stays_in_its_blocks(gpu, nh, nk, hd, window):
+    """A NaN or infinity in a V row: rows that see the key are not finite, rows of a block of 128 that sees one of the
+    same 32 (64) keys may be (with one query head per KV head a block is 128 tokens), all others keep their bits."""
+    new, ctx, P, g, tok = [400, 9, 1], [3000, 70, 900], 64, nh // nk, 32 if hd == 128 else 64
+    batch, bt, kc, vc, q = _case(gpu, new, ctx, P, nh, nk, hd, seed=6, windows=(window,))
+    dq, dk = q.to(gpu), kc.to(gpu)
+    clean, lse = prism_amd.packed_attention(dq, dk, vc.to(gpu), batch, window=window, return_lse=True)
+    first = [0, 400, 409]
+    for b, t, bad in [(0, 3300, float("nan")), (0, 3127, float("inf")), (0, 2950, float("nan")), (1, 74, float("-inf")), (2, 850, float("nan"))]:
+        v = vc.clone()
+        v[int(bt[b, t // P]), t % P, 1, 5] = bad
+        out, lse2 = prism_amd.packed_attention(dq, dk, v.to(gpu), batch, window=window, return_lse=True)
+        assert torch.equal(lse, lse2)
+        may, must = torch.zeros(out.shape[:2], dtype=torch.bool, device=gpu), torch.zeros(out.shape[:2], dtype=torch.bool, device=gpu)
+        rows = torch.arange(new[b] * g, device=gpu)
+        pos = ctx[b] + rows // g
+        sees = (pos >= t) & (pos - t < (window or 1 << 30))
+        for r0 in range(0, new[b] * g, 128):
+            block = rows[r0:r0 + 128]
+            lo, hi = int(pos[r0]) - (window or 1 << 30) + 1, int(pos[block[-1]])
+            if max(lo, 0) // tok <= t // tok <= hi // tok:
+                may[first[b] + block // g, g + block % g] = True
+        must[first[b] + rows[sees] // g, g + rows[sees] % g] = True
+        assert not torch.isfinite(out[must][:, 5]).any()
+        assert torch.equal(out[~may], clean[~may])
+        good = [d for d in range(hd) if d != 5]
+        assert torch.equal(out[..., good], clean[..., good])
