@@ -128,3 +128,15 @@ class LayerCheck:
         mx, mean = attn_errors(got, ref)
         print(f"{what}: max-abs {mx:.3e} mean-abs {mean:.3e} over {got.numel()} outputs", flush=True)
         return mx, mean
+
+
+# packed_attention of blocks of at most 16 rows: lengths of few keys, where one rounding of a probability shows, and of
+# many
+PAIR_CASES = [([1, 1, 1, 1], [1, 6, 13, 40]), ([2, 1, 1], [9, 300, 5000]), ([1, 2], [0, 30])]
+
+
+def pair_tolerance(ref, mag, keys):
+    """Probabilities rounded to a bf16 pair: the second of the pair takes what the first left (2^-8 of it) to 2^-8, so
+    2^-16 of each, of sum_t p_t |v_t|; scores, exponentials and fp32 sums of N(0, 1) inputs below 2^-12 of that and of the
+    output, and 2^-24 per key summed; the output rounded once, 2^-8 of it."""
+    return ref.abs() * 2.0 ** -8 + (mag + ref.abs()) * (2.0 ** -16 + max(2.0 ** -12, keys * 2.0 ** -24))

@@ -5,6 +5,7 @@ import torch
 
 import prism_amd
 from oracle import packed as op
+from pkv_testutil import PAIR_CASES, pair_tolerance
 from prism_amd.attention import read_status
 
 pytestmark = pytest.mark.gpu
@@ -511,3 +512,55 @@ def test_a_bad_value_stays_in_its_blocks(gpu, nh, nk, hd, window):
         assert torch.equal(out[~may], clean[~may])
         good = [d for d in range(hd) if d != 5]
         assert torch.equal(out[..., good], clean[..., good])
+
+
+@pytest.mark.parametrize("new,ctx", PAIR_CASES)
+@pytest.mark.parametrize("nh,nk,hd,P", [(7, 1, 128, 256), (14, 2, 64, 16), (8, 8, 128, 64)])
+def test_decode_rows_round_their_probabilities_to_a_pair(gpu, new, ctx, nh, nk, hd, P):
+    """Blocks of at most 16 rows, whole and in ranges: their outputs are off by little more than their own rounding."""
+    batch, bt, kc, vc, q = _case(gpu, new, ctx, P, nh, nk, hd, seed=21)
+    assert max(new) * (nh // nk) <= 16
+    out = prism_amd.packed_attention(q.to(gpu), kc.to(gpu), vc.to(gpu), batch)
+    ref, _, mag = op.packed_attention64(q, kc, vc, new, ctx, bt)
+    err = (out.double().cpu() - ref).abs()
+    tol = pair_tolerance(ref, mag, max(n + c for n, c in zip(new, ctx)))
+    assert (err <= tol).all(), f"{int((err > tol).sum())} off, worst {float((err / tol).max()):.3g} of the tolerance"
+
+
+@pytest.mark.parametrize("nh,nk,hd", [(28, 4, 128), (14, 2, 64)])
+def test_a_list_with_more_partials_than_the_call(gpu, nh, nk, hd):
+    """Work lists of split blocks, some merged in the launch and some behind it, with room for fewer partials than they
+    name: blocks whose partials fit are done, of the others nothing is written, and nothing past the workspace or the
+    tensors."""
+    new, ctx, P = [1, 40, 1, 3, 40], [9000, 5000, 20, 7000, 30], 64
+    batch, bt, kc, vc, q = _case(gpu, new, ctx, P, nh, nk, hd, seed=14)
+    dq, dk, dv = q.to(gpu), kc.to(gpu), vc.to(gpu)
+    lib, st = prism_amd._lib.load(), prism_amd.attention.status_tensor(gpu)
+    _, items, n_items, merges, n_merges, partials, merge_rows = batch._plans[None]
+    cus = torch.cuda.get_device_properties(gpu).multi_processor_count
+    lengths = [np.asarray(x, np.int32) for x in (new, ctx)]
+    listed, merged, _ = batch._plan((lengths[0].ctypes.data, lengths[1].ctypes.data, len(new)), None, cus)
+    assert len(listed) == n_items and len(merged) == n_merges > 0 and (listed[:, 9] > 0).any() and (listed[:, 7] < 0).any()
+    want = prism_amd.packed_attention(dq, dk, dv, batch)
+    total, g = sum(new), nh // nk
+    for room in sorted({0, 1, partials // 3, partials // 2, partials - 1}):
+        need = lib.pkv_packed_workspace_bytes(room, nk, hd)
+        ws = torch.full((need + 4096,), 0x5A, dtype=torch.uint8, device=gpu)
+        out = torch.full((total + 4, nh, hd), 3.0, dtype=BF16, device=gpu)
+        rc = lib.pkv_packed_attn(dq.data_ptr(), nh * hd, hd, dk.data_ptr(), dv.data_ptr(), dk.stride(0), batch.block_table.data_ptr(),
+                                 batch.max_blocks, out.data_ptr(), nh * hd, hd, 0, 0, items, n_items, merges, n_merges, room,
+                                 merge_rows, ws.data_ptr(), need, total, len(new), nh, nk, hd, P, batch.num_pages,
+                                 batch.max_blocks, 0, hd ** -0.5, st.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and read_status(gpu) == prism_amd._lib.PKV_STATUS_BAD_PAGE
+        done = torch.zeros(total, nh, dtype=torch.bool)
+        for t0, n, _, _, row0, _, _, slot, first, count, *_ in listed.tolist():
+            last = slot if slot < 0 else first + count - 1 if count else \
+                next(m[3] + m[4] - 1 for m in merged.tolist() if (m[0], m[2]) == (t0, row0))
+            rows = torch.arange(row0, min(row0 + 128, n * g))
+            for h in range(nk):
+                done[t0 + rows // g, h * g + rows % g] = last < room
+        done = done.to(gpu)
+        assert done.any() and not done.all()
+        assert torch.equal(out[:total][done], want[done]), room
+        assert (out[:total][~done] == 3.0).all() and (out[total:] == 3.0).all(), room
+        assert (ws[need:] == 0x5A).all(), room

@@ -9,6 +9,7 @@ import prism_amd
 from oracle import epilogue
 from oracle import packed as op
 from oracle import paged_attention as pa
+from pkv_testutil import PAIR_CASES, pair_tolerance
 from prism_amd import _lib
 from prism_amd.kv_cache import FlashAttnKVCache
 
@@ -599,3 +600,31 @@ def test_a_released_batch_keeps_nothing(monkeypatch):
     gc.collect()
     assert gone() is None and kept() is not None
     packed._captured[:] = [t for t in packed._captured if t is not kept()]
+
+
+@pytest.mark.parametrize("new,ctx", PAIR_CASES)
+@pytest.mark.parametrize("nh,nk,hd", [(7, 1, 128), (14, 2, 64), (8, 8, 128)])
+def test_the_pair_tolerance_tells_a_pair_from_one_rounding(new, ctx, nh, nk, hd):
+    """Probabilities rounded once to bf16 are outside it, as a pair inside."""
+    g, bf = torch.Generator().manual_seed(21), torch.bfloat16
+    need = [-(-(n + c) // 64) for n, c in zip(new, ctx)]
+    bt = torch.full((len(new), max(need)), -1, dtype=torch.int32)
+    for b, n in enumerate(need):
+        bt[b, :n] = torch.arange(sum(need[:b]), sum(need[:b]) + n)
+    kc, vc = (torch.randn(sum(need), 64, nk, hd, generator=g).to(bf) for _ in range(2))
+    q = torch.randn(sum(new), nh, hd, generator=g).to(bf)
+    ref, lse, mag = op.packed_attention64(q, kc, vc, new, ctx, bt)
+    got, row = {1: torch.empty_like(ref), 2: torch.empty_like(ref)}, 0
+    for b, (n, c) in enumerate(zip(new, ctx)):
+        for j in range(n):
+            at = torch.arange(c + j + 1)
+            k, v = (x[bt[b].long()[at // 64], at % 64].double() for x in (kc, vc))
+            for h in range(nh):
+                p = torch.exp(k[:, h // (nh // nk)] @ q[row, h].double() / math.sqrt(hd) - lse[row, h])
+                hi = p.to(bf).double()
+                for parts, pr in ((1, hi), (2, hi + (p - hi).to(bf).double())):
+                    got[parts][row, h] = pr @ v[:, h // (nh // nk)]
+            row += 1
+    tol = pair_tolerance(ref, mag, max(n + c for n, c in zip(new, ctx)))
+    assert ((got[2].to(bf).double() - ref).abs() <= tol).all()
+    assert ((got[1].to(bf).double() - ref).abs() > tol).any()
