@@ -3646,7 +3646,7 @@ extern "C" int pkv_prefill_attn(const void* q, int64_t q_sb, int64_t q_ss, int64
 
 namespace pkv {
 // 64 bits that no other call of this process has had, nor likely any memory by chance: a counter from a random start,
-// mixed (a bijection).  Never 0, which is a cleared tag.
+// mixed by the published finaliser of the splitmix64 generator (a bijection).  Never 0, which is a cleared tag.
 static uint64_t random_start() {
   const uint64_t now = uint64_t(std::chrono::steady_clock::now().time_since_epoch().count());
   try {

@@ -520,7 +520,9 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_tile_kernel(const AttnParam
   c = __builtin_amdgcn_readfirstlane(c);
   L = __builtin_amdgcn_readfirstlane(L);
   // PACKED: a chunk's waves go before those of a decode workgroup on the same CU (few_rows), which wait for memory
-  // anyway: 47 decode tokens and two chunks 58.4 -> 55.5 us.  Not at head_dim 64: 208 short chats 19.4 -> 20.4.
+  // anyway: 47 decode tokens and two chunks 47.2 -> 43.5 us (the same inputs over and over); 13 others at head_dim 128
+  // (documents, windows, prompts, decode alone, one to eight KV heads) within 2%.  Not at head_dim 64: 208 short chats
+  // 19.4 -> 20.4.
   constexpr int kPriority = PACKED && HD == 128 ? 1 : 0;
   if constexpr (kPriority > 0) __builtin_amdgcn_s_setprio(kPriority);
   SeqView sv;
