@@ -165,7 +165,7 @@ def _past_weights(shape, g, dev) -> torch.Tensor:
 
 
 def _sample_settings(case: dict, seed: int, dev) -> dict:
-    """temperature, top_k, top_p, min_p: numbers for the whole batch, or a tensor with one for each row."""
+    """temperature, top_k, top_p, min_p (32 bits): numbers for the whole batch, or a tensor with one for each row."""
     if not case["mixed"]:
         return {k: case[k] for k in ("temperature", "top_k", "top_p", "min_p")}
     rng, n = np.random.default_rng(seed + 77), case["rows"]
@@ -302,7 +302,7 @@ def _evict_plain(st: dict):
 def _sample_plain(st: dict):
     x, u, dev = st["logits"].double(), st["uniforms"].double(), st["logits"].device
     n, v = x.shape
-    per_row = lambda a: (a.double() if torch.is_tensor(a) else torch.full((n,), a, dtype=torch.float64, device=dev))[:, None]
+    per_row = lambda a: (a if torch.is_tensor(a) else torch.full((n,), a, dtype=torch.float32, device=dev)).double()[:, None]
     t, k, p, m = (per_row(st["settings"][a]) for a in ("temperature", "top_k", "top_p", "min_p"))
     greedy = t <= 0
     top = x.amax(1, keepdim=True)
@@ -435,7 +435,7 @@ def _sample64(st: dict) -> list:
     at = np.arange(v)
     for i in range(case["rows"]):
         x = st["logits"][i].double().cpu().numpy()
-        t, k, p, m = (float(a[i]) if torch.is_tensor(a) else float(a) for a in
+        t, k, p, m = (float(a[i]) if torch.is_tensor(a) else float(np.float32(a)) for a in
                       (st["settings"][n] for n in ("temperature", "top_k", "top_p", "min_p")))
         order = np.lexsort((at, -x))                        # the largest first, of equal ones the lowest token
         if t <= 0:
