@@ -452,6 +452,81 @@ int pkv_packed_attn(const void* q, int64_t q_st, int64_t q_sh, const void* k_cac
                     int32_t* status, void* stream);
 
 /*
+ * The work list of a pkv_key_weights call, on the host (every pointer here is host memory; nothing is launched).
+ * Sequence b brings new_lens[b] >= 0 tokens behind ctx_lens[b] cached ones; with rows > 0 only the last `rows` of its
+ * new tokens count.  weighed (NULL: ctx_lens): how many of its keys have weights already; the others start from
+ * nothing.  items receives 12 int32 words per item; counts (4 words) the items of its three lists, in the order that
+ * they follow each other in, and the partial sums that the workspace must hold.  items NULL: the counts only.
+ * PKV_ENOSPC where max_items is too few.
+ */
+int pkv_key_weights_plan(const int32_t* new_lens, const int32_t* ctx_lens, const int32_t* weighed, int32_t batch,
+                         int32_t n_heads, int32_t n_kv, int32_t window, int32_t rows, int32_t compute_units,
+                         int32_t* items, int32_t max_items, int32_t* counts);
+
+/* Bytes of workspace a pkv_key_weights call with so many partials needs.  Its contents need not be kept or cleared. */
+size_t pkv_key_weights_workspace_bytes(int32_t partials, int32_t n_kv);
+
+/*
+ * The attention weight that each cached key got from a packed batch's new tokens, added to its sum so far:
+ *   weights[page(t), h, t % page_size] (+)= sum_r sum_i exp(softmax_scale q[r, i] . k[t, h] - lse[r, i])
+ * over the new tokens r that count and see t (causal, with window > 0 the last `window` keys) and the query heads i of
+ * KV head h.  q [tokens, n_heads, head_dim] bf16 and lse (fp32, [tokens, n_heads], the denominators' logarithms) are
+ * pkv_packed_attn's; the keys are in the cache.  weights is fp32 [num_pages, n_kv, page_size] with a page stride.
+ * Keys that the plan lists as not weighed (the new ones) are written, not added to, also where no row sees them.
+ * A row of lse -inf or +inf weighs nothing; masked keys take no part, whatever they hold; a NaN in a row, a key or an
+ * lse makes NaN of the weights of the keys that the row sees, or of that key.  items (device memory, 16-byte aligned)
+ * and the counts are pkv_key_weights_plan's for the same lengths, heads and window; items that do not fit the call are
+ * skipped and flag PKV_STATUS_BAD_PAGE, as is a key that a row sees on a page outside the pool.  Pages of one call
+ * must not be shared by its sequences.  bf16 products, fp32 exponentials and sums, in an order that the list fixes.
+ * No counterpart in the reference, whose pool only ever shrinks by whole sequences (engine/kv_cache.py:87-104).
+ */
+int pkv_key_weights(const void* q, int64_t q_st, int64_t q_sh, const void* k_cache, int64_t cache_page_stride,
+                    const float* lse, int64_t lse_st, float* weights, int64_t weights_page_stride,
+                    const int32_t* block_table, int64_t bt_stride, const int32_t* items, int32_t n_few, int32_t n_many,
+                    int32_t n_merges, int32_t partials, void* workspace, size_t workspace_bytes, int32_t tokens,
+                    int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t page_size,
+                    int32_t num_pages, int32_t max_blocks, int32_t window, float softmax_scale, int32_t* status,
+                    void* stream);
+
+/*
+ * Eviction: of the seq_lens[b] tokens of sequence b (pages block_table[b]), min(keep_lens[b], seq_lens[b]) stay in every
+ * layer and KV head: the first `first`, the last `recent` (as far as they fit, the first ones before them), and of the
+ * others those of the largest weights; of equal weights the earlier token stays, a NaN is above every number.  K, V and
+ * weights of those that stay move, in their order, to the front of the sequence's pages; slots behind them keep what
+ * they hold.  kept (int32 [layers, batch, n_kv, max_keep]) receives the positions, ascending, -1 behind them.  Caches
+ * are bf16 [layers, num_pages, page_size, n_kv, head_dim] with layer and page strides, weights fp32 [layers, num_pages,
+ * n_kv, page_size].  No page may be listed twice in the call.  A sequence whose lengths do not fit the table or
+ * max_keep, or that lists a page outside the pool, is left as it is (kept: -1) and flags PKV_STATUS_BAD_PAGE.
+ * No counterpart in the reference.
+ */
+int pkv_evict(void* k_pool, void* v_pool, int64_t layer_stride, int64_t cache_page_stride, float* weights,
+              int64_t weights_layer_stride, int64_t weights_page_stride, const int32_t* block_table, int64_t bt_stride,
+              const int32_t* seq_lens, const int32_t* keep_lens, int32_t* kept, int32_t layers, int32_t batch,
+              int32_t n_kv, int32_t head_dim, int32_t page_size, int32_t num_pages, int32_t max_blocks,
+              int32_t max_keep, int32_t first, int32_t recent, int32_t* status, void* stream);
+
+/* Bytes of workspace a pkv_sample call of that size needs.  Its contents need not be kept or cleared. */
+size_t pkv_sample_workspace_bytes(int32_t rows, int32_t vocab, int32_t dtype);
+
+/*
+ * The next token of every row of logits [rows, vocab] (PKV_BF16, PKV_FP16 or PKV_FP32; `stride` elements from row to
+ * row).  With w_i = exp((x_i - max x) / temperature) and the tokens in the order (x descending, token ascending): the
+ * first top_k stay (<= 0: all); of those the shortest prefix whose w sum to top_p of theirs (>= 1: all, <= 0: the
+ * first); of those the ones with w_i >= min_p (<= 0: all; more than 1 counts as 1).  tokens[row] = the first token, in
+ * the order of the vocabulary, at which the running sum of the w that stay passes uniforms[row] (0 to 1) times their
+ * sum.  A temperature that is not above 0: the largest logit (of equal ones the lowest token).  Each setting is one
+ * number for all rows, or, where its pointer is not NULL, one a row (device memory).  -inf and NaN logits are never
+ * drawn; where there is no other, tokens[row] = -1 and the logarithm is -inf.  Next to a +inf only its equals weigh
+ * anything.  logprobs (NULL: not wanted): the logarithm of the drawn token's share of the w that stay.  vocab at most
+ * 1000000.  Weights in fp64, sums in fp64 or in integer units of 2^-42 of the largest weight or finer; results repeat
+ * bit for bit.  Replaces the host's argmax and sampling (engine/scheduler.py:266-273).
+ */
+int pkv_sample(const void* logits, int64_t stride, int32_t dtype, const float* uniforms, const float* temperatures,
+               float temperature, const int32_t* top_ks, int32_t top_k, const float* top_ps, float top_p,
+               const float* min_ps, float min_p, int64_t* tokens, float* logprobs, int32_t rows, int32_t vocab,
+               void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * RMSNorm over rows (engine/fused_kernels.py:31-65 fused_rms_norm; called at
  * engine/executor.py:106, :122, :131): out[r] = bf16(h * rsqrt(mean(h^2) + eps) * weight) in
  * fp32, h = x[r], or, when residual is non-NULL, h = bf16(x[r] + residual[r]) (the preceding

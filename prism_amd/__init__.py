@@ -5,7 +5,8 @@ Drop-ins for Prism's engine/kv_cache.py (FlashAttnKVCache), engine/prefix_cache.
 either side of it (QKV split + RoPE, RMSNorm, SiLU-mul; engine/executor.py,
 engine/fused_kernels.py) and a device-resident block table for graph-captured decode batches
 (DecodeBatch, replacing the per-step refill of engine/executor.py:320-356) and the packed step
-of continuous batching (PackedBatch, packed_rope_append, packed_attention; rotate_qk), backed by
+of continuous batching (PackedBatch, packed_rope_append, packed_attention; rotate_qk), eviction of the keys that
+attention weighs least (packed_key_weights, evict_keys), sampling on the device (sample_tokens), backed by
 hand-written gfx950 HIP kernels in libprism_kv.so (C ABI: include/prism_kv.h).  There is no
 CPU path: device ops raise if the library is not built.
 """
@@ -15,9 +16,11 @@ from .attention import (PrismKVStatusError, append_kv, decode_attention, flash_a
 from .decode_batch import DecodeBatch
 from .epilogue import (fused_rms_norm, fused_silu_mul, rms_norm, rope_qk, rope_tables, rotary_tables, rotate_qk,
                        silu_mul)
+from .eviction import evict_keys
 from .kv_cache import FlashAttnKVCache, KVCacheOutOfPages, copy_pages
-from .packed import PackedBatch, packed_attention, packed_rope_append
+from .packed import PackedBatch, packed_attention, packed_key_weights, packed_rope_append
 from .prefix_cache import CachedPrefix, PrefixCache
+from .sampling import sample_tokens
 
 __all__ = [
     "FlashAttnKVCache", "KVCacheOutOfPages", "PrefixCache", "CachedPrefix",
@@ -27,4 +30,5 @@ __all__ = [
     "rope_tables", "rope_qk", "rms_norm", "fused_rms_norm", "silu_mul", "fused_silu_mul",
     "DecodeBatch",
     "PackedBatch", "packed_rope_append", "packed_attention", "rotary_tables", "rotate_qk",
+    "packed_key_weights", "evict_keys", "sample_tokens",
 ]

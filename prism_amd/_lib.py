@@ -173,6 +173,34 @@ _SIGNATURES = {
         _I32, _I32, _I32, _I32, c_float,  # page_size, num_pages, max_blocks, window, scale
         _P, _P,                          # status, stream
     ]),
+    "pkv_key_weights_plan": (c_int32, [_P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P, _I32, _P]),
+    "pkv_key_weights_workspace_bytes": (c_size_t, [_I32] * 2),
+    "pkv_key_weights": (c_int32, [
+        _P, _I64, _I64, _P, _I64,        # q + strides, k_cache
+        _P, _I64, _P, _I64,              # lse, weights
+        _P, _I64,                        # block table
+        _P, _I32, _I32, _I32, _I32,      # items, the three lists' counts, partials
+        _P, c_size_t,                    # workspace
+        _I32, _I32, _I32, _I32, _I32,    # tokens, batch, n_heads, n_kv, head_dim
+        _I32, _I32, _I32, _I32, c_float,  # page_size, num_pages, max_blocks, window, scale
+        _P, _P,                          # status, stream
+    ]),
+    "pkv_evict": (c_int32, [
+        _P, _P, _I64, _I64,              # k_pool, v_pool, layer and page strides
+        _P, _I64, _I64,                  # weights, layer and page strides
+        _P, _I64, _P, _P, _P,            # block table, seq_lens, keep_lens, kept
+        _I32, _I32, _I32, _I32,          # layers, batch, n_kv, head_dim
+        _I32, _I32, _I32, _I32,          # page_size, num_pages, max_blocks, max_keep
+        _I32, _I32, _P, _P,              # first, recent, status, stream
+    ]),
+    "pkv_sample_workspace_bytes": (c_size_t, [_I32] * 3),
+    "pkv_sample": (c_int32, [
+        _P, _I64, _I32, _P,              # logits, stride, dtype, uniforms
+        _P, c_float, _P, _I32,           # temperature, top_k: a row's each or one
+        _P, c_float, _P, c_float,        # top_p, min_p
+        _P, _P, _I32, _I32,              # tokens, logprobs, rows, vocab
+        _P, c_size_t, _P,                # workspace, stream
+    ]),
     "pkv_rms_norm": (c_int32, [
         _P, _I64, _P, _I64, _P, _I64,    # x, residual, h_out
         _P, _P, _I64,                    # weight, out

@@ -21,7 +21,8 @@
 namespace {
 
 // ---- the attached library ----
-#define ENTRIES(X) X(pkv_rotate_qk) X(pkv_packed_rope_append) X(pkv_packed_attn) X(pkv_packed_workspace_bytes) X(pkv_last_error)
+#define ENTRIES(X) X(pkv_rotate_qk) X(pkv_packed_rope_append) X(pkv_packed_attn) X(pkv_packed_workspace_bytes) \
+  X(pkv_key_weights) X(pkv_key_weights_workspace_bytes) X(pkv_sample) X(pkv_sample_workspace_bytes) X(pkv_last_error)
 #define DECLARE(name) decltype(&::name) lib_##name = nullptr;
 ENTRIES(DECLARE)
 PyObject* g_error = nullptr;  // PrismKVError
@@ -370,6 +371,124 @@ PyObject* packed_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// packed_key_weights(q, k_cache, lse, key_weights, batch, plan (window, items, the lists' three counts, partials),
+// softmax_scale or None, status, stream)
+PyObject* packed_key_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9) return PyErr_Format(PyExc_TypeError, "packed_key_weights takes 9 arguments");
+  try {
+    const at::Tensor &q = tensor(a[0], "q"), &kc = tensor(a[1], "k_cache"), &lse = tensor(a[2], "lse"),
+                     &w = tensor(a[3], "key_weights");
+    const Batch& b = batch_of(a[4]);
+    const Rows qr = check_rows(q, "q", b);
+    int32_t* const status = status_word(a[7], b.device);
+    const int64_t page_stride = check_cache(kc, kc, b);
+    on_gpu(lse, "lse");
+    if (lse.scalar_type() != at::kFloat || lse.dim() != 2 || lse.size(0) < b.tokens || lse.size(1) != b.n_heads ||
+        (b.n_heads > 1 && lse.stride(1) != 1) || (b.tokens > 1 && lse.stride(0) < b.n_heads))
+      refuse(c10::str("lse must be float32 [>= ", b.tokens, ", ", b.n_heads, "], contiguous in its last dimension, got ",
+                      shape_of(lse)));
+    on_device(lse, "lse", b.device);
+    on_gpu(w, "key_weights");
+    if (w.scalar_type() != at::kFloat || w.dim() != 3 || w.size(0) < b.num_pages || w.size(1) != b.n_kv ||
+        w.size(2) != b.page_size || w.stride(2) != 1 || (b.n_kv > 1 && w.stride(1) != b.page_size) ||
+        (w.size(0) > 1 && w.stride(0) < b.n_kv * b.page_size))
+      refuse(c10::str("key_weights must be float32 [>= ", b.num_pages, ", ", b.n_kv, ", ", b.page_size,
+                      "], contiguous within a page, got ", shape_of(w)));
+    on_device(w, "key_weights", b.device);
+    if (!PyTuple_Check(a[5]) || PyTuple_GET_SIZE(a[5]) != 6) refuse("a plan of key weights has 6 entries");
+    int64_t plan[6];
+    for (int i = 0; i < 6; ++i) plan[i] = integer(PyTuple_GET_ITEM(a[5], i));
+    const double scale = given(a[6]) ? real(a[6]) : 1.0 / std::sqrt(double(b.head_dim));
+    if (b.tokens > 0) {
+      // the partial sums of this call alone, from torch's allocator: of the current stream, or of the graph it captures
+      at::Tensor ws;
+      const size_t bytes = lib_pkv_key_weights_workspace_bytes(int32_t(plan[5]), int32_t(b.n_kv));
+      if (bytes) ws = at::empty({int64_t(bytes)}, at::TensorOptions().dtype(at::kByte).device(b.device));
+      check(lib_pkv_key_weights(
+                q.data_ptr(), qr.token, qr.head, kc.data_ptr(), page_stride, lse.data_ptr<float>(),
+                b.tokens > 1 ? lse.stride(0) : b.n_heads, w.data_ptr<float>(),
+                w.size(0) > 1 ? w.stride(0) : b.n_kv * b.page_size, b.block_table, b.max_blocks,
+                reinterpret_cast<const int32_t*>(plan[1]), int32_t(plan[2]), int32_t(plan[3]), int32_t(plan[4]),
+                int32_t(plan[5]), bytes ? ws.data_ptr() : nullptr, bytes, int32_t(b.tokens), int32_t(b.batch),
+                int32_t(b.n_heads), int32_t(b.n_kv), int32_t(b.head_dim), int32_t(b.page_size), int32_t(b.num_pages),
+                int32_t(b.max_blocks), int32_t(plan[0]), float(scale), status, address(a[8])),
+            "pkv_key_weights");
+    }
+    return THPVariable_Wrap(w);
+  } catch (const Failed&) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// A setting: a number for every row, or a tensor with one a row.
+struct Setting {
+  const void* rows = nullptr;
+  double all = 0;
+};
+Setting setting(PyObject* o, const char* name, double none, bool whole, int64_t rows, c10::Device d) {
+  if (!given(o)) return {nullptr, none};
+  if (!THPVariable_Check(o)) {
+    if (whole) {
+      const int64_t v = integer(o);
+      return {nullptr, double(v < 0 ? 0 : v > 0x7fffffff ? 0x7fffffff : v)};
+    }
+    const double v = real(o);
+    if (std::isnan(v)) refuse(c10::str(name, " is not a number"));
+    return {nullptr, v};
+  }
+  const at::Tensor& t = THPVariable_Unpack(o);
+  const auto type = whole ? at::kInt : at::kFloat;
+  if (t.scalar_type() != type || t.dim() != 1 || t.size(0) != rows || !t.is_contiguous() || t.device() != d)
+    refuse(c10::str(name, " must be a number, or contiguous ", type, " [", rows, "] on ", d, ", got ", shape_of(t), " on ",
+                    t.device()));
+  return {t.data_ptr(), 0};
+}
+
+// sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p, return_logprobs, stream)
+PyObject* sample_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8) return PyErr_Format(PyExc_TypeError, "sample_tokens takes 8 arguments");
+  try {
+    const at::Tensor &x = tensor(a[0], "logits"), &u = tensor(a[1], "uniforms");
+    on_gpu(x, "logits");
+    const auto dtype = x.scalar_type();
+    const int code = dtype == at::kBFloat16 ? PKV_BF16 : dtype == at::kHalf ? PKV_FP16 : dtype == at::kFloat ? PKV_FP32 : -1;
+    if (code < 0) refuse(c10::str("logits must be bfloat16, float16 or float32, got ", dtype));
+    if (x.dim() != 2 || x.size(1) < 1 || (x.size(1) > 1 && x.stride(1) != 1) || (x.size(0) > 1 && x.stride(0) < x.size(1)))
+      refuse(c10::str("logits must be [rows, vocab], contiguous in vocab and not empty there, got ", shape_of(x)));
+    const int64_t rows = x.size(0), vocab = x.size(1);
+    if (vocab > 1000000 || rows > 65535) refuse(c10::str("at most 65535 rows of 1000000 tokens, got ", x.sizes()));
+    const c10::Device dev = x.device();
+    if (u.scalar_type() != at::kFloat || u.dim() != 1 || u.size(0) != rows || !u.is_contiguous() || u.device() != dev)
+      refuse(c10::str("uniforms must be contiguous float32 [", rows, "] on ", dev, ", got ", shape_of(u), " on ", u.device()));
+    const Setting t = setting(a[2], "temperature", 1.0, false, rows, dev), k = setting(a[3], "top_k", 0.0, true, rows, dev),
+                  p = setting(a[4], "top_p", 1.0, false, rows, dev), m = setting(a[5], "min_p", 0.0, false, rows, dev);
+    if (!t.rows && t.all < 0) refuse("temperature must not be negative (0: the largest logit)");
+    const bool logs = truth(a[6]);
+    at::Tensor tokens = at::empty({rows}, at::TensorOptions().dtype(at::kLong).device(dev)), lp;
+    if (logs) lp = at::empty({rows}, at::TensorOptions().dtype(at::kFloat).device(dev));
+    if (rows > 0) {
+      // of this call alone, from torch's allocator: of the current stream, or of the graph it captures
+      const size_t bytes = lib_pkv_sample_workspace_bytes(int32_t(rows), int32_t(vocab), code);
+      at::Tensor ws = at::empty({int64_t(bytes)}, at::TensorOptions().dtype(at::kByte).device(dev));
+      check(lib_pkv_sample(x.data_ptr(), rows > 1 ? x.stride(0) : vocab, code, u.data_ptr<float>(),
+                           static_cast<const float*>(t.rows), float(t.all), static_cast<const int32_t*>(k.rows),
+                           int32_t(k.all), static_cast<const float*>(p.rows), float(p.all),
+                           static_cast<const float*>(m.rows), float(m.all),
+                           tokens.data_ptr<int64_t>(), logs ? lp.data_ptr<float>() : nullptr, int32_t(rows),
+                           int32_t(vocab), ws.data_ptr(), bytes, address(a[7])),
+            "pkv_sample");
+    }
+    if (!logs) return THPVariable_Wrap(tokens);
+    return Py_BuildValue("(NN)", THPVariable_Wrap(tokens), THPVariable_Wrap(lp));
+  } catch (const Failed&) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
 // attach(handle of a loaded libprism_kv.so, the exception class for its errors)
 PyObject* attach(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 2) return PyErr_Format(PyExc_TypeError, "attach takes 2 arguments");
@@ -386,7 +505,7 @@ PyObject* attach(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(attach), METHOD(rotate_qk), METHOD(new_batch), METHOD(packed_rope_append),
-                         METHOD(packed_attention), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(packed_attention), METHOD(packed_key_weights), METHOD(sample_tokens), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_fastcall", "per-layer calls into libprism_kv.so", -1, methods,
                           nullptr, nullptr, nullptr, nullptr};
 

@@ -63,11 +63,17 @@ class PackedBatch:
     stream, use it behind this one, as any tensor made here; calls there keep its memory until they have run, and a
     call that a graph captures keeps it (a replay reads it, whether the batch lives or not) until ``release``.
 
+    ``evicted[b]`` tokens of the sequence are not in the cache any more (evict_keys): its positions go on behind them.
+    ``weight_rows`` other than 0 lays the batch out for packed_key_weights too: None, every new token's weights count;
+    n, those of each sequence's last n.  ``weighed[b]`` of the cached keys have weights already (all, where it is not
+    given).  The sequences of such a batch share no page.
+
     A page that a new token is written to must belong to one sequence alone, and every page that a token is written
     to or sees must be one of the pool's; columns behind them, or out of every window, may hold anything."""
 
     def __init__(self, new_lens, cache_lens, block_table, *, page_size: int, num_pages: int, n_heads: int, n_kv: int,
-                 head_dim: int, windows: Sequence[int | None] = (None,), device: torch.device | str = "cuda"):
+                 head_dim: int, windows: Sequence[int | None] = (None,), weight_rows: int | None = 0,
+                 weighed=None, evicted=None, device: torch.device | str = "cuda"):
         device = torch.device(device)
         if device.type == "cuda":
             if device.index is None:
@@ -89,6 +95,13 @@ class PackedBatch:
         for w in windows:
             if w is not None and (isinstance(w, bool) or not isinstance(w, (int, np.integer)) or not 1 <= w <= _MAX_KEYS):
                 raise RuntimeError(f"window {w!r} must be None or 1 to 2^27 keys")
+        if weight_rows is not None and (isinstance(weight_rows, bool) or not isinstance(weight_rows, (int, np.integer))
+                                        or not 0 <= weight_rows <= _MAX_KEYS):
+            raise RuntimeError(f"weight_rows {weight_rows!r} must be None (every new token) or 0 to 2^27 tokens")
+        had, gone = (None if x is None else _host_ints(x, name, 1) for x, name in ((weighed, "weighed"), (evicted, "evicted")))
+        for x, name in ((had, "weighed"), (gone, "evicted")):
+            if x is not None and (len(x) != len(new) or (len(x) and x.min() < 0)):
+                raise RuntimeError(f"{name} must have one number, not negative, for each of the {len(new)} sequences")
         self.batch, self.total_tokens = len(new), int(new.sum(dtype=np.int64))
         self.page_size, self.num_pages = page_size, num_pages
         self.n_heads, self.n_kv, self.head_dim, self.device = n_heads, n_kv, head_dim, device
@@ -101,9 +114,21 @@ class PackedBatch:
         widest = 0 if any(w is None for w in windows) else max(windows)
         _lib.check(lib.pkv_packed_layout(*lengths, bt.ctypes.data, bt.shape[1], bt.shape[1], page_size, num_pages, widest,
                                          where[0].ctypes.data, where[1].ctypes.data), "pkv_packed_layout")
+        if gone is not None and total > 0:
+            if any(w is not None for w in windows) and (gone[new > 0] > 0).any():
+                raise RuntimeError("a window counts positions, which an evicted sequence's cached keys do not have any more")
+            if int((ctx.astype(np.int64) + new + gone).max()) > _MAX_KEYS:
+                raise RuntimeError("cached, new and evicted tokens of a sequence: at most 2^27 together")
+            where[0] += np.repeat(gone, new)
         cus = torch.cuda.get_device_properties(device).multi_processor_count if device.type == "cuda" else 256
         plans = {w: self._plan(lengths, w, cus) for w in dict.fromkeys(windows)}
+        weight_plans = {}
+        if weight_rows != 0:
+            self._check_apart(new, ctx, had, bt, widest, int(weight_rows or 0))
+            weight_plans = {w: self._weight_plan(lengths, had, w, int(weight_rows or 0), cus) for w in plans}
         parts = [where[0], where[1], bt.ravel()] + [a.ravel() for items, merges, _ in plans.values() for a in (items, merges)]
+        after = len(parts)
+        parts += [items.ravel() for items, _ in weight_plans.values()]
         starts = np.cumsum([0] + [-(-p.size // 4) * 4 for p in parts])     # 16-byte aligned
         staged = torch.empty(int(starts[-1]) + 4, dtype=torch.int32, pin_memory=device.type == "cuda")
         host = staged.numpy()
@@ -120,6 +145,9 @@ class PackedBatch:
         self._plans = {w: (int(w or 0), base + 4 * int(starts[3 + 2 * i]), len(items), base + 4 * int(starts[4 + 2 * i]),
                            len(merges), int(counts[2]), int(counts[3]))
                        for i, (w, (items, merges, counts)) in enumerate(plans.items())}
+        # the same for the weights: window, items, the number of each of their lists, partials
+        self._weight_plans = {w: (int(w or 0), base + 4 * int(starts[after + i]), *map(int, counts))
+                              for i, (w, (_, counts)) in enumerate(weight_plans.items())}
         self._captured = False
         self._native = _lib.fast().new_batch(self._buf, total, self.batch, n_heads, n_kv, head_dim, page_size, num_pages,
                                              self.max_blocks, self.positions.data_ptr(), self.slots.data_ptr(),
@@ -155,6 +183,33 @@ class PackedBatch:
             room = int(counts[:2].max())
         _lib.check(rc, "pkv_packed_plan")
         return items[:counts[0]], merges[:counts[1]], counts
+
+
+    def _weight_plan(self, lengths, weighed, window, rows, cus):
+        lib = _lib.load()
+        counts = np.zeros(4, np.int32)
+        sizes = (*lengths[:2], 0 if weighed is None else weighed.ctypes.data, self.batch, self.n_heads, self.n_kv,
+                 int(window or 0), rows, cus)
+        _lib.check(lib.pkv_key_weights_plan(*sizes, 0, 0, counts.ctypes.data), "pkv_key_weights_plan")
+        items = np.empty((int(counts[:3].sum()), 12), np.int32)
+        if len(items):
+            _lib.check(lib.pkv_key_weights_plan(*sizes, items.ctypes.data, len(items), counts.ctypes.data),
+                       "pkv_key_weights_plan")
+        return items, counts
+
+    def _check_apart(self, new, ctx, weighed, bt, widest, rows):
+        """The pages whose keys get weights belong to one sequence each: a key's sum is nobody else's."""
+        end = ctx.astype(np.int64) + new
+        first = np.zeros_like(end)
+        if widest > 0:
+            count = np.minimum(new, rows) if rows > 0 else new
+            first = np.minimum(np.maximum(end - count - widest + 1, 0), ctx if weighed is None else np.minimum(weighed, ctx))
+        col = np.arange(bt.shape[1])[None]
+        used = bt[(new > 0)[:, None] & (col >= (first // self.page_size)[:, None]) & (col < (-(-end // self.page_size))[:, None])]
+        used = used[used >= 0]
+        if len(np.unique(used)) < len(used):
+            raise RuntimeError("two sequences of the batch share a page (or one is in it twice): their keys' weights "
+                               "cannot be taken in one step")
 
 
 def packed_rope_append(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, batch: PackedBatch,
@@ -200,3 +255,26 @@ def packed_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         batch._used_on(stream)
         return _lib.fast().packed_attention(q, k_cache, v_cache, batch._native, plan, sinks, softmax_scale, return_lse,
                                             out, status if status is not None else status_tensor(dev), stream)
+
+
+def packed_key_weights(q: torch.Tensor, k_cache: torch.Tensor, lse: torch.Tensor, key_weights: torch.Tensor,
+                       batch: PackedBatch, *, window: int | None = None, softmax_scale: float | None = None,
+                       status: torch.Tensor | None = None) -> torch.Tensor:
+    """Adds to ``key_weights`` (fp32 [num_pages, n_kv, page_size], the cache's pages) the attention weight that every
+    cached key got from the batch's new tokens, summed over them and over the query heads of each KV head, and
+    returns it: what evict_keys goes by.
+
+    ``q``, ``window`` and ``softmax_scale`` are packed_attention's, and ``lse`` (fp32 [tokens, n_heads]) what it
+    returned with ``return_lse``.  Which tokens count, and which keys start from nothing (this step's own), the batch
+    knows: it was laid out with ``weight_rows``.  A row whose lse is infinite weighs nothing."""
+    dev = batch.device
+    _require_gpu(q, "q")
+    plan = batch._weight_plans.get(window)
+    if plan is None:
+        raise RuntimeError("the batch was laid out without weight_rows" if not batch._weight_plans else
+                           f"the batch was laid out for the windows {list(batch._weight_plans)}, not {window}")
+    stream = _raw_stream(dev.index)
+    with _on(dev):
+        batch._used_on(stream)
+        return _lib.fast().packed_key_weights(q, k_cache, lse, key_weights, batch._native, plan, softmax_scale,
+                                              status if status is not None else status_tensor(dev), stream)

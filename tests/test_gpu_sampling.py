@@ -1,0 +1,210 @@
+"""sample_tokens on the device against fp64."""
+import numpy as np
+import pytest
+import torch
+
+import prism_amd
+from oracle import behind as ob
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _expect(x, u, t, k, p, m, got, logs, what):
+    """Equal tokens.  The kernel's sums are within 2^-30 of the oracle's share (weights in fp64 or integers of 2^-42 of the
+    largest, 2^20 of them at most): a number that lies nearer to a border than that decides nothing."""
+    x, n = x.double().cpu().numpy(), len(u)
+    per = lambda a: a.double().cpu().numpy() if torch.is_tensor(a) else np.full(n, np.float64(np.float32(a if a is not None else 0)))
+    t, k, p, m = per(t), per(k), per(1.0 if p is None else p), per(m)
+    u = u.double().cpu().numpy()
+    got, logs = got.cpu().numpy(), None if logs is None else logs.double().cpu().numpy()
+    for i in range(n):
+        token, lp, near = ob.sample64(x[i], u[i], t[i], int(k[i]), p[i], m[i])
+        if near < 2.0 ** -30:
+            continue
+        assert got[i] == token, f"{what} row {i}: {got[i]}, not {token} (t {t[i]} k {k[i]} p {p[i]} m {m[i]} u {u[i]})"
+        if logs is not None:
+            # the sum of the weights to 2^-30, the result rounded to fp32
+            assert logs[i] == lp or abs(logs[i] - lp) <= 2.0 ** -29 + 2.0 ** -23 * abs(lp), f"{what} row {i}: {logs[i]} not {lp}"
+
+
+def _draw(x, u, what, *, temperature=1.0, top_k=None, top_p=None, min_p=None):
+    print(what, tuple(x.shape), x.dtype, flush=True)
+    got, logs = prism_amd.sample_tokens(x, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p,
+                                        return_logprobs=True)
+    _expect(x, u, temperature, top_k, top_p, min_p, got, logs, what)
+    again = prism_amd.sample_tokens(x, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    assert torch.equal(again, got), f"{what}: another token with the same number"
+    return got
+
+
+def _logits(gpu, rows, vocab, dtype, seed, spread=2.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, vocab, generator=g) * spread
+    for i in range(rows):
+        at = torch.randperm(vocab, generator=g)[:min(30, vocab)]
+        x[i, at] = 4 + torch.rand(len(at), generator=g) * 8
+    return x.to(dtype).to(gpu), torch.rand(rows, generator=g).to(gpu)
+
+
+RULES = {
+    "plain": dict(),
+    "cool": dict(temperature=0.6),
+    "greedy": dict(temperature=0.0),
+    "k": dict(top_k=50),
+    "k1": dict(top_k=1),
+    "p": dict(top_p=0.9),
+    "m": dict(min_p=0.05),
+    "kp": dict(temperature=0.8, top_k=40, top_p=0.95),
+    "kpm": dict(temperature=1.2, top_k=400, top_p=0.9, min_p=0.02),
+    "pm": dict(top_p=0.99, min_p=0.001),
+    "wide k": dict(top_k=900, temperature=3.0),
+    "wide p": dict(top_p=0.999, temperature=4.0),
+    "wide m": dict(min_p=1e-4, temperature=2.0),
+    "narrow": dict(top_p=1e-6),
+    "first": dict(top_p=0.0),
+    "top only": dict(min_p=1.0),
+}
+
+
+@pytest.mark.parametrize("rules", list(RULES))
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("vocab", [1, 2, 17, 1000, 4096, 32000, 151003])
+def test_rules(gpu, rules, dtype, vocab):
+    rows = 3 if vocab > 100000 else 12
+    x, u = _logits(gpu, rows, vocab, dtype, seed=vocab)
+    _draw(x, u, f"{rules} {vocab}", **RULES[rules])
+
+
+@pytest.mark.parametrize("rules", ["plain", "kp", "p", "wide p", "wide k", "m"])
+def test_flat_rows(gpu, rules):
+    """Nothing stands out: what stays are tens of thousands of tokens, far more than the lists hold; all equal, the cut
+    is among equals."""
+    for dtype, vocab in ((torch.float32, 100003), (torch.bfloat16, 50000)):
+        x, u = _logits(gpu, 4, vocab, dtype, seed=9, spread=0.3)
+        x[:] = x.clamp(max=1.0)
+        x[1] = 0.25
+        x[2] = torch.where(x[2] > 0, 1.0, -1.0).to(dtype)
+        for more in (dict(), dict(top_k=30000), dict(top_p=0.7), dict(top_k=20000, top_p=0.5, min_p=0.1)):
+            _draw(x, u, f"flat {rules}", **{**RULES[rules], **more})
+
+
+def test_masked_rows(gpu):
+    """-inf, NaN and the type's lowest value as masks; rows with one token left, or none; +inf."""
+    for dtype in DTYPES:
+        x, u = _logits(gpu, 9, 9001, dtype, seed=3)
+        x[0] = -float("inf")
+        x[1] = float("nan")
+        x[2, :] = -float("inf")
+        x[2, 8999] = -3.0
+        x[3, 100:] = float("nan")
+        x[4, ::2] = torch.finfo(dtype).min
+        x[5, 1:] = torch.finfo(dtype).min
+        x[6, [5, 4097, 9000]] = float("inf")
+        x[7, 4000:] = -float("inf")
+        x[8] = torch.finfo(dtype).min
+        for name, rules in RULES.items():
+            got = _draw(x, u, f"masked {name}", **rules)
+            assert got[0] == -1 and got[1] == -1 and got[2] == 8999
+            assert int(got[6]) in (5, 4097, 9000)
+
+
+def test_ties_go_to_the_lowest_token(gpu):
+    x = torch.zeros(6, 20000, device=gpu)
+    u = torch.tensor([0.0, 0.999999, 0.5, 0.3, 0.0, 1.0], device=gpu)
+    assert _draw(x, u, "ties", temperature=0.0).tolist() == [0] * 6
+    got = _draw(x, u, "ties", top_k=10)
+    assert got.tolist() == [0, 9, 5, 3, 0, 9]
+    x[:, 7000:7005] = 1.0
+    assert _draw(x, u, "ties", top_k=2).tolist() == [7000, 7001, 7001, 7000, 7000, 7001]
+    assert _draw(x, u, "ties", temperature=0.0).tolist() == [7000] * 6
+    _draw(x, u, "ties", top_p=0.3)
+
+
+def test_numbers_at_the_ends(gpu):
+    x, _ = _logits(gpu, 6, 5000, torch.float32, seed=4)
+    u = torch.tensor([0.0, 1.0, 1.0 - 2.0 ** -24, 2.0 ** -24, -3.0, 7.0], device=gpu)
+    for name in ("plain", "k", "p", "kpm", "wide p"):
+        _draw(x, u, f"ends {name}", **RULES[name])
+    # the last tokens have no weight at all: 1.0 does not reach them
+    x[:, 4000:] = -1e6
+    got = _draw(x, u, "ends", temperature=0.5)
+    assert int(got.max()) < 4000
+    assert prism_amd.sample_tokens(x, u * float("nan")).tolist() == prism_amd.sample_tokens(x, u * 0).tolist()
+
+
+def test_settings_of_each_row(gpu):
+    rows = 40
+    rng = np.random.default_rng(6)
+    x, u = _logits(gpu, rows, 33001, torch.float32, seed=6)
+    t = torch.from_numpy(rng.choice([0.0, 0.5, 1.0, 2.0, -1.0], rows).astype(np.float32)).to(gpu)
+    k = torch.from_numpy(rng.choice([0, -5, 1, 30, 700, 33000, 33001, 10 ** 9], rows).astype(np.int32)).to(gpu)
+    p = torch.from_numpy(rng.choice([0.0, 0.5, 0.95, 1.0, 2.0], rows).astype(np.float32)).to(gpu)
+    m = torch.from_numpy(rng.choice([0.0, -1.0, 0.01, 0.3, 5.0], rows).astype(np.float32)).to(gpu)
+    _draw(x, u, "rows", temperature=t, top_k=k, top_p=p, min_p=m)
+    _draw(x, u, "rows", temperature=0.7, top_k=k, top_p=0.9, min_p=m)
+
+
+def test_extreme_temperatures(gpu):
+    x, u = _logits(gpu, 5, 3001, torch.float32, seed=11)
+    x[4, :5] = torch.tensor([3e38, 3e38, 2.9e38, -3e38, 0.0])
+    for t in (1e-45, 1e-30, 1e-3, 1e3, 1e30, float("inf")):
+        for more in (dict(), dict(top_k=20), dict(top_p=0.5), dict(min_p=0.1)):
+            _draw(x, u, f"t {t}", temperature=t, **more)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_strided_rows_at_any_alignment(gpu, dtype):
+    wide, u = _logits(gpu, 5, 10007, dtype, seed=12)
+    for off, n in ((0, 10007), (1, 10006), (3, 9999), (7, 1), (5, 4097), (2, 31)):
+        x = wide[:, off:off + n]
+        for name in ("plain", "kp", "p", "greedy", "wide p"):
+            _draw(x, u, f"offset {off} {name}", **RULES[name])
+
+
+@pytest.mark.parametrize("vocab", [262145, 999999, 1000000])
+def test_large_vocabularies(gpu, vocab):
+    x, u = _logits(gpu, 2, vocab, torch.bfloat16, seed=13)
+    for name in ("plain", "kp", "p", "wide p", "greedy"):
+        _draw(x, u, f"large {name}", **RULES[name])
+
+
+def test_many_rows_and_none(gpu):
+    x, u = _logits(gpu, 700, 999, torch.float32, seed=14)
+    _draw(x, u, "many", top_k=20, top_p=0.9)
+    _draw(x, u, "many")
+    empty = prism_amd.sample_tokens(x[:0], u[:0])
+    assert empty.shape == (0,) and empty.dtype == torch.int64
+
+
+def test_the_draws_follow_the_distribution(gpu):
+    """Numbers on a fine grid: each token is drawn as often as its share says, to one grid step at either end."""
+    n = 20000
+    x = torch.tensor([0.5, -1.0, 2.0, -float("inf"), 1.0, 1.9, -4.0], device=gpu).expand(n, 7).contiguous()
+    u = (torch.arange(n, device=gpu) + 0.5) / n
+    got = prism_amd.sample_tokens(x, u, temperature=0.7, top_k=4)
+    share = torch.zeros(7, dtype=torch.float64)
+    kept = torch.tensor([0, 2, 4, 5])
+    share[kept] = torch.softmax(x[0, kept.to(gpu)].double().cpu() / float(np.float32(0.7)), 0)
+    count = torch.bincount(got.cpu(), minlength=7).double()
+    assert (count - share * n).abs().max() <= 2.0
+
+
+def test_streams_and_graphs(gpu):
+    x, u = _logits(gpu, 16, 40001, torch.bfloat16, seed=15)
+    eager = prism_amd.sample_tokens(x, u, top_p=0.9)
+    side = torch.cuda.Stream(gpu)
+    side.wait_stream(torch.cuda.current_stream(gpu))
+    with torch.cuda.stream(side):
+        other = prism_amd.sample_tokens(x, u, top_p=0.9)
+    side.synchronize()
+    assert torch.equal(eager, other)
+    graph, v = torch.cuda.CUDAGraph(), u.clone()
+    with torch.cuda.graph(graph):
+        tokens, logs = prism_amd.sample_tokens(x, v, top_p=0.9, return_logprobs=True)
+    for i in range(4):
+        v.copy_((u + 0.17 * i) % 1.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        want, want_logs = prism_amd.sample_tokens(x, v, top_p=0.9, return_logprobs=True)
+        assert torch.equal(tokens, want) and torch.equal(logs, want_logs)
