@@ -495,7 +495,7 @@ int pkv_key_weights(const void* q, int64_t q_st, int64_t q_sh, const void* k_cac
  * weights of those that stay move, in their order, to the front of the sequence's pages; slots behind them keep what
  * they hold.  kept (int32 [layers, batch, n_kv, max_keep]) receives the positions, ascending, -1 behind them.  Caches
  * are bf16 [layers, num_pages, page_size, n_kv, head_dim] with layer and page strides, weights fp32 [layers, num_pages,
- * n_kv, page_size].  No page may be listed twice in the call.  A sequence whose lengths do not fit the table or
+ * n_kv, page_size].  A page that kept tokens move into must not be listed anywhere else in the call.  A sequence whose lengths do not fit the table or
  * max_keep, or that lists a page outside the pool, is left as it is (kept: -1) and flags PKV_STATUS_BAD_PAGE.
  * No counterpart in the reference.
  */

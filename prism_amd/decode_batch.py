@@ -65,6 +65,9 @@ class DecodeBatch:
             raise ValueError(f"{n_seq} sequences in a batch of {gb} rows (at most {self.max_batch})")
         if len(set(seq_ids)) != n_seq:
             raise ValueError("a sequence appears in two rows")
+        if kv.seq_evicted and any(sid in kv.seq_evicted for sid in seq_ids):
+            raise RuntimeError("tokens were evicted from a sequence: cache_seqlens are not its positions any more "
+                               "(build_packed_batch counts them)")
         if kv.null_page != self.null_page:
             # compact() moved the pool: a fresh null page, every row rewritten
             self.null_page = kv.reserve_null_page()

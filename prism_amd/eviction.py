@@ -41,7 +41,8 @@ def evict_keys(k_pool: torch.Tensor, v_pool: torch.Tensor, key_weights: torch.Te
 
     Pools are [layers, num_pages, page_size, n_kv, head_dim], bf16, weights fp32 [layers, num_pages, n_kv, page_size],
     the table and the lengths int32 on their device; ``max_keep`` bounds what stays of any sequence.  Returns the kept
-    positions, int32 [layers, batch, n_kv, max_keep], ascending, -1 behind them.  No page may be listed twice."""
+    positions, int32 [layers, batch, n_kv, max_keep], ascending, -1 behind them.  A page that kept tokens move into must not
+    be listed anywhere else in the call."""
     ks, vs = _pool_strides(k_pool, "k_pool"), _pool_strides(v_pool, "v_pool")
     dev = k_pool.device
     if v_pool.shape != k_pool.shape or vs != ks or v_pool.device != dev:

@@ -29,7 +29,9 @@ Deliberate differences (each fixes a defect of the reference or extends it):
     (PKV_STATUS_BAD_PAGE) instead of landing in page 0, the first page the allocator hands out;
   * transfer_sequence moves all pages of all layers with one kernel launch (the reference issues
     2 * L * pages copy_ calls, :189-207); migrate_to / compact move every live page (sequences
-    and prefix-cache pages) into another pool, packed, rewriting page ids everywhere.
+    and prefix-cache pages) into another pool, packed, rewriting page ids everywhere;
+  * evict cuts live sequences down to a budget of tokens, dropping the keys that attention weighed least
+    (enable_key_weights, packed_key_weights), and takes their pages back.
 """
 from __future__ import annotations
 
@@ -38,6 +40,7 @@ import torch
 
 from . import _lib
 from .attention import poll_status, status_tensor
+from .eviction import evict_keys
 from .packed import PackedBatch
 
 
@@ -82,6 +85,13 @@ class FlashAttnKVCache:
         self.seq_len: dict[int, int] = {}
         self.seq_owner: dict[int, str] = {}
         self._holders: dict[int, int] = {}     # page -> number of live sequences listing it
+        # tokens that evict() took out of a sequence: its positions go on behind them (sequences without are absent)
+        self.seq_evicted: dict[int, int] = {}
+        # per layer, the attention weight of every cached key, fp32 [max_pages, n_kv, page_size] (enable_key_weights);
+        # of a sequence's keys, the first _weighed[seq] have theirs
+        self.key_weight_pool: torch.Tensor | None = None
+        self.key_weights: list[torch.Tensor] = []
+        self._weighed: dict[int, int] = {}
         self.prefix_cache = None               # set by PrefixCache(kv)
         self._bases: torch.Tensor | None = None
         self.null_page: int | None = None      # reserve_null_page()
@@ -161,6 +171,7 @@ class FlashAttnKVCache:
         self.seq_pages[seq_id] = pages
         self.seq_len[seq_id] = prefix_len if prefix_pages else 0
         self.seq_owner[seq_id] = owner
+        self._weighed[seq_id] = self.seq_len[seq_id]
 
     def fork_sequence(self, src_seq_id: int, dst_seq_id: int, owner: str | None = None) -> None:
         """dst shares every page of src (no copy); the first write into a shared page copies it.
@@ -175,6 +186,12 @@ class FlashAttnKVCache:
         self.seq_pages[dst_seq_id] = pages
         self.seq_len[dst_seq_id] = self.seq_len[src_seq_id]
         self.seq_owner[dst_seq_id] = self.seq_owner.get(src_seq_id, "") if owner is None else owner
+        self._copy_eviction_state(src_seq_id, self, dst_seq_id)
+
+    def _copy_eviction_state(self, src_seq_id: int, target: "FlashAttnKVCache", dst_seq_id: int) -> None:
+        target._weighed[dst_seq_id] = self._weighed.get(src_seq_id, 0)
+        if src_seq_id in self.seq_evicted:
+            target.seq_evicted[dst_seq_id] = self.seq_evicted[src_seq_id]
 
     def free_sequence(self, seq_id: int) -> None:
         if seq_id in self.seq_pages:
@@ -182,6 +199,8 @@ class FlashAttnKVCache:
                 self._release(p)
             del self.seq_len[seq_id]
             self.seq_owner.pop(seq_id, None)
+            self.seq_evicted.pop(seq_id, None)
+            self._weighed.pop(seq_id, None)
 
     def free_model_sequences(self, model_name: str) -> None:
         for sid in [s for s, o in self.seq_owner.items() if o == model_name]:
@@ -192,6 +211,8 @@ class FlashAttnKVCache:
         self.seq_pages.clear()
         self.seq_len.clear()
         self.seq_owner.clear()
+        self.seq_evicted.clear()
+        self._weighed.clear()
         self._holders.clear()
         if self.prefix_cache is not None:
             self.prefix_cache.clear()
@@ -263,6 +284,7 @@ class FlashAttnKVCache:
         dst = [c[1] for c in cow]
         fill = [c[2] for c in cow]
         copy_pages(self, self, src, dst, fill)
+        copy_key_weights(self, self, src, dst)
 
     # ------------------------------------------------------------------ block tables
     def block_table_host(self, seq_ids: list[int]) -> tuple[np.ndarray, np.ndarray]:
@@ -309,10 +331,14 @@ class FlashAttnKVCache:
         return bt, sl
 
     def build_packed_batch(self, seq_ids: list[int], num_new_tokens: int | list[int], n_heads: int,
-                           windows=(None,)) -> PackedBatch:
+                           windows=(None,), weight_rows: int | None = 0) -> PackedBatch:
         """The step's PackedBatch: num_new_tokens[i] tokens of seq_ids[i], to be written behind its seq_len tokens
         (prepare_append first: the pages must be there and not shared).  ``windows`` lists the attention windows
-        that the model's layers use (None: every key)."""
+        that the model's layers use (None: every key).  With ``weight_rows`` (None: every new token's attention counts;
+        n: that of each sequence's last n) the step runs packed_key_weights on ``key_weights`` in every layer, once
+        (enable_key_weights); keys that steps without it appended start from nothing then."""
+        if weight_rows != 0 and self.key_weight_pool is None:
+            raise RuntimeError("the cache keeps no key weights: enable_key_weights first")
         counts = [num_new_tokens] * len(seq_ids) if isinstance(num_new_tokens, int) else list(num_new_tokens)
         if len(counts) != len(seq_ids):
             raise ValueError(f"{len(seq_ids)} sequences but {len(counts)} token counts")
@@ -329,11 +355,106 @@ class FlashAttnKVCache:
             bt, sl = self.block_table_host(seq_ids)
         else:
             bt, sl = np.zeros((0, 1), np.int32), np.zeros(0, np.int32)
+        weighed = [min(self._weighed.get(sid, 0), self.seq_len[sid]) for sid in seq_ids] if weight_rows != 0 else None
+        evicted = [self.seq_evicted.get(sid, 0) for sid in seq_ids] if self.seq_evicted else None
         batch = PackedBatch(counts, sl, bt, page_size=P, num_pages=self.max_pages, n_heads=n_heads,
-                            n_kv=self.num_kv_heads, head_dim=self.head_dim, windows=windows, device=self.device)
+                            n_kv=self.num_kv_heads, head_dim=self.head_dim, windows=windows, weight_rows=weight_rows,
+                            weighed=weighed, evicted=evicted, device=self.device)
+        if weight_rows != 0:
+            for sid, n in zip(seq_ids, counts):
+                if n > 0:
+                    self._weighed[sid] = self.seq_len[sid] + n
         if torch.device(self.device).type == "cuda":
             poll_status(self.device)
         return batch
+
+    # ------------------------------------------------------------------ eviction
+    def enable_key_weights(self) -> list[torch.Tensor]:
+        """Keeps an attention weight for every cached key from now on (fp32, 4 bytes per key and KV head and layer):
+        ``key_weights``, one [max_pages, n_kv, page_size] tensor per layer for packed_key_weights."""
+        if self.key_weight_pool is None:
+            shape = (self.num_layers, self.max_pages, self.num_kv_heads, self.page_size)
+            self.key_weight_pool = torch.zeros(shape, dtype=torch.float32, device=self.device)
+            self.key_weights = list(self.key_weight_pool.unbind(0))
+            self._weighed = dict.fromkeys(self.seq_pages, 0)
+        return self.key_weights
+
+    def next_positions(self, seq_ids: list[int]) -> list[int]:
+        """The position of each sequence's next token: its cached tokens and the evicted ones before them."""
+        return [self.seq_len[sid] + self.seq_evicted.get(sid, 0) for sid in seq_ids]
+
+    def holds_evicted(self, page: int) -> bool:
+        """Whether a sequence that evict() cut lists the page: what it holds need not be a run of tokens."""
+        return any(page in self.seq_pages[sid] for sid in self.seq_evicted if sid in self.seq_pages)
+
+    def evict(self, seq_ids: list[int], budget: int | list[int], *, first: int = 4, recent: int = 64) -> int:
+        """Cuts each sequence that holds more than ``budget`` tokens down to it (evict_keys, every layer in one call):
+        the first ``first`` and the last ``recent`` stay, and of the others those whose keys attention weighed most, in
+        each layer and KV head on its own.  Pages past the budget go back to the pool.  Returns how many it got.
+
+        Between steps: a step's update_seqlens first.  The tokens before the last ``recent`` must have been weighed
+        (steps of build_packed_batch with weight_rows).  Shared pages that would be written to are copied first, which
+        takes free pages for a moment; where there are too few, KVCacheOutOfPages leaves everything as it was.
+        Positions go on as before (build_packed_batch and next_positions count the evicted tokens); cached keys are
+        not at their positions any more, so windows are refused for such a sequence, and PrefixCache.store its pages."""
+        budgets = [budget] * len(seq_ids) if isinstance(budget, int) else list(budget)
+        if self.key_weight_pool is None:
+            raise RuntimeError("the cache keeps no key weights: enable_key_weights first")
+        if len(budgets) != len(seq_ids):
+            raise ValueError(f"{len(seq_ids)} sequences but {len(budgets)} budgets")
+        if len(set(seq_ids)) != len(seq_ids):
+            raise ValueError("a sequence is to be evicted from twice")
+        if any(b < 1 for b in budgets) or first < 0 or recent < 0:
+            raise ValueError("budgets must be at least 1 token, first and recent not negative")
+        P = self.page_size
+        todo = [(sid, self.seq_len[sid], b) for sid, b in zip(seq_ids, budgets) if self.seq_len[sid] > b]
+        for sid, n, keep in todo:
+            tail = min(recent, keep - min(first, keep))
+            if min(self._weighed.get(sid, 0), n) < n - tail:
+                raise RuntimeError(f"sequence {sid}: only {min(self._weighed.get(sid, 0), n)} of the {n - tail} tokens before "
+                                   "the recent ones have been weighed (build_packed_batch with weight_rows)")
+        if not todo:
+            return 0
+        free_before = len(self.free_pages)
+        # pages that the kept tokens move into, and others list too, become the sequence's own: plan, then change.
+        # A page is no longer shared once all but one of its sequences have a copy.
+        holders, copies = dict(self._holders), []
+        for sid, n, keep in todo:
+            for i, page in enumerate(self.seq_pages[sid][:-(-keep // P)]):
+                if holders.get(page, 0) > 1 or self._cached(page):
+                    holders[page] = holders.get(page, 0) - 1
+                    copies.append((sid, i, page))
+        if len(copies) > len(self.free_pages):
+            raise KVCacheOutOfPages(f"{len(copies)} shared pages to copy before the eviction, {len(self.free_pages)} free")
+        if self.k_pool.device.type != "cuda":
+            raise RuntimeError(f"eviction runs on the ROCm device; this cache lives on {self.k_pool.device} (prism_amd has "
+                               "no CPU path)")
+        cow = []
+        for sid, i, old in copies:
+            new = self._pop_page()
+            self._hold(new)
+            self.seq_pages[sid][i] = new
+            cow.append((old, new, P))
+        self._copy_on_write(cow)
+        for _, _, old in copies:
+            self._release(old)
+        bt, _ = self.block_table_host([sid for sid, _, _ in todo])
+        dev = self.k_pool.device
+        ints = _upload(np.concatenate([bt.ravel(), [n for _, n, _ in todo], [keep for _, _, keep in todo]]).tolist(),
+                       torch.int32, dev)
+        table, lens, keeps = ints[:bt.size].view(bt.shape), ints[bt.size:bt.size + len(todo)], ints[bt.size + len(todo):]
+        evict_keys(self.k_pool, self.v_pool, self.key_weight_pool, table, lens, keeps, max(keep for _, _, keep in todo),
+                   first=first, recent=recent)
+        for sid, n, keep in todo:
+            pages = self.seq_pages[sid]
+            for page in pages[-(-keep // P):]:
+                self._release(page)
+            del pages[-(-keep // P):]
+            self.seq_len[sid] = keep
+            self._weighed[sid] = min(self._weighed[sid], n) - (n - keep)
+            self.seq_evicted[sid] = self.seq_evicted.get(sid, 0) + n - keep
+        poll_status(self.device)
+        return len(self.free_pages) - free_before
 
     # ------------------------------------------------------------------ page movement
     def layer_bases(self) -> torch.Tensor:
@@ -358,6 +479,10 @@ class FlashAttnKVCache:
         target_kv.seq_len[dst_seq_id] = src_len
         if n:
             copy_pages(self, target_kv, src_pages[:n], target_kv.seq_pages[dst_seq_id][:n], None, staged)
+            copy_key_weights(self, target_kv, src_pages[:n], target_kv.seq_pages[dst_seq_id][:n])
+        self._copy_eviction_state(seq_id, target_kv, dst_seq_id)
+        if target_kv.key_weight_pool is None or self.key_weight_pool is None:
+            target_kv._weighed[dst_seq_id] = 0
         return n
 
     def live_pages(self) -> list[int]:
@@ -388,6 +513,7 @@ class FlashAttnKVCache:
         remap = {p: target._pop_page() for p in live}
         if live:
             copy_pages(self, target, live, [remap[p] for p in live], None)
+            copy_key_weights(self, target, live, [remap[p] for p in live])
         for sid, pages in self.seq_pages.items():
             new_pages = [remap[p] for p in pages]
             for p in new_pages:
@@ -395,6 +521,9 @@ class FlashAttnKVCache:
             target.seq_pages[sid] = new_pages
             target.seq_len[sid] = self.seq_len[sid]
             target.seq_owner[sid] = self.seq_owner.get(sid, "")
+            self._copy_eviction_state(sid, target, sid)
+            if target.key_weight_pool is None or self.key_weight_pool is None:
+                target._weighed[sid] = 0
         pc = self.prefix_cache
         if pc is not None:
             pc.remap_pages(remap)
@@ -405,6 +534,8 @@ class FlashAttnKVCache:
         self.seq_pages.clear()
         self.seq_len.clear()
         self.seq_owner.clear()
+        self.seq_evicted.clear()
+        self._weighed.clear()
         self._holders.clear()
         return remap
 
@@ -416,6 +547,8 @@ class FlashAttnKVCache:
         """
         fresh = FlashAttnKVCache(self.num_layers, self.num_kv_heads, self.head_dim, self.max_pages,
                                  self.page_size, self.device, self.dtype)
+        if self.key_weight_pool is not None:
+            fresh.enable_key_weights()
         remap = self.migrate_to(fresh)
         self.k_pool, self.v_pool = fresh.k_pool, fresh.v_pool
         self.k_caches[:] = fresh.k_caches
@@ -424,6 +557,9 @@ class FlashAttnKVCache:
         self.free_pages = fresh.free_pages
         self.seq_pages, self.seq_len, self.seq_owner = fresh.seq_pages, fresh.seq_len, fresh.seq_owner
         self._holders = fresh._holders
+        self.seq_evicted, self._weighed = fresh.seq_evicted, fresh._weighed
+        self.key_weight_pool = fresh.key_weight_pool
+        self.key_weights[:] = fresh.key_weights
         if fresh.prefix_cache is not None:
             fresh.prefix_cache.kv = self
             self.prefix_cache = fresh.prefix_cache
@@ -470,6 +606,14 @@ def copy_pages(src: FlashAttnKVCache, dst: FlashAttnKVCache, src_ids: list[int],
         page_stride, dst.k_caches[0].stride(0) * dst.k_pool.element_size(), slot_bytes, src.page_size,
         src.max_pages, dst.max_pages, status_tensor(dev).data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
     _lib.check(rc, "pkv_copy_pages")
+
+
+def copy_key_weights(src: FlashAttnKVCache, dst: FlashAttnKVCache, src_ids: list[int], dst_ids: list[int]) -> None:
+    """The pages' key weights, every layer, behind copy_pages (nothing where one of the caches keeps none)."""
+    if not src_ids or src.key_weight_pool is None or dst.key_weight_pool is None:
+        return
+    a, b = src.key_weight_pool, dst.key_weight_pool
+    b[:, _upload(list(dst_ids), torch.int64, b.device)] = a[:, _upload(list(src_ids), torch.int64, a.device)].to(b.device)
 
 
 def _copy_pages_staged(src: FlashAttnKVCache, dst: FlashAttnKVCache, src_ids, dst_ids, fill) -> None:
