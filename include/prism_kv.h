@@ -488,6 +488,9 @@ int pkv_key_weights(const void* q, int64_t q_st, int64_t q_sh, const void* k_cac
                     int32_t num_pages, int32_t max_blocks, int32_t window, float softmax_scale, int32_t* status,
                     void* stream);
 
+/* Bytes of workspace a pkv_evict call of that size needs.  Its contents need not be kept or cleared. */
+size_t pkv_evict_workspace_bytes(int32_t layers, int32_t batch, int32_t n_kv, int32_t head_dim, int32_t max_keep);
+
 /*
  * Eviction: of the seq_lens[b] tokens of sequence b (pages block_table[b]), min(keep_lens[b], seq_lens[b]) stay in every
  * layer and KV head: the first `first`, the last `recent` (as far as they fit, the first ones before them), and of the
@@ -495,7 +498,7 @@ int pkv_key_weights(const void* q, int64_t q_st, int64_t q_sh, const void* k_cac
  * weights of those that stay move, in their order, to the front of the sequence's pages; slots behind them keep what
  * they hold.  kept (int32 [layers, batch, n_kv, max_keep]) receives the positions, ascending, -1 behind them.  Caches
  * are bf16 [layers, num_pages, page_size, n_kv, head_dim] with layer and page strides, weights fp32 [layers, num_pages,
- * n_kv, page_size].  A page that kept tokens move into must not be listed anywhere else in the call.  A sequence whose lengths do not fit the table or
+ * n_kv, page_size], 16-byte aligned with its strides.  A page that kept tokens move into must not be listed anywhere else in the call.  A sequence whose lengths do not fit the table or
  * max_keep, or that lists a page outside the pool, is left as it is (kept: -1) and flags PKV_STATUS_BAD_PAGE.
  * No counterpart in the reference.
  */
@@ -503,7 +506,8 @@ int pkv_evict(void* k_pool, void* v_pool, int64_t layer_stride, int64_t cache_pa
               int64_t weights_layer_stride, int64_t weights_page_stride, const int32_t* block_table, int64_t bt_stride,
               const int32_t* seq_lens, const int32_t* keep_lens, int32_t* kept, int32_t layers, int32_t batch,
               int32_t n_kv, int32_t head_dim, int32_t page_size, int32_t num_pages, int32_t max_blocks,
-              int32_t max_keep, int32_t first, int32_t recent, int32_t* status, void* stream);
+              int32_t max_keep, int32_t first, int32_t recent, void* workspace, size_t workspace_bytes,
+              int32_t* status, void* stream);
 
 /* Bytes of workspace a pkv_sample call of that size needs.  Its contents need not be kept or cleared. */
 size_t pkv_sample_workspace_bytes(int32_t rows, int32_t vocab, int32_t dtype);

@@ -185,13 +185,15 @@ _SIGNATURES = {
         _I32, _I32, _I32, _I32, c_float,  # page_size, num_pages, max_blocks, window, scale
         _P, _P,                          # status, stream
     ]),
+    "pkv_evict_workspace_bytes": (c_size_t, [_I32] * 5),
     "pkv_evict": (c_int32, [
         _P, _P, _I64, _I64,              # k_pool, v_pool, layer and page strides
         _P, _I64, _I64,                  # weights, layer and page strides
         _P, _I64, _P, _P, _P,            # block table, seq_lens, keep_lens, kept
         _I32, _I32, _I32, _I32,          # layers, batch, n_kv, head_dim
         _I32, _I32, _I32, _I32,          # page_size, num_pages, max_blocks, max_keep
-        _I32, _I32, _P, _P,              # first, recent, status, stream
+        _I32, _I32, _P, c_size_t,        # first, recent, workspace
+        _P, _P,                          # status, stream
     ]),
     "pkv_sample_workspace_bytes": (c_size_t, [_I32] * 3),
     "pkv_sample": (c_int32, [

@@ -3,9 +3,7 @@
 //
 // Two launches.  The first finds each head's threshold, a radix descent over the weights' bits (no sort: what stays is
 // a set, and is written in the order of positions), writes the kept positions and moves the weights.  The second moves
-// K and V.  In place and in order: kept position k[d] goes to d <= k[d], and a chunk of destinations [c, c + C) never
-// holds a source of a later chunk (k[d] >= d >= c + C), so one workgroup that reads a whole chunk before it writes it
-// needs no other care, and may have read the next chunk by then.
+// K and V, in place: the token at position k[d] goes to d <= k[d].
 #include "pkv_common.h"
 
 namespace pkv {
@@ -19,13 +17,16 @@ struct EvictParams {
   const int32_t* lens;
   const int32_t* keeps;
   int32_t* kept;
+  int32_t* marks;  // per layer, sequence, head and K or V: a ticket, then a flag for each workgroup of the second launch
   int32_t* status;
   int64_t k_layer, page_stride, w_layer, w_page, bt_stride;
-  int batch, n_kv, log2_page, num_pages, max_blocks, max_keep, first, recent;
+  int batch, n_kv, log2_page, num_pages, max_blocks, max_keep, first, recent, move_chunks;
 };
 
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWaves = kSelectThreads / 64;
+constexpr int kTableCols = 8192;    // of a sequence's block-table row, held in LDS
+constexpr int kCandidates = 24576;  // keys that share the threshold's first digit, held in LDS
 
 // A sequence's sizes, read by every workgroup that works for it.
 struct Sizes {
@@ -51,20 +52,63 @@ __device__ __forceinline__ uint32_t ordered(float f) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// The place from the top of a histogram of 2^bits counts where the running sum reaches `need`.
+struct Digit {
+  int hist[2048];
+  int wave_sum[kSelectWaves];
+  int bin, above, count;
+};
+__device__ __forceinline__ void find_digit(Digit& sh, int bits, int need) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int top = (1 << bits) - 1 - 2 * tid;  // this thread's two bins, from the top
+  const int c0 = top >= 0 ? sh.hist[top] : 0, c1 = top >= 1 ? sh.hist[top - 1] : 0;
+  int run = c0 + c1;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int up = __shfl_up(run, o);
+    if (lane >= o) run += up;
+  }
+  if (lane == 63) sh.wave_sum[wave] = run;
+  __syncthreads();
+  int before = run - c0 - c1;
+  for (int i = 0; i < wave; ++i) before += sh.wave_sum[i];
+  if (before < need && before + c0 >= need) {
+    sh.bin = top;
+    sh.above = before;
+    sh.count = c0;
+  } else if (before + c0 < need && before + c0 + c1 >= need) {
+    sh.bin = top - 1;
+    sh.above = before + c0;
+    sh.count = c1;
+  }
+  __syncthreads();
+}
+
+// A workgroup per layer, sequence and head.  Reads the weights three times (first digit; the keys of that digit, which
+// then lie in LDS; the kept ones), 16 bytes a lane with the next ones on the way: 28 layers' one head of 100 k tokens
+// take .. us.
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const EvictParams p) {
-  constexpr int BITS = 11, BINS = 1 << BITS;
-  __shared__ int hist[BINS];
-  __shared__ int wave_sum[kSelectWaves];
-  __shared__ int found_bin, found_above;
+  __shared__ Digit sh;
+  __shared__ int table[kTableCols];
+  __shared__ uint32_t keys[kCandidates];
+  __shared__ int candidates;
   const int h = blockIdx.x, b = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Sizes s = sizes_of(p, b);
-  int32_t* kept = p.kept + ((int64_t(layer) * p.batch + b) * p.n_kv + h) * p.max_keep;
+  const int64_t head = (int64_t(layer) * p.batch + b) * p.n_kv + h;
+  int32_t* kept = p.kept + head * p.max_keep;
+  // the second launch's tickets and flags
+  for (int i = tid; i < 2 * (1 + p.move_chunks); i += kSelectThreads) p.marks[head * 2 * (1 + p.move_chunks) + i] = 0;
   const int32_t* bt = p.bt + b * p.bt_stride;
   bool bad = s.bad;
   if (!bad) {
     const int pages = (s.n + (1 << p.log2_page) - 1) >> p.log2_page;
-    for (int c = tid; c < pages; c += kSelectThreads) bad |= unsigned(bt[c]) >= unsigned(p.num_pages);
+    for (int c = tid; c < pages; c += kSelectThreads) {
+      const int page = bt[c];
+      bad |= unsigned(page) >= unsigned(p.num_pages);
+      if (c < kTableCols) table[c] = page;
+    }
   }
+  if (tid == 0) candidates = 0;
   if (__syncthreads_or(bad)) {
     if (tid == 0) flag_status(p.status, PKV_STATUS_BAD_PAGE);
     for (int d = tid; d < p.max_keep; d += kSelectThreads) kept[d] = -1;
@@ -77,71 +121,116 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
   }
   float* const w = p.w + layer * p.w_layer + (int64_t(h) << p.log2_page);
   const int in_page = (1 << p.log2_page) - 1;
-  auto place = [&](int t) -> float* { return w + bt[t >> p.log2_page] * p.w_page + (t & in_page); };
+  auto place = [&](int t) -> float* {
+    const int col = t >> p.log2_page;
+    return w + (col < kTableCols ? table[col] : bt[col]) * p.w_page + (t & in_page);
+  };
   const int lo = s.first, hi = s.n - s.recent;  // whose weights decide
   int need = s.keep - s.first - s.recent;       // how many of them stay
+  const bool choose = need > 0;
+  // f(t, four weights) for every group of four tokens, kUnroll of a thread's loads on the way at once
+  constexpr int kUnroll = 4;
+  auto each = [&](auto&& f) {
+    for (int t0 = tid * 4; t0 < s.n; t0 += kUnroll * kSelectThreads * 4) {
+      f32x4 x[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int t = t0 + u * kSelectThreads * 4;
+        if (t < s.n) x[u] = *reinterpret_cast<const f32x4*>(place(t));
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int t = t0 + u * kSelectThreads * 4;
+        if (t < s.n) f(t, x[u]);
+      }
+    }
+  };
   // the need-th largest key, digit by digit; `need` becomes how many of those equal to it stay
   uint32_t threshold = 0xffffffffu;
-  if (need > 0) {
+  if (choose) {
     threshold = 0;
+    bool listed = false;
+    int n_listed = 0;
     for (int shift = 32; shift > 0;) {
-      const int bits = min(BITS, shift);
+      const int bits = min(11, shift);
       shift -= bits;
-      for (int i = tid; i < BINS; i += kSelectThreads) hist[i] = 0;
+      for (int i = tid; i < 2048; i += kSelectThreads) sh.hist[i] = 0;
       __syncthreads();
-      const uint32_t above_mask = shift + bits == 32 ? 0 : ~0u << (shift + bits);
-      for (int t = lo + tid; t < hi; t += kSelectThreads) {
-        const uint32_t key = ordered(*place(t));
-        if ((key & above_mask) == threshold) atomicAdd(&hist[(key >> shift) & ((1 << bits) - 1)], 1);
+      const uint32_t done = shift + bits == 32 ? 0 : ~0u << (shift + bits), mask = (1u << bits) - 1;
+      if (listed) {
+        for (int i = tid; i < n_listed; i += kSelectThreads)
+          if ((keys[i] & done) == threshold) atomicAdd(&sh.hist[(keys[i] >> shift) & mask], 1);
+      } else {
+        each([&](int t, f32x4 x) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t key = ordered(x[i]);
+            if (t + i >= lo && t + i < hi && (key & done) == threshold) atomicAdd(&sh.hist[(key >> shift) & mask], 1);
+          }
+        });
       }
       __syncthreads();
-      // counts from the top: thread i has two bins, largest digits first
-      const int top = (1 << bits) - 1 - 2 * tid;
-      const int c0 = top >= 0 ? hist[top] : 0, c1 = top >= 1 ? hist[top - 1] : 0;
-      int run = c0 + c1;
-      for (int o = 1; o < 64; o <<= 1) {
-        const int up = __shfl_up(run, o);
-        if (lane >= o) run += up;
-      }
-      if (lane == 63) wave_sum[wave] = run;
-      __syncthreads();
-      int before = run - c0 - c1;
-      for (int i = 0; i < wave; ++i) before += wave_sum[i];
-      if (before < need && before + c0 >= need) {
-        found_bin = top;
-        found_above = before;
-      } else if (before + c0 < need && before + c0 + c1 >= need) {
-        found_bin = top - 1;
-        found_above = before + c0;
+      find_digit(sh, bits, need);
+      threshold |= uint32_t(sh.bin) << shift;
+      need -= sh.above;
+      n_listed = sh.count;
+      if (!listed && shift > 0 && n_listed <= kCandidates) {
+        listed = true;
+        const uint32_t upto = ~0u << shift;
+        each([&](int t, f32x4 x) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t key = ordered(x[i]);
+            if (t + i >= lo && t + i < hi && (key & upto) == threshold) keys[atomicAdd(&candidates, 1)] = key;
+          }
+        });
       }
       __syncthreads();
-      threshold |= uint32_t(found_bin) << shift;
-      need -= found_above;
+      if (listed) n_listed = candidates;
     }
   }
-  // in the order of positions: what lies above the threshold, and the first `need` that equal it
+  // in the order of positions: what lies above the threshold, and the first `need` that equal it.  A kept weight moves to
+  // d <= t: never to where a later chunk's lie, and this chunk's are in registers by then.
   int above = 0, equal = 0;  // so far
-  for (int t0 = 0; t0 < s.n; t0 += kSelectThreads) {
-    const int t = t0 + tid;
-    const float f = t < s.n ? *place(t) : 0.0f;
-    const bool middle = t >= lo && t < hi;
-    const uint32_t key = ordered(f);
-    const bool is_above = t < s.n && (!middle || (s.keep > s.first + s.recent && key > threshold));
-    const bool is_equal = middle && s.keep > s.first + s.recent && key == threshold;
-    const uint64_t a = __ballot(is_above), e = __ballot(is_equal), below = (uint64_t(1) << lane) - 1;
-    if (lane == 0) wave_sum[wave] = __popcll(a) << 16 | __popcll(e);
-    __syncthreads();  // and every weight of this chunk is read
-    int packed = 0, all = 0;
-    for (int i = 0; i < kSelectWaves; ++i) {
-      if (i == wave) packed = all;
-      all += wave_sum[i];
+  f32x4 next = {};
+  if (tid * 4 < s.n) next = *reinterpret_cast<const f32x4*>(place(tid * 4));
+  for (int t0 = 0; t0 < s.n; t0 += kSelectThreads * 4) {
+    const int t = t0 + tid * 4;
+    const f32x4 x = next;
+    if (t + kSelectThreads * 4 < s.n) next = *reinterpret_cast<const f32x4*>(place(t + kSelectThreads * 4));
+    uint32_t is_above = 0, is_equal = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool middle = t + i >= lo && t + i < hi;
+      const uint32_t key = ordered(x[i]);
+      is_above |= uint32_t(t + i < s.n && (!middle || (choose && key > threshold))) << i;
+      is_equal |= uint32_t(choose && middle && key == threshold) << i;
     }
-    const int my_above = above + (packed >> 16) + __popcll(a & below);
-    const int my_equal = equal + (packed & 0xffff) + __popcll(e & below);
-    if (is_above || (is_equal && my_equal < need)) {
-      const int d = my_above + min(my_equal, need);
-      kept[d] = t;
-      if (d != t) *place(d) = f;
+    const int mine = __popc(is_above) << 16 | __popc(is_equal);
+    int run = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(run, o);
+      if (lane >= o) run += up;
+    }
+    if (lane == 63) sh.wave_sum[wave] = run;
+    __syncthreads();
+    int before = run - mine, all = 0;
+    for (int i = 0; i < kSelectWaves; ++i) {
+      if (i < wave) before += sh.wave_sum[i];
+      all += sh.wave_sum[i];
+    }
+    int my_above = above + (before >> 16), my_equal = equal + (before & 0xffff);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool a = is_above >> i & 1, e = is_equal >> i & 1;
+      if (a || (e && my_equal < need)) {
+        const int d = my_above + min(my_equal, need);
+        kept[d] = t + i;
+        if (d != t + i) *place(d) = x[i];
+      }
+      my_above += a;
+      my_equal += e;
     }
     above += all >> 16;
     equal += all & 0xffff;
@@ -149,57 +238,102 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
   }
 }
 
-// One workgroup moves `PART` 16-byte chunks of every kept row of K or of V of one head.
-template <int THREADS, int U>
-__global__ __launch_bounds__(THREADS) void evict_move_kernel(const EvictParams p, int chunks, int log2_part) {
-  const int parts = chunks >> log2_part;
-  const int stream = blockIdx.x % (2 * parts), b = blockIdx.y, layer = blockIdx.z, h = blockIdx.x / (2 * parts);
+// ---- K and V ----
+// A workgroup takes 32 KB of destination rows of K or of V of one head: it reads their sources, and writes them once the
+// sources that lie in its destinations have been read by the workgroups that they belong to.  Those have smaller
+// destinations (k[d] >= d), and a workgroup's place in that order is a ticket that it draws when it starts: whoever it
+// waits for has started, reads without waiting for anybody, and then raises its flag.  So every wait ends, whatever
+// else runs on the device.
+template <int U>
+__global__ __launch_bounds__(256) void evict_move_kernel(const EvictParams p, int log2_chunks) {
+  __shared__ int ticket_lds, wait_lds[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int stream = blockIdx.x / p.move_chunks, b = blockIdx.y, layer = blockIdx.z, h = stream >> 1;
   const Sizes s = sizes_of(p, b);
-  if (s.bad || s.keep == s.n) return;
-  const int32_t* kept = p.kept + ((int64_t(layer) * p.batch + b) * p.n_kv + h) * p.max_keep;
+  const int rows = 256 >> log2_chunks;  // a pass of the workgroup
+  const int per = rows * U;
+  if (s.bad || s.keep == s.n || int(blockIdx.x % p.move_chunks) * per >= s.keep) return;  // as many as the kept rows need go on
+  const int64_t head = (int64_t(layer) * p.batch + b) * p.n_kv + h;
+  const int32_t* kept = p.kept + head * p.max_keep;
+  int32_t* const marks = p.marks + (head * 2 + (stream & 1)) * (1 + p.move_chunks);
+  if (tid == 0) {
+    ticket_lds = atomicAdd(&marks[0], 1);
+    wait_lds[0] = wait_lds[1] = -1;
+  }
+  __syncthreads();
+  const int mine = ticket_lds, d0 = mine * per, d1 = min(d0 + per, s.keep);
+  const int last = kept[d1 - 1];
+  if (last < 0 || last == d1 - 1) return;  // refused by the first launch, or all in place (nobody else reads these slots)
   const int32_t* bt = p.bt + b * p.bt_stride;
-  const int lane_chunk = threadIdx.x & ((1 << log2_part) - 1), row = threadIdx.x >> log2_part;
-  const int rows = THREADS >> log2_part;  // a pass
-  uint16_t* const base = (stream < parts ? p.k : p.v) + layer * p.k_layer +
-                         (h * chunks + (stream % parts << log2_part) + lane_chunk) * 8;
-  const int64_t key_st = int64_t(p.n_kv) * chunks * 8;
+  const int chunk = tid & ((1 << log2_chunks) - 1), row = tid >> log2_chunks;
+  const int64_t key_st = int64_t(p.n_kv) << (log2_chunks + 3);
+  uint16_t* const base = (stream & 1 ? p.v : p.k) + layer * p.k_layer + (((h << log2_chunks) + chunk) << 3);
   const int in_page = (1 << p.log2_page) - 1;
   auto place = [&](int t) { return base + bt[t >> p.log2_page] * p.page_stride + (t & in_page) * key_st; };
-  // nothing before the first evicted position moves: kept[d] == d up to there
-  int d0 = 0;
-  for (int end = s.keep; d0 < end;) {
-    const int mid = (d0 + end) >> 1;
-    if (kept[mid] == mid)
-      d0 = mid + 1;
-    else
-      end = mid;
-  }
-  if (d0 >= s.keep || kept[0] < 0) return;
-  u32x4 now[U];
-  for (int c = d0; c < s.keep; c += U * rows) {
+  int from[U];
+  u32x4 x[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int d = c + u * rows + row;
-      if (d < s.keep) now[u] = ld16(place(kept[d]));
-    }
-    __syncthreads();  // every source of the chunk is read
+  for (int u = 0; u < U; ++u) from[u] = kept[min(d0 + u * rows + row, d1 - 1)];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int d = c + u * rows + row;
-      if (d < s.keep) st16(place(d), now[u]);
+  for (int u = 0; u < U; ++u) x[u] = ld16(place(from[u]));
+  // meanwhile: the destinations [a, b) whose sources lie in this workgroup's, 64 places tried at once.  At most `per`
+  // of them, so they belong to two workgroups at most.
+  if (wave < 2) {
+    const int want = wave == 0 ? d0 : d1;
+    int lo = 0, hi = d1;  // the first d with kept[d] >= want lies in [lo, hi] (kept[d] >= d)
+    while (lo < hi) {
+      const int step = (hi - lo + 63) >> 6;
+      const int at = min(lo + (lane + 1) * step - 1, hi - 1);
+      const int less = __popcll(__ballot(kept[at] < want && lo + (lane + 1) * step - 1 < hi));
+      const int next = min(lo + less * step, hi);
+      hi = min(next + step - 1, hi);
+      lo = next;
+      if (step == 1) {
+        hi = lo;
+      }
     }
+    if (lane == 0) wait_lds[wave] = lo;
   }
+  __syncthreads();
+  const int a = wait_lds[0], e = wait_lds[1];
+  // the loads have arrived
+#pragma unroll
+  for (int u = 0; u < U; ++u) asm volatile("" ::"v"(x[u]));
+  __syncthreads();
+  if (tid == 0) {
+    __hip_atomic_store(&marks[1 + mine], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (e > a)
+      for (int i = a / per; i <= min((e - 1) / per, mine - 1); ++i)
+        while (__hip_atomic_load(&marks[1 + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0) __builtin_amdgcn_s_sleep(1);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int d = d0 + u * rows + row;
+    if (d < d1 && from[u] != d) st16(place(d), x[u]);
+  }
+}
+
+constexpr int kMoveUnroll = 8;
+int move_chunks(int max_keep, int head_dim) {
+  const int per = 256 / (head_dim / 8) * kMoveUnroll;
+  return (max_keep + per - 1) / per;
 }
 
 }  // namespace
 }  // namespace pkv
+
+extern "C" size_t pkv_evict_workspace_bytes(int32_t layers, int32_t batch, int32_t n_kv, int32_t head_dim, int32_t max_keep) {
+  if (layers <= 0 || batch <= 0 || n_kv <= 0 || max_keep <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
+  return size_t(layers) * batch * n_kv * 2 * (1 + pkv::move_chunks(max_keep, head_dim)) * sizeof(int32_t);
+}
 
 extern "C" int pkv_evict(void* k_pool, void* v_pool, int64_t layer_stride, int64_t cache_page_stride, float* weights,
                          int64_t weights_layer_stride, int64_t weights_page_stride, const int32_t* block_table,
                          int64_t bt_stride, const int32_t* seq_lens, const int32_t* keep_lens, int32_t* kept,
                          int32_t layers, int32_t batch, int32_t n_kv, int32_t head_dim, int32_t page_size,
                          int32_t num_pages, int32_t max_blocks, int32_t max_keep, int32_t first, int32_t recent,
-                         int32_t* status, void* stream) {
+                         void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
   using namespace pkv;
   clear_error();
   const char* fn = "pkv_evict";
@@ -209,12 +343,19 @@ extern "C" int pkv_evict(void* k_pool, void* v_pool, int64_t layer_stride, int64
                           page_size, num_pages, max_blocks);
   if (rc) return rc;
   if (!weights || !keep_lens || (max_keep > 0 && !kept)) return fail(PKV_EINVAL, "%s: null argument", fn);
-  if ((reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(kept)) & 3u)
-    return fail(PKV_EINVAL, "%s: weights/kept not 4-byte aligned", fn);
+  if (!aligned16(weights) || weights_layer_stride % 4 || weights_page_stride % 4)
+    return fail(PKV_EINVAL, "%s: weights or their strides not 16-byte aligned", fn);
+  if (reinterpret_cast<uintptr_t>(kept) & 3u) return fail(PKV_EINVAL, "%s: kept not 4-byte aligned", fn);
   if (layer_stride % 8 || weights_page_stride < int64_t(n_kv) * page_size)
     return fail(PKV_EINVAL, "%s: layer stride not 16-byte aligned, or the weights' pages overlap", fn);
   if (layers > 65535 || batch > 65535) return fail(PKV_EINVAL, "%s: layers/batch exceed the grid limit", fn);
   if (layers == 0 || batch == 0 || max_keep == 0) return PKV_OK;
+  const size_t need = pkv_evict_workspace_bytes(layers, batch, n_kv, head_dim, max_keep);
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 3u))
+    return fail(PKV_EINVAL, "%s: workspace null or not 4-byte aligned", fn);
+  if (workspace_bytes < need) return fail(PKV_ENOSPC, "%s: workspace %zu bytes < %zu needed", fn, workspace_bytes, need);
+  const int64_t wgs = int64_t(n_kv) * 2 * move_chunks(max_keep, head_dim);
+  if (wgs * 256 > 0x7fffffff) return fail(PKV_EINVAL, "%s: %d heads of %d kept tokens exceed the grid limit", fn, n_kv, max_keep);
   EvictParams p;
   p.k = static_cast<uint16_t*>(k_pool);
   p.v = static_cast<uint16_t*>(v_pool);
@@ -238,8 +379,9 @@ extern "C" int pkv_evict(void* k_pool, void* v_pool, int64_t layer_stride, int64
   p.first = first;
   p.recent = recent;
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  p.marks = static_cast<int32_t*>(workspace);
+  p.move_chunks = move_chunks(max_keep, head_dim);
   evict_select_kernel<<<dim3(n_kv, batch, layers), kSelectThreads, 0, s>>>(p);
-  const int chunks = head_dim / 8;
-  evict_move_kernel<1024, 4><<<dim3(n_kv * 2, batch, layers), 1024, 0, s>>>(p, chunks, ilog2(chunks));
+  evict_move_kernel<kMoveUnroll><<<dim3(unsigned(wgs), batch, layers), 256, 0, s>>>(p, ilog2(head_dim / 8));
   return check_launch(fn);
 }

@@ -69,8 +69,12 @@ def evict_keys(k_pool: torch.Tensor, v_pool: torch.Tensor, key_weights: torch.Te
         kept = torch.empty((layers, batch, nk, max_keep), dtype=torch.int32, device=dev)
         if kept.numel() == 0 or blocks == 0:
             return kept.fill_(-1)
-        rc = _lib.load().pkv_evict(k_pool.data_ptr(), v_pool.data_ptr(), *ks, key_weights.data_ptr(),
-                                   *key_weights.stride()[:2], bt, blocks, lens, keeps, kept.data_ptr(), layers, batch, nk, hd,
-                                   P, pages, blocks, max_keep, first, recent, status.data_ptr(), _raw_stream(dev.index))
+        lib = _lib.load()
+        # of this call alone, from torch's allocator: of the current stream, or of the graph it captures
+        ws = torch.empty(lib.pkv_evict_workspace_bytes(layers, batch, nk, hd, max_keep), dtype=torch.uint8, device=dev)
+        rc = lib.pkv_evict(k_pool.data_ptr(), v_pool.data_ptr(), *ks, key_weights.data_ptr(),
+                           *key_weights.stride()[:2], bt, blocks, lens, keeps, kept.data_ptr(), layers, batch, nk, hd,
+                           P, pages, blocks, max_keep, first, recent, ws.data_ptr(), ws.numel(), status.data_ptr(),
+                           _raw_stream(dev.index))
         _lib.check(rc, "pkv_evict")
     return kept

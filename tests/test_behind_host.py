@@ -176,7 +176,8 @@ def test_weights_argument_errors():
 
 def _evict_call(lib, **over):
     a = dict(k=A16, v=A16, layer=1 << 16, page=2048, w=A16, w_layer=640, w_page=32, bt=A16, bt_st=2, lens=A16, keeps=A16,
-             kept=A16, layers=0, batch=1, nk=2, hd=64, P=16, pages=20, blocks=2, max_keep=4, first=0, recent=0)
+             kept=A16, layers=0, batch=1, nk=2, hd=64, P=16, pages=20, blocks=2, max_keep=4, first=0, recent=0, ws=A16,
+             ws_bytes=1 << 20)
     a.update(over)
     return lib.pkv_evict(*a.values(), None, None)
 
@@ -185,11 +186,13 @@ def test_evict_argument_errors():
     lib = _lib.load()
     assert _evict_call(lib) == 0
     for over, msg in [(dict(k=A16 + 8), "aligned"), (dict(w=0), "null"), (dict(keeps=0), "null"), (dict(kept=0), "null"),
-                      (dict(w=A16 + 2), "4-byte"), (dict(layer=12), "layer stride"), (dict(w_page=31), "overlap"),
+                      (dict(w=A16 + 4), "16-byte"), (dict(w_layer=6), "16-byte"), (dict(w_page=34), "16-byte"), (dict(kept=A16 + 2), "4-byte"),
+                      (dict(layers=1, ws=0), "workspace"), (dict(layers=1, ws=A16 + 2), "workspace"),
+                      (dict(layers=1, ws_bytes=8), "needed"), (dict(layer=12), "layer stride"), (dict(w_page=28), "overlap"),
                       (dict(layers=-1), "sizes"), (dict(max_keep=-1), "sizes"), (dict(first=-1), "sizes"), (dict(recent=-1), "sizes"),
                       (dict(layers=70000), "grid"), (dict(hd=80), "head_dim"), (dict(P=8), "page_size"), (dict(bt=0), "null"),
                       (dict(lens=0), "null")]:
-        assert _evict_call(lib, **over) == _lib.PKV_EINVAL, over
+        assert _evict_call(lib, **over) in (_lib.PKV_EINVAL, _lib.PKV_ENOSPC), over
         assert msg in lib.pkv_last_error().decode(), (over, lib.pkv_last_error())
 
 
