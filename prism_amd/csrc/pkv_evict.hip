@@ -129,7 +129,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
   int need = s.keep - s.first - s.recent;       // how many of them stay
   const bool choose = need > 0;
   // f(t, four weights) for every group of four tokens, kUnroll of a thread's loads on the way at once
-  constexpr int kUnroll = 4;
+  constexpr int kUnroll = 8;
   auto each = [&](auto&& f) {
     for (int t0 = tid * 4; t0 < s.n; t0 += kUnroll * kSelectThreads * 4) {
       f32x4 x[kUnroll];
@@ -191,18 +191,28 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
   }
   // in the order of positions: what lies above the threshold, and the first `need` that equal it.  A kept weight moves to
   // d <= t: never to where a later chunk's lie, and this chunk's are in registers by then.
+  constexpr int G = 4;  // groups of four tokens a thread and chunk
   int above = 0, equal = 0;  // so far
-  f32x4 next = {};
-  if (tid * 4 < s.n) next = *reinterpret_cast<const f32x4*>(place(tid * 4));
-  for (int t0 = 0; t0 < s.n; t0 += kSelectThreads * 4) {
-    const int t = t0 + tid * 4;
-    const f32x4 x = next;
-    if (t + kSelectThreads * 4 < s.n) next = *reinterpret_cast<const f32x4*>(place(t + kSelectThreads * 4));
+  f32x4 next[G] = {};
+  auto load = [&](int t0) {
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      const int t = t0 + (tid * G + j) * 4;
+      if (t < s.n) next[j] = *reinterpret_cast<const f32x4*>(place(t));
+    }
+  };
+  load(0);
+  for (int t0 = 0; t0 < s.n; t0 += kSelectThreads * 4 * G) {
+    const int t = t0 + tid * 4 * G;
+    f32x4 x[G];
+#pragma unroll
+    for (int j = 0; j < G; ++j) x[j] = next[j];
+    load(t0 + kSelectThreads * 4 * G);
     uint32_t is_above = 0, is_equal = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 4 * G; ++i) {
       const bool middle = t + i >= lo && t + i < hi;
-      const uint32_t key = ordered(x[i]);
+      const uint32_t key = ordered(x[i >> 2][i & 3]);
       is_above |= uint32_t(t + i < s.n && (!middle || (choose && key > threshold))) << i;
       is_equal |= uint32_t(choose && middle && key == threshold) << i;
     }
@@ -222,12 +232,12 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
     }
     int my_above = above + (before >> 16), my_equal = equal + (before & 0xffff);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 4 * G; ++i) {
       const bool a = is_above >> i & 1, e = is_equal >> i & 1;
       if (a || (e && my_equal < need)) {
         const int d = my_above + min(my_equal, need);
         kept[d] = t + i;
-        if (d != t + i) *place(d) = x[i];
+        if (d != t + i) *place(d) = x[i >> 2][i & 3];
       }
       my_above += a;
       my_equal += e;

@@ -5,10 +5,14 @@
 // a prefix of that order, so nothing has to be sorted: what stays is all that lies before one place in it.  The drawn token is the
 // first, in the order of the vocabulary, at which the running sum of the weights that stay passes u times their sum.
 //
-// Two launches.  The first has a workgroup per slice of a row: its maximum, the sum of its weights (fp64, from its own
-// maximum on) and, where a rule is set, a list of its largest tokens.  The second has a workgroup per row, which finds
-// the place among the lists where they hold it (all above the largest token that any slice left out), else among the
-// row's logits themselves, by a radix descent over sums in 64-bit integers.
+// Two launches.  The first has a workgroup per slice of a row: its maximum and what the row's rules need of it.
+//   no rule:          the sum of its weights
+//   top-p or min-p:   the running sums of its weights over classes of value, 1/16 octave of weight each
+//   top-k:            a list of its largest tokens
+// The second has a workgroup per row.  It joins the slices, finds the place where the order is cut (among the few
+// tokens of one class, or on the lists), then the slice that the draw falls into, and reads that one again.  Rows whose
+// cut lies in none of these (thousands of equal logits, top-k past the lists) are searched through by a radix descent
+// over all their tokens.
 //
 // A decision can fall between tokens 1e-6 of the sum apart, so the weights are taken in fp64 and their sums are fp64 in
 // a fixed order or integers (2^-42 of the largest weight or finer): no order of atomics changes a token.
@@ -24,17 +28,21 @@ constexpr int kSliceThreads = 256;
 constexpr int kRowThreads = 1024;
 constexpr int kRowWaves = kRowThreads / 64;
 constexpr int kListMax = 8192;   // tokens that a row's lists hold together
-constexpr int kSlicesMax = 512;
+constexpr int kSlicesMax = 256;
 constexpr int kBins = 2048;
 constexpr int kBinBits = 11;
+constexpr int kClasses = 512;    // of value, kPerOctave to the octave of weight
+constexpr double kPerOctave = 16.0;
+constexpr int kClassBits = 50;   // the classes' sums are in units of 2^-50 of the slice's reference
 
 struct SliceHead {
   uint64_t best;   // (ordered value, ~token) of the largest, 0: no token of the slice can be drawn
-  double sum;      // of the weights, relative to the slice's own maximum
+  double sum;      // no rule: of the weights, relative to the slice's own maximum.  Classes: of all, in their units
+  double ref;      // classes: the octave that they count from
   uint32_t count;  // listed tokens
   uint32_t left;   // the largest ordered value among those not listed, 0: every one is
   uint32_t valid;  // tokens that can be drawn
-  uint32_t pad;
+  uint32_t pad[3];
 };
 
 struct Setting {
@@ -48,10 +56,11 @@ struct SampleParams {
   int64_t* tokens;
   float* logprobs;
   SliceHead* heads;
-  uint2* lists;  // (ordered value, token)
+  void* lists;  // a slice's part: `cap` tokens as (ordered value, token), or kClasses running sums
   Setting temperature, top_k, top_p, min_p;
   int64_t stride;
   int vocab, slices, cap;
+  int64_t part;  // bytes of a slice's part
 };
 
 // What a row asks for.
@@ -60,9 +69,8 @@ struct Rules {
   double top_p, min_p;
   int top_k;     // 0: off
   bool greedy, use_p, use_m;
-  __device__ __forceinline__ bool filtered() const { return top_k > 0 || use_p || use_m; }
-  // the weights of the whole row are summed: to draw from, or for top-p's share
-  __device__ __forceinline__ bool summed() const { return !greedy && top_k == 0 && (use_p || !use_m); }
+  __device__ __forceinline__ bool lists() const { return top_k > 0; }
+  __device__ __forceinline__ bool classes() const { return top_k == 0 && (use_p || use_m); }
 };
 
 __device__ __forceinline__ double setting(const Setting& s, int row) {
@@ -94,9 +102,9 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return key == 0 ? -INFINITY : __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// 2^t, t <= 0: the series of exp(f ln 2) on |f| <= 1/2 to its 11th power (6e-15), scaled by the whole part; nothing
-// below 2^-1000.
-__device__ __forceinline__ double exp2_neg(double t) {
+// 2^t: the series of exp(f ln 2) on |f| <= 1/2 to its 11th power (6e-15), scaled by the whole part; nothing below
+// 2^-1000.
+__device__ __forceinline__ double exp2_of(double t) {
   if (t < -1000.0) return 0.0;
   const double n = rint(t), f = t - n;
   double r = 4.4455382718708114e-10;
@@ -118,7 +126,7 @@ __device__ __forceinline__ double exp2_neg(double t) {
 __device__ __forceinline__ double weight_of(float x, float top, double scale) {
   if (x == top) return 1.0;
   if (!(x > -INFINITY) || top == INFINITY) return 0.0;
-  return exp2_neg((double(x) - double(top)) * scale);
+  return exp2_of((double(x) - double(top)) * scale);
 }
 
 template <class T>
@@ -129,6 +137,20 @@ template <>
 __device__ __forceinline__ float to_float(__bf16 v) { return float(v); }
 template <>
 __device__ __forceinline__ float to_float(_Float16 v) { return float(v); }
+
+// The same where no maximum of the row is known yet: x / T in octaves, from a reference octave at or above the
+// largest (with +inf, whose equals alone weigh anything, 2^28, which leaves nothing to any other).
+__device__ __forceinline__ double octave_of(float top, double scale) {
+  return top == INFINITY ? 268435456.0 : ceil(double(top) * scale);
+}
+__device__ __forceinline__ double octaves_below(float x, double ref, double scale) {  // 0 or less; -1e300: no weight
+#pragma clang fp contract(off)  // the same bits wherever it is computed, and 0 for a product that is whole
+  if (!(x > -INFINITY)) return -1e300;
+  if (x == INFINITY) return 0.0;
+  const double octaves = double(x) * scale;
+  return fmin(octaves - ref, 0.0);
+}
+__device__ __forceinline__ int class_of(double t) { return int(fmin(-t * kPerOctave, 1e9)); }
 
 // A row as 16-byte pieces from the 16-byte boundary at or before its start on (a piece that holds any of the row lies
 // in the row's own allocation, whose start and size are multiples of 16 bytes at least): element j of them is token j - skip.
@@ -185,18 +207,18 @@ __device__ __forceinline__ int distance_bin(float x, float top) {
 template <class T, int E>
 __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const SampleParams p) {
   constexpr int V = Row<T>::kVec, L = E / V, W = kSliceThreads / 64;
-  __shared__ uint64_t best_lds[W];
+  __shared__ uint64_t best_lds[W], classes[kClasses], total_lds[W];
   __shared__ double sum_lds[W];
   __shared__ int hist[1024];
   __shared__ int count_lds[W], taken, bins_lds[2];
   __shared__ uint32_t left_lds[W];
   const int slice = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const Rules rules = rules_of(p, row);
   const Row<T> src(p, row);
   float x[L][V];
   const int piece0 = slice * (kSliceThreads * L);
 #pragma unroll
   for (int l = 0; l < L; ++l) src.get(piece0 + l * kSliceThreads + tid, x[l]);
+  const Rules rules = rules_of(p, row);
   auto token = [&](int l, int e) { return (piece0 + l * kSliceThreads + tid) * V + e - src.skip; };
   uint64_t best = 0;
 #pragma unroll
@@ -209,7 +231,10 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
   // of equal values the lowest token: a thread meets its own in ascending order, other threads' are compared by ~token
   best = wave_max(best);
   if (lane == 0) best_lds[wave] = best;
-  for (int i = tid; i < 1024; i += kSliceThreads) hist[i] = 0;
+  if (rules.lists())
+    for (int i = tid; i < 1024; i += kSliceThreads) hist[i] = 0;
+  else if (rules.classes())
+    for (int i = tid; i < kClasses; i += kSliceThreads) classes[i] = 0;
   if (tid == 0) taken = 0;
   if (tid < 2) bins_lds[tid] = 0;
   __syncthreads();
@@ -217,40 +242,90 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
   for (int i = 0; i < W; ++i) best = max(best, best_lds[i]);
   const float top = value_of(uint32_t(best >> 32));
   SliceHead* const head = p.heads + int64_t(row) * p.slices + slice;
+  char* const part = static_cast<char*>(p.lists) + (int64_t(row) * p.slices + slice) * p.part;
   if (rules.greedy || best == 0) {
-    if (tid == 0) *head = SliceHead{best, 0.0, 0, 0, 0, 0};
+    if (tid == 0) *head = SliceHead{best, 0.0, 0.0, 0, 0, 0, {}};
     return;
   }
-  double sum = 0.0;
-  if (rules.summed()) {
+  if (!rules.lists() && !rules.classes()) {
+    double sum = 0.0;
 #pragma unroll
     for (int l = 0; l < L; ++l)
 #pragma unroll
       for (int e = 0; e < V; ++e) sum += weight_of(x[l][e], top, rules.scale);
     sum = wave_sum(sum);
     if (lane == 0) sum_lds[wave] = sum;
+    __syncthreads();
+    if (tid == 0) {
+      sum = 0.0;
+      for (int i = 0; i < W; ++i) sum += sum_lds[i];
+      *head = SliceHead{best, sum, 0.0, 0, 0, 0, {}};
+    }
+    return;
   }
-  int valid = 0;
-  if (rules.filtered()) {
+  if (rules.classes()) {
+    const double ref = octave_of(top, rules.scale);
+    uint64_t low = 0;  // behind the last class
+    int valid = 0;
 #pragma unroll
     for (int l = 0; l < L; ++l)
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (x[l][e] > -INFINITY) {
-          ++valid;
-          atomicAdd(&hist[distance_bin(x[l][e], top)], 1);
-        }
-  }
-  __syncthreads();
-  sum = 0.0;
-  if (rules.summed())
+      for (int e = 0; e < V; ++e) {
+        const double t = octaves_below(x[l][e], ref, rules.scale);
+        const uint64_t w = uint64_t(exp2_of(t + kClassBits) + 0.5);
+        const int c = class_of(t);
+        valid += x[l][e] > -INFINITY;
+        if (c < kClasses)
+          atomicAdd(reinterpret_cast<unsigned long long*>(&classes[c]), (unsigned long long)w);
+        else
+          low += w;
+      }
 #pragma unroll
-    for (int i = 0; i < W; ++i) sum += sum_lds[i];
-  if (!rules.filtered()) {
-    if (tid == 0) *head = SliceHead{best, sum, 0, 0, 0, 0};
+    for (int o = 32; o > 0; o >>= 1) {
+      low += __shfl_xor((unsigned long long)low, o);
+      valid += __shfl_xor(valid, o);
+    }
+    __syncthreads();
+    // running sums, two classes a thread
+    const uint64_t c0 = classes[2 * tid], c1 = classes[2 * tid + 1];
+    uint64_t run = c0 + c1;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint64_t up = __shfl_up((unsigned long long)run, o);
+      if (lane >= o) run += up;
+    }
+    if (lane == 63) total_lds[wave] = run;
+    if (lane == 0) {
+      best_lds[wave] = low;
+      count_lds[wave] = valid;
+    }
+    __syncthreads();
+    for (int i = 0; i < wave; ++i) run += total_lds[i];
+    uint64_t* const sums = reinterpret_cast<uint64_t*>(part);
+    *reinterpret_cast<u32x4*>(&sums[2 * tid]) =
+        u32x4{uint32_t(run - c1), uint32_t((run - c1) >> 32), uint32_t(run), uint32_t(run >> 32)};
+    if (tid == 0) {
+      uint64_t all = 0;
+      valid = 0;
+      for (int i = 0; i < W; ++i) {
+        all += total_lds[i] + best_lds[i];
+        valid += count_lds[i];
+      }
+      *head = SliceHead{best, double(all), ref, 0, 0, uint32_t(valid), {}};
+    }
     return;
   }
-  // how many classes fit the list, and how many hold the first top_k
+  int valid = 0;
+#pragma unroll
+  for (int l = 0; l < L; ++l)
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (x[l][e] > -INFINITY) {
+        ++valid;
+        atomicAdd(&hist[distance_bin(x[l][e], top)], 1);
+      }
+  __syncthreads();
+  // how many bins fit the list, and how many hold the first top_k
   int c[4], run = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -278,15 +353,15 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
   for (int o = 32; o > 0; o >>= 1) {
     fit += __shfl_xor(fit, o);
     less += __shfl_xor(less, o);
+    valid += __shfl_xor(valid, o);
   }
   if (lane == 0) {
     atomicAdd(&bins_lds[0], fit);
     atomicAdd(&bins_lds[1], less);
   }
   __syncthreads();
-  int bins = bins_lds[0];
-  if (rules.top_k > 0) bins = min(bins, bins_lds[1] + 1);
-  uint2* const list = p.lists + (int64_t(row) * p.slices + slice) * p.cap;
+  const int bins = min(bins_lds[0], bins_lds[1] + 1);
+  uint2* const list = reinterpret_cast<uint2*>(part);
   uint32_t left = 0;
 #pragma unroll
   for (int l = 0; l < L; ++l)
@@ -300,21 +375,18 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
         left = max(left, key);
     }
   left = uint32_t(wave_max(uint64_t(left)));
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) valid += __shfl_xor(valid, o);
-  __syncthreads();
   if (lane == 0) {
     left_lds[wave] = left;
-    count_lds[wave] = valid;
+    total_lds[wave] = valid;
   }
   __syncthreads();
   if (tid == 0) {
     valid = 0;
     for (int i = 0; i < W; ++i) {
       left = max(left, left_lds[i]);
-      valid += count_lds[i];
+      valid += int(total_lds[i]);
     }
-    *head = SliceHead{best, sum, uint32_t(taken), left, uint32_t(valid), 0};
+    *head = SliceHead{best, 0.0, 0.0, uint32_t(taken), left, uint32_t(valid), {}};
   }
 }
 
@@ -512,180 +584,393 @@ struct RowSource {
   }
 };
 
+// One key a thread, the largest first, over the first n threads (a power of two).  Every thread calls it.
+__device__ uint64_t sort_down(uint64_t* lds, uint64_t key, int n) {
+  const int tid = threadIdx.x;
+  for (int size = 2; size <= n; size <<= 1)
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      uint64_t other;
+      if (stride >= 64) {
+        __syncthreads();
+        if (tid < n) lds[tid] = key;
+        __syncthreads();
+        other = tid < n ? lds[tid ^ stride] : 0;
+      } else {
+        other = __shfl_xor((unsigned long long)key, stride);
+      }
+      const bool larger = ((tid & size) == 0) == ((tid & stride) == 0);  // this place takes the larger of the two
+      key = (key > other) == larger ? key : other;
+    }
+  return key;
+}
+
+// The running sum over the first n threads, in their order; `all` the sum.
+__device__ __forceinline__ double running_sum(double* lds, double x, int n, double& all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = (n + 63) >> 6;
+  double run = x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double up = __shfl_up(run, o);
+    if (lane >= o) run += up;
+  }
+  __syncthreads();
+  if (lane == 63) lds[wave] = run;
+  __syncthreads();
+  double before = 0.0;
+  all = 0.0;
+  for (int i = 0; i < waves; ++i) {
+    if (i < wave) before += lds[i];
+    all += lds[i];
+  }
+  return before + run;
+}
+
+struct RowLds {
+  RowShared sh;
+  union {
+    struct {
+      uint32_t keys[kListMax], tokens[kListMax];
+      uint64_t weights[kListMax];
+    } list;
+    uint64_t sort[kRowThreads];
+  };
+  uint64_t best[kRowWaves];
+  uint32_t left[kRowWaves], valid[kRowWaves];
+  double ref[kRowWaves];
+  double slice[kSlicesMax];     // its weights that stay, in order
+  double factor[kSlicesMax];    // of its sums to the row's reference
+  int shift[kSlicesMax];        // of its classes
+  unsigned long long extra[kSlicesMax];  // what stays of the cut class
+  double class_sum[kClasses];
+  int cut;
+};
+
+// The draw among `weights of the slices` (lds.slice, summing to total in that order): the slice, then the token in it;
+// weight(x, token) is 0 for what does not stay.  -> the token.
+template <class T, class Weight>
+__device__ int draw_from_slices(RowLds& lds, const SampleParams& p, const Row<T>& src, int row, double target, int slice_size,
+                                Weight&& weight) {
+  RowShared& sh = lds.sh;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (wave == 0) {
+    // 64 slices at a time; the sums run on in order
+    double run = 0.0, before = 0.0;
+    int at = -1;
+    for (int s0 = 0; s0 < p.slices; s0 += 64) {
+      const double mine = s0 + lane < p.slices ? lds.slice[s0 + lane] : 0.0;
+      double sum = mine;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const double up = __shfl_up(sum, o);
+        if (lane >= o) sum += up;
+      }
+      sum += run;
+      const uint64_t past = __ballot(mine > 0.0 && sum > target), some = __ballot(mine > 0.0);
+      if (some) {
+        const int i = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);  // else the last that has any, so far
+        at = s0 + i;
+        before = __shfl(sum, i) - __shfl(mine, i);
+      }
+      if (past) break;
+      run = __shfl(sum, 63);
+    }
+    if (lane == 0) {
+      sh.slice = at;
+      sh.target = target - before;
+      sh.token = -1;
+    }
+  }
+  __syncthreads();
+  const int per = slice_size / kRowThreads;
+  const int first = sh.slice * slice_size + tid * per - src.skip;
+  const T* values = static_cast<const T*>(p.logits) + row * p.stride;
+  double mine = 0.0;
+  int last = -1;  // this thread's last token with any weight
+  for (int e = 0; e < per; ++e)
+    if (unsigned(first + e) < unsigned(p.vocab)) {
+      const float x = to_float(values[first + e]);
+      const double w = x == x ? weight(x, first + e) : 0.0;
+      mine += w;
+      if (w > 0.0) last = first + e;
+    }
+  double run = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double up = __shfl_up(run, o);
+    if (lane >= o) run += up;
+  }
+  if (lane == 63) sh.wave_d[wave] = run;
+  // the sums of this order may fall short of the slice's own by their rounding: then it is the last token
+  atomicMax(&sh.token, last);
+  __syncthreads();
+  const int fallback = sh.token;
+  double before = 0.0;
+  for (int i = 0; i < wave; ++i) before += sh.wave_d[i];
+  before += run - mine;
+  __syncthreads();
+  if (tid == 0) sh.token = 0x7fffffff;
+  __syncthreads();
+  if (before + mine > sh.target) {
+    double sum = before;
+    for (int e = 0; e < per; ++e)
+      if (unsigned(first + e) < unsigned(p.vocab)) {
+        const float x = to_float(values[first + e]);
+        const double w = x == x ? weight(x, first + e) : 0.0;
+        sum += w;
+        if (w > 0.0 && sum > sh.target) {
+          atomicMin(&sh.token, first + e);
+          break;
+        }
+      }
+  }
+  __syncthreads();
+  return min(max(sh.token == 0x7fffffff ? fallback : sh.token, 0), p.vocab - 1);
+}
+
 template <class T>
 __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleParams p, int slice_size) {
-  __shared__ RowShared sh;
-  __shared__ uint32_t list_keys[kListMax], list_tokens[kListMax];
-  __shared__ uint64_t list_weights[kListMax];
-  __shared__ uint64_t best_lds[kRowWaves];
-  __shared__ uint32_t left_lds[kRowWaves], valid_lds[kRowWaves];
-  __shared__ double slice_sums[kSlicesMax];
+  __shared__ RowLds lds;
+  RowShared& sh = lds.sh;
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Rules rules = rules_of(p, row);
   const Row<T> src(p, row);
-  const SliceHead* heads = p.heads + int64_t(row) * p.slices;
   SliceHead head = {};
-  if (tid < p.slices) head = heads[tid];
+  if (tid < p.slices) head = p.heads[int64_t(row) * p.slices + tid];
   uint64_t best = wave_max(head.best);
   uint32_t left = uint32_t(wave_max(uint64_t(head.left)));
   uint32_t valid = head.valid;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) valid += __shfl_xor(valid, o);
   if (lane == 0) {
-    best_lds[wave] = best;
-    left_lds[wave] = left;
-    valid_lds[wave] = valid;
+    lds.best[wave] = best;
+    lds.left[wave] = left;
+    lds.valid[wave] = valid;
   }
   if (tid == 0) sh.n = 0;
   __syncthreads();
   valid = 0;
 #pragma unroll
   for (int i = 0; i < kRowWaves; ++i) {
-    best = max(best, best_lds[i]);
-    left = max(left, left_lds[i]);
-    valid += valid_lds[i];
+    best = max(best, lds.best[i]);
+    left = max(left, lds.left[i]);
+    valid += lds.valid[i];
   }
   const float top = value_of(uint32_t(best >> 32));
-  const int best_token = int(~uint32_t(best));
+  const T* const values = static_cast<const T*>(p.logits) + row * p.stride;
   if (best == 0 || rules.greedy) {  // nothing to draw, or nothing to choose
     if (tid == 0) {
-      p.tokens[row] = best == 0 ? -1 : best_token;
+      p.tokens[row] = best == 0 ? -1 : int(~uint32_t(best));
       if (p.logprobs) p.logprobs[row] = best == 0 ? -INFINITY : 0.0f;
     }
     return;
   }
-  const double u = p.uniforms[row];
-  double total = 0.0;
-  if (rules.summed()) {
-    if (tid < p.slices)
-      slice_sums[tid] = head.best ? head.sum * weight_of(value_of(uint32_t(head.best >> 32)), top, rules.scale) : 0.0;
-    __syncthreads();
-    // in order, by every thread alike
-    for (int i = 0; i < p.slices; ++i) total += slice_sums[i];
-  }
-  if (!rules.filtered()) {
-    // the slice, then the token in it
-    const double target = fmin(fmax(u, 0.0), 1.0) * total;
+  const double u = fmin(fmax(double(p.uniforms[row]), 0.0), 1.0);
+  const char* const parts = static_cast<const char*>(p.lists) + int64_t(row) * p.slices * p.part;
+  auto finish = [&](int token, double total) {  // total: of the weights that stay, relative to the largest
     if (tid == 0) {
-      double run = 0.0;
-      int at = -1;
-      double at_before = 0.0;
-      for (int i = 0; i < p.slices; ++i) {
-        if (slice_sums[i] > 0.0) {
-          at = i;
-          at_before = run;
-        }
-        run += slice_sums[i];
-        if (run > target) break;
-      }
-      sh.slice = at;
-      sh.target = target - at_before;
-      sh.token = -1;
-    }
-    __syncthreads();
-    const int per = slice_size / kRowThreads;
-    const int first = sh.slice * slice_size + tid * per - src.skip;
-    double mine = 0.0;
-    int last = -1;  // this thread's last token with any weight
-    const T* values = static_cast<const T*>(p.logits) + row * p.stride;
-    for (int e = 0; e < per; ++e)
-      if (unsigned(first + e) < unsigned(p.vocab)) {
-        const float x = to_float(values[first + e]);
-        const double w = x == x ? weight_of(x, top, rules.scale) : 0.0;
-        mine += w;
-        if (w > 0.0) last = first + e;
-      }
-    double run = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double up = __shfl_up(run, o);
-      if (lane >= o) run += up;
-    }
-    if (lane == 63) sh.wave_d[wave] = run;
-    // the sums of this order may fall short of the slice's own by their rounding: then it is the last token
-    atomicMax(&sh.token, last);
-    __syncthreads();
-    const int fallback = sh.token;
-    double before = 0.0;
-    for (int i = 0; i < wave; ++i) before += sh.wave_d[i];
-    before += run - mine;
-    __syncthreads();
-    if (tid == 0) sh.token = 0x7fffffff;
-    __syncthreads();
-    if (before + mine > sh.target) {
-      double sum = before;
-      for (int e = 0; e < per; ++e)
-        if (unsigned(first + e) < unsigned(p.vocab)) {
-          const float x = to_float(values[first + e]);
-          const double w = x == x ? weight_of(x, top, rules.scale) : 0.0;
-          sum += w;
-          if (w > 0.0 && sum > sh.target) {
-            atomicMin(&sh.token, first + e);
-            break;
-          }
-        }
-    }
-    __syncthreads();
-    if (tid == 0) {
-      const int token = sh.token == 0x7fffffff ? fallback : sh.token;
       p.tokens[row] = token;
       if (p.logprobs) {
         const float x = to_float(values[token]);
-        p.logprobs[row] = float((x == top ? 0.0 : (double(x) - double(top)) * rules.scale / 1.4426950408889634) - log(total));
+        p.logprobs[row] =
+            float((x == top ? 0.0 : (double(x) - double(top)) * rules.scale * 0.69314718055994531) - log(total));
       }
     }
+  };
+  double total = 0.0;  // of the row's weights
+  if (rules.lists()) {
+    // the lists, as far as they are whole: above the largest value that some slice left out
+    for (int s = wave; s < p.slices; s += kRowWaves) {
+      const int count = min(int(p.heads[int64_t(row) * p.slices + s].count), p.cap);
+      const uint2* list = reinterpret_cast<const uint2*>(parts + s * p.part);
+      for (int i0 = 0; i0 < count; i0 += 64) {
+        const uint2 it = i0 + lane < count ? list[i0 + lane] : uint2{0, 0};
+        const bool take = it.x > left;
+        const uint64_t all = __ballot(take);
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&sh.n, __popcll(all));
+        at = __builtin_amdgcn_readfirstlane(at) + __popcll(all & ((uint64_t(1) << lane) - 1));
+        if (take && at < kListMax) {
+          lds.list.keys[at] = it.x;
+          lds.list.tokens[at] = it.y;
+        }
+      }
+    }
+    __syncthreads();
+    const int n = min(sh.n, kListMax);
+    if (n <= kRowThreads && (left == 0 || n >= rules.top_k)) {
+      // sorted, a token a thread: top-k is the first so many, top-p and min-p a prefix of them
+      uint64_t key = tid < n ? uint64_t(lds.list.keys[tid]) << 32 | uint32_t(~lds.list.tokens[tid]) : 0;
+      __syncthreads();
+      int size = 64;
+      while (size < n) size <<= 1;
+      key = sort_down(lds.sort, key, size);
+      const int k = min(n, rules.top_k);
+      const float x = value_of(uint32_t(key >> 32));
+      double w = tid < k ? weight_of(x, top, rules.scale) : 0.0, all;
+      int stay = k;
+      if (rules.use_p) {
+        const double run = running_sum(sh.wave_d, w, k, all);
+        stay = __syncthreads_count(tid < k && (tid == 0 || run - w < rules.top_p * all));
+      }
+      if (rules.use_m) stay = min(stay, __syncthreads_count(tid < k && w >= rules.min_p));
+      // and by token, for the draw
+      w = tid < stay ? w : 0.0;
+      key = tid < stay ? uint64_t(uint32_t(key)) << 32 | uint32_t(tid) : 0;
+      __syncthreads();
+      if (tid < stay) lds.list.weights[kListMax / 2 + tid] = __double_as_longlong(w);  // out of the sort's way
+      size = 64;
+      while (size < stay) size <<= 1;
+      key = sort_down(lds.sort, key, size);
+      __syncthreads();
+      w = tid < stay ? __longlong_as_double(lds.list.weights[kListMax / 2 + uint32_t(key)]) : 0.0;
+      const double run = running_sum(sh.wave_d, w, stay, all);
+      // the first past the target; rounding aside there is one, else the last with any weight
+      const int before = __syncthreads_count(tid < stay && !(run > u * all));
+      int pick = before;
+      if (before >= stay) {
+        if (tid == 0) sh.token = 0;
+        __syncthreads();
+        if (tid < stay && w > 0.0) atomicMax(&sh.token, tid);
+        __syncthreads();
+        pick = sh.token;
+      }
+      if (tid == pick) sh.slice = int(~uint32_t(key >> 32));
+      __syncthreads();
+      finish(sh.slice, all);
+      return;
+    }
+    if (left == 0 || n >= rules.top_k) {
+      constexpr int kListBits = 49;
+      for (int i = tid; i < n; i += kRowThreads)
+        lds.list.weights[i] = uint64_t(weight_of(value_of(lds.list.keys[i]), top, rules.scale) * ldexp(1.0, kListBits) + 0.5);
+      __syncthreads();
+      const Drawn got = choose(sh, ListSource{lds.list.keys, lds.list.tokens, lds.list.weights, n, p.vocab}, rules, 0.0,
+                               uint64_t(n), u, kListBits);
+      finish(got.token, got.total);
+      return;
+    }
+  } else if (!rules.classes()) {
+    if (tid < p.slices)
+      lds.slice[tid] = head.best ? head.sum * weight_of(value_of(uint32_t(head.best >> 32)), top, rules.scale) : 0.0;
+    __syncthreads();
+    for (int i = 0; i < p.slices; ++i) total += lds.slice[i];  // in order, by every thread alike
+    const int token = draw_from_slices<T>(lds, p, src, row, u * total, slice_size,
+                                          [&](float x, int) { return weight_of(x, top, rules.scale); });
+    finish(token, total);
     return;
-  }
-  // the lists, as far as they are whole: above the largest value that some slice left out
-  constexpr int kListBits = 49;
-  const double list_unit = ldexp(1.0, kListBits);
-  uint64_t sum = 0;
-  for (int s = wave; s < p.slices; s += kRowWaves) {
-    const int count = min(int(heads[s].count), p.cap);
-    const uint2* list = p.lists + (int64_t(row) * p.slices + s) * p.cap;
-    for (int i0 = 0; i0 < count; i0 += 64) {
-      const uint2 it = i0 + lane < count ? list[i0 + lane] : uint2{0, 0};
-      const bool take = it.x > left;
-      const uint64_t all = __ballot(take);
-      int at = 0;
-      if (lane == 0) at = atomicAdd(&sh.n, __popcll(all));
-      at = __builtin_amdgcn_readfirstlane(at) + __popcll(all & ((uint64_t(1) << lane) - 1));
-      if (take && at < kListMax) {
-        const uint64_t w = uint64_t(weight_of(value_of(it.x), top, rules.scale) * list_unit + 0.5);
-        list_keys[at] = it.x;
-        list_tokens[at] = it.y;
-        list_weights[at] = w;
-        sum += w;
+  } else {
+    // the row's classes: the slices' counted from the row's reference
+    const double ref = octave_of(top, rules.scale);
+    if (tid < p.slices) {
+      const double down = head.best ? fmin(ref - head.ref, 4096.0) : 4096.0;
+      lds.shift[tid] = int(down) * int(kPerOctave);
+      lds.factor[tid] = head.best ? exp2_of(-down) : 0.0;
+      lds.slice[tid] = head.best ? head.sum * lds.factor[tid] : 0.0;
+      lds.extra[tid] = 0;
+    }
+    if (tid == 0) lds.cut = kClasses;
+    __syncthreads();
+    for (int i = 0; i < p.slices; ++i) total += lds.slice[i];
+    auto upto = [&](int s, int c) -> double {  // slice s's weights in classes 0 .. c, in units of 2^-kClassBits
+      const int at = min(c - lds.shift[s], kClasses - 1);
+      if (at < 0 || lds.factor[s] == 0.0) return 0.0;
+      return double(reinterpret_cast<const uint64_t*>(parts + s * p.part)[at]) * lds.factor[s];
+    };
+    if (tid < kClasses) {
+      double sum = 0.0;
+#pragma unroll 8
+      for (int s = 0; s < p.slices; ++s) sum += upto(s, tid);
+      lds.class_sum[tid] = sum;
+    }
+    __syncthreads();
+    // the largest weight lies below the reference by up to an octave
+    const double t_top = octaves_below(top, ref, rules.scale);
+    const double t_min = rules.use_m ? t_top + log2(rules.min_p) : -1e300;
+    const double target = rules.top_p * total;
+    if (tid < kClasses && rules.use_p && lds.class_sum[tid] >= target) atomicMin(&lds.cut, tid);
+    __syncthreads();
+    const int p_cut = lds.cut;
+    const int cut = rules.use_m ? min(p_cut, class_of(t_min)) : p_cut;
+    if (cut < kClasses) {
+      const double above = cut > 0 ? lds.class_sum[cut - 1] : 0.0;
+      // the cut class's tokens: those between the logits that bound it (a little more, then exactly)
+      const double inv = 1.0 / rules.scale;
+      const double slack = 1e-9 * (1.0 + fabs(ref));  // the octaves' own rounding, far from the reference's whole part
+      double hi = (ref - cut / kPerOctave + slack) * inv, lo = (ref - (cut + 1) / kPerOctave - slack) * inv;
+      hi += 1e-6 * fabs(hi);
+      lo -= 1e-6 * fabs(lo);
+      const bool infinite = top == INFINITY;
+      const float x_hi = infinite ? INFINITY : float(hi), x_lo = infinite ? INFINITY : float(lo);
+      const int pieces = (src.skip + p.vocab + Row<T>::kVec - 1) / Row<T>::kVec;
+      constexpr int kAhead = 4;
+      for (int i0 = tid; i0 < pieces; i0 += kAhead * kRowThreads) {
+        float x[kAhead][Row<T>::kVec];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) src.get(i0 + a * kRowThreads, x[a]);
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+          for (int e = 0; e < Row<T>::kVec; ++e)
+            if (x[a][e] >= x_lo && x[a][e] <= x_hi) {
+              const double t = octaves_below(x[a][e], ref, rules.scale);
+              if (class_of(t) != cut) continue;
+              const int at = atomicAdd(&sh.n, 1);
+              if (at < kListMax) {
+                lds.list.keys[at] = ordered(x[a][e]);
+                lds.list.tokens[at] = uint32_t((i0 + a * kRowThreads) * Row<T>::kVec + e - src.skip);
+                lds.list.weights[at] = uint64_t(exp2_of(t + kClassBits) + 0.5);
+              }
+            }
+      }
+      __syncthreads();
+      const int n = sh.n;
+      if (n <= kListMax) {
+        const ListSource list = {lds.list.keys, lds.list.tokens, lds.list.weights, n, p.vocab};
+        Cut at = {0, kTokenMask};
+        if (p_cut == cut) {
+          uint64_t here = 0;
+          for (int i = tid; i < n; i += kRowThreads) here += lds.list.weights[i];
+          here = block_sum(sh, here);
+          const double rest = target - above;
+          const uint64_t need = max(uint64_t(ceil(fmax(rest, 0.0))), uint64_t(1));
+          if (need < here) at = cut_at(sh, list, at, need, [](auto&& w) { return w(); });
+        }
+        auto stays = [&](double t, uint32_t key, uint32_t token) {
+          const int c = class_of(t);
+          return c < cut || (c == cut && t >= t_min && at.keeps(key, token));
+        };
+        for (int i = tid; i < n; i += kRowThreads) {
+          const uint32_t key = lds.list.keys[i], token = lds.list.tokens[i];
+          if (stays(octaves_below(value_of(key), ref, rules.scale), key, token))
+            atomicAdd(&lds.extra[(token + src.skip) / slice_size], (unsigned long long)lds.list.weights[i]);
+        }
+        __syncthreads();
+        if (tid < p.slices) lds.slice[tid] = (cut > 0 ? upto(tid, cut - 1) : 0.0) + double(lds.extra[tid]);
+        __syncthreads();
+        double kept = 0.0;
+        for (int i = 0; i < p.slices; ++i) kept += lds.slice[i];
+        const double unit = ldexp(1.0, kClassBits);
+        const int token = draw_from_slices<T>(lds, p, src, row, u * kept, slice_size, [&](float x, int token) {
+          const double t = octaves_below(x, ref, rules.scale);
+          return stays(t, ordered(x), token) ? exp2_of(t) * unit : 0.0;
+        });
+        finish(token, kept / unit / exp2_of(t_top));
+        return;
       }
     }
+    total = total / ldexp(1.0, kClassBits) / exp2_of(t_top);
   }
-  sum = block_sum(sh, sum);
-  const int n = min(sh.n, kListMax);
-  const bool min_within = rules.use_m && weight_of(value_of(left), top, rules.scale) < rules.min_p;
-  const bool whole = left == 0 ||
-                     (rules.top_k > 0 ? uint32_t(n) >= uint32_t(rules.top_k) || (!rules.use_p && min_within)
-                                      : (rules.use_p && double(sum) >= rules.top_p * total * list_unit) || min_within);
-  Drawn got;
-  if (whole) {
-    got = choose(sh, ListSource{list_keys, list_tokens, list_weights, n, p.vocab}, rules, total, uint64_t(n), u, kListBits);
-  } else {
-    const int bits = 62 - kTokenBits;
-    const int pieces = (src.skip + p.vocab + Row<T>::kVec - 1) / Row<T>::kVec;
-    got = choose(sh, RowSource<T>{src, top, rules.scale, ldexp(1.0, bits), pieces, p.vocab}, rules, total, valid, u, bits);
-  }
-  if (tid == 0) {
-    p.tokens[row] = got.token;
-    if (p.logprobs) {
-      const float x = to_float((static_cast<const T*>(p.logits) + row * p.stride)[got.token]);
-      p.logprobs[row] = float((x == top ? 0.0 : (double(x) - double(top)) * rules.scale / 1.4426950408889634) - log(got.total));
-    }
-  }
+  const int bits = 62 - kTokenBits;
+  const int pieces = (src.skip + p.vocab + Row<T>::kVec - 1) / Row<T>::kVec;
+  const Drawn got = choose(sh, RowSource<T>{src, top, rules.scale, ldexp(1.0, bits), pieces, p.vocab}, rules, total, valid, u, bits);
+  finish(got.token, got.total);
 }
 
 // ---- the host side ----
 struct Split {
   int elements;  // of a slice, a thread
   int slices, cap;
+  int64_t part;  // bytes of a slice's list or classes
 };
 // Slices of 4096 tokens.
 Split split_of(int64_t rows, int vocab, int dtype) {
@@ -694,6 +979,7 @@ Split split_of(int64_t rows, int vocab, int dtype) {
   const int size = kSliceThreads * s.elements;
   s.slices = s.elements ? (vocab + 7 + size - 1) / size : 0;
   s.cap = s.slices ? std::min(512, kListMax / s.slices) : 0;
+  s.part = (std::max<int64_t>(s.cap * sizeof(uint2), kClasses * sizeof(uint64_t)) + 15) / 16 * 16;
   return s;
 }
 
@@ -710,7 +996,7 @@ extern "C" size_t pkv_sample_workspace_bytes(int32_t rows, int32_t vocab, int32_
   using namespace pkv;
   if (rows <= 0 || vocab <= 0) return 0;
   const Split s = split_of(rows, vocab, dtype);
-  return size_t(rows) * s.slices * (sizeof(SliceHead) + size_t(s.cap) * sizeof(uint2));
+  return size_t(rows) * s.slices * (sizeof(SliceHead) + s.part);
 }
 
 extern "C" int pkv_sample(const void* logits, int64_t stride, int32_t dtype, const float* uniforms,
@@ -745,7 +1031,7 @@ extern "C" int pkv_sample(const void* logits, int64_t stride, int32_t dtype, con
   p.tokens = tokens;
   p.logprobs = logprobs;
   p.heads = static_cast<SliceHead*>(workspace);
-  p.lists = reinterpret_cast<uint2*>(p.heads + size_t(rows) * s.slices);
+  p.lists = p.heads + size_t(rows) * s.slices;
   p.temperature = {temperatures, temperature};
   p.top_k = {top_ks, double(top_k)};
   p.top_p = {top_ps, top_p};
@@ -754,6 +1040,7 @@ extern "C" int pkv_sample(const void* logits, int64_t stride, int32_t dtype, con
   p.vocab = vocab;
   p.slices = s.slices;
   p.cap = s.cap;
+  p.part = s.part;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == PKV_BF16)
     launch<__bf16>(p, s, rows, st);
