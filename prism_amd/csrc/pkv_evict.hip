@@ -191,7 +191,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
   }
   // in the order of positions: what lies above the threshold, and the first `need` that equal it.  A kept weight moves to
   // d <= t: never to where a later chunk's lie, and this chunk's are in registers by then.
-  constexpr int G = 4;  // groups of four tokens a thread and chunk
+  constexpr int G = 1;  // groups of four tokens a thread and chunk
   int above = 0, equal = 0;  // so far
   f32x4 next[G] = {};
   auto load = [&](int t0) {

@@ -28,8 +28,15 @@ struct WeightParams {
   int64_t q_st, q_sh, page_stride, lse_st, w_page, bt_stride;
   float scale2;  // softmax scale times log2 e
   int tokens, batch, n_kv, g, log2_page, num_pages, max_blocks, n_parts;
+  uint32_t g_mul, g_shift;  // row / g
   uint32_t window;  // a row sees the keys with pos - t < window, unsigned
 };
+
+// row / g for 0 <= row < 2^30: with shift = ceil(log2 g) and mul = ceil(2^(31 + shift) / g), less than 2^32, the product
+// exceeds row * 2^(31 + shift) / g by less than row < 2^31, so by less than 1 / g of the quotient's unit.
+__device__ __forceinline__ int token_of(const WeightParams& p, int row) {
+  return int((uint64_t(uint32_t(row)) * p.g_mul) >> (31 + p.g_shift));
+}
 
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -39,6 +46,7 @@ __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
 }
 __device__ __forceinline__ bf16x8 frag(u32x4 v) { return __builtin_bit_cast(bf16x8, v); }
 
+constexpr int kFewPerCu = 4;  // workgroups of weigh_few_kernel on a CU at once
 constexpr float kLog2e = 1.4426950408889634f;
 
 // A row's denominator in log2; one that saw nothing (-inf) weighs nothing, as one of +inf does.
@@ -64,12 +72,13 @@ __device__ __forceinline__ bool seen(int pos0, int last, uint32_t window, int t0
   return t0 <= last && t1 - 1 > int64_t(pos0) - window;
 }
 
-__device__ __forceinline__ float row16_sum(float x) {  // over the 16 lanes of a row, in every lane
-  x += __shfl_xor(x, 1);
-  x += __shfl_xor(x, 2);
-  x += __shfl_xor(x, 4);
-  x += __shfl_xor(x, 8);
-  return x;
+// Over the 16 lanes of a row, in every lane: rotations within the row, no way through LDS.
+template <int CTRL>
+__device__ __forceinline__ float add_rotated(float x) {
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float row16_sum(float x) {
+  return add_rotated<0x121>(add_rotated<0x122>(add_rotated<0x124>(add_rotated<0x128>(x))));
 }
 
 // ---- few query rows: the keys stream past them ----
@@ -77,7 +86,7 @@ __device__ __forceinline__ float row16_sum(float x) {  // over the 16 lanes of a
 // takes a run of 32-key tiles straight into the A operand (16 keys x 32 elements an instruction, a lane's 16 bytes
 // of its key's row), the rows are the columns of the product: C[key, row], a lane has 4 keys of one row.
 template <int HD>
-__global__ __launch_bounds__(256) void weigh_few_kernel(const WeightParams p) {
+__global__ __launch_bounds__(256, kFewPerCu) void weigh_few_kernel(const WeightParams p) {
   constexpr int KS = HD / 32, CH = HD / 8;  // steps of the contraction, 16-byte chunks of a row
   __shared__ u32x4 q_lds[kWeightFewRows * CH];
   __shared__ float lse_lds[kWeightFewRows];
@@ -93,11 +102,11 @@ __global__ __launch_bounds__(256) void weigh_few_kernel(const WeightParams p) {
   const int cols = (it.rows + 15) & ~15;
   for (int i = threadIdx.x; i < cols * CH; i += 256) {
     const int r = i / CH, c = i % CH, row = it.row0 + min(r, it.rows - 1);
-    const int tok = it.tok0 + row / p.g, head = h * p.g + row % p.g;
+    const int j = token_of(p, row), tok = it.tok0 + j, head = h * p.g + row - j * p.g;
     q_lds[r * CH + (c ^ (r & 7))] = ld16(p.q + tok * p.q_st + head * p.q_sh + c * 8);
     if (c == 0) {
       lse_lds[r] = row_lse2(p.lse[tok * p.lse_st + head]);
-      pos_lds[r] = r < it.rows ? it.pos0 + row / p.g : -(1 << 30);
+      pos_lds[r] = r < it.rows ? it.pos0 + j : -(1 << 30);
     }
   }
   __syncthreads();
@@ -211,13 +220,14 @@ __global__ __launch_bounds__(256) void weigh_many_kernel(const WeightParams p) {
 #pragma unroll
     for (int u = 0; u < LOADS; ++u) {
       const int i = threadIdx.x + u * 256, r = i / CH, c = i % CH;
-      const int row = it.row0 + min(step * 32 + r, it.rows - 1);
-      stage[u] = ld16(p.q + int64_t(it.tok0 + row / p.g) * p.q_st + (h * p.g + row % p.g) * p.q_sh + c * 8);
+      const int row = it.row0 + min(step * 32 + r, it.rows - 1), j = token_of(p, row);
+      stage[u] = ld16(p.q + (it.tok0 + j) * p.q_st + (h * p.g + row - j * p.g) * p.q_sh + c * 8);
     }
     if (threadIdx.x < 32) {
       const int r = step * 32 + threadIdx.x, row = it.row0 + min(r, it.rows - 1);
-      stage_lse = row_lse2(p.lse[int64_t(it.tok0 + row / p.g) * p.lse_st + h * p.g + row % p.g]);
-      stage_pos = r < it.rows ? it.pos0 + row / p.g : -(1 << 30);
+      const int j = token_of(p, row);
+      stage_lse = row_lse2(p.lse[(it.tok0 + j) * p.lse_st + h * p.g + row - j * p.g]);
+      stage_pos = r < it.rows ? it.pos0 + j : -(1 << 30);
     }
   };
   auto put = [&](int buf) {
@@ -244,7 +254,7 @@ __global__ __launch_bounds__(256) void weigh_many_kernel(const WeightParams p) {
     const float lse2 = lse_lds[buf][n32];
     // positions grow with the rows: the first and last lane's say what the step's rows see
     const int lo = __builtin_amdgcn_readlane(pos, 0), full = __builtin_amdgcn_readlane(pos, 31);
-    const int hi = full >= 0 ? full : it.pos0 + (it.row0 + it.rows - 1) / p.g;
+    const int hi = full >= 0 ? full : it.pos0 + token_of(p, it.row0 + it.rows - 1);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int t0 = base + s * 32;
@@ -319,7 +329,6 @@ __global__ __launch_bounds__(kWeightBlock) void weigh_merge_kernel(const WeightP
 // ---- the host side ----
 // Few rows: pieces of the keys for four workgroups per CU, of 128 keys at least (a tile per wave).
 // Many rows: blocks of 256 keys; a block's rows are split where there are fewer than two blocks per CU.
-constexpr int kFewPerCu = 4;
 constexpr int kManyPerCu = 2;
 constexpr int kMinSteps = 8;  // of 32 rows: below that a partial's way through memory costs more than it saves
 
@@ -371,8 +380,18 @@ void weight_plan(const int32_t* new_lens, const int32_t* ctx_lens, const int32_t
       }
     }
   }
-  const int64_t few_share = (few_keys * n_kv + int64_t(cus) * kFewPerCu - 1) / (int64_t(cus) * kFewPerCu);
-  const int piece = int(std::min<int64_t>(std::max<int64_t>((few_share + 127) / 128 * 128, 128), kWeightFewKeys));
+  // the shortest pieces, in whole tiles for each of four waves, that all run at once
+  int piece = 128;
+  if (few_keys > 0) {
+    const int64_t slots = int64_t(cus) * kFewPerCu;
+    piece = int(std::min<int64_t>((few_keys * n_kv / slots + 127) / 128 * 128, kWeightFewKeys));
+    for (piece = std::max(piece, 128); piece < kWeightFewKeys; piece += 128) {
+      int64_t count = 0;
+      for (const Seq& s : seqs)
+        if (s.it.rows <= kWeightFewRows) count += (s.end - (s.first & ~31) + piece - 1) / piece;
+      if (count * n_kv <= slots) break;
+    }
+  }
   const int64_t many_share = std::max<int64_t>((many_steps * n_kv + int64_t(cus) * kManyPerCu - 1) / (int64_t(cus) * kManyPerCu), kMinSteps);
   for (const Seq& s : seqs) {
     if (s.it.rows <= kWeightFewRows) {
@@ -517,6 +536,8 @@ extern "C" int pkv_key_weights(const void* q, int64_t q_st, int64_t q_sh, const 
   p.batch = batch;
   p.n_kv = n_kv;
   p.g = n_heads / n_kv;
+  p.g_shift = uint32_t(ilog2(p.g));
+  p.g_mul = uint32_t(((uint64_t(1) << (31 + p.g_shift)) + p.g - 1) / p.g);
   p.log2_page = ilog2(page_size);
   p.num_pages = num_pages;
   p.max_blocks = max_blocks;
