@@ -86,27 +86,28 @@ __device__ __forceinline__ float row16_sum(float x) {
 // takes a run of 32-key tiles straight into the A operand (16 keys x 32 elements an instruction, a lane's 16 bytes
 // of its key's row), the rows are the columns of the product: C[key, row], a lane has 4 keys of one row.
 template <int HD>
-__global__ __launch_bounds__(256, kFewPerCu) void weigh_few_kernel(const WeightParams p) {
+struct FewLds {
+  u32x4 q[kWeightFewRows * (HD / 8)];
+  float lse[kWeightFewRows];
+  int pos[kWeightFewRows];
+};
+template <int HD>
+__device__ __forceinline__ void weigh_few(const WeightParams& p, const WeightItem it, int h, FewLds<HD>& lds) {
   constexpr int KS = HD / 32, CH = HD / 8;  // steps of the contraction, 16-byte chunks of a row
-  __shared__ u32x4 q_lds[kWeightFewRows * CH];
-  __shared__ float lse_lds[kWeightFewRows];
-  __shared__ int pos_lds[kWeightFewRows];
-  const int h = blockIdx.x % p.n_kv;
-  const WeightItem it = p.items[blockIdx.x / p.n_kv];
   if (!fits(it, p) || it.rows > kWeightFewRows || it.keys > kWeightFewKeys) {  // also what keeps a wave's page ids in its lanes
     if (threadIdx.x == 0) flag_status(p.status, PKV_STATUS_BAD_PAGE);
     return;
   }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int32_t* bt = p.bt + it.seq * p.bt_stride;
   const int cols = (it.rows + 15) & ~15;
   for (int i = threadIdx.x; i < cols * CH; i += 256) {
     const int r = i / CH, c = i % CH, row = it.row0 + min(r, it.rows - 1);
     const int j = token_of(p, row), tok = it.tok0 + j, head = h * p.g + row - j * p.g;
-    q_lds[r * CH + (c ^ (r & 7))] = ld16(p.q + tok * p.q_st + head * p.q_sh + c * 8);
+    lds.q[r * CH + (c ^ (r & 7))] = ld16(p.q + tok * p.q_st + head * p.q_sh + c * 8);
     if (c == 0) {
-      lse_lds[r] = row_lse2(p.lse[tok * p.lse_st + head]);
-      pos_lds[r] = r < it.rows ? it.pos0 + j : -(1 << 30);
+      lds.lse[r] = row_lse2(p.lse[tok * p.lse_st + head]);
+      lds.pos[r] = r < it.rows ? it.pos0 + j : -(1 << 30);
     }
   }
   __syncthreads();
@@ -143,12 +144,12 @@ __global__ __launch_bounds__(256, kFewPerCu) void weigh_few_kernel(const WeightP
       const int r = c0 + n16;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const bf16x8 b = frag(q_lds[r * CH + ((ks * 4 + quad) ^ (r & 7))]);
+        const bf16x8 b = frag(lds.q[r * CH + ((ks * 4 + quad) ^ (r & 7))]);
         acc[0] = mfma16(frag(a[0][ks]), b, acc[0]);
         acc[1] = mfma16(frag(a[1][ks]), b, acc[1]);
       }
-      const float lse2 = lse_lds[r];
-      const int ahead = pos_lds[r] - t0 - quad * 4;
+      const float lse2 = lds.lse[r];
+      const int ahead = lds.pos[r] - t0 - quad * 4;
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -183,20 +184,23 @@ __global__ __launch_bounds__(256, kFewPerCu) void weigh_few_kernel(const WeightP
 // ---- many query rows: a block of keys stays, the rows go past it ----
 // Prompt chunks: 4 waves hold 64 keys each as the A operand, 32 query rows at a time come through LDS (two buffers, one
 // barrier a step) as B: C[key, row], a lane has 16 keys of one row twice, so the row's lse is one value a lane and a
-// key's sum stays in the lane until the end.
+// key's sum stays in the lane until the end.  Exponentials bound it: of 32 x 32 scores the products take 256 cycles of
+// the matrix pipe, their 16 multiply-adds, exponentials and sums a lane 384 of the vector ALU.  So the products of one
+// 32 keys are issued between the exponentials of the other, one product for every two.
 template <int HD>
-__global__ __launch_bounds__(256) void weigh_many_kernel(const WeightParams p) {
+struct ManyLds {
+  u32x4 q[2][32 * (HD / 8)];
+  float lse[2][32];
+  int pos[2][32];
+};
+template <int HD>
+__device__ __forceinline__ void weigh_many(const WeightParams& p, const WeightItem it, int h, ManyLds<HD>& lds) {
   constexpr int KS = HD / 16, CH = HD / 8, LOADS = 32 * CH / 256;
-  __shared__ u32x4 q_lds[2][32 * CH];
-  __shared__ float lse_lds[2][32];
-  __shared__ int pos_lds[2][32];
-  const int h = blockIdx.x % p.n_kv;
-  const WeightItem it = p.items[blockIdx.x / p.n_kv];
   if (!fits(it, p) || it.keys > kWeightBlock || it.part >= p.n_parts) {
     if (threadIdx.x == 0) flag_status(p.status, PKV_STATUS_BAD_PAGE);
     return;
   }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int32_t* bt = p.bt + it.seq * p.bt_stride;
   const int n32 = lane & 31, half = lane >> 5;
   const int64_t key_st = int64_t(p.n_kv) * HD;
@@ -213,6 +217,12 @@ __global__ __launch_bounds__(256) void weigh_many_kernel(const WeightParams p) {
     for (int ks = 0; ks < KS; ++ks) a[s][ks] = frag(ld16(src + ks * 16));
   }
   const int steps = (it.rows + 31) >> 5;
+  // held in registers for the loop
+  const int rows = __builtin_amdgcn_readfirstlane(it.rows), row0 = __builtin_amdgcn_readfirstlane(it.row0);
+  const int pos0 = __builtin_amdgcn_readfirstlane(it.pos0);
+  const uint16_t* const q = p.q + it.tok0 * p.q_st + h * p.g * p.q_sh;
+  const float* const lse = p.lse + it.tok0 * p.lse_st + h * p.g;
+  const uint32_t q_st = uint32_t(p.q_st), q_sh = uint32_t(p.q_sh), lse_st = uint32_t(p.lse_st);
   u32x4 stage[LOADS];
   float stage_lse;
   int stage_pos;
@@ -220,28 +230,53 @@ __global__ __launch_bounds__(256) void weigh_many_kernel(const WeightParams p) {
 #pragma unroll
     for (int u = 0; u < LOADS; ++u) {
       const int i = threadIdx.x + u * 256, r = i / CH, c = i % CH;
-      const int row = it.row0 + min(step * 32 + r, it.rows - 1), j = token_of(p, row);
-      stage[u] = ld16(p.q + (it.tok0 + j) * p.q_st + (h * p.g + row - j * p.g) * p.q_sh + c * 8);
+      const uint32_t row = row0 + min(step * 32 + r, rows - 1), j = token_of(p, row);
+      stage[u] = ld16(q + uint64_t(j) * q_st + uint64_t(row - j * p.g) * q_sh + c * 8);
     }
     if (threadIdx.x < 32) {
-      const int r = step * 32 + threadIdx.x, row = it.row0 + min(r, it.rows - 1);
-      const int j = token_of(p, row);
-      stage_lse = row_lse2(p.lse[(it.tok0 + j) * p.lse_st + h * p.g + row - j * p.g]);
-      stage_pos = r < it.rows ? it.pos0 + j : -(1 << 30);
+      const int r = step * 32 + threadIdx.x;
+      const uint32_t row = row0 + min(r, rows - 1), j = token_of(p, row);
+      stage_lse = lse[uint64_t(j) * lse_st + (row - j * p.g)];
+      stage_pos = r < rows ? pos0 + int(j) : -(1 << 30);
     }
   };
   auto put = [&](int buf) {
 #pragma unroll
     for (int u = 0; u < LOADS; ++u) {
       const int i = threadIdx.x + u * 256, r = i / CH, c = i % CH;
-      q_lds[buf][r * CH + (c ^ (r & 7))] = stage[u];
+      lds.q[buf][r * CH + (c ^ (r & 7))] = stage[u];
     }
     if (threadIdx.x < 32) {
-      lse_lds[buf][threadIdx.x] = stage_lse;
-      pos_lds[buf][threadIdx.x] = stage_pos;
+      lds.lse[buf][threadIdx.x] = row_lse2(stage_lse);
+      lds.pos[buf][threadIdx.x] = stage_pos;
     }
   };
   float sum[2][16] = {};
+  // the scores waiting for their exponentials: of the second 32 keys and the step before, of the first 32 and this one
+  f32x16 acc[2];
+  float wait_lse = 0.0f;  // of acc[1]'s step
+  int wait_pos = 0;
+  enum { kNone, kSome, kAll };
+  int wait = kNone;  // how many of acc[1]'s scores count
+  auto consume = [&](const f32x16& c, float (&sums)[16], float lse2) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sums[i] += __builtin_amdgcn_exp2f(__builtin_fmaf(c[i], p.scale2, -lse2));
+  };
+  auto consume_some = [&](const f32x16& c, float (&sums)[16], float lse2, int ahead) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(c[i], p.scale2, -lse2));
+      sums[i] += uint32_t(ahead - (i & 3) - 8 * (i >> 2)) < p.window ? e : 0.0f;
+    }
+  };
+  // one product, then two scores' worth of the vector ALU (a product takes 32 cycles, a score's work 24)
+  auto interleave = [] {
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x402, 48 / KS, 0);
+    }
+  };
   if (steps > 0) {
     fetch(0);
     put(0);
@@ -250,35 +285,57 @@ __global__ __launch_bounds__(256) void weigh_many_kernel(const WeightParams p) {
   for (int step = 0; step < steps; ++step) {
     const int buf = step & 1;
     if (step + 1 < steps) fetch(step + 1);
-    const int pos = pos_lds[buf][n32];
-    const float lse2 = lse_lds[buf][n32];
+    const int pos = lds.pos[buf][n32];
+    const float lse2 = lds.lse[buf][n32];
     // positions grow with the rows: the first and last lane's say what the step's rows see
     const int lo = __builtin_amdgcn_readlane(pos, 0), full = __builtin_amdgcn_readlane(pos, 31);
-    const int hi = full >= 0 ? full : it.pos0 + token_of(p, it.row0 + it.rows - 1);
+    const int hi = full >= 0 ? full : pos0 + token_of(p, row0 + rows - 1);
+    int see[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int t0 = base + s * 32;
-      if (t0 >= end || !seen(lo, hi, p.window, t0, t0 + 32)) continue;
-      f32x16 acc = {};
+      see[s] = t0 >= end || !seen(lo, hi, p.window, t0, t0 + 32)               ? kNone
+               : full >= 0 && t0 + 31 <= lo && int64_t(hi) - t0 < p.window ? kAll
+                                                                           : kSome;
+    }
+    bf16x8 b[KS];
+    if (see[0] | see[1]) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        acc = mfma32(a[s][ks], frag(q_lds[buf][n32 * CH + ((ks * 2 + half) ^ (n32 & 7))]), acc);
-      if (full >= 0 && t0 + 31 <= lo && int64_t(hi) - t0 < p.window) {
+      for (int ks = 0; ks < KS; ++ks) b[ks] = frag(lds.q[buf][n32 * CH + ((ks * 2 + half) ^ (n32 & 7))]);
+    }
+    if (see[0] == kAll && see[1] == kAll && wait == kAll) {
+      acc[0] = f32x16{};
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          sum[s][i] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i], p.scale2, -lse2));
-      } else {
-        const int ahead = pos - t0 - half * 4;
+      for (int ks = 0; ks < KS; ++ks) acc[0] = mfma32(a[0][ks], b[ks], acc[0]);
+      consume(acc[1], sum[1], wait_lse);
+      interleave();
+      acc[1] = f32x16{};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i], p.scale2, -lse2));
-          sum[s][i] += uint32_t(ahead - (i & 3) - 8 * (i >> 2)) < p.window ? e : 0.0f;
-        }
+      for (int ks = 0; ks < KS; ++ks) acc[1] = mfma32(a[1][ks], b[ks], acc[1]);
+      consume(acc[0], sum[0], lse2);
+      interleave();
+    } else {
+      if (wait == kAll) consume(acc[1], sum[1], wait_lse);
+      if (wait == kSome) consume_some(acc[1], sum[1], wait_lse, wait_pos - base - 32 - half * 4);
+      if (see[0]) {
+        acc[0] = f32x16{};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) acc[0] = mfma32(a[0][ks], b[ks], acc[0]);
+        consume_some(acc[0], sum[0], lse2, pos - base - half * 4);
+      }
+      if (see[1]) {
+        acc[1] = f32x16{};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) acc[1] = mfma32(a[1][ks], b[ks], acc[1]);
       }
     }
+    wait = see[1];
+    wait_lse = lse2;
+    wait_pos = pos;
     if (step + 1 < steps) put(buf ^ 1);
     __syncthreads();
   }
+  if (wait) consume_some(acc[1], sum[1], wait_lse, wait_pos - base - 32 - half * 4);
   // over the 32 rows of a half wave; then lane i of it has key (i & 3) + 8 (i >> 2) + 4 half of the first 16 sums
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
@@ -305,6 +362,31 @@ __global__ __launch_bounds__(256) void weigh_many_kernel(const WeightParams p) {
   }
 }
 
+template <int HD>
+__global__ __launch_bounds__(256, kFewPerCu) void weigh_few_kernel(const WeightParams p) {
+  __shared__ FewLds<HD> lds;
+  weigh_few<HD>(p, p.items[blockIdx.x / p.n_kv], blockIdx.x % p.n_kv, lds);
+}
+template <int HD>
+__global__ __launch_bounds__(256) void weigh_many_kernel(const WeightParams p) {
+  __shared__ ManyLds<HD> lds;
+  weigh_many<HD>(p, p.items[blockIdx.x / p.n_kv], blockIdx.x % p.n_kv, lds);
+}
+// Both, in turn: the blocks of many rows keep the matrix and vector units busy while the others read.
+template <int HD>
+__global__ __launch_bounds__(256) void weigh_both_kernel(const WeightParams p, int n_few, int n_many) {
+  __shared__ union {
+    FewLds<HD> few;
+    ManyLds<HD> many;
+  } lds;
+  const int i = blockIdx.x / p.n_kv, h = blockIdx.x % p.n_kv, pairs = min(n_few, n_many);
+  const int at = i < 2 * pairs ? i >> 1 : i - pairs;
+  if (i < 2 * pairs ? i & 1 : n_few > n_many)
+    weigh_few<HD>(p, p.items[at], h, lds.few);
+  else
+    weigh_many<HD>(p, p.items[n_few + at], h, lds.many);
+}
+
 // The blocks whose rows were split: their partial sums, in the list's order.
 __global__ __launch_bounds__(kWeightBlock) void weigh_merge_kernel(const WeightParams p) {
   const int h = blockIdx.x % p.n_kv;
@@ -329,8 +411,8 @@ __global__ __launch_bounds__(kWeightBlock) void weigh_merge_kernel(const WeightP
 // ---- the host side ----
 // Few rows: pieces of the keys for four workgroups per CU, of 128 keys at least (a tile per wave).
 // Many rows: blocks of 256 keys; a block's rows are split where there are fewer than two blocks per CU.
-constexpr int kManyPerCu = 2;
-constexpr int kMinSteps = 8;  // of 32 rows: below that a partial's way through memory costs more than it saves
+constexpr int kManyPerCu = 8;
+constexpr int kMinSteps = 12;  // of 32 rows: below that a partial's way through memory costs more than it saves
 
 struct Lists {
   std::vector<WeightItem> few, many, merges;
@@ -506,6 +588,8 @@ extern "C" int pkv_key_weights(const void* q, int64_t q_st, int64_t q_sh, const 
   if (!(softmax_scale > 0.f) || !std::isfinite(softmax_scale)) return fail(PKV_EINVAL, "%s: bad softmax_scale", fn);
   if ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(weights)) & 3u)
     return fail(PKV_EINVAL, "%s: lse/weights not 4-byte aligned", fn);
+  if (q_st < 0 || q_sh < 0 || q_st > 0x7fffffff || q_sh > 0x7fffffff || lse_st > 0x7fffffff)
+    return fail(PKV_EINVAL, "%s: strides of q or lse past 2^31 elements", fn);
   if (lse_st < n_heads || weights_page_stride < int64_t(n_kv) * page_size)
     return fail(PKV_EINVAL, "%s: lse or weights rows overlap", fn);
   if (n_few + int64_t(n_many) + n_merges == 0) return PKV_OK;
@@ -544,16 +628,17 @@ extern "C" int pkv_key_weights(const void* q, int64_t q_st, int64_t q_sh, const 
   p.n_parts = partials;
   p.window = window > 0 ? uint32_t(window) : 0x7fffffffu;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (n_few > 0) {
+  if (n_few > 0 && n_many > 0) {
+    auto* kernel = head_dim == 128 ? weigh_both_kernel<128> : weigh_both_kernel<64>;
+    kernel<<<unsigned(n_few + n_many) * n_kv, 256, 0, s>>>(p, n_few, n_many);
+  } else if (n_few > 0) {
     auto* kernel = head_dim == 128 ? weigh_few_kernel<128> : weigh_few_kernel<64>;
     kernel<<<unsigned(n_few) * n_kv, 256, 0, s>>>(p);
-    p.items += n_few;
-  }
-  if (n_many > 0) {
+  } else if (n_many > 0) {
     auto* kernel = head_dim == 128 ? weigh_many_kernel<128> : weigh_many_kernel<64>;
     kernel<<<unsigned(n_many) * n_kv, 256, 0, s>>>(p);
-    p.items += n_many;
   }
+  p.items += n_few + n_many;
   if (n_merges > 0) weigh_merge_kernel<<<unsigned(n_merges) * n_kv, kWeightBlock, 0, s>>>(p);
   return check_launch(fn);
 }
