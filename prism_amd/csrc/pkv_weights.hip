@@ -69,7 +69,7 @@ __device__ __forceinline__ int page_of(const WeightParams& p, const int32_t* row
 
 // Whether some row of positions [pos0, last] sees some key of [t0, t1).
 __device__ __forceinline__ bool seen(int pos0, int last, uint32_t window, int t0, int t1) {
-  return t0 <= last && t1 - 1 > int64_t(pos0) - window;
+  return t0 <= last && t1 - 1 > pos0 - int(window);  // positions are not negative, windows at most 2^31 - 1
 }
 
 // Over the 16 lanes of a row, in every lane: rotations within the row, no way through LDS.
@@ -185,8 +185,8 @@ __device__ __forceinline__ void weigh_few(const WeightParams& p, const WeightIte
 // Prompt chunks: 4 waves hold 64 keys each as the A operand, 32 query rows at a time come through LDS (two buffers, one
 // barrier a step) as B: C[key, row], a lane has 16 keys of one row twice, so the row's lse is one value a lane and a
 // key's sum stays in the lane until the end.  Exponentials bound it: of 32 x 32 scores the products take 256 cycles of
-// the matrix pipe, their 16 multiply-adds, exponentials and sums a lane 384 of the vector ALU.  So the products of one
-// 32 keys are issued between the exponentials of the other, one product for every two.
+// the matrix pipe, their 16 multiply-adds, exponentials and sums a lane 384 of the vector ALU.  So the products of the
+// second 32 keys are issued between the exponentials of the first, and the other wave of the SIMD fills the rest.
 template <int HD>
 struct ManyLds {
   u32x4 q[2][32 * (HD / 8)];
@@ -252,12 +252,7 @@ __device__ __forceinline__ void weigh_many(const WeightParams& p, const WeightIt
     }
   };
   float sum[2][16] = {};
-  // the scores waiting for their exponentials: of the second 32 keys and the step before, of the first 32 and this one
-  f32x16 acc[2];
-  float wait_lse = 0.0f;  // of acc[1]'s step
-  int wait_pos = 0;
-  enum { kNone, kSome, kAll };
-  int wait = kNone;  // how many of acc[1]'s scores count
+  enum { kNone, kSome, kAll };  // of a tile's scores count
   auto consume = [&](const f32x16& c, float (&sums)[16], float lse2) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) sums[i] += __builtin_amdgcn_exp2f(__builtin_fmaf(c[i], p.scale2, -lse2));
@@ -277,6 +272,10 @@ __device__ __forceinline__ void weigh_many(const WeightParams& p, const WeightIt
       __builtin_amdgcn_sched_group_barrier(0x402, 48 / KS, 0);
     }
   };
+  // chunk ks * 2 + half of a row lies at that number ^ (row & 7): the exclusive or reaches the lowest three bits alone
+  int at[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) at[i] = n32 * CH * 16 + (((i * 2 + half) ^ (n32 & 7)) << 4);
   if (steps > 0) {
     fetch(0);
     put(0);
@@ -287,6 +286,10 @@ __device__ __forceinline__ void weigh_many(const WeightParams& p, const WeightIt
     if (step + 1 < steps) fetch(step + 1);
     const int pos = lds.pos[buf][n32];
     const float lse2 = lds.lse[buf][n32];
+    const char* const tile = reinterpret_cast<const char*>(lds.q[buf]);
+    bf16x8 b[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) b[ks] = frag(*reinterpret_cast<const u32x4*>(tile + at[ks & 3] + (ks >> 2) * 128));
     // positions grow with the rows: the first and last lane's say what the step's rows see
     const int lo = __builtin_amdgcn_readlane(pos, 0), full = __builtin_amdgcn_readlane(pos, 31);
     const int hi = full >= 0 ? full : pos0 + token_of(p, row0 + rows - 1);
@@ -294,48 +297,34 @@ __device__ __forceinline__ void weigh_many(const WeightParams& p, const WeightIt
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int t0 = base + s * 32;
-      see[s] = t0 >= end || !seen(lo, hi, p.window, t0, t0 + 32)               ? kNone
-               : full >= 0 && t0 + 31 <= lo && int64_t(hi) - t0 < p.window ? kAll
-                                                                           : kSome;
+      see[s] = t0 >= end || !seen(lo, hi, p.window, t0, t0 + 32)           ? kNone
+               : full >= 0 && t0 + 31 <= lo && hi - t0 < int(p.window) ? kAll
+                                                                       : kSome;
     }
-    bf16x8 b[KS];
-    if (see[0] | see[1]) {
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) b[ks] = frag(lds.q[buf][n32 * CH + ((ks * 2 + half) ^ (n32 & 7))]);
-    }
-    if (see[0] == kAll && see[1] == kAll && wait == kAll) {
-      acc[0] = f32x16{};
+    f32x16 acc[2];
+    if (see[0] == kAll && see[1] == kAll) {
+      acc[0] = acc[1] = f32x16{};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) acc[0] = mfma32(a[0][ks], b[ks], acc[0]);
-      consume(acc[1], sum[1], wait_lse);
-      interleave();
-      acc[1] = f32x16{};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) acc[1] = mfma32(a[1][ks], b[ks], acc[1]);
       consume(acc[0], sum[0], lse2);
+      __builtin_amdgcn_sched_group_barrier(0x008, KS, 0);
       interleave();
+      consume(acc[1], sum[1], lse2);
     } else {
-      if (wait == kAll) consume(acc[1], sum[1], wait_lse);
-      if (wait == kSome) consume_some(acc[1], sum[1], wait_lse, wait_pos - base - 32 - half * 4);
-      if (see[0]) {
-        acc[0] = f32x16{};
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) acc[0] = mfma32(a[0][ks], b[ks], acc[0]);
-        consume_some(acc[0], sum[0], lse2, pos - base - half * 4);
-      }
-      if (see[1]) {
-        acc[1] = f32x16{};
+      for (int s = 0; s < 2; ++s)
+        if (see[s]) {
+          acc[s] = f32x16{};
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) acc[1] = mfma32(a[1][ks], b[ks], acc[1]);
-      }
+          for (int ks = 0; ks < KS; ++ks) acc[s] = mfma32(a[s][ks], b[ks], acc[s]);
+          consume_some(acc[s], sum[s], lse2, pos - base - s * 32 - half * 4);
+        }
     }
-    wait = see[1];
-    wait_lse = lse2;
-    wait_pos = pos;
     if (step + 1 < steps) put(buf ^ 1);
     __syncthreads();
   }
-  if (wait) consume_some(acc[1], sum[1], wait_lse, wait_pos - base - 32 - half * 4);
   // over the 32 rows of a half wave; then lane i of it has key (i & 3) + 8 (i >> 2) + 4 half of the first 16 sums
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
