@@ -216,22 +216,41 @@ __device__ __forceinline__ void weigh_many(const WeightParams& p, const WeightIt
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) a[s][ks] = frag(ld16(src + ks * 16));
   }
+  // waited for here: in the loop the wait would take in the rows on their way too
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(a[s][ks]));
   const int steps = (it.rows + 31) >> 5;
   // held in registers for the loop
   const int rows = __builtin_amdgcn_readfirstlane(it.rows), row0 = __builtin_amdgcn_readfirstlane(it.row0);
   const int pos0 = __builtin_amdgcn_readfirstlane(it.pos0);
-  const uint16_t* const q = p.q + it.tok0 * p.q_st + h * p.g * p.q_sh;
   const float* const lse = p.lse + it.tok0 * p.lse_st + h * p.g;
-  const uint32_t q_st = uint32_t(p.q_st), q_sh = uint32_t(p.q_sh), lse_st = uint32_t(p.lse_st);
+  const uint32_t lse_st = uint32_t(p.lse_st);
+  // A thread's rows are 32 apart: (token, head) goes on by a quotient and a remainder, and wraps at the group's end.
+  // Behind the last row it stays where it is: what it reads there is not counted.
+  const int skip_j = 32 / p.g, skip_i = 32 - skip_j * p.g;
+  const int64_t ahead = skip_j * p.q_st + skip_i * p.q_sh, wrap = p.q_st - p.g * p.q_sh;
+  const uint16_t* src[LOADS];
+  int head[LOADS], left[LOADS];
+#pragma unroll
+  for (int u = 0; u < LOADS; ++u) {
+    const int i = threadIdx.x + u * 256, r = i / CH, c = i % CH, row = row0 + max(min(r, rows - 1), 0), j = token_of(p, row);
+    src[u] = p.q + (it.tok0 + j) * p.q_st + (h * p.g + row - j * p.g) * p.q_sh + c * 8;
+    head[u] = row - j * p.g;
+    left[u] = rows - r;  // rows from this one on
+  }
   u32x4 stage[LOADS];
   float stage_lse;
   int stage_pos;
   auto fetch = [&](int step) {
 #pragma unroll
     for (int u = 0; u < LOADS; ++u) {
-      const int i = threadIdx.x + u * 256, r = i / CH, c = i % CH;
-      const uint32_t row = row0 + min(step * 32 + r, rows - 1), j = token_of(p, row);
-      stage[u] = ld16(q + uint64_t(j) * q_st + uint64_t(row - j * p.g) * q_sh + c * 8);
+      stage[u] = ld16(src[u]);
+      left[u] -= 32;
+      const bool more = left[u] > 0, over = head[u] + skip_i >= p.g;
+      head[u] += over ? skip_i - p.g : skip_i;
+      src[u] += more ? ahead + (over ? wrap : 0) : 0;
     }
     if (threadIdx.x < 32) {
       const int r = step * 32 + threadIdx.x;
@@ -252,26 +271,31 @@ __device__ __forceinline__ void weigh_many(const WeightParams& p, const WeightIt
     }
   };
   float sum[2][16] = {};
-  enum { kNone, kSome, kAll };  // of a tile's scores count
-  auto consume = [&](const f32x16& c, float (&sums)[16], float lse2) {
+  // scores to weights, all of them or what a row sees
+  auto weights = [&](f32x16& c, float lse2) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sums[i] += __builtin_amdgcn_exp2f(__builtin_fmaf(c[i], p.scale2, -lse2));
+    for (int i = 0; i < 16; ++i) c[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(c[i], p.scale2, -lse2));
   };
-  auto consume_some = [&](const f32x16& c, float (&sums)[16], float lse2, int ahead) {
+  auto weights_seen = [&](f32x16& c, float lse2, int ahead) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(c[i], p.scale2, -lse2));
-      sums[i] += uint32_t(ahead - (i & 3) - 8 * (i >> 2)) < p.window ? e : 0.0f;
+      c[i] = uint32_t(ahead - (i & 3) - 8 * (i >> 2)) < p.window ? e : 0.0f;
     }
   };
-  // one product, then two scores' worth of the vector ALU (a product takes 32 cycles, a score's work 24)
+  // one product, then two scores' worth of the vector ALU
   auto interleave = [] {
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x402, 48 / KS, 0);
+      __builtin_amdgcn_sched_group_barrier(0x402, 32 / KS, 0);
     }
   };
+  // Steps all of whose rows see all 64 keys: from the first whose first row is past them to the last whose last row's
+  // window still begins before them.
+  const int64_t past = int64_t(base + 63 - pos0) * p.g - row0, before = (int64_t(base) + p.window - pos0) * p.g - row0;
+  const int full0 = base < end ? int(min(max((past + 31) >> 5, int64_t(0)), int64_t(steps))) : steps;
+  const int full1 = int(min(max(before >> 5, int64_t(0)), int64_t(rows >> 5)));
   // chunk ks * 2 + half of a row lies at that number ^ (row & 7): the exclusive or reaches the lowest three bits alone
   int at[4];
 #pragma unroll
@@ -284,44 +308,40 @@ __device__ __forceinline__ void weigh_many(const WeightParams& p, const WeightIt
   for (int step = 0; step < steps; ++step) {
     const int buf = step & 1;
     if (step + 1 < steps) fetch(step + 1);
-    const int pos = lds.pos[buf][n32];
     const float lse2 = lds.lse[buf][n32];
     const char* const tile = reinterpret_cast<const char*>(lds.q[buf]);
     bf16x8 b[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) b[ks] = frag(*reinterpret_cast<const u32x4*>(tile + at[ks & 3] + (ks >> 2) * 128));
-    // positions grow with the rows: the first and last lane's say what the step's rows see
-    const int lo = __builtin_amdgcn_readlane(pos, 0), full = __builtin_amdgcn_readlane(pos, 31);
-    const int hi = full >= 0 ? full : pos0 + token_of(p, row0 + rows - 1);
-    int see[2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int t0 = base + s * 32;
-      see[s] = t0 >= end || !seen(lo, hi, p.window, t0, t0 + 32)           ? kNone
-               : full >= 0 && t0 + 31 <= lo && hi - t0 < int(p.window) ? kAll
-                                                                       : kSome;
-    }
     f32x16 acc[2];
-    if (see[0] == kAll && see[1] == kAll) {
+    if (step >= full0 && step < full1) {
       acc[0] = acc[1] = f32x16{};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) acc[0] = mfma32(a[0][ks], b[ks], acc[0]);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) acc[1] = mfma32(a[1][ks], b[ks], acc[1]);
-      consume(acc[0], sum[0], lse2);
+      weights(acc[0], lse2);
       __builtin_amdgcn_sched_group_barrier(0x008, KS, 0);
       interleave();
-      consume(acc[1], sum[1], lse2);
+      weights(acc[1], lse2);
     } else {
+      // positions grow with the rows: the first and last row's say what the step's rows see
+      const int pos = lds.pos[buf][n32];
+      const int lo = __builtin_amdgcn_readlane(pos, 0), hi = pos0 + token_of(p, row0 + min(step * 32 + 31, rows - 1));
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        if (see[s]) {
-          acc[s] = f32x16{};
+      for (int s = 0; s < 2; ++s) {
+        const int t0 = base + s * 32;
+        acc[s] = f32x16{};
+        if (t0 >= end || !seen(lo, hi, p.window, t0, t0 + 32)) continue;
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) acc[s] = mfma32(a[s][ks], b[ks], acc[s]);
-          consume_some(acc[s], sum[s], lse2, pos - base - s * 32 - half * 4);
-        }
+        for (int ks = 0; ks < KS; ++ks) acc[s] = mfma32(a[s][ks], b[ks], acc[s]);
+        weights_seen(acc[s], lse2, pos - t0 - half * 4);
+      }
     }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum[s][i] += acc[s][i];
     if (step + 1 < steps) put(buf ^ 1);
     __syncthreads();
   }
