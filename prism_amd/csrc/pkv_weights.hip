@@ -182,20 +182,21 @@ __device__ __forceinline__ void weigh_few(const WeightParams& p, const WeightIte
 }
 
 // ---- many query rows: a block of keys stays, the rows go past it ----
-// Prompt chunks: 4 waves hold 64 keys each as the A operand, 32 query rows at a time come through LDS (two buffers, one
-// barrier a step) as B: C[key, row], a lane has 16 keys of one row twice, so the row's lse is one value a lane and a
+// Prompt chunks: 4 waves hold 64 keys each as the A operand, 64 query rows at a time come through LDS (two buffers, one
+// barrier a step) as B, 32 a product: C[key, row], a lane has 16 keys of one row twice, so the row's lse is one value a lane and a
 // key's sum stays in the lane until the end.  Exponentials bound it: of 32 x 32 scores the products take 256 cycles of
 // the matrix pipe, their 16 multiply-adds, exponentials and sums a lane 384 of the vector ALU.  So the products of the
 // second 32 keys are issued between the exponentials of the first, and the other wave of the SIMD fills the rest.
+constexpr int kStepRows = 64;
 template <int HD>
 struct ManyLds {
-  u32x4 q[2][32 * (HD / 8)];
-  float lse[2][32];
-  int pos[2][32];
+  u32x4 q[2][kStepRows * (HD / 8)];
+  float lse[2][kStepRows];
+  int pos[2][kStepRows];
 };
 template <int HD>
 __device__ __forceinline__ void weigh_many(const WeightParams& p, const WeightItem it, int h, ManyLds<HD>& lds) {
-  constexpr int KS = HD / 16, CH = HD / 8, LOADS = 32 * CH / 256;
+  constexpr int KS = HD / 16, CH = HD / 8, LOADS = kStepRows * CH / 256;
   if (!fits(it, p) || it.keys > kWeightBlock || it.part >= p.n_parts) {
     if (threadIdx.x == 0) flag_status(p.status, PKV_STATUS_BAD_PAGE);
     return;
@@ -221,15 +222,15 @@ __device__ __forceinline__ void weigh_many(const WeightParams& p, const WeightIt
   for (int s = 0; s < 2; ++s)
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(a[s][ks]));
-  const int steps = (it.rows + 31) >> 5;
+  const int steps = (it.rows + kStepRows - 1) / kStepRows;
   // held in registers for the loop
   const int rows = __builtin_amdgcn_readfirstlane(it.rows), row0 = __builtin_amdgcn_readfirstlane(it.row0);
   const int pos0 = __builtin_amdgcn_readfirstlane(it.pos0);
   const float* const lse = p.lse + it.tok0 * p.lse_st + h * p.g;
   const uint32_t lse_st = uint32_t(p.lse_st);
-  // A thread's rows are 32 apart: (token, head) goes on by a quotient and a remainder, and wraps at the group's end.
+  // A thread's rows are a step apart: (token, head) goes on by a quotient and a remainder, and wraps at the group's end.
   // Behind the last row it stays where it is: what it reads there is not counted.
-  const int skip_j = 32 / p.g, skip_i = 32 - skip_j * p.g;
+  const int skip_j = kStepRows / p.g, skip_i = kStepRows - skip_j * p.g;
   const int64_t ahead = skip_j * p.q_st + skip_i * p.q_sh, wrap = p.q_st - p.g * p.q_sh;
   const uint16_t* src[LOADS];
   int head[LOADS], left[LOADS];
@@ -247,13 +248,13 @@ __device__ __forceinline__ void weigh_many(const WeightParams& p, const WeightIt
 #pragma unroll
     for (int u = 0; u < LOADS; ++u) {
       stage[u] = ld16(src[u]);
-      left[u] -= 32;
+      left[u] -= kStepRows;
       const bool more = left[u] > 0, over = head[u] + skip_i >= p.g;
       head[u] += over ? skip_i - p.g : skip_i;
       src[u] += more ? ahead + (over ? wrap : 0) : 0;
     }
-    if (threadIdx.x < 32) {
-      const int r = step * 32 + threadIdx.x;
+    if (threadIdx.x < kStepRows) {
+      const int r = step * kStepRows + threadIdx.x;
       const uint32_t row = row0 + min(r, rows - 1), j = token_of(p, row);
       stage_lse = lse[uint64_t(j) * lse_st + (row - j * p.g)];
       stage_pos = r < rows ? pos0 + int(j) : -(1 << 30);
@@ -265,7 +266,7 @@ __device__ __forceinline__ void weigh_many(const WeightParams& p, const WeightIt
       const int i = threadIdx.x + u * 256, r = i / CH, c = i % CH;
       lds.q[buf][r * CH + (c ^ (r & 7))] = stage[u];
     }
-    if (threadIdx.x < 32) {
+    if (threadIdx.x < kStepRows) {
       lds.lse[buf][threadIdx.x] = row_lse2(stage_lse);
       lds.pos[buf][threadIdx.x] = stage_pos;
     }
@@ -291,10 +292,10 @@ __device__ __forceinline__ void weigh_many(const WeightParams& p, const WeightIt
       __builtin_amdgcn_sched_group_barrier(0x402, 32 / KS, 0);
     }
   };
-  // Steps all of whose rows see all 64 keys: from the first whose first row is past them to the last whose last row's
+  // Tiles of 32 rows that all see all 64 keys: from the first whose first row is past them to the last whose last row's
   // window still begins before them.
   const int64_t past = int64_t(base + 63 - pos0) * p.g - row0, before = (int64_t(base) + p.window - pos0) * p.g - row0;
-  const int full0 = base < end ? int(min(max((past + 31) >> 5, int64_t(0)), int64_t(steps))) : steps;
+  const int full0 = base < end ? int(min(max((past + 31) >> 5, int64_t(0)), int64_t(1 << 30))) : 1 << 30;
   const int full1 = int(min(max(before >> 5, int64_t(0)), int64_t(rows >> 5)));
   // chunk ks * 2 + half of a row lies at that number ^ (row & 7): the exclusive or reaches the lowest three bits alone
   int at[4];
@@ -308,40 +309,44 @@ __device__ __forceinline__ void weigh_many(const WeightParams& p, const WeightIt
   for (int step = 0; step < steps; ++step) {
     const int buf = step & 1;
     if (step + 1 < steps) fetch(step + 1);
-    const float lse2 = lds.lse[buf][n32];
-    const char* const tile = reinterpret_cast<const char*>(lds.q[buf]);
-    bf16x8 b[KS];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) b[ks] = frag(*reinterpret_cast<const u32x4*>(tile + at[ks & 3] + (ks >> 2) * 128));
-    f32x16 acc[2];
-    if (step >= full0 && step < full1) {
-      acc[0] = acc[1] = f32x16{};
+    for (int sub = 0; sub < kStepRows / 32; ++sub) {
+      const int tile = step * (kStepRows / 32) + sub;
+      const float lse2 = lds.lse[buf][sub * 32 + n32];
+      const char* const q_tile = reinterpret_cast<const char*>(lds.q[buf] + sub * 32 * CH);
+      bf16x8 b[KS];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) acc[0] = mfma32(a[0][ks], b[ks], acc[0]);
+      for (int ks = 0; ks < KS; ++ks) b[ks] = frag(*reinterpret_cast<const u32x4*>(q_tile + at[ks & 3] + (ks >> 2) * 128));
+      f32x16 acc[2];
+      if (tile >= full0 && tile < full1) {
+        acc[0] = acc[1] = f32x16{};
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) acc[1] = mfma32(a[1][ks], b[ks], acc[1]);
-      weights(acc[0], lse2);
-      __builtin_amdgcn_sched_group_barrier(0x008, KS, 0);
-      interleave();
-      weights(acc[1], lse2);
-    } else {
-      // positions grow with the rows: the first and last row's say what the step's rows see
-      const int pos = lds.pos[buf][n32];
-      const int lo = __builtin_amdgcn_readlane(pos, 0), hi = pos0 + token_of(p, row0 + min(step * 32 + 31, rows - 1));
+        for (int ks = 0; ks < KS; ++ks) acc[0] = mfma32(a[0][ks], b[ks], acc[0]);
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int t0 = base + s * 32;
-        acc[s] = f32x16{};
-        if (t0 >= end || !seen(lo, hi, p.window, t0, t0 + 32)) continue;
+        for (int ks = 0; ks < KS; ++ks) acc[1] = mfma32(a[1][ks], b[ks], acc[1]);
+        weights(acc[0], lse2);
+        __builtin_amdgcn_sched_group_barrier(0x008, KS, 0);
+        interleave();
+        weights(acc[1], lse2);
+      } else {
+        // positions grow with the rows: the first and last row's say what the tile's rows see
+        const int pos = lds.pos[buf][sub * 32 + n32];
+        const int lo = max(__builtin_amdgcn_readlane(pos, 0), 0), hi = pos0 + token_of(p, row0 + min(tile * 32 + 31, rows - 1));
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) acc[s] = mfma32(a[s][ks], b[ks], acc[s]);
-        weights_seen(acc[s], lse2, pos - t0 - half * 4);
+        for (int s = 0; s < 2; ++s) {
+          const int t0 = base + s * 32;
+          acc[s] = f32x16{};
+          if (t0 >= end || !seen(lo, hi, p.window, t0, t0 + 32)) continue;
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) acc[s] = mfma32(a[s][ks], b[ks], acc[s]);
+          weights_seen(acc[s], lse2, pos - t0 - half * 4);
+        }
       }
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum[s][i] += acc[s][i];
     }
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sum[s][i] += acc[s][i];
     if (step + 1 < steps) put(buf ^ 1);
     __syncthreads();
   }
@@ -503,7 +508,7 @@ void weight_plan(const int32_t* new_lens, const int32_t* ctx_lens, const int32_t
       block_rows(s, it.key0, it.key0 + it.keys, r0, r1);
       const int64_t steps = (r1 - r0 + 31) / 32;
       const int pieces = int(std::max<int64_t>(std::min((steps + many_share - 1) / many_share, steps / kMinSteps), 1));
-      const int64_t per = (steps + pieces - 1) / pieces * 32;
+      const int64_t per = ((steps + pieces - 1) / pieces + 1) / 2 * 64;
       it.row0 = r0;
       it.rows = r1 - r0;
       if (per >= r1 - r0) {
