@@ -18,6 +18,7 @@
 // a fixed order or integers (2^-42 of the largest weight or finer): no order of atomics changes a token.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "pkv_common.h"
 
@@ -102,24 +103,28 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return key == 0 ? -INFINITY : __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// 2^t: the series of exp(f ln 2) on |f| <= 1/2 to its 11th power (6e-15), scaled by the whole part; nothing below
-// 2^-1000.
-__device__ __forceinline__ double exp2_of(double t) {
-  if (t < -1000.0) return 0.0;
-  const double n = rint(t), f = t - n;
-  double r = 4.4455382718708114e-10;
-  r = fma(r, f, 7.0549116208011233e-09);
-  r = fma(r, f, 1.0178086009239699e-07);
-  r = fma(r, f, 1.3215486790144309e-06);
-  r = fma(r, f, 1.5252733804059841e-05);
-  r = fma(r, f, 1.5403530393381608e-04);
-  r = fma(r, f, 1.3333558146428443e-03);
-  r = fma(r, f, 9.6181291076284771e-03);
-  r = fma(r, f, 5.5504108664821580e-02);
-  r = fma(r, f, 2.4022650695910072e-01);
-  r = fma(r, f, 6.9314718055994531e-01);
+// 2^t for -1000 <= t <= 60: on |f| <= 1/2 the polynomial of degree 9 through the Chebyshev points (3e-14), its exponent
+// raised by the whole part, which t + 1.5 * 2^52 has rounded into its lowest bits.
+__device__ __forceinline__ double exp2_within(double t) {
+  constexpr double kWhole = 6755399441055744.0;
+  const double n = t + kWhole, f = t - (n - kWhole);
+  double r = 1.0209419265549968e-07;
+  r = fma(r, f, 1.3259628068862384e-06);
+  r = fma(r, f, 1.5252653613517797e-05);
+  r = fma(r, f, 1.5403433825801269e-04);
+  r = fma(r, f, 1.3333558236151045e-03);
+  r = fma(r, f, 9.6181291938355444e-03);
+  r = fma(r, f, 5.5504108664411090e-02);
+  r = fma(r, f, 2.4022650695640746e-01);
+  r = fma(r, f, 6.9314718055995062e-01);
   r = fma(r, f, 1.0);
-  return ldexp(r, int(n));
+  return __hiloint2double(__double2hiint(r) + (__double2loint(n) << 20), __double2loint(r));
+}
+// The same, nothing below 2^-1000.
+__device__ __forceinline__ double exp2_of(double t) { return t < -1000.0 ? 0.0 : exp2_within(t); }
+// A weight of at most 2^51 units as an integer, rounded by the sum's last place.
+__device__ __forceinline__ uint64_t whole(double units) {
+  return uint64_t(__double_as_longlong(units + 4503599627370496.0)) & 0xfffffffffffffull;
 }
 
 // exp((x - top) / T); an infinite top leaves weight to its equals alone.
@@ -139,9 +144,9 @@ template <>
 __device__ __forceinline__ float to_float(_Float16 v) { return float(v); }
 
 // The same where no maximum of the row is known yet: x / T in octaves, from a reference octave at or above the
-// largest (with +inf, whose equals alone weigh anything, 2^28, which leaves nothing to any other).
+// largest (with +inf, whose equals alone weigh anything, one that leaves nothing to any other).
 __device__ __forceinline__ double octave_of(float top, double scale) {
-  return top == INFINITY ? 268435456.0 : ceil(double(top) * scale);
+  return top == INFINITY ? 1e300 : ceil(double(top) * scale);
 }
 __device__ __forceinline__ double octaves_below(float x, double ref, double scale) {  // 0 or less; -1e300: no weight
 #pragma clang fp contract(off)  // the same bits wherever it is computed, and 0 for a product that is whole
@@ -157,6 +162,8 @@ __device__ __forceinline__ int class_of(double t) { return int(fmin(-t * kPerOct
 template <class T>
 struct Row {
   static constexpr int kVec = 16 / sizeof(T);
+  // lowest bits of the ordered values that are alike for all of one sign
+  static constexpr int kZeros = std::is_same<T, float>::value ? 0 : std::is_same<T, __bf16>::value ? 16 : 13;
   const u32x4* pieces;
   int skip, vocab;
   __device__ __forceinline__ Row(const SampleParams& p, int row) {
@@ -164,6 +171,17 @@ struct Row {
     pieces = reinterpret_cast<const u32x4*>(at & ~uintptr_t(15));
     skip = int(at & 15) / int(sizeof(T));
     vocab = p.vocab;
+  }
+  // piece i as it is, its values whatever they are outside the row
+  __device__ __forceinline__ u32x4 raw(int i) const {
+    const int first = i * kVec - skip;
+    return first < vocab && first + kVec > 0 ? pieces[i] : u32x4{};
+  }
+  __device__ __forceinline__ static float value(const u32x4& v, int e) {
+    struct alignas(16) Values {
+      T v[kVec];
+    };
+    return to_float(__builtin_bit_cast(Values, v).v[e]);
   }
   // piece i's values, -inf outside the row
   __device__ __forceinline__ void get(int i, float (&x)[kVec]) const {
@@ -204,12 +222,13 @@ __device__ __forceinline__ int distance_bin(float x, float top) {
   return min(max(b, 0), 1023);
 }
 
-template <class T, int E>
+// PLAIN: no row has a rule (the settings are numbers, and none of them is one).
+template <class T, int E, bool PLAIN>
 __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const SampleParams p) {
   constexpr int V = Row<T>::kVec, L = E / V, W = kSliceThreads / 64;
-  __shared__ uint64_t best_lds[W], classes[kClasses], total_lds[W];
+  __shared__ uint64_t best_lds[W], classes[PLAIN ? 1 : kClasses], total_lds[W];
   __shared__ double sum_lds[W];
-  __shared__ int hist[1024];
+  __shared__ int hist[PLAIN ? 1 : 1024];
   __shared__ int count_lds[W], taken, bins_lds[2];
   __shared__ uint32_t left_lds[W];
   const int slice = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -231,12 +250,14 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
   // of equal values the lowest token: a thread meets its own in ascending order, other threads' are compared by ~token
   best = wave_max(best);
   if (lane == 0) best_lds[wave] = best;
-  if (rules.lists())
-    for (int i = tid; i < 1024; i += kSliceThreads) hist[i] = 0;
-  else if (rules.classes())
-    for (int i = tid; i < kClasses; i += kSliceThreads) classes[i] = 0;
-  if (tid == 0) taken = 0;
-  if (tid < 2) bins_lds[tid] = 0;
+  if constexpr (!PLAIN) {
+    if (rules.lists())
+      for (int i = tid; i < 1024; i += kSliceThreads) hist[i] = 0;
+    else if (rules.classes())
+      for (int i = tid; i < kClasses; i += kSliceThreads) classes[i] = 0;
+    if (tid == 0) taken = 0;
+    if (tid < 2) bins_lds[tid] = 0;
+  }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < W; ++i) best = max(best, best_lds[i]);
@@ -247,12 +268,21 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
     if (tid == 0) *head = SliceHead{best, 0.0, 0.0, 0, 0, 0, {}};
     return;
   }
-  if (!rules.lists() && !rules.classes()) {
+  if (PLAIN || (!rules.lists() && !rules.classes())) {
     double sum = 0.0;
+    const double bias = -double(top) * rules.scale;
+    if (rules.scale > 0.0 && fabs(bias) < 1e6) {  // rounded to 2^-33 of an octave at most, for all of the slice alike
+      // -inf comes out as 2^-1000 of the slice's own largest: nothing
 #pragma unroll
-    for (int l = 0; l < L; ++l)
+      for (int l = 0; l < L; ++l)
 #pragma unroll
-      for (int e = 0; e < V; ++e) sum += weight_of(x[l][e], top, rules.scale);
+        for (int e = 0; e < V; ++e) sum += exp2_within(fmax(fma(double(x[l][e]), rules.scale, bias), -1000.0));
+    } else {
+#pragma unroll
+      for (int l = 0; l < L; ++l)
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum += weight_of(x[l][e], top, rules.scale);
+    }
     sum = wave_sum(sum);
     if (lane == 0) sum_lds[wave] = sum;
     __syncthreads();
@@ -263,6 +293,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
     }
     return;
   }
+  if constexpr (PLAIN) return;
   if (rules.classes()) {
     const double ref = octave_of(top, rules.scale);
     uint64_t low = 0;  // behind the last class
@@ -271,10 +302,11 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
     for (int l = 0; l < L; ++l)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const double t = octaves_below(x[l][e], ref, rules.scale);
-        const uint64_t w = uint64_t(exp2_of(t + kClassBits) + 0.5);
+        if (!(x[l][e] > -INFINITY)) continue;
+        ++valid;
+        const double t = fmax(octaves_below(x[l][e], ref, rules.scale), -900.0);
+        const uint64_t w = whole(exp2_within(t + kClassBits));
         const int c = class_of(t);
-        valid += x[l][e] > -INFINITY;
         if (c < kClasses)
           atomicAdd(reinterpret_cast<unsigned long long*>(&classes[c]), (unsigned long long)w);
         else
@@ -398,8 +430,8 @@ struct RowShared {
   uint64_t found_before, found_value;
   int found_bin;
   int n;
-  double total, target;
-  int slice, token;
+  double target;
+  int slice, token, first;
 };
 
 // The first place of a descending order at which the running sum of values reaches `target` (1 or more, and the sum
@@ -478,13 +510,16 @@ constexpr int kTokenBits = 20;
 constexpr uint32_t kTokenMask = (1u << kTokenBits) - 1;
 
 // The shortest prefix, within `cut`, whose values sum to `target`.
+// The keys lie in [low, low + 2^bits << zeros), their lowest `zeros` bits are low's.
 template <class Source, class Value>
-__device__ Cut cut_at(RowShared& sh, const Source& src, Cut cut, uint64_t target, Value&& value) {
-  const Place at = descend(sh, 32, target, [&](auto&& add) {
+__device__ Cut cut_at(RowShared& sh, const Source& src, Cut cut, uint64_t target, Value&& value, uint32_t low = 0,
+                      int bits = 32, int zeros = 0) {
+  Place at = descend(sh, bits, target, [&](auto&& add) {
     src.each([&](uint32_t k, uint32_t t, auto&& w) {
-      if (cut.keeps(k, t)) add(k, value(w));
+      if (cut.keeps(k, t)) add((k - low) >> zeros, value(w));
     });
   });
+  at.key = (at.key << zeros) + low;
   // of the tokens with that very value, all of one weight, the lowest
   uint64_t one = 0;
   src.each([&](uint32_t k, uint32_t t, auto&& w) {
@@ -584,24 +619,73 @@ struct RowSource {
   }
 };
 
-// One key a thread, the largest first, over the first n threads (a power of two).  Every thread calls it.
+// Lane l's partner l ^ MASK, without a way through LDS.
+template <int CTRL>
+__device__ __forceinline__ uint32_t moved(uint32_t x) {
+  return uint32_t(__builtin_amdgcn_update_dpp(0, int(x), CTRL, 0xf, 0xf, true));
+}
+template <int MASK>
+__device__ __forceinline__ uint32_t across(uint32_t x) {
+  if constexpr (MASK == 1) return moved<0xb1>(x);            // quad 1 0 3 2
+  if constexpr (MASK == 2) return moved<0x4e>(x);            // quad 2 3 0 1
+  if constexpr (MASK == 4) return moved<0x141>(moved<0x1b>(x));  // within eight: 7 - l of quad 3 2 1 0
+  if constexpr (MASK == 8) return moved<0x128>(x);           // a row of 16 turned by 8
+  if constexpr (MASK == 16) {
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return __lane_id() & 16 ? a[0] : a[1];
+  }
+  if constexpr (MASK == 32) {
+    const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return __lane_id() & 32 ? a[0] : a[1];
+  }
+}
+template <int MASK>
+__device__ __forceinline__ uint64_t across(uint64_t x) {
+  return uint64_t(across<MASK>(uint32_t(x >> 32))) << 32 | across<MASK>(uint32_t(x));
+}
+// Strides STRIDE .. 1 of a bitonic merge of blocks of `size`.
+template <int STRIDE>
+__device__ __forceinline__ uint64_t merge_down(uint64_t key, int size) {
+  const uint64_t other = across<STRIDE>(key);
+  const bool larger = ((threadIdx.x & size) == 0) == ((threadIdx.x & STRIDE) == 0);  // this place takes the larger
+  key = (key > other) == larger ? key : other;
+  if constexpr (STRIDE > 1) return merge_down<STRIDE / 2>(key, size);
+  return key;
+}
+// 64 keys of a wave, each block of them by `size`'s direction (64: the largest first).
+__device__ __forceinline__ uint64_t sort_wave(uint64_t key) {
+  key = merge_down<1>(key, 2);
+  key = merge_down<2>(key, 4);
+  key = merge_down<4>(key, 8);
+  key = merge_down<8>(key, 16);
+  key = merge_down<16>(key, 32);
+  return merge_down<32>(key, 64);
+}
+// One key a thread, the largest first, over the first n threads (a power of two from 64 on).  Every thread calls it.
 __device__ uint64_t sort_down(uint64_t* lds, uint64_t key, int n) {
   const int tid = threadIdx.x;
-  for (int size = 2; size <= n; size <<= 1)
-    for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      uint64_t other;
-      if (stride >= 64) {
-        __syncthreads();
-        if (tid < n) lds[tid] = key;
-        __syncthreads();
-        other = tid < n ? lds[tid ^ stride] : 0;
-      } else {
-        other = __shfl_xor((unsigned long long)key, stride);
-      }
-      const bool larger = ((tid & size) == 0) == ((tid & stride) == 0);  // this place takes the larger of the two
+  key = sort_wave(key);
+  for (int size = 128; size <= n; size <<= 1) {
+    for (int stride = size >> 1; stride >= 64; stride >>= 1) {
+      __syncthreads();
+      if (tid < n) lds[tid] = key;
+      __syncthreads();
+      const uint64_t other = tid < n ? lds[tid ^ stride] : 0;
+      const bool larger = ((tid & size) == 0) == ((tid & stride) == 0);
       key = (key > other) == larger ? key : other;
     }
+    key = merge_down<32>(key, size);
+  }
   return key;
+}
+
+__device__ __forceinline__ double wave_running_sum(double x) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double up = __shfl_up(x, o);
+    if (int(threadIdx.x & 63) >= o) x += up;
+  }
+  return x;
 }
 
 // The running sum over the first n threads, in their order; `all` the sum.
@@ -645,12 +729,16 @@ struct RowLds {
   int cut;
 };
 
+// The logarithm of a token's share of `total`, which is relative to the largest weight.
+__device__ __forceinline__ float log_share(float x, float top, const Rules& r, double total) {
+  return float((x == top ? 0.0 : (double(x) - double(top)) * r.scale * 0.69314718055994531) - log(total));
+}
+
 // The draw among `weights of the slices` (lds.slice, summing to total in that order): the slice, then the token in it;
 // weight(x, token) is 0 for what does not stay.  -> the token.
-template <class T, class Weight>
-__device__ int draw_from_slices(RowLds& lds, const SampleParams& p, const Row<T>& src, int row, double target, int slice_size,
-                                Weight&& weight) {
-  RowShared& sh = lds.sh;
+template <int PER, class T, class Lds, class Weight>
+__device__ int draw_from_slices(Lds& lds, const SampleParams& p, const Row<T>& src, int row, double target, Weight&& weight) {
+  auto& sh = lds.sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (wave == 0) {
     // 64 slices at a time; the sums run on in order
@@ -678,57 +766,91 @@ __device__ int draw_from_slices(RowLds& lds, const SampleParams& p, const Row<T>
       sh.slice = at;
       sh.target = target - before;
       sh.token = -1;
+      sh.first = 0x7fffffff;
     }
   }
   __syncthreads();
-  const int per = slice_size / kRowThreads;
-  const int first = sh.slice * slice_size + tid * per - src.skip;
+  const int first = (sh.slice * kRowThreads + tid) * PER - src.skip;
   const T* values = static_cast<const T*>(p.logits) + row * p.stride;
-  double mine = 0.0;
-  int last = -1;  // this thread's last token with any weight
-  for (int e = 0; e < per; ++e)
-    if (unsigned(first + e) < unsigned(p.vocab)) {
-      const float x = to_float(values[first + e]);
-      const double w = x == x ? weight(x, first + e) : 0.0;
-      mine += w;
-      if (w > 0.0) last = first + e;
-    }
-  double run = mine;
+  float x[PER];
+  double w[PER], mine = 0.0;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double up = __shfl_up(run, o);
-    if (lane >= o) run += up;
+  for (int e = 0; e < PER; ++e) x[e] = unsigned(first + e) < unsigned(p.vocab) ? to_float(values[first + e]) : -INFINITY;
+  int last = -1;  // this thread's last token with any weight
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    w[e] = x[e] > -INFINITY ? weight(x[e], first + e) : 0.0;
+    mine += w[e];
+    if (w[e] > 0.0) last = first + e;
   }
+  const double run = wave_running_sum(mine);
   if (lane == 63) sh.wave_d[wave] = run;
   // the sums of this order may fall short of the slice's own by their rounding: then it is the last token
-  atomicMax(&sh.token, last);
+  if (last >= 0) atomicMax(&sh.token, last);
   __syncthreads();
-  const int fallback = sh.token;
-  double before = 0.0;
-  for (int i = 0; i < wave; ++i) before += sh.wave_d[i];
-  before += run - mine;
-  __syncthreads();
-  if (tid == 0) sh.token = 0x7fffffff;
-  __syncthreads();
-  if (before + mine > sh.target) {
-    double sum = before;
-    for (int e = 0; e < per; ++e)
-      if (unsigned(first + e) < unsigned(p.vocab)) {
-        const float x = to_float(values[first + e]);
-        const double w = x == x ? weight(x, first + e) : 0.0;
-        sum += w;
-        if (w > 0.0 && sum > sh.target) {
-          atomicMin(&sh.token, first + e);
-          break;
-        }
-      }
+  double sum = 0.0;
+  for (int i = 0; i < wave; ++i) sum += sh.wave_d[i];
+  sum += run - mine;
+  int got = 0x7fffffff;
+#pragma unroll
+  for (int e = PER - 1; e >= 0; --e) {
+    double upto = sum;
+#pragma unroll
+    for (int j = 0; j <= e; ++j) upto += w[j];
+    if (w[e] > 0.0 && upto > sh.target) got = first + e;
   }
+  if (got != 0x7fffffff) atomicMin(&sh.first, got);
   __syncthreads();
-  return min(max(sh.token == 0x7fffffff ? fallback : sh.token, 0), p.vocab - 1);
+  return min(max(sh.first == 0x7fffffff ? sh.token : sh.first, 0), p.vocab - 1);
 }
 
-template <class T>
-__global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleParams p, int slice_size) {
+// Rows without a rule.
+struct PlainLds {
+  struct {
+    double wave_d[kRowWaves], target;
+    int slice, token, first;
+  } sh;
+  uint64_t best[kRowWaves];
+  double slice[kSlicesMax];
+};
+template <class T, int PER>
+__global__ __launch_bounds__(kRowThreads) void sample_plain_row_kernel(const SampleParams p) {
+  __shared__ PlainLds lds;
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  SliceHead head = {};
+  if (tid < p.slices) head = p.heads[int64_t(row) * p.slices + tid];
+  const double u = fmin(fmax(double(p.uniforms[row]), 0.0), 1.0);
+  const Rules rules = rules_of(p, row);
+  const Row<T> src(p, row);
+  uint64_t best = wave_max(head.best);
+  if (lane == 0) lds.best[wave] = best;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kRowWaves; ++i) best = max(best, lds.best[i]);
+  if (best == 0) {
+    if (tid == 0) {
+      p.tokens[row] = -1;
+      if (p.logprobs) p.logprobs[row] = -INFINITY;
+    }
+    return;
+  }
+  const float top = value_of(uint32_t(best >> 32));
+  if (tid < p.slices)
+    lds.slice[tid] = head.best ? head.sum * weight_of(value_of(uint32_t(head.best >> 32)), top, rules.scale) : 0.0;
+  __syncthreads();
+  double total = 0.0;
+  for (int i = 0; i < p.slices; ++i) total += lds.slice[i];  // in order, by every thread alike
+  const int token = draw_from_slices<PER>(lds, p, src, row, u * total,
+                                          [&](float x, int) { return weight_of(x, top, rules.scale); });
+  if (tid == 0) {
+    p.tokens[row] = token;
+    if (p.logprobs) p.logprobs[row] = log_share(to_float((static_cast<const T*>(p.logits) + row * p.stride)[token]), top, rules, total);
+  }
+}
+
+template <class T, int PER>
+__global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleParams p) {
+  constexpr int slice_size = PER * kRowThreads;
   __shared__ RowLds lds;
   RowShared& sh = lds.sh;
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -769,11 +891,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SamplePar
   auto finish = [&](int token, double total) {  // total: of the weights that stay, relative to the largest
     if (tid == 0) {
       p.tokens[row] = token;
-      if (p.logprobs) {
-        const float x = to_float(values[token]);
-        p.logprobs[row] =
-            float((x == top ? 0.0 : (double(x) - double(top)) * rules.scale * 0.69314718055994531) - log(total));
-      }
+      if (p.logprobs) p.logprobs[row] = log_share(to_float(values[token]), top, rules, total);
     }
   };
   double total = 0.0;  // of the row's weights
@@ -805,6 +923,26 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SamplePar
       while (size < n) size <<= 1;
       key = sort_down(lds.sort, key, size);
       const int k = min(n, rules.top_k);
+      if (k <= 64) {  // all in the first wave: nothing to wait for
+        if (wave > 0) return;
+        double w = lane < k ? weight_of(value_of(uint32_t(key >> 32)), top, rules.scale) : 0.0;
+        int stay = k;
+        if (rules.use_p) {
+          const double run = wave_running_sum(w), all = __shfl(run, 63);
+          stay = __popcll(__ballot(lane < k && (lane == 0 || run - w < rules.top_p * all)));
+        }
+        if (rules.use_m) stay = min(stay, int(__popcll(__ballot(lane < k && w >= rules.min_p))));
+        // and by token, for the draw
+        w = lane < stay ? w : 0.0;
+        key = sort_wave(lane < stay ? uint64_t(uint32_t(key)) << 32 | uint32_t(lane) : 0);
+        w = lane < stay ? __shfl(w, int(uint32_t(key))) : 0.0;
+        const double run = wave_running_sum(w), all = __shfl(run, 63);
+        // the first past the target, else (roundings aside there is one) the last with any weight
+        const uint64_t past = __ballot(lane < stay && run > u * all), some = __ballot(w > 0.0);
+        const int pick = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+        finish(int(~uint32_t(__shfl((unsigned long long)key, pick) >> 32)), all);
+        return;
+      }
       const float x = value_of(uint32_t(key >> 32));
       double w = tid < k ? weight_of(x, top, rules.scale) : 0.0, all;
       int stay = k;
@@ -854,8 +992,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SamplePar
       lds.slice[tid] = head.best ? head.sum * weight_of(value_of(uint32_t(head.best >> 32)), top, rules.scale) : 0.0;
     __syncthreads();
     for (int i = 0; i < p.slices; ++i) total += lds.slice[i];  // in order, by every thread alike
-    const int token = draw_from_slices<T>(lds, p, src, row, u * total, slice_size,
-                                          [&](float x, int) { return weight_of(x, top, rules.scale); });
+    const int token = draw_from_slices<PER>(lds, p, src, row, u * total,
+                                            [&](float x, int) { return weight_of(x, top, rules.scale); });
     finish(token, total);
     return;
   } else {
@@ -876,11 +1014,26 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SamplePar
       if (at < 0 || lds.factor[s] == 0.0) return 0.0;
       return double(reinterpret_cast<const uint64_t*>(parts + s * p.part)[at]) * lds.factor[s];
     };
-    if (tid < kClasses) {
+    {
+      // the even and the odd slices, by the two halves of the workgroup, eight loads on their way
+      const int c = tid & (kClasses - 1), odd = tid / kClasses;
       double sum = 0.0;
-#pragma unroll 8
-      for (int s = 0; s < p.slices; ++s) sum += upto(s, tid);
-      lds.class_sum[tid] = sum;
+      for (int s0 = odd; s0 < p.slices; s0 += 16) {
+        uint64_t v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int s = min(s0 + 2 * i, p.slices - 1);
+          v[i] = reinterpret_cast<const uint64_t*>(parts + s * p.part)[min(max(c - lds.shift[s], 0), kClasses - 1)];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int s = s0 + 2 * i;
+          if (s < p.slices && c >= lds.shift[s] && lds.factor[s] != 0.0) sum += double(v[i]) * lds.factor[s];
+        }
+      }
+      if (odd) lds.class_sum[c] = sum;
+      __syncthreads();
+      if (!odd) lds.class_sum[c] += sum;
     }
     __syncthreads();
     // the largest weight lies below the reference by up to an octave
@@ -902,25 +1055,27 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SamplePar
       const bool infinite = top == INFINITY;
       const float x_hi = infinite ? INFINITY : float(hi), x_lo = infinite ? INFINITY : float(lo);
       const int pieces = (src.skip + p.vocab + Row<T>::kVec - 1) / Row<T>::kVec;
-      constexpr int kAhead = 4;
+      constexpr int kAhead = 8;
       for (int i0 = tid; i0 < pieces; i0 += kAhead * kRowThreads) {
-        float x[kAhead][Row<T>::kVec];
+        u32x4 v[kAhead];
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a) src.get(i0 + a * kRowThreads, x[a]);
+        for (int a = 0; a < kAhead; ++a) v[a] = src.raw(i0 + a * kRowThreads);
 #pragma unroll
         for (int a = 0; a < kAhead; ++a)
 #pragma unroll
-          for (int e = 0; e < Row<T>::kVec; ++e)
-            if (x[a][e] >= x_lo && x[a][e] <= x_hi) {
-              const double t = octaves_below(x[a][e], ref, rules.scale);
-              if (class_of(t) != cut) continue;
-              const int at = atomicAdd(&sh.n, 1);
-              if (at < kListMax) {
-                lds.list.keys[at] = ordered(x[a][e]);
-                lds.list.tokens[at] = uint32_t((i0 + a * kRowThreads) * Row<T>::kVec + e - src.skip);
-                lds.list.weights[at] = uint64_t(exp2_of(t + kClassBits) + 0.5);
-              }
+          for (int e = 0; e < Row<T>::kVec; ++e) {
+            const float x = Row<T>::value(v[a], e);
+            if (!(x >= x_lo && x <= x_hi)) continue;
+            const uint32_t token = uint32_t((i0 + a * kRowThreads) * Row<T>::kVec + e - src.skip);
+            const double t = octaves_below(x, ref, rules.scale);
+            if (token >= uint32_t(p.vocab) || class_of(t) != cut) continue;
+            const int at = atomicAdd(&sh.n, 1);
+            if (at < kListMax) {
+              lds.list.keys[at] = ordered(x);
+              lds.list.tokens[at] = token;
+              lds.list.weights[at] = whole(exp2_within(t + kClassBits));
             }
+          }
       }
       __syncthreads();
       const int n = sh.n;
@@ -933,7 +1088,30 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SamplePar
           here = block_sum(sh, here);
           const double rest = target - above;
           const uint64_t need = max(uint64_t(ceil(fmax(rest, 0.0))), uint64_t(1));
-          if (need < here) at = cut_at(sh, list, at, need, [](auto&& w) { return w(); });
+          if (need < here) {
+            // few bits tell a class's values apart
+            uint32_t low = ~0u, high = 0;
+            for (int i = tid; i < n; i += kRowThreads) {
+              low = min(low, lds.list.keys[i]);
+              high = max(high, lds.list.keys[i]);
+            }
+            const uint64_t span = wave_max(uint64_t(~low)), up = wave_max(uint64_t(high));
+            if (lane == 0) {
+              lds.left[wave] = uint32_t(span);
+              lds.valid[wave] = uint32_t(up);
+            }
+            __syncthreads();
+            low = lds.left[0];
+            high = lds.valid[0];
+            for (int i = 1; i < kRowWaves; ++i) {
+              low = max(low, lds.left[i]);
+              high = max(high, lds.valid[i]);
+            }
+            low = ~low;
+            const int zeros = (low ^ high) >> 31 ? 0 : Row<T>::kZeros;
+            const int bits = 32 - int(__builtin_clz(((high - low) >> zeros) | 1));
+            at = cut_at(sh, list, at, need, [](auto&& w) { return w(); }, low, bits, zeros);
+          }
         }
         auto stays = [&](double t, uint32_t key, uint32_t token) {
           const int c = class_of(t);
@@ -950,7 +1128,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SamplePar
         double kept = 0.0;
         for (int i = 0; i < p.slices; ++i) kept += lds.slice[i];
         const double unit = ldexp(1.0, kClassBits);
-        const int token = draw_from_slices<T>(lds, p, src, row, u * kept, slice_size, [&](float x, int token) {
+        const int token = draw_from_slices<PER>(lds, p, src, row, u * kept, [&](float x, int token) {
           const double t = octaves_below(x, ref, rules.scale);
           return stays(t, ordered(x), token) ? exp2_of(t) * unit : 0.0;
         });
@@ -984,9 +1162,15 @@ Split split_of(int64_t rows, int vocab, int dtype) {
 }
 
 template <class T>
-void launch(const SampleParams& p, const Split& s, int rows, hipStream_t stream) {
-  sample_slice_kernel<T, 16><<<dim3(s.slices, rows), kSliceThreads, 0, stream>>>(p);
-  sample_row_kernel<T><<<rows, kRowThreads, 0, stream>>>(p, kSliceThreads * s.elements);
+void launch(const SampleParams& p, bool plain, int rows, hipStream_t stream) {
+  constexpr int E = 16, PER = E * kSliceThreads / kRowThreads;
+  if (plain) {
+    sample_slice_kernel<T, E, true><<<dim3(p.slices, rows), kSliceThreads, 0, stream>>>(p);
+    sample_plain_row_kernel<T, PER><<<rows, kRowThreads, 0, stream>>>(p);
+  } else {
+    sample_slice_kernel<T, E, false><<<dim3(p.slices, rows), kSliceThreads, 0, stream>>>(p);
+    sample_row_kernel<T, PER><<<rows, kRowThreads, 0, stream>>>(p);
+  }
 }
 
 }  // namespace
@@ -1042,11 +1226,13 @@ extern "C" int pkv_sample(const void* logits, int64_t stride, int32_t dtype, con
   p.cap = s.cap;
   p.part = s.part;
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool plain = !temperatures && temperature > 0.f && !top_ks && (top_k <= 0 || top_k >= vocab) && !top_ps &&
+                     !(top_p < 1.f) && !min_ps && !(min_p > 0.f);
   if (dtype == PKV_BF16)
-    launch<__bf16>(p, s, rows, st);
+    launch<__bf16>(p, plain, rows, st);
   else if (dtype == PKV_FP16)
-    launch<_Float16>(p, s, rows, st);
+    launch<_Float16>(p, plain, rows, st);
   else
-    launch<float>(p, s, rows, st);
+    launch<float>(p, plain, rows, st);
   return check_launch(fn);
 }
