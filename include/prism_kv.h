@@ -510,7 +510,7 @@ int pkv_evict(void* k_pool, void* v_pool, int64_t layer_stride, int64_t cache_pa
               int32_t* status, void* stream);
 
 /* Bytes of workspace a pkv_sample call of that size needs.  Its contents need not be kept or cleared. */
-size_t pkv_sample_workspace_bytes(int32_t rows, int32_t vocab, int32_t dtype);
+size_t pkv_sample_workspace_bytes(int32_t rows, int32_t vocab);
 
 /*
  * The next token of every row of logits [rows, vocab] (PKV_BF16, PKV_FP16 or PKV_FP32; `stride` elements from row to

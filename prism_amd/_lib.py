@@ -195,7 +195,7 @@ _SIGNATURES = {
         _I32, _I32, _P, c_size_t,        # first, recent, workspace
         _P, _P,                          # status, stream
     ]),
-    "pkv_sample_workspace_bytes": (c_size_t, [_I32] * 3),
+    "pkv_sample_workspace_bytes": (c_size_t, [_I32] * 2),
     "pkv_sample": (c_int32, [
         _P, _I64, _I32, _P,              # logits, stride, dtype, uniforms
         _P, c_float, _P, _I32,           # temperature, top_k: a row's each or one

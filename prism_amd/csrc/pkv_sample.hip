@@ -70,8 +70,8 @@ struct Rules {
   double top_p, min_p;
   int top_k;     // 0: off
   bool greedy, use_p, use_m;
-  __device__ __forceinline__ bool lists() const { return top_k > 0; }
-  __device__ __forceinline__ bool classes() const { return top_k == 0 && (use_p || use_m); }
+  __device__ __forceinline__ bool lists() const { return !greedy && top_k > 0; }
+  __device__ __forceinline__ bool classes() const { return !greedy && top_k == 0 && (use_p || use_m); }
 };
 
 __device__ __forceinline__ double setting(const Setting& s, int row) {
@@ -432,61 +432,8 @@ struct RowShared {
   int n;
   double target;
   int slice, token, first;
+  uint32_t cut_key, cut_token;
 };
-
-// The first place of a descending order at which the running sum of values reaches `target` (1 or more, and the sum
-// of all is no less): digit by digit from the top, f(add) calls add(sort key, value) for every element.
-struct Place {
-  uint32_t key;
-  uint64_t left;   // of the target, at that key
-  uint64_t value;  // of all elements of that key
-};
-template <class F>
-__device__ Place descend(RowShared& sh, int bits_total, uint64_t target, F&& f) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  uint32_t key = 0;
-  Place out = {0, target, 0};
-  for (int shift = bits_total; shift > 0;) {
-    const int bits = min(kBinBits, shift);
-    shift -= bits;
-    for (int i = tid; i < kBins; i += kRowThreads) sh.hist[i] = 0;
-    __syncthreads();
-    const uint32_t done = shift + bits >= 32 ? 0u : ~0u << (shift + bits);
-    f([&](uint32_t k, uint64_t v) {
-      if ((k & done) == key && v > 0)
-        atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[(k >> shift) & ((1u << bits) - 1)]), (unsigned long long)v);
-    });
-    __syncthreads();
-    const int at = (1 << bits) - 1 - 2 * tid;  // this thread's two bins, from the top
-    const uint64_t v0 = at >= 0 ? sh.hist[at] : 0, v1 = at >= 1 ? sh.hist[at - 1] : 0;
-    uint64_t run = v0 + v1;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint64_t up = __shfl_up((unsigned long long)run, o);
-      if (lane >= o) run += up;
-    }
-    if (lane == 63) sh.wave[wave] = run;
-    __syncthreads();
-    uint64_t before = run - v0 - v1;
-    for (int i = 0; i < wave; ++i) before += sh.wave[i];
-    if (before < out.left && before + v0 >= out.left) {
-      sh.found_bin = at;
-      sh.found_before = before;
-      sh.found_value = v0;
-    } else if (before + v0 < out.left && before + v0 + v1 >= out.left) {
-      sh.found_bin = at - 1;
-      sh.found_before = before + v0;
-      sh.found_value = v1;
-    }
-    __syncthreads();
-    key |= uint32_t(sh.found_bin) << shift;
-    out.left -= sh.found_before;
-    out.value = sh.found_value;
-  }
-  out.key = key;
-  __syncthreads();
-  return out;
-}
 
 __device__ __forceinline__ uint64_t block_sum(RowShared& sh, uint64_t x) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -501,89 +448,115 @@ __device__ __forceinline__ uint64_t block_sum(RowShared& sh, uint64_t x) {
   return x;
 }
 
+constexpr int kTokenBits = 20;
+constexpr uint32_t kTokenMask = (1u << kTokenBits) - 1;
+
 // Where in the order (value descending, token ascending) the last token that stays lies.
 struct Cut {
   uint32_t key, token;
   __device__ __forceinline__ bool keeps(uint32_t k, uint32_t t) const { return k > key || (k == key && t <= token); }
 };
-constexpr int kTokenBits = 20;
-constexpr uint32_t kTokenMask = (1u << kTokenBits) - 1;
 
-// The shortest prefix, within `cut`, whose values sum to `target`.
-// The keys lie in [low, low + 2^bits << zeros), their lowest `zeros` bits are low's.
-template <class Source, class Value>
-__device__ Cut cut_at(RowShared& sh, const Source& src, Cut cut, uint64_t target, Value&& value, uint32_t low = 0,
-                      int bits = 32, int zeros = 0) {
-  Place at = descend(sh, bits, target, [&](auto&& add) {
-    src.each([&](uint32_t k, uint32_t t, auto&& w) {
-      if (cut.keeps(k, t)) add((k - low) >> zeros, value(w));
-    });
-  });
-  at.key = (at.key << zeros) + low;
-  // of the tokens with that very value, all of one weight, the lowest
-  uint64_t one = 0;
-  src.each([&](uint32_t k, uint32_t t, auto&& w) {
-    if (k == at.key && cut.keeps(k, t)) one = value(w);
-  });
-  uint64_t m = one;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = max(m, uint64_t(__shfl_xor((unsigned long long)m, o)));
-  if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = m;
-  __syncthreads();
-  one = 0;
-  for (int i = 0; i < kRowWaves; ++i) one = max(one, sh.wave[i]);
-  __syncthreads();
-  const uint64_t ties = at.value / one, stay = (at.left + one - 1) / one;
-  if (stay >= ties) return {at.key, cut.key == at.key ? cut.token : kTokenMask};
-  const Place last = descend(sh, kTokenBits, stay, [&](auto&& add) {
-    src.each([&](uint32_t k, uint32_t t, auto&&) {
-      if (k == at.key && cut.keeps(k, t)) add(kTokenMask - t, 1);
-    });
-  });
-  return {at.key, kTokenMask - last.key};
-}
-
-struct Drawn {
+// A search through (ordered value, token, weight in units) by radix descents, each to the place of a descending order
+// where a running sum reaches a target.  Five steps use the one loop: the first top_k by value, and by token among
+// those of the last value; the shortest prefix of top_p by value, and by token; the token drawn.  (One piece of code,
+// not five: it is rarely run, and the registers of the kernels around it are better left to them.)
+enum { kByCount, kCountTies, kByShare, kShareTies, kDraw };
+struct Search {
+  Cut cut;
+  int top_k;          // 0: not a rule
+  double top_p;       // 1 or more: not a rule
+  double row_units;   // the whole row's weights, for top_p where there is no top_k; negative: the sum of what is searched
+  uint64_t least;     // min_p's weight, 1 or more
+  double u;
+  uint64_t need;      // kByShare: where not 0, the sum that the prefix has to reach
+  // results of the draw
   uint32_t token;
-  double total;  // of the weights that stay
+  uint64_t total;
 };
-
-// The rules and the draw over a source of (ordered value, token, weight in units of 2^-bits of the largest).
-// row_total: the whole row's weights (only where no top-k limits it).
 template <class Source>
-__device__ Drawn choose(RowShared& sh, const Source& src, const Rules& r, double row_total, uint64_t valid, double u, int bits) {
-  const double unit = ldexp(1.0, bits);
-  Cut cut = {0, kTokenMask};
-  if (r.top_k > 0 && uint64_t(r.top_k) < valid) cut = cut_at(sh, src, cut, uint64_t(r.top_k), [](auto&&) { return uint64_t(1); });
-  if (r.use_p) {
-    uint64_t here = 0;
-    src.each([&](uint32_t k, uint32_t t, auto&& w) {
-      if (cut.keeps(k, t)) here += w();
-    });
-    here = block_sum(sh, here);
-    const double share = r.top_p * (r.top_k > 0 ? double(here) : row_total * unit);
-    const uint64_t target = max(uint64_t(ceil(share)), uint64_t(1));
-    if (target < here) cut = cut_at(sh, src, cut, target, [](auto&& w) { return w(); });
-  }
-  const uint64_t least = r.use_m ? max(uint64_t(r.min_p * unit), uint64_t(1)) : 1;
-  uint64_t total = 0;
-  src.each([&](uint32_t k, uint32_t t, auto&& w) {
-    if (cut.keeps(k, t)) {
-      const uint64_t v = w();
-      if (v >= least) total += v;
-    }
-  });
-  total = block_sum(sh, total);
-  const uint64_t below = min(uint64_t(fmin(fmax(u, 0.0), 1.0) * double(total)), total - 1);
-  const Place at = descend(sh, kTokenBits, below + 1, [&](auto&& add) {
-    src.each([&](uint32_t k, uint32_t t, auto&& w) {
-      if (cut.keeps(k, t)) {
+__device__ __forceinline__ void search(RowShared& sh, const Source& src, Search& st, int from, int to) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  uint64_t ties = 0;  // how many of the last value stay; 0: all
+  for (int step = from; step <= to; ++step) {
+    uint64_t target = ties, sum = 0;
+    if (step == kByShare || step == kDraw) {
+      const uint64_t least = step == kDraw ? st.least : 1;
+      src.each([&](uint32_t k, uint32_t t, auto&& w) {
+        if (!st.cut.keeps(k, t)) return;
         const uint64_t v = w();
-        if (v >= least) add(kTokenMask - t, v);
+        if (v >= least) sum += v;
+      });
+      sum = block_sum(sh, sum);
+    }
+    if (step == kByCount) target = st.top_k;
+    if (step == kByShare) {
+      target = st.need;
+      if (target == 0) target = max(uint64_t(ceil(st.top_p * (st.row_units < 0.0 ? double(sum) : st.row_units))), uint64_t(1));
+      if (st.top_p >= 1.0 || target >= sum) target = 0;
+    }
+    if (step == kDraw) {
+      st.total = sum;
+      target = min(uint64_t(st.u * double(sum)), sum - 1) + 1;
+    }
+    ties = 0;
+    if (target == 0) continue;
+    const bool by_value = step == kByCount || step == kByShare, weighted = step == kByShare || step == kDraw;
+    const bool tied = step == kCountTies || step == kShareTies;
+    uint32_t key = 0;
+    uint64_t value = 0;  // of all that have the key
+    for (int shift = by_value ? 32 : kTokenBits; shift > 0;) {
+      const int bits = min(kBinBits, shift);
+      shift -= bits;
+      for (int i = tid; i < kBins; i += kRowThreads) sh.hist[i] = 0;
+      __syncthreads();
+      const uint32_t done = shift + bits >= 32 ? 0u : ~0u << (shift + bits);
+      src.each([&](uint32_t k, uint32_t t, auto&& w) {
+        if (!st.cut.keeps(k, t) || (tied && k != st.cut.key)) return;
+        const uint32_t order = by_value ? k : kTokenMask - t;
+        if ((order & done) != key) return;
+        uint64_t v = weighted ? w() : 1;
+        if (step == kDraw && v < st.least) v = 0;
+        if (v > 0)
+          atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[(order >> shift) & ((1u << bits) - 1)]), (unsigned long long)v);
+      });
+      __syncthreads();
+      const int at = (1 << bits) - 1 - 2 * tid;  // this thread's two bins, from the top
+      const uint64_t v0 = at >= 0 ? sh.hist[at] : 0, v1 = at >= 1 ? sh.hist[at - 1] : 0;
+      uint64_t run = v0 + v1;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const uint64_t up = __shfl_up((unsigned long long)run, o);
+        if (lane >= o) run += up;
       }
-    });
-  });
-  return {min(kTokenMask - at.key, uint32_t(src.vocab - 1)), double(total) / unit};
+      if (lane == 63) sh.wave[wave] = run;
+      __syncthreads();
+      uint64_t before = run - v0 - v1;
+      for (int i = 0; i < wave; ++i) before += sh.wave[i];
+      const bool first = before < target && before + v0 >= target;
+      if (first || (before + v0 < target && before + v0 + v1 >= target)) {
+        sh.found_bin = first ? at : at - 1;
+        sh.found_before = first ? before : before + v0;
+        sh.found_value = first ? v0 : v1;
+      }
+      __syncthreads();
+      key |= uint32_t(sh.found_bin) << shift;
+      target -= sh.found_before;
+      value = sh.found_value;
+    }
+    __syncthreads();
+    if (step == kDraw) {
+      st.token = min(kTokenMask - key, uint32_t(src.vocab - 1));
+    } else if (tied) {
+      st.cut.token = kTokenMask - key;
+    } else {
+      // of the tokens of that very value, all of one weight, the lowest
+      const uint64_t one = weighted ? max(src.weight(key), uint64_t(1)) : 1;
+      const uint64_t stay = (target + one - 1) / one;
+      if (st.cut.key != key) st.cut = {key, kTokenMask};
+      if (stay * one < value) ties = stay;
+    }
+  }
 }
 
 struct ListSource {
@@ -591,9 +564,17 @@ struct ListSource {
   const uint32_t* tokens;
   const uint64_t* weights;
   int n, vocab;
+  float top;
+  double ref, scale, unit;  // ref: the octave that units count from; NaN: they are of the largest weight
   template <class F>
   __device__ __forceinline__ void each(F&& f) const {
     for (int i = threadIdx.x; i < n; i += kRowThreads) f(keys[i], tokens[i], [&] { return weights[i]; });
+  }
+  // the same bits as the list's
+  __device__ __forceinline__ uint64_t weight(uint32_t key) const {
+    const float x = value_of(key);
+    return ref == ref ? whole(exp2_within(octaves_below(x, ref, scale) + kClassBits))
+                      : uint64_t(weight_of(x, top, scale) * unit + 0.5);
   }
 };
 
@@ -603,6 +584,9 @@ struct RowSource {
   float top;
   double scale, unit;
   int pieces, vocab;
+  __device__ __forceinline__ uint64_t weight(uint32_t key) const {
+    return uint64_t(weight_of(value_of(key), top, scale) * unit + 0.5);
+  }
   template <class F>
   __device__ __forceinline__ void each(F&& f) const {
     constexpr int V = Row<T>::kVec;
@@ -612,12 +596,23 @@ struct RowSource {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const uint32_t key = ordered(x[e]);
-        if (key != 0)
-          f(key, uint32_t(i * V + e - row.skip), [&] { return uint64_t(weight_of(x[e], top, scale) * unit + 0.5); });
+        if (key != 0) f(key, uint32_t(i * V + e - row.skip), [&] { return uint64_t(weight_of(x[e], top, scale) * unit + 0.5); });
       }
     }
   }
 };
+
+// All the rules: of weights in `unit`s of the largest, where `valid` tokens can be drawn.
+__device__ __forceinline__ Search whole_search(const Rules& r, double u, double unit, double row_units, uint32_t valid) {
+  Search st = {};
+  st.cut = {0, kTokenMask};
+  st.top_k = uint32_t(r.top_k) < valid ? r.top_k : 0;
+  st.top_p = r.use_p ? r.top_p : 1.0;
+  st.row_units = row_units;
+  st.least = r.use_m ? max(uint64_t(r.min_p * unit), uint64_t(1)) : 1;
+  st.u = u;
+  return st;
+}
 
 // Lane l's partner l ^ MASK, without a way through LDS.
 template <int CTRL>
@@ -711,13 +706,10 @@ __device__ __forceinline__ double running_sum(double* lds, double x, int n, doub
 
 struct RowLds {
   RowShared sh;
-  union {
-    struct {
-      uint32_t keys[kListMax], tokens[kListMax];
-      uint64_t weights[kListMax];
-    } list;
-    uint64_t sort[kRowThreads];
-  };
+  struct {
+    uint32_t keys[kListMax], tokens[kListMax];
+    uint64_t weights[kListMax];
+  } list;
   uint64_t best[kRowWaves];
   uint32_t left[kRowWaves], valid[kRowWaves];
   double ref[kRowWaves];
@@ -814,7 +806,7 @@ struct PlainLds {
   double slice[kSlicesMax];
 };
 template <class T, int PER>
-__global__ __launch_bounds__(kRowThreads) void sample_plain_row_kernel(const SampleParams p) {
+__global__ __launch_bounds__(kRowThreads) void sample_plain_kernel(const SampleParams p) {
   __shared__ PlainLds lds;
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   SliceHead head = {};
@@ -848,13 +840,161 @@ __global__ __launch_bounds__(kRowThreads) void sample_plain_row_kernel(const Sam
   }
 }
 
+// Rows with top-k.
+template <class T>
+__global__ __launch_bounds__(kRowThreads) void sample_lists_kernel(const SampleParams p) {
+  __shared__ RowLds lds;
+  RowShared& sh = lds.sh;
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const Rules rules = rules_of(p, row);
+  if (!rules.lists()) return;
+  const Row<T> src(p, row);
+  SliceHead head = {};
+  if (tid < p.slices) head = p.heads[int64_t(row) * p.slices + tid];
+  uint64_t best = wave_max(head.best);
+  uint32_t left = uint32_t(wave_max(uint64_t(head.left)));
+  uint32_t valid = head.valid;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) valid += __shfl_xor(valid, o);
+  if (lane == 0) {
+    lds.best[wave] = best;
+    lds.left[wave] = left;
+    lds.valid[wave] = valid;
+  }
+  if (tid == 0) sh.n = 0;
+  __syncthreads();
+  valid = 0;
+#pragma unroll
+  for (int i = 0; i < kRowWaves; ++i) {
+    best = max(best, lds.best[i]);
+    left = max(left, lds.left[i]);
+    valid += lds.valid[i];
+  }
+  const float top = value_of(uint32_t(best >> 32));
+  const T* const values = static_cast<const T*>(p.logits) + row * p.stride;
+  if (best == 0) {  // nothing to draw
+    if (tid == 0) {
+      p.tokens[row] = -1;
+      if (p.logprobs) p.logprobs[row] = -INFINITY;
+    }
+    return;
+  }
+  const double u = fmin(fmax(double(p.uniforms[row]), 0.0), 1.0);
+  const char* const parts = static_cast<const char*>(p.lists) + int64_t(row) * p.slices * p.part;
+  auto finish = [&](int token, double total) {  // total: of the weights that stay, relative to the largest
+    if (tid == 0) {
+      p.tokens[row] = token;
+      if (p.logprobs) p.logprobs[row] = log_share(to_float(values[token]), top, rules, total);
+    }
+  };
+  // the lists, as far as they are whole: above the largest value that some slice left out
+  for (int s = wave; s < p.slices; s += kRowWaves) {
+    const int count = min(int(p.heads[int64_t(row) * p.slices + s].count), p.cap);
+    const uint2* list = reinterpret_cast<const uint2*>(parts + s * p.part);
+    for (int i0 = 0; i0 < count; i0 += 64) {
+      const uint2 it = i0 + lane < count ? list[i0 + lane] : uint2{0, 0};
+      const bool take = it.x > left;
+      const uint64_t all = __ballot(take);
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&sh.n, __popcll(all));
+      at = __builtin_amdgcn_readfirstlane(at) + __popcll(all & ((uint64_t(1) << lane) - 1));
+      if (take && at < kListMax) {
+        lds.list.keys[at] = it.x;
+        lds.list.tokens[at] = it.y;
+      }
+    }
+  }
+  __syncthreads();
+  const int n = min(sh.n, kListMax);
+  if (n <= kRowThreads && (left == 0 || n >= rules.top_k)) {
+    // sorted, a token a thread: top-k is the first so many, top-p and min-p a prefix of them
+    uint64_t key = tid < n ? uint64_t(lds.list.keys[tid]) << 32 | uint32_t(~lds.list.tokens[tid]) : 0;
+    __syncthreads();
+    int size = 64;
+    while (size < n) size <<= 1;
+    key = sort_down(sh.hist, key, size);
+    const int k = min(n, rules.top_k);
+    if (k <= 64) {  // all in the first wave: nothing to wait for
+      if (wave > 0) return;
+      double w = lane < k ? weight_of(value_of(uint32_t(key >> 32)), top, rules.scale) : 0.0;
+      int stay = k;
+      if (rules.use_p) {
+        const double run = wave_running_sum(w), all = __shfl(run, 63);
+        stay = __popcll(__ballot(lane < k && (lane == 0 || run - w < rules.top_p * all)));
+      }
+      if (rules.use_m) stay = min(stay, int(__popcll(__ballot(lane < k && w >= rules.min_p))));
+      // and by token, for the draw
+      w = lane < stay ? w : 0.0;
+      key = sort_wave(lane < stay ? uint64_t(uint32_t(key)) << 32 | uint32_t(lane) : 0);
+      w = lane < stay ? __shfl(w, int(uint32_t(key))) : 0.0;
+      const double run = wave_running_sum(w), all = __shfl(run, 63);
+      // the first past the target, else (roundings aside there is one) the last with any weight
+      const uint64_t past = __ballot(lane < stay && run > u * all), some = __ballot(w > 0.0);
+      const int pick = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+      finish(int(~uint32_t(__shfl((unsigned long long)key, pick) >> 32)), all);
+      return;
+    }
+    const float x = value_of(uint32_t(key >> 32));
+    double w = tid < k ? weight_of(x, top, rules.scale) : 0.0, all;
+    int stay = k;
+    if (rules.use_p) {
+      const double run = running_sum(sh.wave_d, w, k, all);
+      stay = __syncthreads_count(tid < k && (tid == 0 || run - w < rules.top_p * all));
+    }
+    if (rules.use_m) stay = min(stay, __syncthreads_count(tid < k && w >= rules.min_p));
+    // and by token, for the draw
+    w = tid < stay ? w : 0.0;
+    key = tid < stay ? uint64_t(uint32_t(key)) << 32 | uint32_t(tid) : 0;
+    __syncthreads();
+    if (tid < stay) lds.list.weights[tid] = __double_as_longlong(w);
+    size = 64;
+    while (size < stay) size <<= 1;
+    key = sort_down(sh.hist, key, size);
+    __syncthreads();
+    w = tid < stay ? __longlong_as_double(lds.list.weights[uint32_t(key)]) : 0.0;
+    const double run = running_sum(sh.wave_d, w, stay, all);
+    // the first past the target; rounding aside there is one, else the last with any weight
+    const int before = __syncthreads_count(tid < stay && !(run > u * all));
+    int pick = before;
+    if (before >= stay) {
+      if (tid == 0) sh.token = 0;
+      __syncthreads();
+      if (tid < stay && w > 0.0) atomicMax(&sh.token, tid);
+      __syncthreads();
+      pick = sh.token;
+    }
+    if (tid == pick) sh.slice = int(~uint32_t(key >> 32));
+    __syncthreads();
+    finish(sh.slice, all);
+    return;
+  }
+  if (left == 0 || n >= rules.top_k) {
+    constexpr int kListBits = 49;
+    const double unit = ldexp(1.0, kListBits);
+    for (int i = tid; i < n; i += kRowThreads)
+      lds.list.weights[i] = uint64_t(weight_of(value_of(lds.list.keys[i]), top, rules.scale) * unit + 0.5);
+    __syncthreads();
+    Search st = whole_search(rules, u, unit, -1.0, uint32_t(n));
+    search(sh, ListSource{lds.list.keys, lds.list.tokens, lds.list.weights, n, p.vocab, top, NAN, rules.scale, unit}, st, kByCount, kDraw);
+    finish(int(st.token), double(st.total) / unit);
+    return;
+  }
+  const double unit = ldexp(1.0, 62 - kTokenBits);
+  const int pieces = (src.skip + p.vocab + Row<T>::kVec - 1) / Row<T>::kVec;
+  Search st = whole_search(rules, u, unit, -1.0, valid);
+  search(sh, RowSource<T>{src, top, rules.scale, unit, pieces, p.vocab}, st, kByCount, kDraw);
+  finish(int(st.token), double(st.total) / unit);
+}
+
+// Every other row, where some have rules.
 template <class T, int PER>
-__global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleParams p) {
+__global__ __launch_bounds__(kRowThreads) void sample_classes_kernel(const SampleParams p) {
   constexpr int slice_size = PER * kRowThreads;
   __shared__ RowLds lds;
   RowShared& sh = lds.sh;
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Rules rules = rules_of(p, row);
+  if (rules.lists()) return;
   const Row<T> src(p, row);
   SliceHead head = {};
   if (tid < p.slices) head = p.heads[int64_t(row) * p.slices + tid];
@@ -895,99 +1035,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SamplePar
     }
   };
   double total = 0.0;  // of the row's weights
-  if (rules.lists()) {
-    // the lists, as far as they are whole: above the largest value that some slice left out
-    for (int s = wave; s < p.slices; s += kRowWaves) {
-      const int count = min(int(p.heads[int64_t(row) * p.slices + s].count), p.cap);
-      const uint2* list = reinterpret_cast<const uint2*>(parts + s * p.part);
-      for (int i0 = 0; i0 < count; i0 += 64) {
-        const uint2 it = i0 + lane < count ? list[i0 + lane] : uint2{0, 0};
-        const bool take = it.x > left;
-        const uint64_t all = __ballot(take);
-        int at = 0;
-        if (lane == 0) at = atomicAdd(&sh.n, __popcll(all));
-        at = __builtin_amdgcn_readfirstlane(at) + __popcll(all & ((uint64_t(1) << lane) - 1));
-        if (take && at < kListMax) {
-          lds.list.keys[at] = it.x;
-          lds.list.tokens[at] = it.y;
-        }
-      }
-    }
-    __syncthreads();
-    const int n = min(sh.n, kListMax);
-    if (n <= kRowThreads && (left == 0 || n >= rules.top_k)) {
-      // sorted, a token a thread: top-k is the first so many, top-p and min-p a prefix of them
-      uint64_t key = tid < n ? uint64_t(lds.list.keys[tid]) << 32 | uint32_t(~lds.list.tokens[tid]) : 0;
-      __syncthreads();
-      int size = 64;
-      while (size < n) size <<= 1;
-      key = sort_down(lds.sort, key, size);
-      const int k = min(n, rules.top_k);
-      if (k <= 64) {  // all in the first wave: nothing to wait for
-        if (wave > 0) return;
-        double w = lane < k ? weight_of(value_of(uint32_t(key >> 32)), top, rules.scale) : 0.0;
-        int stay = k;
-        if (rules.use_p) {
-          const double run = wave_running_sum(w), all = __shfl(run, 63);
-          stay = __popcll(__ballot(lane < k && (lane == 0 || run - w < rules.top_p * all)));
-        }
-        if (rules.use_m) stay = min(stay, int(__popcll(__ballot(lane < k && w >= rules.min_p))));
-        // and by token, for the draw
-        w = lane < stay ? w : 0.0;
-        key = sort_wave(lane < stay ? uint64_t(uint32_t(key)) << 32 | uint32_t(lane) : 0);
-        w = lane < stay ? __shfl(w, int(uint32_t(key))) : 0.0;
-        const double run = wave_running_sum(w), all = __shfl(run, 63);
-        // the first past the target, else (roundings aside there is one) the last with any weight
-        const uint64_t past = __ballot(lane < stay && run > u * all), some = __ballot(w > 0.0);
-        const int pick = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
-        finish(int(~uint32_t(__shfl((unsigned long long)key, pick) >> 32)), all);
-        return;
-      }
-      const float x = value_of(uint32_t(key >> 32));
-      double w = tid < k ? weight_of(x, top, rules.scale) : 0.0, all;
-      int stay = k;
-      if (rules.use_p) {
-        const double run = running_sum(sh.wave_d, w, k, all);
-        stay = __syncthreads_count(tid < k && (tid == 0 || run - w < rules.top_p * all));
-      }
-      if (rules.use_m) stay = min(stay, __syncthreads_count(tid < k && w >= rules.min_p));
-      // and by token, for the draw
-      w = tid < stay ? w : 0.0;
-      key = tid < stay ? uint64_t(uint32_t(key)) << 32 | uint32_t(tid) : 0;
-      __syncthreads();
-      if (tid < stay) lds.list.weights[kListMax / 2 + tid] = __double_as_longlong(w);  // out of the sort's way
-      size = 64;
-      while (size < stay) size <<= 1;
-      key = sort_down(lds.sort, key, size);
-      __syncthreads();
-      w = tid < stay ? __longlong_as_double(lds.list.weights[kListMax / 2 + uint32_t(key)]) : 0.0;
-      const double run = running_sum(sh.wave_d, w, stay, all);
-      // the first past the target; rounding aside there is one, else the last with any weight
-      const int before = __syncthreads_count(tid < stay && !(run > u * all));
-      int pick = before;
-      if (before >= stay) {
-        if (tid == 0) sh.token = 0;
-        __syncthreads();
-        if (tid < stay && w > 0.0) atomicMax(&sh.token, tid);
-        __syncthreads();
-        pick = sh.token;
-      }
-      if (tid == pick) sh.slice = int(~uint32_t(key >> 32));
-      __syncthreads();
-      finish(sh.slice, all);
-      return;
-    }
-    if (left == 0 || n >= rules.top_k) {
-      constexpr int kListBits = 49;
-      for (int i = tid; i < n; i += kRowThreads)
-        lds.list.weights[i] = uint64_t(weight_of(value_of(lds.list.keys[i]), top, rules.scale) * ldexp(1.0, kListBits) + 0.5);
-      __syncthreads();
-      const Drawn got = choose(sh, ListSource{lds.list.keys, lds.list.tokens, lds.list.weights, n, p.vocab}, rules, 0.0,
-                               uint64_t(n), u, kListBits);
-      finish(got.token, got.total);
-      return;
-    }
-  } else if (!rules.classes()) {
+  if (!rules.classes()) {
     if (tid < p.slices)
       lds.slice[tid] = head.best ? head.sum * weight_of(value_of(uint32_t(head.best >> 32)), top, rules.scale) : 0.0;
     __syncthreads();
@@ -996,152 +1044,161 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SamplePar
                                             [&](float x, int) { return weight_of(x, top, rules.scale); });
     finish(token, total);
     return;
-  } else {
-    // the row's classes: the slices' counted from the row's reference
-    const double ref = octave_of(top, rules.scale);
-    if (tid < p.slices) {
-      const double down = head.best ? fmin(ref - head.ref, 4096.0) : 4096.0;
-      lds.shift[tid] = int(down) * int(kPerOctave);
-      lds.factor[tid] = head.best ? exp2_of(-down) : 0.0;
-      lds.slice[tid] = head.best ? head.sum * lds.factor[tid] : 0.0;
-      lds.extra[tid] = 0;
-    }
-    if (tid == 0) lds.cut = kClasses;
-    __syncthreads();
-    for (int i = 0; i < p.slices; ++i) total += lds.slice[i];
-    auto upto = [&](int s, int c) -> double {  // slice s's weights in classes 0 .. c, in units of 2^-kClassBits
-      const int at = min(c - lds.shift[s], kClasses - 1);
-      if (at < 0 || lds.factor[s] == 0.0) return 0.0;
-      return double(reinterpret_cast<const uint64_t*>(parts + s * p.part)[at]) * lds.factor[s];
-    };
-    {
-      // the even and the odd slices, by the two halves of the workgroup, eight loads on their way
-      const int c = tid & (kClasses - 1), odd = tid / kClasses;
-      double sum = 0.0;
-      for (int s0 = odd; s0 < p.slices; s0 += 16) {
-        uint64_t v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int s = min(s0 + 2 * i, p.slices - 1);
-          v[i] = reinterpret_cast<const uint64_t*>(parts + s * p.part)[min(max(c - lds.shift[s], 0), kClasses - 1)];
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int s = s0 + 2 * i;
-          if (s < p.slices && c >= lds.shift[s] && lds.factor[s] != 0.0) sum += double(v[i]) * lds.factor[s];
-        }
-      }
-      if (odd) lds.class_sum[c] = sum;
-      __syncthreads();
-      if (!odd) lds.class_sum[c] += sum;
-    }
-    __syncthreads();
-    // the largest weight lies below the reference by up to an octave
-    const double t_top = octaves_below(top, ref, rules.scale);
-    const double t_min = rules.use_m ? t_top + log2(rules.min_p) : -1e300;
-    const double target = rules.top_p * total;
-    if (tid < kClasses && rules.use_p && lds.class_sum[tid] >= target) atomicMin(&lds.cut, tid);
-    __syncthreads();
-    const int p_cut = lds.cut;
-    const int cut = rules.use_m ? min(p_cut, class_of(t_min)) : p_cut;
-    if (cut < kClasses) {
-      const double above = cut > 0 ? lds.class_sum[cut - 1] : 0.0;
-      // the cut class's tokens: those between the logits that bound it (a little more, then exactly)
-      const double inv = 1.0 / rules.scale;
-      const double slack = 1e-9 * (1.0 + fabs(ref));  // the octaves' own rounding, far from the reference's whole part
-      double hi = (ref - cut / kPerOctave + slack) * inv, lo = (ref - (cut + 1) / kPerOctave - slack) * inv;
-      hi += 1e-6 * fabs(hi);
-      lo -= 1e-6 * fabs(lo);
-      const bool infinite = top == INFINITY;
-      const float x_hi = infinite ? INFINITY : float(hi), x_lo = infinite ? INFINITY : float(lo);
-      const int pieces = (src.skip + p.vocab + Row<T>::kVec - 1) / Row<T>::kVec;
-      constexpr int kAhead = 8;
-      for (int i0 = tid; i0 < pieces; i0 += kAhead * kRowThreads) {
-        u32x4 v[kAhead];
-#pragma unroll
-        for (int a = 0; a < kAhead; ++a) v[a] = src.raw(i0 + a * kRowThreads);
-#pragma unroll
-        for (int a = 0; a < kAhead; ++a)
-#pragma unroll
-          for (int e = 0; e < Row<T>::kVec; ++e) {
-            const float x = Row<T>::value(v[a], e);
-            if (!(x >= x_lo && x <= x_hi)) continue;
-            const uint32_t token = uint32_t((i0 + a * kRowThreads) * Row<T>::kVec + e - src.skip);
-            const double t = octaves_below(x, ref, rules.scale);
-            if (token >= uint32_t(p.vocab) || class_of(t) != cut) continue;
-            const int at = atomicAdd(&sh.n, 1);
-            if (at < kListMax) {
-              lds.list.keys[at] = ordered(x);
-              lds.list.tokens[at] = token;
-              lds.list.weights[at] = whole(exp2_within(t + kClassBits));
-            }
-          }
-      }
-      __syncthreads();
-      const int n = sh.n;
-      if (n <= kListMax) {
-        const ListSource list = {lds.list.keys, lds.list.tokens, lds.list.weights, n, p.vocab};
-        Cut at = {0, kTokenMask};
-        if (p_cut == cut) {
-          uint64_t here = 0;
-          for (int i = tid; i < n; i += kRowThreads) here += lds.list.weights[i];
-          here = block_sum(sh, here);
-          const double rest = target - above;
-          const uint64_t need = max(uint64_t(ceil(fmax(rest, 0.0))), uint64_t(1));
-          if (need < here) {
-            // few bits tell a class's values apart
-            uint32_t low = ~0u, high = 0;
-            for (int i = tid; i < n; i += kRowThreads) {
-              low = min(low, lds.list.keys[i]);
-              high = max(high, lds.list.keys[i]);
-            }
-            const uint64_t span = wave_max(uint64_t(~low)), up = wave_max(uint64_t(high));
-            if (lane == 0) {
-              lds.left[wave] = uint32_t(span);
-              lds.valid[wave] = uint32_t(up);
-            }
-            __syncthreads();
-            low = lds.left[0];
-            high = lds.valid[0];
-            for (int i = 1; i < kRowWaves; ++i) {
-              low = max(low, lds.left[i]);
-              high = max(high, lds.valid[i]);
-            }
-            low = ~low;
-            const int zeros = (low ^ high) >> 31 ? 0 : Row<T>::kZeros;
-            const int bits = 32 - int(__builtin_clz(((high - low) >> zeros) | 1));
-            at = cut_at(sh, list, at, need, [](auto&& w) { return w(); }, low, bits, zeros);
-          }
-        }
-        auto stays = [&](double t, uint32_t key, uint32_t token) {
-          const int c = class_of(t);
-          return c < cut || (c == cut && t >= t_min && at.keeps(key, token));
-        };
-        for (int i = tid; i < n; i += kRowThreads) {
-          const uint32_t key = lds.list.keys[i], token = lds.list.tokens[i];
-          if (stays(octaves_below(value_of(key), ref, rules.scale), key, token))
-            atomicAdd(&lds.extra[(token + src.skip) / slice_size], (unsigned long long)lds.list.weights[i]);
-        }
-        __syncthreads();
-        if (tid < p.slices) lds.slice[tid] = (cut > 0 ? upto(tid, cut - 1) : 0.0) + double(lds.extra[tid]);
-        __syncthreads();
-        double kept = 0.0;
-        for (int i = 0; i < p.slices; ++i) kept += lds.slice[i];
-        const double unit = ldexp(1.0, kClassBits);
-        const int token = draw_from_slices<PER>(lds, p, src, row, u * kept, [&](float x, int token) {
-          const double t = octaves_below(x, ref, rules.scale);
-          return stays(t, ordered(x), token) ? exp2_of(t) * unit : 0.0;
-        });
-        finish(token, kept / unit / exp2_of(t_top));
-        return;
-      }
-    }
-    total = total / ldexp(1.0, kClassBits) / exp2_of(t_top);
   }
-  const int bits = 62 - kTokenBits;
+  // the row's classes: the slices' counted from the row's reference
+  const double ref = octave_of(top, rules.scale);
+  if (tid < p.slices) {
+    const double down = head.best ? fmin(ref - head.ref, 4096.0) : 4096.0;
+    lds.shift[tid] = int(down) * int(kPerOctave);
+    lds.factor[tid] = head.best ? exp2_of(-down) : 0.0;
+    lds.slice[tid] = head.best ? head.sum * lds.factor[tid] : 0.0;
+    lds.extra[tid] = 0;
+  }
+  if (tid == 0) {
+    lds.cut = kClasses;
+    sh.cut_key = 0;  // all of the class stays where its sum falls short
+    sh.cut_token = kTokenMask;
+  }
+  __syncthreads();
+  for (int i = 0; i < p.slices; ++i) total += lds.slice[i];
+  auto upto = [&](int s, int c) -> double {  // slice s's weights in classes 0 .. c, in units of 2^-kClassBits
+    const int at = min(c - lds.shift[s], kClasses - 1);
+    if (at < 0 || lds.factor[s] == 0.0) return 0.0;
+    return double(reinterpret_cast<const uint64_t*>(parts + s * p.part)[at]) * lds.factor[s];
+  };
+  {
+    // the even and the odd slices, by the two halves of the workgroup, eight loads on their way
+    const int c = tid & (kClasses - 1), odd = tid / kClasses;
+    double sum = 0.0;
+    for (int s0 = odd; s0 < p.slices; s0 += 16) {
+      uint64_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int s = min(s0 + 2 * i, p.slices - 1);
+        v[i] = reinterpret_cast<const uint64_t*>(parts + s * p.part)[min(max(c - lds.shift[s], 0), kClasses - 1)];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int s = s0 + 2 * i;
+        if (s < p.slices && c >= lds.shift[s] && lds.factor[s] != 0.0) sum += double(v[i]) * lds.factor[s];
+      }
+    }
+    if (odd) lds.class_sum[c] = sum;
+    __syncthreads();
+    if (!odd) lds.class_sum[c] += sum;
+  }
+  __syncthreads();
+  // the largest weight lies below the reference by up to an octave
+  const double t_top = octaves_below(top, ref, rules.scale);
+  const double t_min = rules.use_m ? t_top + log2(rules.min_p) : -1e300;
+  const double target = rules.top_p * total;
+  if (tid < kClasses && rules.use_p && lds.class_sum[tid] >= target) atomicMin(&lds.cut, tid);
+  __syncthreads();
+  const int p_cut = lds.cut;
+  const int cut = rules.use_m ? min(p_cut, class_of(t_min)) : p_cut;
+  if (cut < kClasses) {
+    const double above = cut > 0 ? lds.class_sum[cut - 1] : 0.0;
+    // the cut class's tokens: those between the logits that bound it (a little more, then exactly)
+    const double inv = 1.0 / rules.scale;
+    const double slack = 1e-9 * (1.0 + fabs(ref));  // the octaves' own rounding, far from the reference's whole part
+    double hi = (ref - cut / kPerOctave + slack) * inv, lo = (ref - (cut + 1) / kPerOctave - slack) * inv;
+    hi += 1e-6 * fabs(hi);
+    lo -= 1e-6 * fabs(lo);
+    const bool infinite = top == INFINITY;
+    const float x_hi = infinite ? INFINITY : float(hi), x_lo = infinite ? INFINITY : float(lo);
+    const int pieces = (src.skip + p.vocab + Row<T>::kVec - 1) / Row<T>::kVec;
+    constexpr int kAhead = 6, V = Row<T>::kVec;
+    for (int i0 = tid; i0 < pieces; i0 += kAhead * kRowThreads) {
+      u32x4 v[kAhead];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) v[a] = src.raw(i0 + a * kRowThreads);
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        float x[V], most = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          x[e] = Row<T>::value(v[a], e);
+          most = fmaxf(most, x[e]);
+        }
+        if (!(most >= x_lo)) continue;  // most pieces hold nothing so large
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          if (!(x[e] >= x_lo && x[e] <= x_hi)) continue;
+          const uint32_t token = uint32_t((i0 + a * kRowThreads) * V + e - src.skip);
+          const double t = octaves_below(x[e], ref, rules.scale);
+          if (token >= uint32_t(p.vocab) || class_of(t) != cut) continue;
+          const int at = atomicAdd(&sh.n, 1);
+          if (at < kListMax) {
+            lds.list.keys[at] = ordered(x[e]);
+            lds.list.tokens[at] = token;
+            lds.list.weights[at] = whole(exp2_within(t + kClassBits));
+          }
+        }
+      }
+    }
+    __syncthreads();
+    const int n = sh.n;
+    if (n <= kListMax) {
+      Cut at = {0, kTokenMask};
+      if (p_cut == cut && n <= kRowThreads) {
+        // sorted: the place where the running sum gets there
+        const double rest = target - above;
+        const uint64_t need = max(uint64_t(ceil(fmax(rest, 0.0))), uint64_t(1));
+        uint64_t key = tid < n ? uint64_t(lds.list.keys[tid]) << 32 | uint64_t(kTokenMask - lds.list.tokens[tid]) << 10 | uint32_t(tid) : 0;
+        int size = 64;
+        while (size < n) size <<= 1;
+        key = sort_down(sh.hist, key, size);
+        const uint64_t mine = tid < n ? lds.list.weights[uint32_t(key) & (kRowThreads - 1)] : 0;
+        uint64_t run = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const uint64_t up = __shfl_up((unsigned long long)run, o);
+          if (lane >= o) run += up;
+        }
+        if (lane == 63) sh.wave[wave] = run;
+        __syncthreads();
+        for (int i = 0; i < wave; ++i) run += sh.wave[i];
+        if (tid < n && run >= need && run - mine < need) {
+          sh.cut_key = uint32_t(key >> 32);
+          sh.cut_token = kTokenMask - (uint32_t(key) >> 10 & kTokenMask);
+        }
+        __syncthreads();
+        at = {sh.cut_key, sh.cut_token};
+      } else if (p_cut == cut) {
+        Search st = {{0, kTokenMask}, 0, 0.0, 0.0, 1, 0.0, max(uint64_t(ceil(fmax(target - above, 0.0))), uint64_t(1)), 0, 0};
+        search(sh, ListSource{lds.list.keys, lds.list.tokens, lds.list.weights, n, p.vocab, top, ref, rules.scale, 0.0}, st,
+               kByShare, kShareTies);
+        at = st.cut;
+      }
+      auto stays = [&](double t, uint32_t key, uint32_t token) {
+        const int c = class_of(t);
+        return c < cut || (c == cut && t >= t_min && at.keeps(key, token));
+      };
+      for (int i = tid; i < n; i += kRowThreads) {
+        const uint32_t key = lds.list.keys[i], token = lds.list.tokens[i];
+        if (stays(octaves_below(value_of(key), ref, rules.scale), key, token))
+          atomicAdd(&lds.extra[(token + src.skip) / slice_size], (unsigned long long)lds.list.weights[i]);
+      }
+      __syncthreads();
+      if (tid < p.slices) lds.slice[tid] = (cut > 0 ? upto(tid, cut - 1) : 0.0) + double(lds.extra[tid]);
+      __syncthreads();
+      double kept = 0.0;
+      for (int i = 0; i < p.slices; ++i) kept += lds.slice[i];
+      const double unit = ldexp(1.0, kClassBits);
+      const int token = draw_from_slices<PER>(lds, p, src, row, u * kept, [&](float x, int token) {
+        const double t = octaves_below(x, ref, rules.scale);
+        return stays(t, ordered(x), token) ? exp2_of(t) * unit : 0.0;
+      });
+      finish(token, kept / unit / exp2_of(t_top));
+      return;
+    }
+  }
+  total = total / ldexp(1.0, kClassBits) / exp2_of(t_top);
+  const double unit = ldexp(1.0, 62 - kTokenBits);
   const int pieces = (src.skip + p.vocab + Row<T>::kVec - 1) / Row<T>::kVec;
-  const Drawn got = choose(sh, RowSource<T>{src, top, rules.scale, ldexp(1.0, bits), pieces, p.vocab}, rules, total, valid, u, bits);
-  finish(got.token, got.total);
+  Search st = whole_search(rules, u, unit, total * unit, valid);
+  search(sh, RowSource<T>{src, top, rules.scale, unit, pieces, p.vocab}, st, kByCount, kDraw);
+  finish(int(st.token), double(st.total) / unit);
 }
 
 // ---- the host side ----
@@ -1150,36 +1207,45 @@ struct Split {
   int slices, cap;
   int64_t part;  // bytes of a slice's list or classes
 };
-// Slices of 4096 tokens.
-Split split_of(int64_t rows, int vocab, int dtype) {
+// Slices of 4096 tokens, of 8192 for many plain rows: 256 of 131072 .. us in 8192, .. in 4096.
+Split split_of(int64_t rows, int vocab, bool plain) {
   Split s;
-  s.elements = vocab > 4096 * 256 - 16 ? 0 : 16;
+  s.elements = plain && rows * vocab > int64_t(8192) * 1024 ? 32 : 16;
   const int size = kSliceThreads * s.elements;
-  s.slices = s.elements ? (vocab + 7 + size - 1) / size : 0;
-  s.cap = s.slices ? std::min(512, kListMax / s.slices) : 0;
+  s.slices = (vocab + 7 + size - 1) / size;
+  s.cap = std::min(512, kListMax / s.slices);
   s.part = (std::max<int64_t>(s.cap * sizeof(uint2), kClasses * sizeof(uint64_t)) + 15) / 16 * 16;
   return s;
 }
 
+// Which rows there are: plain ones alone, with top-k, any others.
+struct Kinds {
+  bool plain, lists, others;
+};
 template <class T>
-void launch(const SampleParams& p, bool plain, int rows, hipStream_t stream) {
-  constexpr int E = 16, PER = E * kSliceThreads / kRowThreads;
-  if (plain) {
-    sample_slice_kernel<T, E, true><<<dim3(p.slices, rows), kSliceThreads, 0, stream>>>(p);
-    sample_plain_row_kernel<T, PER><<<rows, kRowThreads, 0, stream>>>(p);
+void launch(const SampleParams& p, const Split& s, const Kinds& k, int rows, hipStream_t stream) {
+  constexpr int PER = 16 * kSliceThreads / kRowThreads;
+  const dim3 slices(p.slices, rows);
+  if (s.elements == 32) {
+    sample_slice_kernel<T, 32, true><<<slices, kSliceThreads, 0, stream>>>(p);
+    sample_plain_kernel<T, 2 * PER><<<rows, kRowThreads, 0, stream>>>(p);
+  } else if (k.plain) {
+    sample_slice_kernel<T, 16, true><<<slices, kSliceThreads, 0, stream>>>(p);
+    sample_plain_kernel<T, PER><<<rows, kRowThreads, 0, stream>>>(p);
   } else {
-    sample_slice_kernel<T, E, false><<<dim3(p.slices, rows), kSliceThreads, 0, stream>>>(p);
-    sample_row_kernel<T, PER><<<rows, kRowThreads, 0, stream>>>(p);
+    sample_slice_kernel<T, 16, false><<<slices, kSliceThreads, 0, stream>>>(p);
+    if (k.lists) sample_lists_kernel<T><<<rows, kRowThreads, 0, stream>>>(p);
+    if (k.others) sample_classes_kernel<T, PER><<<rows, kRowThreads, 0, stream>>>(p);
   }
 }
 
 }  // namespace
 }  // namespace pkv
 
-extern "C" size_t pkv_sample_workspace_bytes(int32_t rows, int32_t vocab, int32_t dtype) {
+extern "C" size_t pkv_sample_workspace_bytes(int32_t rows, int32_t vocab) {
   using namespace pkv;
-  if (rows <= 0 || vocab <= 0) return 0;
-  const Split s = split_of(rows, vocab, dtype);
+  if (rows <= 0 || vocab <= 0 || vocab > 1000000) return 0;
+  const Split s = split_of(rows, vocab, false);
   return size_t(rows) * s.slices * (sizeof(SliceHead) + s.part);
 }
 
@@ -1204,11 +1270,16 @@ extern "C" int pkv_sample(const void* logits, int64_t stride, int32_t dtype, con
        reinterpret_cast<uintptr_t>(top_ps) | reinterpret_cast<uintptr_t>(min_ps) | reinterpret_cast<uintptr_t>(logprobs)) & 3u)
     return fail(PKV_EINVAL, "%s: an array of 4-byte values is not aligned to them", fn);
   if (reinterpret_cast<uintptr_t>(tokens) & 7u) return fail(PKV_EINVAL, "%s: tokens not 8-byte aligned", fn);
-  const size_t need = pkv_sample_workspace_bytes(rows, vocab, dtype);
+  const size_t need = pkv_sample_workspace_bytes(rows, vocab);
   if (!workspace || !aligned16(workspace)) return fail(PKV_EINVAL, "%s: workspace null or not 16-byte aligned", fn);
   if (workspace_bytes < need)
     return fail(PKV_ENOSPC, "%s: workspace %zu bytes < %zu needed", fn, workspace_bytes, need);
-  const Split s = split_of(rows, vocab, dtype);
+  const bool warm = !temperatures && temperature > 0.f, no_k = !top_ks && (top_k <= 0 || top_k >= vocab);
+  Kinds kinds;
+  kinds.plain = warm && no_k && !top_ps && !(top_p < 1.f) && !min_ps && !(min_p > 0.f);
+  kinds.lists = !no_k;
+  kinds.others = no_k || top_ks || !warm || top_ps || top_p <= 0.f || top_k == 1;  // greedy rows among them
+  const Split s = split_of(rows, vocab, kinds.plain);
   SampleParams p;
   p.logits = logits;
   p.uniforms = uniforms;
@@ -1226,13 +1297,11 @@ extern "C" int pkv_sample(const void* logits, int64_t stride, int32_t dtype, con
   p.cap = s.cap;
   p.part = s.part;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const bool plain = !temperatures && temperature > 0.f && !top_ks && (top_k <= 0 || top_k >= vocab) && !top_ps &&
-                     !(top_p < 1.f) && !min_ps && !(min_p > 0.f);
   if (dtype == PKV_BF16)
-    launch<__bf16>(p, plain, rows, st);
+    launch<__bf16>(p, s, kinds, rows, st);
   else if (dtype == PKV_FP16)
-    launch<_Float16>(p, plain, rows, st);
+    launch<_Float16>(p, s, kinds, rows, st);
   else
-    launch<float>(p, plain, rows, st);
+    launch<float>(p, s, kinds, rows, st);
   return check_launch(fn);
 }

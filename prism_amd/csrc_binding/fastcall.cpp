@@ -471,7 +471,7 @@ PyObject* sample_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (logs) lp = at::empty({rows}, at::TensorOptions().dtype(at::kFloat).device(dev));
     if (rows > 0) {
       // of this call alone, from torch's allocator: of the current stream, or of the graph it captures
-      const size_t bytes = lib_pkv_sample_workspace_bytes(int32_t(rows), int32_t(vocab), code);
+      const size_t bytes = lib_pkv_sample_workspace_bytes(int32_t(rows), int32_t(vocab));
       at::Tensor ws = at::empty({int64_t(bytes)}, at::TensorOptions().dtype(at::kByte).device(dev));
       check(lib_pkv_sample(x.data_ptr(), rows > 1 ? x.stride(0) : vocab, code, u.data_ptr<float>(),
                            static_cast<const float*>(t.rows), float(t.all), static_cast<const int32_t*>(k.rows),

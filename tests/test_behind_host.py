@@ -206,8 +206,8 @@ def _sample_call(lib, **over):
 def test_sample_argument_errors():
     lib = _lib.load()
     assert _sample_call(lib) == 0
-    need = lib.pkv_sample_workspace_bytes(2, 100, _lib.PKV_FP32)
-    assert need > 0 and lib.pkv_sample_workspace_bytes(0, 100, 0) == 0
+    need = lib.pkv_sample_workspace_bytes(2, 100)
+    assert need > 0 and lib.pkv_sample_workspace_bytes(0, 100) == 0
     two = dict(rows=2, ws=A16, ws_bytes=need)
     for over, msg in [(dict(rows=-1), "vocabulary"), (dict(vocab=0), "vocabulary"), (dict(vocab=1000001), "vocabulary"),
                       (dict(rows=65536), "grid"), (dict(dtype=3), "dtype"), (dict(two, x=0), "null"), (dict(two, u=0), "null"),
