@@ -726,6 +726,13 @@ __device__ __forceinline__ float log_share(float x, float top, const Rules& r, d
   return float((x == top ? 0.0 : (double(x) - double(top)) * r.scale * 0.69314718055994531) - log(total));
 }
 
+// The slices' weights together: every lane and wave adds in the same tree, and gets the same bits.
+__device__ __forceinline__ double slices_sum(const double* slice, int n) {
+  double x = 0.0;
+  for (int s = threadIdx.x & 63; s < n; s += 64) x += slice[s];
+  return wave_sum(x);
+}
+
 // The draw among `weights of the slices` (lds.slice, summing to total in that order): the slice, then the token in it;
 // weight(x, token) is 0 for what does not stay.  -> the token.
 template <int PER, class T, class Lds, class Weight>
@@ -831,7 +838,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_plain_kernel(const SampleP
     lds.slice[tid] = head.best ? head.sum * weight_of(value_of(uint32_t(head.best >> 32)), top, rules.scale) : 0.0;
   __syncthreads();
   double total = 0.0;
-  for (int i = 0; i < p.slices; ++i) total += lds.slice[i];  // in order, by every thread alike
+  total = slices_sum(lds.slice, p.slices);
   const int token = draw_from_slices<PER>(lds, p, src, row, u * total,
                                           [&](float x, int) { return weight_of(x, top, rules.scale); });
   if (tid == 0) {
@@ -842,12 +849,9 @@ __global__ __launch_bounds__(kRowThreads) void sample_plain_kernel(const SampleP
 
 // Rows with top-k.
 template <class T>
-__global__ __launch_bounds__(kRowThreads) void sample_lists_kernel(const SampleParams p) {
-  __shared__ RowLds lds;
+__device__ __forceinline__ void lists_row(const SampleParams& p, const Rules& rules, int row, RowLds& lds) {
   RowShared& sh = lds.sh;
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const Rules rules = rules_of(p, row);
-  if (!rules.lists()) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Row<T> src(p, row);
   SliceHead head = {};
   if (tid < p.slices) head = p.heads[int64_t(row) * p.slices + tid];
@@ -905,8 +909,48 @@ __global__ __launch_bounds__(kRowThreads) void sample_lists_kernel(const SampleP
     }
   }
   __syncthreads();
-  const int n = min(sh.n, kListMax);
-  if (n <= kRowThreads && (left == 0 || n >= rules.top_k)) {
+  int n = min(sh.n, kListMax);
+  const bool enough = left == 0 || n >= rules.top_k;
+  if (n > kRowThreads && enough && rules.top_k < kRowThreads) {
+    // first down to those in the classes of distance that the first top_k reach
+    int* const hist = reinterpret_cast<int*>(sh.hist);
+    hist[tid] = 0;
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+    uint32_t keys[kListMax / kRowThreads], tokens[kListMax / kRowThreads];
+    int bins[kListMax / kRowThreads];
+#pragma unroll
+    for (int j = 0; j < kListMax / kRowThreads; ++j) {
+      const int i = tid + j * kRowThreads;
+      bins[j] = 1024;
+      if (i >= n) continue;
+      keys[j] = lds.list.keys[i];
+      tokens[j] = lds.list.tokens[i];
+      bins[j] = distance_bin(value_of(keys[j]), top);
+      atomicAdd(&hist[bins[j]], 1);
+    }
+    __syncthreads();
+    int run = hist[tid];
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(run, o);
+      if (lane >= o) run += up;
+    }
+    if (lane == 63) lds.left[wave] = uint32_t(run);
+    __syncthreads();
+    for (int i = 0; i < wave; ++i) run += int(lds.left[i]);
+    const int last = __syncthreads_count(run < rules.top_k);  // the class that the first top_k end in
+#pragma unroll
+    for (int j = 0; j < kListMax / kRowThreads; ++j)
+      if (bins[j] <= last && bins[j] < 1024) {
+        const int at = atomicAdd(&sh.n, 1);
+        lds.list.keys[at] = keys[j];
+        lds.list.tokens[at] = tokens[j];
+      }
+    __syncthreads();
+    n = sh.n;
+  }
+  if (n <= kRowThreads && enough) {
     // sorted, a token a thread: top-k is the first so many, top-p and min-p a prefix of them
     uint64_t key = tid < n ? uint64_t(lds.list.keys[tid]) << 32 | uint32_t(~lds.list.tokens[tid]) : 0;
     __syncthreads();
@@ -968,7 +1012,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_lists_kernel(const SampleP
     finish(sh.slice, all);
     return;
   }
-  if (left == 0 || n >= rules.top_k) {
+  if (enough) {
     constexpr int kListBits = 49;
     const double unit = ldexp(1.0, kListBits);
     for (int i = tid; i < n; i += kRowThreads)
@@ -988,13 +1032,10 @@ __global__ __launch_bounds__(kRowThreads) void sample_lists_kernel(const SampleP
 
 // Every other row, where some have rules.
 template <class T, int PER>
-__global__ __launch_bounds__(kRowThreads) void sample_classes_kernel(const SampleParams p) {
+__device__ __forceinline__ void classes_row(const SampleParams& p, const Rules& rules, int row, RowLds& lds) {
   constexpr int slice_size = PER * kRowThreads;
-  __shared__ RowLds lds;
   RowShared& sh = lds.sh;
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const Rules rules = rules_of(p, row);
-  if (rules.lists()) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Row<T> src(p, row);
   SliceHead head = {};
   if (tid < p.slices) head = p.heads[int64_t(row) * p.slices + tid];
@@ -1039,7 +1080,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_classes_kernel(const Sampl
     if (tid < p.slices)
       lds.slice[tid] = head.best ? head.sum * weight_of(value_of(uint32_t(head.best >> 32)), top, rules.scale) : 0.0;
     __syncthreads();
-    for (int i = 0; i < p.slices; ++i) total += lds.slice[i];  // in order, by every thread alike
+    total = slices_sum(lds.slice, p.slices);
     const int token = draw_from_slices<PER>(lds, p, src, row, u * total,
                                             [&](float x, int) { return weight_of(x, top, rules.scale); });
     finish(token, total);
@@ -1060,7 +1101,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_classes_kernel(const Sampl
     sh.cut_token = kTokenMask;
   }
   __syncthreads();
-  for (int i = 0; i < p.slices; ++i) total += lds.slice[i];
+  total = slices_sum(lds.slice, p.slices);
   auto upto = [&](int s, int c) -> double {  // slice s's weights in classes 0 .. c, in units of 2^-kClassBits
     const int at = min(c - lds.shift[s], kClasses - 1);
     if (at < 0 || lds.factor[s] == 0.0) return 0.0;
@@ -1120,18 +1161,14 @@ __global__ __launch_bounds__(kRowThreads) void sample_classes_kernel(const Sampl
           x[e] = Row<T>::value(v[a], e);
           most = fmaxf(most, x[e]);
         }
-        if (!(most >= x_lo)) continue;  // most pieces hold nothing so large
+        if (!(most >= x_lo) || i0 + a * kRowThreads >= pieces) continue;  // most pieces hold nothing so large
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           if (!(x[e] >= x_lo && x[e] <= x_hi)) continue;
-          const uint32_t token = uint32_t((i0 + a * kRowThreads) * V + e - src.skip);
-          const double t = octaves_below(x[e], ref, rules.scale);
-          if (token >= uint32_t(p.vocab) || class_of(t) != cut) continue;
           const int at = atomicAdd(&sh.n, 1);
           if (at < kListMax) {
-            lds.list.keys[at] = ordered(x[e]);
-            lds.list.tokens[at] = token;
-            lds.list.weights[at] = whole(exp2_within(t + kClassBits));
+            lds.list.keys[at] = __float_as_uint(x[e]);
+            lds.list.tokens[at] = uint32_t((i0 + a * kRowThreads) * V + e - src.skip);
           }
         }
       }
@@ -1139,6 +1176,16 @@ __global__ __launch_bounds__(kRowThreads) void sample_classes_kernel(const Sampl
     __syncthreads();
     const int n = sh.n;
     if (n <= kListMax) {
+      // now exactly: what is not of the class weighs nothing
+      for (int i = tid; i < n; i += kRowThreads) {
+        const float x = __uint_as_float(lds.list.keys[i]);
+        const double t = octaves_below(x, ref, rules.scale);
+        const bool in = lds.list.tokens[i] < uint32_t(p.vocab) && class_of(t) == cut;
+        lds.list.keys[i] = in ? ordered(x) : 0;
+        lds.list.weights[i] = in ? whole(exp2_within(t + kClassBits)) : 0;
+        if (!in) lds.list.tokens[i] = 0;
+      }
+      __syncthreads();
       Cut at = {0, kTokenMask};
       if (p_cut == cut && n <= kRowThreads) {
         // sorted: the place where the running sum gets there
@@ -1182,8 +1229,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_classes_kernel(const Sampl
       __syncthreads();
       if (tid < p.slices) lds.slice[tid] = (cut > 0 ? upto(tid, cut - 1) : 0.0) + double(lds.extra[tid]);
       __syncthreads();
-      double kept = 0.0;
-      for (int i = 0; i < p.slices; ++i) kept += lds.slice[i];
+      const double kept = slices_sum(lds.slice, p.slices);
       const double unit = ldexp(1.0, kClassBits);
       const int token = draw_from_slices<PER>(lds, p, src, row, u * kept, [&](float x, int token) {
         const double t = octaves_below(x, ref, rules.scale);
@@ -1201,17 +1247,29 @@ __global__ __launch_bounds__(kRowThreads) void sample_classes_kernel(const Sampl
   finish(int(st.token), double(st.total) / unit);
 }
 
+// The rows with top-k, or the others; where a call has both, each kernel leaves the other's.
+enum { kListRows, kOtherRows };
+template <class T, int PER, int ROWS>
+__global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleParams p) {
+  __shared__ RowLds lds;
+  const int row = blockIdx.x;
+  const Rules rules = rules_of(p, row);
+  if (rules.lists() != (ROWS == kListRows)) return;
+  if constexpr (ROWS == kListRows)
+    lists_row<T>(p, rules, row, lds);
+  else
+    classes_row<T, PER>(p, rules, row, lds);
+}
+
 // ---- the host side ----
 struct Split {
-  int elements;  // of a slice, a thread
   int slices, cap;
   int64_t part;  // bytes of a slice's list or classes
 };
-// Slices of 4096 tokens, of 8192 for many plain rows: 256 of 131072 .. us in 8192, .. in 4096.
-Split split_of(int64_t rows, int vocab, bool plain) {
+constexpr int kSlice = 16 * kSliceThreads;  // 256 plain rows of 131072 take 59 us in slices of 4096, 62 in 8192
+Split split_of(int vocab) {
   Split s;
-  s.elements = plain && rows * vocab > int64_t(8192) * 1024 ? 32 : 16;
-  const int size = kSliceThreads * s.elements;
+  const int size = kSlice;
   s.slices = (vocab + 7 + size - 1) / size;
   s.cap = std::min(512, kListMax / s.slices);
   s.part = (std::max<int64_t>(s.cap * sizeof(uint2), kClasses * sizeof(uint64_t)) + 15) / 16 * 16;
@@ -1223,19 +1281,17 @@ struct Kinds {
   bool plain, lists, others;
 };
 template <class T>
-void launch(const SampleParams& p, const Split& s, const Kinds& k, int rows, hipStream_t stream) {
-  constexpr int PER = 16 * kSliceThreads / kRowThreads;
+void launch(const SampleParams& p, const Kinds& k, int rows, hipStream_t stream) {
+  constexpr int PER = kSlice / kRowThreads;
   const dim3 slices(p.slices, rows);
-  if (s.elements == 32) {
-    sample_slice_kernel<T, 32, true><<<slices, kSliceThreads, 0, stream>>>(p);
-    sample_plain_kernel<T, 2 * PER><<<rows, kRowThreads, 0, stream>>>(p);
-  } else if (k.plain) {
+  if (k.plain) {
     sample_slice_kernel<T, 16, true><<<slices, kSliceThreads, 0, stream>>>(p);
     sample_plain_kernel<T, PER><<<rows, kRowThreads, 0, stream>>>(p);
   } else {
     sample_slice_kernel<T, 16, false><<<slices, kSliceThreads, 0, stream>>>(p);
-    if (k.lists) sample_lists_kernel<T><<<rows, kRowThreads, 0, stream>>>(p);
-    if (k.others) sample_classes_kernel<T, PER><<<rows, kRowThreads, 0, stream>>>(p);
+    // two kernels, not one with both: that one would have to spill
+    if (k.lists) sample_row_kernel<T, PER, kListRows><<<rows, kRowThreads, 0, stream>>>(p);
+    if (k.others) sample_row_kernel<T, PER, kOtherRows><<<rows, kRowThreads, 0, stream>>>(p);
   }
 }
 
@@ -1245,7 +1301,7 @@ void launch(const SampleParams& p, const Split& s, const Kinds& k, int rows, hip
 extern "C" size_t pkv_sample_workspace_bytes(int32_t rows, int32_t vocab) {
   using namespace pkv;
   if (rows <= 0 || vocab <= 0 || vocab > 1000000) return 0;
-  const Split s = split_of(rows, vocab, false);
+  const Split s = split_of(vocab);
   return size_t(rows) * s.slices * (sizeof(SliceHead) + s.part);
 }
 
@@ -1279,7 +1335,7 @@ extern "C" int pkv_sample(const void* logits, int64_t stride, int32_t dtype, con
   kinds.plain = warm && no_k && !top_ps && !(top_p < 1.f) && !min_ps && !(min_p > 0.f);
   kinds.lists = !no_k;
   kinds.others = no_k || top_ks || !warm || top_ps || top_p <= 0.f || top_k == 1;  // greedy rows among them
-  const Split s = split_of(rows, vocab, kinds.plain);
+  const Split s = split_of(vocab);
   SampleParams p;
   p.logits = logits;
   p.uniforms = uniforms;
@@ -1298,10 +1354,10 @@ extern "C" int pkv_sample(const void* logits, int64_t stride, int32_t dtype, con
   p.part = s.part;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == PKV_BF16)
-    launch<__bf16>(p, s, kinds, rows, st);
+    launch<__bf16>(p, kinds, rows, st);
   else if (dtype == PKV_FP16)
-    launch<_Float16>(p, s, kinds, rows, st);
+    launch<_Float16>(p, kinds, rows, st);
   else
-    launch<float>(p, s, kinds, rows, st);
+    launch<float>(p, kinds, rows, st);
   return check_launch(fn);
 }
