@@ -37,7 +37,8 @@ constexpr double kPerOctave = 16.0;
 constexpr int kClassBits = 50;   // the classes' sums are in units of 2^-50 of the slice's reference
 
 struct SliceHead {
-  uint64_t best;   // (ordered value, ~token) of the largest, 0: no token of the slice can be drawn
+  uint64_t best;   // (ordered value, ~token) of the largest, 0: no token of the slice can be drawn.  The token for
+                   // greedy rows alone
   double sum;      // no rule: of the weights, relative to the slice's own maximum.  Classes: of all, in their units
   double ref;      // classes: the octave that they count from
   uint32_t count;  // listed tokens
@@ -50,6 +51,7 @@ struct Setting {
   const void* rows;  // one value a row, or NULL: `all`
   double all;
 };
+constexpr double kLog2e = 1.4426950408889634;
 
 struct SampleParams {
   const void* logits;
@@ -59,6 +61,7 @@ struct SampleParams {
   SliceHead* heads;
   void* lists;  // a slice's part: `cap` tokens as (ordered value, token), or kClasses running sums
   Setting temperature, top_k, top_p, min_p;
+  double scale;  // log2 e / T, where T is one number
   int64_t stride;
   int vocab, slices, cap;
   int64_t part;  // bytes of a slice's part
@@ -81,7 +84,7 @@ __device__ __forceinline__ Rules rules_of(const SampleParams& p, int row) {
   Rules r;
   const double t = setting(p.temperature, row);
   r.greedy = !(t > 0.0);
-  r.scale = 1.4426950408889634 / t;
+  r.scale = p.temperature.rows ? kLog2e / t : p.scale;
   const int k = p.top_k.rows ? static_cast<const int32_t*>(p.top_k.rows)[row] : int(p.top_k.all);
   r.top_k = k > 0 && k < p.vocab ? k : 0;
   if (r.top_k == 1) r.greedy = true;
@@ -183,7 +186,11 @@ struct Row {
     };
     return to_float(__builtin_bit_cast(Values, v).v[e]);
   }
-  // piece i's values, -inf outside the row
+  // whether pieces [i, i + n) lie in the row with all they hold
+  __device__ __forceinline__ bool inside(int i, int n) const {
+    return i * kVec >= skip && (i + n) * kVec - skip <= vocab;
+  }
+  // piece i's values, -inf outside the row and for NaN
   __device__ __forceinline__ void get(int i, float (&x)[kVec]) const {
     const int first = i * kVec - skip;
     if (first >= vocab || first + kVec <= 0) {
@@ -203,15 +210,58 @@ struct Row {
   }
 };
 
+// Lane l's partner l ^ MASK, without a way through LDS.
+template <int CTRL>
+__device__ __forceinline__ uint32_t moved(uint32_t x) {
+  return uint32_t(__builtin_amdgcn_update_dpp(0, int(x), CTRL, 0xf, 0xf, true));
+}
+template <int MASK>
+__device__ __forceinline__ uint32_t across(uint32_t x) {
+  if constexpr (MASK == 1) return moved<0xb1>(x);            // quad 1 0 3 2
+  if constexpr (MASK == 2) return moved<0x4e>(x);            // quad 2 3 0 1
+  if constexpr (MASK == 4) return moved<0x141>(moved<0x1b>(x));  // within eight: 7 - l of quad 3 2 1 0
+  if constexpr (MASK == 8) return moved<0x128>(x);           // a row of 16 turned by 8
+  if constexpr (MASK == 16) {
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return __lane_id() & 16 ? a[0] : a[1];
+  }
+  if constexpr (MASK == 32) {
+    const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return __lane_id() & 32 ? a[0] : a[1];
+  }
+}
+template <int MASK>
+__device__ __forceinline__ uint64_t across(uint64_t x) {
+  return uint64_t(across<MASK>(uint32_t(x >> 32))) << 32 | across<MASK>(uint32_t(x));
+}
+template <int MASK>
+__device__ __forceinline__ float across(float x) {
+  return __uint_as_float(across<MASK>(__float_as_uint(x)));
+}
+__device__ __forceinline__ float wave_top(float x) {
+  x = fmaxf(x, across<1>(x));
+  x = fmaxf(x, across<2>(x));
+  x = fmaxf(x, across<4>(x));
+  x = fmaxf(x, across<8>(x));
+  x = fmaxf(x, across<16>(x));
+  return fmaxf(x, across<32>(x));
+}
+template <int MASK>
+__device__ __forceinline__ double across(double x) {
+  return __longlong_as_double(int64_t(across<MASK>(uint64_t(__double_as_longlong(x)))));
+}
 __device__ __forceinline__ uint64_t wave_max(uint64_t x) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) x = max(x, uint64_t(__shfl_xor((unsigned long long)x, o)));
   return x;
 }
 __device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-  return x;
+  x += across<32>(x);
+  x += across<16>(x);
+  x += across<8>(x);
+  x += across<4>(x);
+  x += across<2>(x);
+  return x + across<1>(x);
 }
 
 // ---- a slice of a row ----
@@ -226,8 +276,9 @@ __device__ __forceinline__ int distance_bin(float x, float top) {
 template <class T, int E, bool PLAIN>
 __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const SampleParams p) {
   constexpr int V = Row<T>::kVec, L = E / V, W = kSliceThreads / 64;
-  __shared__ uint64_t best_lds[W], classes[PLAIN ? 1 : kClasses], total_lds[W];
+  __shared__ uint64_t low_lds[W], classes[PLAIN ? 1 : kClasses], total_lds[W];
   __shared__ double sum_lds[W];
+  __shared__ float top_lds[W];
   __shared__ int hist[PLAIN ? 1 : 1024];
   __shared__ int count_lds[W], taken, bins_lds[2];
   __shared__ uint32_t left_lds[W];
@@ -235,37 +286,56 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
   const Row<T> src(p, row);
   float x[L][V];
   const int piece0 = slice * (kSliceThreads * L);
+  if (src.inside(piece0, kSliceThreads * L)) {
+    u32x4 raw[L];
 #pragma unroll
-  for (int l = 0; l < L; ++l) src.get(piece0 + l * kSliceThreads + tid, x[l]);
+    for (int l = 0; l < L; ++l) raw[l] = src.pieces[piece0 + l * kSliceThreads + tid];
+#pragma unroll
+    for (int l = 0; l < L; ++l)
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[l][e] = fmaxf(Row<T>::value(raw[l], e), -INFINITY);  // NaN to -inf
+  } else {
+#pragma unroll
+    for (int l = 0; l < L; ++l) src.get(piece0 + l * kSliceThreads + tid, x[l]);
+  }
   const Rules rules = rules_of(p, row);
   auto token = [&](int l, int e) { return (piece0 + l * kSliceThreads + tid) * V + e - src.skip; };
-  uint64_t best = 0;
+  float top = -INFINITY;
 #pragma unroll
   for (int l = 0; l < L; ++l)
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const uint32_t key = ordered(x[l][e]);
-      if (key > uint32_t(best >> 32)) best = uint64_t(key) << 32 | uint32_t(~token(l, e));
-    }
-  // of equal values the lowest token: a thread meets its own in ascending order, other threads' are compared by ~token
-  best = wave_max(best);
-  if (lane == 0) best_lds[wave] = best;
+    for (int e = 0; e < V; ++e) top = fmaxf(top, x[l][e]);
+  top = wave_top(top);
+  if (lane == 0) top_lds[wave] = top;
   if constexpr (!PLAIN) {
     if (rules.lists())
       for (int i = tid; i < 1024; i += kSliceThreads) hist[i] = 0;
     else if (rules.classes())
       for (int i = tid; i < kClasses; i += kSliceThreads) classes[i] = 0;
-    if (tid == 0) taken = 0;
+    if (tid == 0) taken = rules.greedy ? 0x7fffffff : 0;
     if (tid < 2) bins_lds[tid] = 0;
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < W; ++i) best = max(best, best_lds[i]);
-  const float top = value_of(uint32_t(best >> 32));
+  for (int i = 0; i < W; ++i) top = fmaxf(top, top_lds[i]);
   SliceHead* const head = p.heads + int64_t(row) * p.slices + slice;
   char* const part = static_cast<char*>(p.lists) + (int64_t(row) * p.slices + slice) * p.part;
-  if (rules.greedy || best == 0) {
-    if (tid == 0) *head = SliceHead{best, 0.0, 0.0, 0, 0, 0, {}};
+  if (top == -INFINITY) {
+    if (tid == 0) *head = SliceHead{0, 0.0, 0.0, 0, 0, 0, {}};
+    return;
+  }
+  uint64_t best = uint64_t(ordered(top)) << 32;
+  if (!PLAIN && rules.greedy) {
+    // of equal values the lowest token
+    int first = 0x7fffffff;
+#pragma unroll
+    for (int l = L - 1; l >= 0; --l)
+#pragma unroll
+      for (int e = V - 1; e >= 0; --e)
+        if (x[l][e] == top) first = token(l, e);
+    if (first != 0x7fffffff) atomicMin(&taken, first);
+    __syncthreads();
+    if (tid == 0) *head = SliceHead{best | uint32_t(~taken), 0.0, 0.0, 0, 0, 0, {}};
     return;
   }
   if (PLAIN || (!rules.lists() && !rules.classes())) {
@@ -328,7 +398,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
     }
     if (lane == 63) total_lds[wave] = run;
     if (lane == 0) {
-      best_lds[wave] = low;
+      low_lds[wave] = low;
       count_lds[wave] = valid;
     }
     __syncthreads();
@@ -340,7 +410,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
       uint64_t all = 0;
       valid = 0;
       for (int i = 0; i < W; ++i) {
-        all += total_lds[i] + best_lds[i];
+        all += total_lds[i] + low_lds[i];
         valid += count_lds[i];
       }
       *head = SliceHead{best, double(all), ref, 0, 0, uint32_t(valid), {}};
@@ -614,30 +684,6 @@ __device__ __forceinline__ Search whole_search(const Rules& r, double u, double 
   return st;
 }
 
-// Lane l's partner l ^ MASK, without a way through LDS.
-template <int CTRL>
-__device__ __forceinline__ uint32_t moved(uint32_t x) {
-  return uint32_t(__builtin_amdgcn_update_dpp(0, int(x), CTRL, 0xf, 0xf, true));
-}
-template <int MASK>
-__device__ __forceinline__ uint32_t across(uint32_t x) {
-  if constexpr (MASK == 1) return moved<0xb1>(x);            // quad 1 0 3 2
-  if constexpr (MASK == 2) return moved<0x4e>(x);            // quad 2 3 0 1
-  if constexpr (MASK == 4) return moved<0x141>(moved<0x1b>(x));  // within eight: 7 - l of quad 3 2 1 0
-  if constexpr (MASK == 8) return moved<0x128>(x);           // a row of 16 turned by 8
-  if constexpr (MASK == 16) {
-    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-    return __lane_id() & 16 ? a[0] : a[1];
-  }
-  if constexpr (MASK == 32) {
-    const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    return __lane_id() & 32 ? a[0] : a[1];
-  }
-}
-template <int MASK>
-__device__ __forceinline__ uint64_t across(uint64_t x) {
-  return uint64_t(across<MASK>(uint32_t(x >> 32))) << 32 | across<MASK>(uint32_t(x));
-}
 // Strides STRIDE .. 1 of a bitonic merge of blocks of `size`.
 template <int STRIDE>
 __device__ __forceinline__ uint64_t merge_down(uint64_t key, int size) {
@@ -733,42 +779,11 @@ __device__ __forceinline__ double slices_sum(const double* slice, int n) {
   return wave_sum(x);
 }
 
-// The draw among `weights of the slices` (lds.slice, summing to total in that order): the slice, then the token in it;
-// weight(x, token) is 0 for what does not stay.  -> the token.
-template <int PER, class T, class Lds, class Weight>
-__device__ int draw_from_slices(Lds& lds, const SampleParams& p, const Row<T>& src, int row, double target, Weight&& weight) {
-  auto& sh = lds.sh;
+// The token in the slice that the draw fell into (sh.slice, sh.target from its start on); weight(x, token) is 0 for what
+// does not stay.
+template <int PER, class T, class Shared, class Weight>
+__device__ __forceinline__ int draw_in_slice(Shared& sh, const SampleParams& p, const Row<T>& src, int row, Weight&& weight) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (wave == 0) {
-    // 64 slices at a time; the sums run on in order
-    double run = 0.0, before = 0.0;
-    int at = -1;
-    for (int s0 = 0; s0 < p.slices; s0 += 64) {
-      const double mine = s0 + lane < p.slices ? lds.slice[s0 + lane] : 0.0;
-      double sum = mine;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const double up = __shfl_up(sum, o);
-        if (lane >= o) sum += up;
-      }
-      sum += run;
-      const uint64_t past = __ballot(mine > 0.0 && sum > target), some = __ballot(mine > 0.0);
-      if (some) {
-        const int i = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);  // else the last that has any, so far
-        at = s0 + i;
-        before = __shfl(sum, i) - __shfl(mine, i);
-      }
-      if (past) break;
-      run = __shfl(sum, 63);
-    }
-    if (lane == 0) {
-      sh.slice = at;
-      sh.target = target - before;
-      sh.token = -1;
-      sh.first = 0x7fffffff;
-    }
-  }
-  __syncthreads();
   const int first = (sh.slice * kRowThreads + tid) * PER - src.skip;
   const T* values = static_cast<const T*>(p.logits) + row * p.stride;
   float x[PER];
@@ -803,47 +818,117 @@ __device__ int draw_from_slices(Lds& lds, const SampleParams& p, const Row<T>& s
   return min(max(sh.first == 0x7fffffff ? sh.token : sh.first, 0), p.vocab - 1);
 }
 
-// Rows without a rule.
+// The draw among the weights of the slices (lds.slice): the slice, then the token in it.
+template <int PER, class T, class Lds, class Weight>
+__device__ int draw_from_slices(Lds& lds, const SampleParams& p, const Row<T>& src, int row, double target, Weight&& weight) {
+  auto& sh = lds.sh;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (wave == 0) {
+    // 64 slices at a time; the sums run on in order
+    double run = 0.0, before = 0.0;
+    int at = -1;
+    for (int s0 = 0; s0 < p.slices; s0 += 64) {
+      const double mine = s0 + lane < p.slices ? lds.slice[s0 + lane] : 0.0;
+      double sum = mine;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const double up = __shfl_up(sum, o);
+        if (lane >= o) sum += up;
+      }
+      sum += run;
+      const uint64_t past = __ballot(mine > 0.0 && sum > target), some = __ballot(mine > 0.0);
+      if (some) {
+        const int i = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);  // else the last that has any, so far
+        at = s0 + i;
+        before = __shfl(sum, i) - __shfl(mine, i);
+      }
+      if (past) break;
+      run = __shfl(sum, 63);
+    }
+    if (lane == 0) {
+      sh.slice = at;
+      sh.target = target - before;
+      sh.token = -1;
+      sh.first = 0x7fffffff;
+    }
+  }
+  __syncthreads();
+  return draw_in_slice<PER>(sh, p, src, row, weight);
+}
+
+// Rows without a rule: the first wave takes all slices' sums, four a lane, and picks the slice.
 struct PlainLds {
   struct {
     double wave_d[kRowWaves], target;
     int slice, token, first;
   } sh;
-  uint64_t best[kRowWaves];
-  double slice[kSlicesMax];
+  double total;
+  float top;
 };
 template <class T, int PER>
 __global__ __launch_bounds__(kRowThreads) void sample_plain_kernel(const SampleParams p) {
+  static_assert(kSlicesMax == 256, "four slices a lane");
   __shared__ PlainLds lds;
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  SliceHead head = {};
-  if (tid < p.slices) head = p.heads[int64_t(row) * p.slices + tid];
-  const double u = fmin(fmax(double(p.uniforms[row]), 0.0), 1.0);
   const Rules rules = rules_of(p, row);
   const Row<T> src(p, row);
-  uint64_t best = wave_max(head.best);
-  if (lane == 0) lds.best[wave] = best;
-  __syncthreads();
+  if (wave == 0) {
+    const SliceHead* heads = p.heads + int64_t(row) * p.slices;
+    float tops[4], top = -INFINITY;
+    double w[4], mine = 0.0;
 #pragma unroll
-  for (int i = 0; i < kRowWaves; ++i) best = max(best, lds.best[i]);
-  if (best == 0) {
+    for (int j = 0; j < 4; ++j) {
+      const int s = lane * 4 + j;
+      const uint64_t best = s < p.slices ? heads[s].best : 0;
+      w[j] = s < p.slices ? heads[s].sum : 0.0;
+      tops[j] = value_of(uint32_t(best >> 32));
+      top = fmaxf(top, tops[j]);
+    }
+    const double u = fmin(fmax(double(p.uniforms[row]), 0.0), 1.0);
+    top = wave_top(top);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[j] *= weight_of(tops[j], top, rules.scale);
+      mine += w[j];
+    }
+    const double run = wave_running_sum(mine), total = __shfl(run, 63), target = u * total;
+    const uint64_t past = __ballot(mine > 0.0 && run > target), some = __ballot(mine > 0.0);
+    if (lane == (past ? __builtin_ctzll(past) : some ? 63 - __builtin_clzll(some) : 0)) {
+      // the first slice past the target, else the last that weighs anything
+      int at = 0;
+      double upto = run - mine, before = upto;
+      bool found = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (!found && w[j] > 0.0) {
+          at = lane * 4 + j;
+          before = upto;
+          found = upto + w[j] > target;
+        }
+        upto += w[j];
+      }
+      lds.sh.slice = at;
+      lds.sh.target = target - before;
+      lds.sh.token = -1;
+      lds.sh.first = 0x7fffffff;
+      lds.total = total;
+      lds.top = top;
+    }
+  }
+  __syncthreads();
+  const float top = lds.top;
+  if (top == -INFINITY) {
     if (tid == 0) {
       p.tokens[row] = -1;
       if (p.logprobs) p.logprobs[row] = -INFINITY;
     }
     return;
   }
-  const float top = value_of(uint32_t(best >> 32));
-  if (tid < p.slices)
-    lds.slice[tid] = head.best ? head.sum * weight_of(value_of(uint32_t(head.best >> 32)), top, rules.scale) : 0.0;
-  __syncthreads();
-  double total = 0.0;
-  total = slices_sum(lds.slice, p.slices);
-  const int token = draw_from_slices<PER>(lds, p, src, row, u * total,
-                                          [&](float x, int) { return weight_of(x, top, rules.scale); });
+  const int token = draw_in_slice<PER>(lds.sh, p, src, row, [&](float x, int) { return weight_of(x, top, rules.scale); });
   if (tid == 0) {
     p.tokens[row] = token;
-    if (p.logprobs) p.logprobs[row] = log_share(to_float((static_cast<const T*>(p.logits) + row * p.stride)[token]), top, rules, total);
+    if (p.logprobs)
+      p.logprobs[row] = log_share(to_float((static_cast<const T*>(p.logits) + row * p.stride)[token]), top, rules, lds.total);
   }
 }
 
@@ -891,21 +976,28 @@ __device__ __forceinline__ void lists_row(const SampleParams& p, const Rules& ru
       if (p.logprobs) p.logprobs[row] = log_share(to_float(values[token]), top, rules, total);
     }
   };
-  // the lists, as far as they are whole: above the largest value that some slice left out
-  for (int s = wave; s < p.slices; s += kRowWaves) {
-    const int count = min(int(p.heads[int64_t(row) * p.slices + s].count), p.cap);
-    const uint2* list = reinterpret_cast<const uint2*>(parts + s * p.part);
-    for (int i0 = 0; i0 < count; i0 += 64) {
-      const uint2 it = i0 + lane < count ? list[i0 + lane] : uint2{0, 0};
-      const bool take = it.x > left;
-      const uint64_t all = __ballot(take);
-      int at = 0;
-      if (lane == 0) at = atomicAdd(&sh.n, __popcll(all));
-      at = __builtin_amdgcn_readfirstlane(at) + __popcll(all & ((uint64_t(1) << lane) - 1));
-      if (take && at < kListMax) {
-        lds.list.keys[at] = it.x;
-        lds.list.tokens[at] = it.y;
-      }
+  // the lists, as far as they are whole: above the largest value that some slice left out.  All loads at once: a list
+  // has `cap` places, kListMax together at most.
+  if (tid < p.slices) lds.shift[tid] = min(int(head.count), p.cap);
+  __syncthreads();
+  uint2 it[kListMax / kRowThreads];
+#pragma unroll
+  for (int j = 0; j < kListMax / kRowThreads; ++j) {
+    const int i = tid + j * kRowThreads, s = i / p.cap;
+    it[j] = uint2{0, 0};
+    if (s < p.slices && i - s * p.cap < lds.shift[s]) it[j] = reinterpret_cast<const uint2*>(parts + s * p.part)[i - s * p.cap];
+  }
+#pragma unroll
+  for (int j = 0; j < kListMax / kRowThreads; ++j) {
+    const bool take = it[j].x > left;
+    const uint64_t all = __ballot(take);
+    if (!all) continue;
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&sh.n, __popcll(all));
+    at = __builtin_amdgcn_readfirstlane(at) + __popcll(all & ((uint64_t(1) << lane) - 1));
+    if (take) {
+      lds.list.keys[at] = it[j].x;
+      lds.list.tokens[at] = it[j].y;
     }
   }
   __syncthreads();
@@ -1344,6 +1436,7 @@ extern "C" int pkv_sample(const void* logits, int64_t stride, int32_t dtype, con
   p.heads = static_cast<SliceHead*>(workspace);
   p.lists = p.heads + size_t(rows) * s.slices;
   p.temperature = {temperatures, temperature};
+  p.scale = kLog2e / double(temperature);
   p.top_k = {top_ks, double(top_k)};
   p.top_p = {top_ps, top_p};
   p.min_p = {min_ps, min_p};
