@@ -26,6 +26,7 @@ namespace pkv {
 namespace {
 
 constexpr int kSliceThreads = 256;
+constexpr int kSlice = 16 * kSliceThreads;  // 256 plain rows of 131072 take 59 us in slices of 4096, 62 in 8192
 constexpr int kRowThreads = 1024;
 constexpr int kRowWaves = kRowThreads / 64;
 constexpr int kListMax = 8192;   // tokens that a row's lists hold together
@@ -781,10 +782,10 @@ __device__ __forceinline__ double slices_sum(const double* slice, int n) {
 
 // The token in the slice that the draw fell into (sh.slice, sh.target from its start on); weight(x, token) is 0 for what
 // does not stay.
-template <int PER, class T, class Shared, class Weight>
+template <int PER, int THREADS, class T, class Shared, class Weight>
 __device__ __forceinline__ int draw_in_slice(Shared& sh, const SampleParams& p, const Row<T>& src, int row, Weight&& weight) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int first = (sh.slice * kRowThreads + tid) * PER - src.skip;
+  const int first = (sh.slice * THREADS + tid) * PER - src.skip;
   const T* values = static_cast<const T*>(p.logits) + row * p.stride;
   float x[PER];
   double w[PER], mine = 0.0;
@@ -853,7 +854,7 @@ __device__ int draw_from_slices(Lds& lds, const SampleParams& p, const Row<T>& s
     }
   }
   __syncthreads();
-  return draw_in_slice<PER>(sh, p, src, row, weight);
+  return draw_in_slice<PER, kRowThreads>(sh, p, src, row, weight);
 }
 
 // Rows without a rule: the first wave takes all slices' sums, four a lane, and picks the slice.
@@ -865,8 +866,10 @@ struct PlainLds {
   double total;
   float top;
 };
-template <class T, int PER>
-__global__ __launch_bounds__(kRowThreads) void sample_plain_kernel(const SampleParams p) {
+constexpr int kPlainThreads = 256;
+template <class T>
+__global__ __launch_bounds__(kPlainThreads) void sample_plain_kernel(const SampleParams p) {
+  constexpr int PER = kSlice / kPlainThreads;
   static_assert(kSlicesMax == 256, "four slices a lane");
   __shared__ PlainLds lds;
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -924,7 +927,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_plain_kernel(const SampleP
     }
     return;
   }
-  const int token = draw_in_slice<PER>(lds.sh, p, src, row, [&](float x, int) { return weight_of(x, top, rules.scale); });
+  const int token = draw_in_slice<PER, kPlainThreads>(lds.sh, p, src, row, [&](float x, int) { return weight_of(x, top, rules.scale); });
   if (tid == 0) {
     p.tokens[row] = token;
     if (p.logprobs)
@@ -1358,7 +1361,6 @@ struct Split {
   int slices, cap;
   int64_t part;  // bytes of a slice's list or classes
 };
-constexpr int kSlice = 16 * kSliceThreads;  // 256 plain rows of 131072 take 59 us in slices of 4096, 62 in 8192
 Split split_of(int vocab) {
   Split s;
   const int size = kSlice;
@@ -1378,7 +1380,7 @@ void launch(const SampleParams& p, const Kinds& k, int rows, hipStream_t stream)
   const dim3 slices(p.slices, rows);
   if (k.plain) {
     sample_slice_kernel<T, 16, true><<<slices, kSliceThreads, 0, stream>>>(p);
-    sample_plain_kernel<T, PER><<<rows, kRowThreads, 0, stream>>>(p);
+    sample_plain_kernel<T><<<rows, kPlainThreads, 0, stream>>>(p);
   } else {
     sample_slice_kernel<T, 16, false><<<slices, kSliceThreads, 0, stream>>>(p);
     // two kernels, not one with both: that one would have to spill
