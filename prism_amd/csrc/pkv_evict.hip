@@ -55,19 +55,27 @@ __device__ __forceinline__ uint32_t ordered(float f) {
 // The place from the top of a histogram of 2^bits counts where the running sum reaches `need`.
 struct Digit {
   int hist[2048];
-  int wave_sum[kSelectWaves];
+  int wave_sum[kSelectWaves], chunk_sum[2][kSelectWaves];
   int bin, above, count;
 };
+// Sums of a wave up to each lane: within rows of 16, then from row to row.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int add_from(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_running_sum(int x) {
+  x = add_from<0x111, 0xf>(x);  // the lane before, two, four, eight before
+  x = add_from<0x112, 0xf>(x);
+  x = add_from<0x114, 0xf>(x);
+  x = add_from<0x118, 0xf>(x);
+  x = add_from<0x142, 0xa>(x);         // lane 15 of the row before, into rows 1 and 3
+  return add_from<0x143, 0xc>(x);      // lane 31, into rows 2 and 3
+}
 __device__ __forceinline__ void find_digit(Digit& sh, int bits, int need) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int top = (1 << bits) - 1 - 2 * tid;  // this thread's two bins, from the top
   const int c0 = top >= 0 ? sh.hist[top] : 0, c1 = top >= 1 ? sh.hist[top - 1] : 0;
-  int run = c0 + c1;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int up = __shfl_up(run, o);
-    if (lane >= o) run += up;
-  }
+  const int run = wave_running_sum(c0 + c1);
   if (lane == 63) sh.wave_sum[wave] = run;
   __syncthreads();
   int before = run - c0 - c1;
@@ -128,20 +136,35 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
   const int lo = s.first, hi = s.n - s.recent;  // whose weights decide
   int need = s.keep - s.first - s.recent;       // how many of them stay
   const bool choose = need > 0;
-  // f(t, four weights) for every group of four tokens, kUnroll of a thread's loads on the way at once
-  constexpr int kUnroll = 8;
+  // f(t, four keys) for every group of four tokens some of whose weights decide, 0 for those that do not; a batch of
+  // loads is on its way while the one before it is worked on
+  constexpr int kUnroll = 4, kStride = kSelectThreads * 4;
   auto each = [&](auto&& f) {
-    for (int t0 = tid * 4; t0 < s.n; t0 += kUnroll * kSelectThreads * 4) {
+    f32x4 next[kUnroll];
+    auto load = [&](int t0) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (t0 + u * kStride < s.n) next[u] = *reinterpret_cast<const f32x4*>(place(t0 + u * kStride));
+    };
+    load(tid * 4);
+    for (int t0 = tid * 4; t0 < s.n; t0 += kUnroll * kStride) {
       f32x4 x[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int t = t0 + u * kSelectThreads * 4;
-        if (t < s.n) x[u] = *reinterpret_cast<const f32x4*>(place(t));
-      }
+      for (int u = 0; u < kUnroll; ++u) x[u] = next[u];
+      load(t0 + kUnroll * kStride);
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
-        const int t = t0 + u * kSelectThreads * 4;
-        if (t < s.n) f(t, x[u]);
+        const int t = t0 + u * kStride;
+        if (t + 3 < lo || t >= hi) continue;
+        uint32_t key[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) key[i] = ordered(x[u][i]);
+        if (t < lo || t + 3 >= hi) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (t + i < lo || t + i >= hi) key[i] = 0;
+        }
+        f(key);
       }
     }
   };
@@ -161,12 +184,10 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
         for (int i = tid; i < n_listed; i += kSelectThreads)
           if ((keys[i] & done) == threshold) atomicAdd(&sh.hist[(keys[i] >> shift) & mask], 1);
       } else {
-        each([&](int t, f32x4 x) {
+        each([&](const uint32_t (&key)[4]) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t key = ordered(x[i]);
-            if (t + i >= lo && t + i < hi && (key & done) == threshold) atomicAdd(&sh.hist[(key >> shift) & mask], 1);
-          }
+          for (int i = 0; i < 4; ++i)
+            if (key[i] != 0 && (key[i] & done) == threshold) atomicAdd(&sh.hist[(key[i] >> shift) & mask], 1);
         });
       }
       __syncthreads();
@@ -177,12 +198,10 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
       if (!listed && shift > 0 && n_listed <= kCandidates) {
         listed = true;
         const uint32_t upto = ~0u << shift;
-        each([&](int t, f32x4 x) {
+        each([&](const uint32_t (&key)[4]) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t key = ordered(x[i]);
-            if (t + i >= lo && t + i < hi && (key & upto) == threshold) keys[atomicAdd(&candidates, 1)] = key;
-          }
+          for (int i = 0; i < 4; ++i)
+            if (key[i] != 0 && (key[i] & upto) == threshold) keys[atomicAdd(&candidates, 1)] = key[i];
         });
       }
       __syncthreads();
@@ -191,60 +210,55 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
   }
   // in the order of positions: what lies above the threshold, and the first `need` that equal it.  A kept weight moves to
   // d <= t: never to where a later chunk's lie, and this chunk's are in registers by then.
-  constexpr int G = 1;  // groups of four tokens a thread and chunk
+  constexpr int kAhead = 4;  // chunks on their way
   int above = 0, equal = 0;  // so far
-  f32x4 next[G] = {};
-  auto load = [&](int t0) {
-#pragma unroll
-    for (int j = 0; j < G; ++j) {
-      const int t = t0 + (tid * G + j) * 4;
-      if (t < s.n) next[j] = *reinterpret_cast<const f32x4*>(place(t));
-    }
+  f32x4 next[kAhead];
+  auto load = [&](int j, int t) {
+    if (t < s.n) next[j] = *reinterpret_cast<const f32x4*>(place(t));
   };
-  load(0);
-  for (int t0 = 0; t0 < s.n; t0 += kSelectThreads * 4 * G) {
-    const int t = t0 + tid * 4 * G;
-    f32x4 x[G];
 #pragma unroll
-    for (int j = 0; j < G; ++j) x[j] = next[j];
-    load(t0 + kSelectThreads * 4 * G);
-    uint32_t is_above = 0, is_equal = 0;
+  for (int j = 0; j < kAhead; ++j) load(j, tid * 4 + j * kStride);
+  for (int base = 0; base < s.n; base += kAhead * kStride) {
 #pragma unroll
-    for (int i = 0; i < 4 * G; ++i) {
-      const bool middle = t + i >= lo && t + i < hi;
-      const uint32_t key = ordered(x[i >> 2][i & 3]);
-      is_above |= uint32_t(t + i < s.n && (!middle || (choose && key > threshold))) << i;
-      is_equal |= uint32_t(choose && middle && key == threshold) << i;
-    }
-    const int mine = __popc(is_above) << 16 | __popc(is_equal);
-    int run = mine;
+    for (int j = 0; j < kAhead; ++j) {
+      if (base + j * kStride >= s.n) break;
+      const int t = base + j * kStride + tid * 4;
+      const f32x4 x = next[j];
+      load(j, t + kAhead * kStride);
+      uint32_t is_above = 0, is_equal = 0;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int up = __shfl_up(run, o);
-      if (lane >= o) run += up;
-    }
-    if (lane == 63) sh.wave_sum[wave] = run;
-    __syncthreads();
-    int before = run - mine, all = 0;
-    for (int i = 0; i < kSelectWaves; ++i) {
-      if (i < wave) before += sh.wave_sum[i];
-      all += sh.wave_sum[i];
-    }
-    int my_above = above + (before >> 16), my_equal = equal + (before & 0xffff);
-#pragma unroll
-    for (int i = 0; i < 4 * G; ++i) {
-      const bool a = is_above >> i & 1, e = is_equal >> i & 1;
-      if (a || (e && my_equal < need)) {
-        const int d = my_above + min(my_equal, need);
-        kept[d] = t + i;
-        if (d != t + i) *place(d) = x[i >> 2][i & 3];
+      for (int i = 0; i < 4; ++i) {
+        const bool middle = t + i >= lo && t + i < hi;
+        const uint32_t key = ordered(x[i]);
+        is_above |= uint32_t(t + i < s.n && (!middle || (choose && key > threshold))) << i;
+        is_equal |= uint32_t(choose && middle && key == threshold) << i;
       }
-      my_above += a;
-      my_equal += e;
+      const int mine = __popc(is_above) << 16 | __popc(is_equal), run = wave_running_sum(mine);
+      int* const sums = sh.chunk_sum[j & 1];  // the other one may still be read
+      if (lane == 63) sums[wave] = run;
+      __syncthreads();
+      int before = run - mine, all = 0;
+#pragma unroll
+      for (int i = 0; i < kSelectWaves; ++i) {
+        const int v = sums[i];
+        before += i < wave ? v : 0;
+        all += v;
+      }
+      int my_above = above + (before >> 16), my_equal = equal + (before & 0xffff);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool a = is_above >> i & 1, e = is_equal >> i & 1;
+        if (a || (e && my_equal < need)) {
+          const int d = my_above + min(my_equal, need);
+          kept[d] = t + i;
+          if (d != t + i) *place(d) = x[i];
+        }
+        my_above += a;
+        my_equal += e;
+      }
+      above += all >> 16;
+      equal += all & 0xffff;
     }
-    above += all >> 16;
-    equal += all & 0xffff;
-    __syncthreads();
   }
 }
 
