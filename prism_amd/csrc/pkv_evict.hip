@@ -25,7 +25,7 @@ struct EvictParams {
 
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWaves = kSelectThreads / 64;
-constexpr int kTableCols = 8192;    // of a sequence's block-table row, held in LDS
+constexpr int kTableCols = 8192;    // of block tables no wider than that, a sequence's row is held in LDS
 constexpr int kCandidates = 24576;  // keys that share the threshold's first digit, held in LDS
 
 // A sequence's sizes, read by every workgroup that works for it.
@@ -95,12 +95,14 @@ __device__ __forceinline__ void find_digit(Digit& sh, int bits, int need) {
 // A workgroup per layer, sequence and head.  Reads the weights three times (first digit; the keys of that digit, which
 // then lie in LDS; the kept ones), 16 bytes a lane with the next ones on the way: 28 layers' one head of 100 k tokens
 // take .. us.
+// TABLE: a sequence's row of the block table lies in LDS.
+template <bool TABLE>
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const EvictParams p) {
   __shared__ Digit sh;
-  __shared__ int table[kTableCols];
-  __shared__ uint32_t keys[kCandidates];
+  __shared__ int table[TABLE ? kTableCols : 1];
+  __shared__ __align__(16) uint32_t keys[kCandidates];  // later what stays of a chunk, twice
   __shared__ int candidates;
-  const int h = blockIdx.x, b = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int h = blockIdx.x, b = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Sizes s = sizes_of(p, b);
   const int64_t head = (int64_t(layer) * p.batch + b) * p.n_kv + h;
   int32_t* kept = p.kept + head * p.max_keep;
@@ -113,7 +115,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
     for (int c = tid; c < pages; c += kSelectThreads) {
       const int page = bt[c];
       bad |= unsigned(page) >= unsigned(p.num_pages);
-      if (c < kTableCols) table[c] = page;
+      if constexpr (TABLE) table[c] = page;
     }
   }
   if (tid == 0) candidates = 0;
@@ -131,7 +133,12 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
   const int in_page = (1 << p.log2_page) - 1;
   auto place = [&](int t) -> float* {
     const int col = t >> p.log2_page;
-    return w + (col < kTableCols ? table[col] : bt[col]) * p.w_page + (t & in_page);
+    int page;
+    if constexpr (TABLE)
+      page = table[col];
+    else
+      page = bt[col];
+    return w + page * p.w_page + (t & in_page);
   };
   const int lo = s.first, hi = s.n - s.recent;  // whose weights decide
   int need = s.keep - s.first - s.recent;       // how many of them stay
@@ -225,39 +232,49 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
       const int t = base + j * kStride + tid * 4;
       const f32x4 x = next[j];
       load(j, t + kAhead * kStride);
+      // without a choice (need 0) the threshold is above every key but NaN's, and none of those equal to it stay
       uint32_t is_above = 0, is_equal = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const bool middle = t + i >= lo && t + i < hi;
         const uint32_t key = ordered(x[i]);
-        is_above |= uint32_t(t + i < s.n && (!middle || (choose && key > threshold))) << i;
-        is_equal |= uint32_t(choose && middle && key == threshold) << i;
+        is_above |= uint32_t(key > threshold) << i;
+        is_equal |= uint32_t(key == threshold) << i;
+      }
+      if (t < lo || t + 3 >= hi) {
+        const uint32_t inside = t + 3 < s.n ? 15 : t < s.n ? (1u << (s.n - t)) - 1 : 0;
+        uint32_t middle = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) middle |= uint32_t(t + i >= lo && t + i < hi) << i;
+        is_above = (is_above & middle) | (inside & ~middle);
+        is_equal &= middle;
       }
       const int mine = __popc(is_above) << 16 | __popc(is_equal), run = wave_running_sum(mine);
       int* const sums = sh.chunk_sum[j & 1];  // the other one may still be read
       if (lane == 63) sums[wave] = run;
       __syncthreads();
-      int before = run - mine, all = 0;
-#pragma unroll
-      for (int i = 0; i < kSelectWaves; ++i) {
-        const int v = sums[i];
-        before += i < wave ? v : 0;
-        all += v;
-      }
+      const int waves = wave_running_sum(lane < kSelectWaves ? sums[lane] : 0);  // up to each of them
+      const int all = __builtin_amdgcn_readlane(waves, kSelectWaves - 1);
+      const int before = (wave > 0 ? __builtin_amdgcn_readlane(waves, wave - 1) : 0) + run - mine;
       int my_above = above + (before >> 16), my_equal = equal + (before & 0xffff);
+      const int start = above + min(equal, need);
+      uint2* const stage = reinterpret_cast<uint2*>(keys) + (j & 1) * kStride;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const bool a = is_above >> i & 1, e = is_equal >> i & 1;
-        if (a || (e && my_equal < need)) {
-          const int d = my_above + min(my_equal, need);
-          kept[d] = t + i;
-          if (d != t + i) *place(d) = x[i];
-        }
+        if (a || (e && my_equal < need)) stage[my_above + min(my_equal, need) - start] = uint2{uint32_t(t + i), __float_as_uint(x[i])};
         my_above += a;
         my_equal += e;
       }
       above += all >> 16;
       equal += all & 0xffff;
+      const int count = above + min(equal, need) - start;
+      __syncthreads();
+      for (int i = tid; i < count; i += kSelectThreads) {
+        const uint2 it = stage[i];
+        const int d = start + i;
+        kept[d] = int(it.x);
+        if (d != int(it.x)) *place(d) = __uint_as_float(it.y);
+      }
     }
   }
 }
@@ -405,7 +422,8 @@ extern "C" int pkv_evict(void* k_pool, void* v_pool, int64_t layer_stride, int64
   const hipStream_t s = static_cast<hipStream_t>(stream);
   p.marks = static_cast<int32_t*>(workspace);
   p.move_chunks = move_chunks(max_keep, head_dim);
-  evict_select_kernel<<<dim3(n_kv, batch, layers), kSelectThreads, 0, s>>>(p);
+  auto* select = max_blocks <= kTableCols ? evict_select_kernel<true> : evict_select_kernel<false>;
+  select<<<dim3(n_kv, batch, layers), kSelectThreads, 0, s>>>(p);
   evict_move_kernel<kMoveUnroll><<<dim3(unsigned(wgs), batch, layers), 256, 0, s>>>(p, ilog2(head_dim / 8));
   return check_launch(fn);
 }

@@ -69,6 +69,14 @@ def test_long(gpu, lens, keeps):
     _check(gpu, k, v, w, bt, lens, keeps, 4, 100)
 
 
+def test_tables_wider_than_the_kernel_holds(gpu):
+    """8200 columns, and a sequence that uses more than 8192 of them."""
+    lens, keeps = [131200 - 5, 700], [9000, 300]
+    k, v, w, bt = _pools(1, lens, 16, 1, 64, seed=8)
+    assert bt.shape[1] > 8192
+    _check(gpu, k, v, w, bt, lens, keeps, 4, 100)
+
+
 def test_ties_and_odd_values(gpu):
     """Equal weights (zeros of both signs among them) go by age; NaN is above +inf, negative weights are below zero."""
     lens, keeps = [3000, 1500, 5000, 2000], [1000, 700, 4000, 900]
