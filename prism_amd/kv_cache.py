@@ -92,6 +92,7 @@ class FlashAttnKVCache:
         self.key_weight_pool: torch.Tensor | None = None
         self.key_weights: list[torch.Tensor] = []
         self._weighed: dict[int, int] = {}
+        self._weighed_pages: set[int] = set()  # pages all of whose keys have theirs: as a prefix, they count as weighed
         self.prefix_cache = None               # set by PrefixCache(kv)
         self._bases: torch.Tensor | None = None
         self.null_page: int | None = None      # reserve_null_page()
@@ -117,7 +118,9 @@ class FlashAttnKVCache:
     def _pop_page(self) -> int:
         if not self.free_pages:
             raise KVCacheOutOfPages(f"Out of KV cache pages ({self.max_pages} total)")
-        return self.free_pages.pop()
+        page = self.free_pages.pop()
+        self._weighed_pages.discard(page)
+        return page
 
     def _all_pages_free(self) -> list[int]:
         return [p for p in range(self.max_pages - 1, -1, -1) if p != self.null_page]
@@ -171,7 +174,8 @@ class FlashAttnKVCache:
         self.seq_pages[seq_id] = pages
         self.seq_len[seq_id] = prefix_len if prefix_pages else 0
         self.seq_owner[seq_id] = owner
-        self._weighed[seq_id] = self.seq_len[seq_id]
+        first_without = next((i for i, p in enumerate(pages) if p not in self._weighed_pages), len(pages))
+        self._weighed[seq_id] = min(self.seq_len[seq_id], first_without * self.page_size)
 
     def fork_sequence(self, src_seq_id: int, dst_seq_id: int, owner: str | None = None) -> None:
         """dst shares every page of src (no copy); the first write into a shared page copies it.
@@ -361,9 +365,10 @@ class FlashAttnKVCache:
                             n_kv=self.num_kv_heads, head_dim=self.head_dim, windows=windows, weight_rows=weight_rows,
                             weighed=weighed, evicted=evicted, device=self.device)
         if weight_rows != 0:
-            for sid, n in zip(seq_ids, counts):
+            for sid, n, had in zip(seq_ids, counts, weighed):
                 if n > 0:
                     self._weighed[sid] = self.seq_len[sid] + n
+                    self._weighed_pages.update(self.seq_pages[sid][had // P:(self.seq_len[sid] + n) // P])
         if torch.device(self.device).type == "cuda":
             poll_status(self.device)
         return batch
@@ -377,6 +382,7 @@ class FlashAttnKVCache:
             self.key_weight_pool = torch.zeros(shape, dtype=torch.float32, device=self.device)
             self.key_weights = list(self.key_weight_pool.unbind(0))
             self._weighed = dict.fromkeys(self.seq_pages, 0)
+            self._weighed_pages.clear()
         return self.key_weights
 
     def next_positions(self, seq_ids: list[int]) -> list[int]:
@@ -524,6 +530,8 @@ class FlashAttnKVCache:
             self._copy_eviction_state(sid, target, sid)
             if target.key_weight_pool is None or self.key_weight_pool is None:
                 target._weighed[sid] = 0
+        if target.key_weight_pool is not None and self.key_weight_pool is not None:
+            target._weighed_pages.update(remap[p] for p in live if p in self._weighed_pages)
         pc = self.prefix_cache
         if pc is not None:
             pc.remap_pages(remap)
@@ -536,6 +544,7 @@ class FlashAttnKVCache:
         self.seq_owner.clear()
         self.seq_evicted.clear()
         self._weighed.clear()
+        self._weighed_pages.clear()
         self._holders.clear()
         return remap
 
@@ -557,7 +566,7 @@ class FlashAttnKVCache:
         self.free_pages = fresh.free_pages
         self.seq_pages, self.seq_len, self.seq_owner = fresh.seq_pages, fresh.seq_len, fresh.seq_owner
         self._holders = fresh._holders
-        self.seq_evicted, self._weighed = fresh.seq_evicted, fresh._weighed
+        self.seq_evicted, self._weighed, self._weighed_pages = fresh.seq_evicted, fresh._weighed, fresh._weighed_pages
         self.key_weight_pool = fresh.key_weight_pool
         self.key_weights[:] = fresh.key_weights
         if fresh.prefix_cache is not None:

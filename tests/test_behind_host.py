@@ -303,3 +303,33 @@ def test_cache_book_keeping_without_a_device(monkeypatch):
     kv.free_sequence(1)
     kv.free_sequence(5)
     assert not kv.seq_evicted
+
+
+def test_a_prefix_whose_keys_were_never_weighed_starts_from_nothing():
+    """Only pages that steps with weights filled count as weighed where they are a new sequence's prefix, whoever had
+    them before."""
+    kv = FlashAttnKVCache(1, 2, 64, 12, 16, "cpu")
+    pc = prism_amd.PrefixCache(kv, 16)
+    kv.enable_key_weights()
+
+    def run(sid, counts, weights):
+        for n, w in zip(counts, weights):
+            kv.prepare_append([sid], n)
+            kv.build_packed_batch([sid], n, 4, weight_rows=None if w else 0)
+            kv.update_seqlens([sid], n)
+
+    def weighed_as_prefix(tokens):
+        pages, n = pc.lookup(tokens, "m")
+        kv.new_sequence(9, prefix_pages=pages, prefix_len=n)
+        got = kv._weighed[9]
+        kv.free_sequence(9)
+        return n, got
+
+    for sid, weights, want in ((1, (1, 1), 48), (2, (0, 0), 0), (3, (0, 1), 48), (4, (1, 0), 32)):
+        tokens = [100 * sid + i for i in range(48)]
+        kv.new_sequence(sid)
+        run(sid, (40, 8), weights)
+        pc.store(tokens, kv.seq_pages[sid][:3], "m")
+        assert weighed_as_prefix(tokens) == (48, want)
+        kv.free_sequence(sid)
+        pc.evict_lru(3)  # its pages go to the next one
