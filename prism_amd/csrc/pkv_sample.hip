@@ -92,8 +92,9 @@ __device__ __forceinline__ Rules rules_of(const SampleParams& p, int row) {
   r.top_p = setting(p.top_p, row);
   r.use_p = r.top_p < 1.0;
   if (r.top_p <= 0.0) r.greedy = true;
-  r.min_p = fmin(setting(p.min_p, row), 1.0);
-  r.use_m = r.min_p > 0.0;
+  const double m = setting(p.min_p, row);
+  r.use_m = m > 0.0;  // not a NaN: a setting that is none takes nothing away
+  r.min_p = fmin(m, 1.0);
   return r;
 }
 

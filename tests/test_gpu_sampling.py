@@ -145,6 +145,18 @@ def test_settings_of_each_row(gpu):
     _draw(x, u, "rows", temperature=0.7, top_k=k, top_p=0.9, min_p=m)
 
 
+def test_settings_of_rows_that_are_no_number(gpu):
+    """NaN: no rule, and the largest logit as a temperature."""
+    x, u = _logits(gpu, 4, 9001, torch.float32, seed=17)
+    nan, one = torch.full((4,), float("nan"), device=gpu), torch.full((4,), 1.0, device=gpu)
+    want = prism_amd.sample_tokens(x, u)
+    assert torch.equal(prism_amd.sample_tokens(x, u, top_p=nan), want)
+    assert torch.equal(prism_amd.sample_tokens(x, u, min_p=nan), want)
+    assert torch.equal(prism_amd.sample_tokens(x, u, top_p=0.5 * one, min_p=nan), prism_amd.sample_tokens(x, u, top_p=0.5))
+    assert torch.equal(prism_amd.sample_tokens(x, u, top_k=40, min_p=nan), prism_amd.sample_tokens(x, u, top_k=40))
+    assert torch.equal(prism_amd.sample_tokens(x, u, temperature=nan), x.argmax(1))
+
+
 def test_extreme_temperatures(gpu):
     x, u = _logits(gpu, 5, 3001, torch.float32, seed=11)
     x[4, :5] = torch.tensor([3e38, 3e38, 2.9e38, -3e38, 0.0])
