@@ -608,7 +608,7 @@ extern "C" int pkv_key_weights(const void* q, int64_t q_st, int64_t q_sh, const 
     return fail(PKV_EINVAL, "%s: lse or weights rows overlap", fn);
   if (n_few + int64_t(n_many) + n_merges == 0) return PKV_OK;
   if (!items || !aligned16(items)) return fail(PKV_EINVAL, "%s: work list null or not 16-byte aligned", fn);
-  if ((n_few + int64_t(n_many) + n_merges) * n_kv > 0x7fffffff) return fail(PKV_EINVAL, "%s: too many work items", fn);
+  if ((n_few + int64_t(n_many) + n_merges) * n_kv * 256 > 0x7fffffff) return fail(PKV_EINVAL, "%s: too many work items", fn);
   const size_t need = pkv_key_weights_workspace_bytes(partials, n_kv);
   if (need > 0 && (!workspace || !aligned16(workspace)))
     return fail(PKV_EINVAL, "%s: workspace null or not 16-byte aligned", fn);

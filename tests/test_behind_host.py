@@ -174,6 +174,13 @@ def test_weights_argument_errors():
     assert lib.pkv_key_weights_workspace_bytes(3, 4) == 3 * 4 * 256 * 4
 
 
+def test_weights_work_lists_past_the_grid():
+    """2^31 threads and more are refused, before anything is launched."""
+    lib = _lib.load()
+    for over in (dict(few=1 << 22), dict(few=1 << 21, many=1 << 21), dict(few=0, merges=1 << 22)):
+        assert _weights_call(lib, **over) == _lib.PKV_EINVAL and b"too many" in lib.pkv_last_error(), over
+
+
 def _evict_call(lib, **over):
     a = dict(k=A16, v=A16, layer=1 << 16, page=2048, w=A16, w_layer=640, w_page=32, bt=A16, bt_st=2, lens=A16, keeps=A16,
              kept=A16, layers=0, batch=1, nk=2, hd=64, P=16, pages=20, blocks=2, max_keep=4, first=0, recent=0, ws=A16,
