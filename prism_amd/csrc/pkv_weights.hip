@@ -32,7 +32,7 @@ struct WeightParams {
   uint32_t window;  // a row sees the keys with pos - t < window, unsigned
 };
 
-// row / g for 0 <= row < 2^30: with shift = ceil(log2 g) and mul = ceil(2^(31 + shift) / g), less than 2^32, the product
+// row / g for 0 <= row < 2^30: with shift = log2 g, rounded up, and mul = ceil(2^(31 + shift) / g), less than 2^32, the product
 // exceeds row * 2^(31 + shift) / g by less than row < 2^31, so by less than 1 / g of the quotient's unit.
 __device__ __forceinline__ int token_of(const WeightParams& p, int row) {
   return int((uint64_t(uint32_t(row)) * p.g_mul) >> (31 + p.g_shift));
@@ -46,7 +46,9 @@ __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
 }
 __device__ __forceinline__ bf16x8 frag(u32x4 v) { return __builtin_bit_cast(bf16x8, v); }
 
-constexpr int kFewPerCu = 4;  // workgroups of weigh_few_kernel on a CU at once
+// Workgroups of weigh_few_kernel on a CU at once.  48 sequences of 2500 keys, 28 heads on 4: 2 of them 35 us, 4 31, 6 46
+// (too few registers).
+constexpr int kFewPerCu = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // A row's denominator in log2; one that saw nothing (-inf) weighs nothing, as one of +inf does.
@@ -84,7 +86,9 @@ __device__ __forceinline__ float row16_sum(float x) {
 // ---- few query rows: the keys stream past them ----
 // Decode tokens and verify rows: the reading of K is all there is to do.  The item's query rows lie in LDS, every wave
 // takes a run of 32-key tiles straight into the A operand (16 keys x 32 elements an instruction, a lane's 16 bytes
-// of its key's row), the rows are the columns of the product: C[key, row], a lane has 4 keys of one row.
+// of its key's row), the rows are the columns of the product: C[key, row], a lane has 4 keys of one row.  The next tile
+// is on its way meanwhile.  48 sequences of 2500 keys (4 KV heads of 128, 135 MB): 30 us, 4.5 TB/s; 7 of 50 k keys on one
+// KV head (106 MB): 25 us, 4.2 TB/s.  A copy of this size runs at 4.9.
 template <int HD>
 struct FewLds {
   u32x4 q[kWeightFewRows * (HD / 8)];
@@ -183,10 +187,11 @@ __device__ __forceinline__ void weigh_few(const WeightParams& p, const WeightIte
 
 // ---- many query rows: a block of keys stays, the rows go past it ----
 // Prompt chunks: 4 waves hold 64 keys each as the A operand, 64 query rows at a time come through LDS (two buffers, one
-// barrier a step) as B, 32 a product: C[key, row], a lane has 16 keys of one row twice, so the row's lse is one value a lane and a
-// key's sum stays in the lane until the end.  Exponentials bound it: of 32 x 32 scores the products take 256 cycles of
-// the matrix pipe, their 16 multiply-adds, exponentials and sums a lane 384 of the vector ALU.  So the products of the
-// second 32 keys are issued between the exponentials of the first, and the other wave of the SIMD fills the rest.
+// barrier a step; 32 a step took 10 % longer) as B, 32 a product: C[key, row], a lane has 16 keys of one row twice, so the
+// row's lse is one value a lane and a key's sum stays in the lane until the end.  Exponentials bound it: of 32 x 32 scores
+// the products take 256 cycles of the matrix pipe, their 16 multiply-adds, exponentials and sums a lane 384 of the vector
+// ALU.  So the products of the second 32 keys are issued between the exponentials of the first, and the other wave of the
+// SIMD fills the rest.  Four prompts of 1800 to 3500 tokens (28 heads of 128 on 4): 184 us, 0.75 PFLOP/s.
 constexpr int kStepRows = 64;
 template <int HD>
 struct ManyLds {
@@ -424,9 +429,12 @@ __global__ __launch_bounds__(kWeightBlock) void weigh_merge_kernel(const WeightP
 
 // ---- the host side ----
 // Few rows: pieces of the keys for four workgroups per CU, of 128 keys at least (a tile per wave).
-// Many rows: blocks of 256 keys; a block's rows are split where there are fewer than two blocks per CU.
+// Many rows: blocks of 256 keys, their rows in pieces for eight workgroups per CU (four prompts: 4 of them 206 us, 8 197,
+// 16 213), of 12 steps of 32 rows at least, as a partial's way through memory has its price (4 steps: a prompt of 2048
+// tokens 67 us in place of 45, decode tokens beside chunks 91 in place of 68, but one of 512 18 in place of 22; 24 steps:
+// 46, 74 and 35).
 constexpr int kManyPerCu = 8;
-constexpr int kMinSteps = 12;  // of 32 rows: below that a partial's way through memory costs more than it saves
+constexpr int kMinSteps = 12;
 
 struct Lists {
   std::vector<WeightItem> few, many, merges;

@@ -50,7 +50,7 @@ def test_every_visible_pair_once(nh, nk, window, rows):
                 assert fresh == (ctx[b] if had is None else had[b])
                 assert 0 < nk_ <= (3968 if kind == "few" else 256) and 0 <= r0 and r0 + nr <= nt * g
                 if kind == "few":
-                    assert (r0, nr, part) == (0, nt * g, -1) and nr <= 64
+                    assert (r0, nr, part) == (0, nt * g, -1) and nr <= 128
                 else:
                     assert r0 % g == 0 or part >= 0
                 rows_of.setdefault((b, k0, nk_), []).append((r0, nr))

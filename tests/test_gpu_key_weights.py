@@ -71,6 +71,17 @@ def test_weights(gpu, lengths, nh, nk, hd, P):
             _check(got, want, gain, w, max(new) * (nh // nk), f"{lengths} rows {rows} window {window}")
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_row_counts_on_either_side_of_the_two_ways(gpu, hd):
+    """128 query rows of a sequence stream its keys, 132 are streamed past them."""
+    new, ctx = [32, 33, 31, 1], [5000, 300, 31, 4000]
+    batch, bt, kc, q, lse, w = _case(gpu, new, ctx, 64, 16, 4, hd, seed=hd)
+    assert batch._weight_plans[None][2] > 0 and batch._weight_plans[None][3] == 2  # 333 keys, blocks of 256
+    want, gain = ob.key_weights64(q, kc, lse, w, new, ctx, bt)
+    got = prism_amd.packed_key_weights(q.to(gpu), kc.to(gpu), lse.to(gpu), w.to(gpu), batch)
+    _check(got, want, gain, w, 33 * 4, f"head_dim {hd}")
+
+
 @pytest.mark.parametrize("new,ctx,nh,nk,hd", [([2000], [0], 28, 4, 128), ([900, 1, 1400], [3000, 9000, 100], 14, 2, 64),
                                               ([700, 300], [0, 12000], 7, 1, 128)])
 def test_split_rows(gpu, new, ctx, nh, nk, hd):
