@@ -498,8 +498,9 @@ size_t pkv_evict_workspace_bytes(int32_t layers, int32_t batch, int32_t n_kv, in
  * weights of those that stay move, in their order, to the front of the sequence's pages; slots behind them keep what
  * they hold.  kept (int32 [layers, batch, n_kv, max_keep]) receives the positions, ascending, -1 behind them.  Caches
  * are bf16 [layers, num_pages, page_size, n_kv, head_dim] with layer and page strides, weights fp32 [layers, num_pages,
- * n_kv, page_size], 16-byte aligned with its strides.  A page that kept tokens move into must not be listed anywhere else in the call.  A sequence whose lengths do not fit the table or
- * max_keep, or that lists a page outside the pool, is left as it is (kept: -1) and flags PKV_STATUS_BAD_PAGE.
+ * n_kv, page_size], 16-byte aligned with its strides.  A page that kept tokens move into must not be listed anywhere
+ * else in the call.  A sequence whose lengths do not fit the table or max_keep, or that lists a page outside the pool,
+ * is left as it is (kept: -1) and flags PKV_STATUS_BAD_PAGE.
  * No counterpart in the reference.
  */
 int pkv_evict(void* k_pool, void* v_pool, int64_t layer_stride, int64_t cache_page_stride, float* weights,

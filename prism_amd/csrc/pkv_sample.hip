@@ -2,10 +2,12 @@
 //
 // With w_i = exp((x_i - max x) / T) and the tokens in the order (x descending, token ascending): the first k stay; of
 // those the shortest prefix whose weights sum to top_p of theirs; of those the ones with w_i >= min_p.  Each rule keeps
-// a prefix of that order, so nothing has to be sorted: what stays is all that lies before one place in it.  The drawn token is the
-// first, in the order of the vocabulary, at which the running sum of the weights that stay passes u times their sum.
+// a prefix of that order, so nothing has to be sorted: what stays is all that lies before one place in it.  The drawn
+// token is the first, in the order of the vocabulary, at which the running sum of the weights that stay passes u times
+// their sum.
 //
-// Two launches.  The first has a workgroup per slice of a row: its maximum and what the row's rules need of it.
+// Two launches, three where some rows have top-k and some do not.  The first has a workgroup per slice of a row: its
+// maximum and what the row's rules need of it.
 //   no rule:          the sum of its weights
 //   top-p or min-p:   the running sums of its weights over classes of value, 1/16 octave of weight each
 //   top-k:            a list of its largest tokens
@@ -13,6 +15,11 @@
 // tokens of one class, or on the lists), then the slice that the draw falls into, and reads that one again.  Rows whose
 // cut lies in none of these (thousands of equal logits, top-k past the lists) are searched through by a radix descent
 // over all their tokens.
+//
+// The first launch is bound by fp64, an exponential a token: 256 plain fp32 rows of 131072 take 31 us (134 MB, 4.3 TB/s),
+// 32 bf16 rows of 151003 with top-p 13.  The second by the latency of its steps, one workgroup a row: plain rows 13 us,
+// top-p 33 (2 to join the slices' heads, 2 their sums, 5 the classes, 10 to read the row for the cut class, 4 to sort it,
+// 5 to draw), top-k 11 for one row of 32000, 35 for 60 of 128000 with settings of their own.
 //
 // A decision can fall between tokens 1e-6 of the sum apart, so the weights are taken in fp64 and their sums are fp64 in
 // a fixed order or integers (2^-42 of the largest weight or finer): no order of atomics changes a token.
@@ -26,7 +33,8 @@ namespace pkv {
 namespace {
 
 constexpr int kSliceThreads = 256;
-constexpr int kSlice = 16 * kSliceThreads;  // 256 plain rows of 131072 take 59 us in slices of 4096, 62 in 8192
+// In slices of 8192, 256 plain rows of 131072 take 53 us, not 47, 32 of 151003 with top-p 53, not 49.
+constexpr int kSlice = 16 * kSliceThreads;
 constexpr int kRowThreads = 1024;
 constexpr int kRowWaves = kRowThreads / 64;
 constexpr int kListMax = 8192;   // tokens that a row's lists hold together
@@ -858,7 +866,8 @@ __device__ int draw_from_slices(Lds& lds, const SampleParams& p, const Row<T>& s
   return draw_in_slice<PER, kRowThreads>(sh, p, src, row, weight);
 }
 
-// Rows without a rule: the first wave takes all slices' sums, four a lane, and picks the slice.
+// Rows without a rule: the first wave takes all slices' sums, four a lane, and picks the slice.  256 rows of 131072 take
+// 47 us with both launches, by the kernel of the other rows 51; one row 16 and 17.
 struct PlainLds {
   struct {
     double wave_d[kRowWaves], target;
@@ -1384,7 +1393,7 @@ void launch(const SampleParams& p, const Kinds& k, int rows, hipStream_t stream)
     sample_plain_kernel<T><<<rows, kPlainThreads, 0, stream>>>(p);
   } else {
     sample_slice_kernel<T, 16, false><<<slices, kSliceThreads, 0, stream>>>(p);
-    // two kernels, not one with both: that one would have to spill
+    // two kernels, not one with both: that one would have to spill (60 rows, some of either kind: 35 and 40 us)
     if (k.lists) sample_row_kernel<T, PER, kListRows><<<rows, kRowThreads, 0, stream>>>(p);
     if (k.others) sample_row_kernel<T, PER, kOtherRows><<<rows, kRowThreads, 0, stream>>>(p);
   }

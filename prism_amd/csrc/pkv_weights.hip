@@ -191,7 +191,7 @@ __device__ __forceinline__ void weigh_few(const WeightParams& p, const WeightIte
 // row's lse is one value a lane and a key's sum stays in the lane until the end.  Exponentials bound it: of 32 x 32 scores
 // the products take 256 cycles of the matrix pipe, their 16 multiply-adds, exponentials and sums a lane 384 of the vector
 // ALU.  So the products of the second 32 keys are issued between the exponentials of the first, and the other wave of the
-// SIMD fills the rest.  Four prompts of 1800 to 3500 tokens (28 heads of 128 on 4): 184 us, 0.75 PFLOP/s.
+// SIMD fills the rest.  Four prompts of 2600 to 3400 tokens (28 heads of 128 on 4): 184 us, 0.75 PFLOP/s.
 constexpr int kStepRows = 64;
 template <int HD>
 struct ManyLds {
