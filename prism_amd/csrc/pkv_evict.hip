@@ -52,6 +52,20 @@ __device__ __forceinline__ uint32_t ordered(float f) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// Four at once: sums of exponentials are as they should be, not negative and no NaN.
+__device__ __forceinline__ void ordered4(f32x4 x, uint32_t (&key)[4]) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(x[i]);
+  const bool fine = max(max(u[0], u[1]), max(u[2], u[3])) <= 0x7f800000u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) key[i] = u[i] | 0x80000000u;
+  if (!fine) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) key[i] = ordered(x[i]);
+  }
+}
+
 // The place from the top of a histogram of 2^bits counts where the running sum reaches `need`.
 struct Digit {
   int hist[2048];
@@ -94,7 +108,7 @@ __device__ __forceinline__ void find_digit(Digit& sh, int bits, int need) {
 
 // A workgroup per layer, sequence and head.  Reads the weights three times (first digit; the keys of that digit, which
 // then lie in LDS; the kept ones), 16 bytes a lane with the next ones on the way.  What bounds it is a CU's vector ALU:
-// 28 layers' one head of 100 k tokens take 72 us on 28 of 256 CUs, 1 us for 4096 weights and pass; 28 layers of
+// 28 layers' one head of 100 k tokens take 66 us on 28 of 256 CUs, 0.9 us for 4096 weights and pass; 28 layers of
 // 6 sequences of 2800 tokens with 4 heads, which fill the device, 32 us.  More workgroups to a head would need four
 // launches, and the move of K and V behind it is the longer one already (110 and 205 us).
 // TABLE: a sequence's row of the block table lies in LDS, as it does up to 8192 columns.  From global memory the long
@@ -147,8 +161,8 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
   const int lo = s.first, hi = s.n - s.recent;  // whose weights decide
   int need = s.keep - s.first - s.recent;       // how many of them stay
   const bool choose = need > 0;
-  // f(t, four keys) for every group of four tokens some of whose weights decide, 0 for those that do not; a batch of
-  // loads is on its way while the one before it is worked on
+  // f(four keys, whether all of them count) for every group of four tokens some of whose weights decide, 0 for those that
+  // do not; a batch of loads is on its way while the one before it is worked on
   constexpr int kUnroll = 4, kStride = kSelectThreads * 4;
   auto each = [&](auto&& f) {
     f32x4 next[kUnroll];
@@ -168,14 +182,14 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
         const int t = t0 + u * kStride;
         if (t + 3 < lo || t >= hi) continue;
         uint32_t key[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) key[i] = ordered(x[u][i]);
-        if (t < lo || t + 3 >= hi) {
+        ordered4(x[u], key);
+        const bool whole = t >= lo && t + 3 < hi;
+        if (!whole) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (t + i < lo || t + i >= hi) key[i] = 0;
         }
-        f(key);
+        f(key, whole);
       }
     }
   };
@@ -195,7 +209,12 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
         for (int i = tid; i < n_listed; i += kSelectThreads)
           if ((keys[i] & done) == threshold) atomicAdd(&sh.hist[(keys[i] >> shift) & mask], 1);
       } else {
-        each([&](const uint32_t (&key)[4]) {
+        each([&](const uint32_t (&key)[4], bool whole) {
+          if (done == 0 && whole) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) atomicAdd(&sh.hist[key[i] >> 21], 1);
+            return;
+          }
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (key[i] != 0 && (key[i] & done) == threshold) atomicAdd(&sh.hist[(key[i] >> shift) & mask], 1);
@@ -209,10 +228,10 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
       if (!listed && shift > 0 && n_listed <= kCandidates) {
         listed = true;
         const uint32_t upto = ~0u << shift;
-        each([&](const uint32_t (&key)[4]) {
+        each([&](const uint32_t (&key)[4], bool whole) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (key[i] != 0 && (key[i] & upto) == threshold) keys[atomicAdd(&candidates, 1)] = key[i];
+            if ((key[i] & upto) == threshold && (whole || key[i] != 0)) keys[atomicAdd(&candidates, 1)] = key[i];
         });
       }
       __syncthreads();
@@ -237,12 +256,12 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
       const f32x4 x = next[j];
       load(j, t + kAhead * kStride);
       // without a choice (need 0) the threshold is above every key but NaN's, and none of those equal to it stay
-      uint32_t is_above = 0, is_equal = 0;
+      uint32_t key[4], is_above = 0, is_equal = 0;
+      ordered4(x, key);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t key = ordered(x[i]);
-        is_above |= uint32_t(key > threshold) << i;
-        is_equal |= uint32_t(key == threshold) << i;
+        is_above |= uint32_t(key[i] > threshold) << i;
+        is_equal |= uint32_t(key[i] == threshold) << i;
       }
       if (t < lo || t + 3 >= hi) {
         const uint32_t inside = t + 3 < s.n ? 15 : t < s.n ? (1u << (s.n - t)) - 1 : 0;
