@@ -23,11 +23,6 @@ struct EvictParams {
   int batch, n_kv, log2_page, num_pages, max_blocks, max_keep, first, recent, move_chunks;
 };
 
-constexpr int kSelectThreads = 1024;
-constexpr int kSelectWaves = kSelectThreads / 64;
-constexpr int kTableCols = 8192;    // of a block table's row, held in LDS
-constexpr int kCandidates = 24576;  // keys that share the threshold's first digit, held in LDS
-
 // A sequence's sizes, read by every workgroup that works for it.
 struct Sizes {
   int n, keep, first, recent;  // keep < n: something goes
@@ -66,12 +61,6 @@ __device__ __forceinline__ void ordered4(f32x4 x, uint32_t (&key)[4]) {
   }
 }
 
-// The place from the top of a histogram of 2^bits counts where the running sum reaches `need`.
-struct Digit {
-  int hist[2048];
-  int wave_sum[kSelectWaves], chunk_sum[2][kSelectWaves];
-  int bin, above, count;
-};
 // Sums of a wave up to each lane: within rows of 16, then from row to row.
 template <int CTRL, int ROWS>
 __device__ __forceinline__ int add_from(int x) {
@@ -85,39 +74,57 @@ __device__ __forceinline__ int wave_running_sum(int x) {
   x = add_from<0x142, 0xa>(x);         // lane 15 of the row before, into rows 1 and 3
   return add_from<0x143, 0xc>(x);      // lane 31, into rows 2 and 3
 }
-__device__ __forceinline__ void find_digit(Digit& sh, int bits, int need) {
+
+// The place from the top of a histogram of 2^bits counts where the running sum reaches `need`.
+template <int THREADS>
+struct Digit {
+  int hist[2048];
+  int wave_sum[THREADS / 64], chunk_sum[2][THREADS / 64];
+  int bin, above, count;
+};
+template <int THREADS>
+__device__ __forceinline__ void find_digit(Digit<THREADS>& sh, int bits, int need) {
+  constexpr int PER = 2048 / THREADS;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int top = (1 << bits) - 1 - 2 * tid;  // this thread's two bins, from the top
-  const int c0 = top >= 0 ? sh.hist[top] : 0, c1 = top >= 1 ? sh.hist[top - 1] : 0;
-  const int run = wave_running_sum(c0 + c1);
+  const int top = (1 << bits) - 1 - PER * tid;  // this thread's bins, from the top
+  int c[PER], mine = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    c[i] = top >= i ? sh.hist[top - i] : 0;
+    mine += c[i];
+  }
+  const int run = wave_running_sum(mine);
   if (lane == 63) sh.wave_sum[wave] = run;
   __syncthreads();
-  int before = run - c0 - c1;
+  int before = run - mine;
   for (int i = 0; i < wave; ++i) before += sh.wave_sum[i];
-  if (before < need && before + c0 >= need) {
-    sh.bin = top;
-    sh.above = before;
-    sh.count = c0;
-  } else if (before + c0 < need && before + c0 + c1 >= need) {
-    sh.bin = top - 1;
-    sh.above = before + c0;
-    sh.count = c1;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (before < need && before + c[i] >= need) {
+      sh.bin = top - i;
+      sh.above = before;
+      sh.count = c[i];
+    }
+    before += c[i];
   }
   __syncthreads();
 }
 
 // A workgroup per layer, sequence and head.  Reads the weights three times (first digit; the keys of that digit, which
-// then lie in LDS; the kept ones), 16 bytes a lane with the next ones on the way.  What bounds it is a CU's vector ALU:
-// 28 layers' one head of 100 k tokens take 66 us on 28 of 256 CUs, 0.9 us for 4096 weights and pass; 28 layers of
-// 6 sequences of 2800 tokens with 4 heads, which fill the device, 32 us.  More workgroups to a head would need four
-// launches, and the move of K and V behind it is the longer one already (110 and 205 us).
-// TABLE: a sequence's row of the block table lies in LDS, as it does up to 8192 columns.  From global memory the long
-// eviction takes 11 us more, those of six sequences the same.
-template <bool TABLE>
-__global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const EvictParams p) {
-  __shared__ Digit sh;
-  __shared__ int table[TABLE ? kTableCols : 1];
-  __shared__ __align__(16) uint32_t keys[kCandidates];  // later what stays of a chunk, twice
+// then lie in LDS where CANDIDATES hold them; the kept ones), 16 bytes a lane with the next ones on the way.  What bounds
+// it is a CU's vector ALU: 28 layers' one head of 105 k tokens take 66 us on 28 of 256 CUs, 0.9 us for 4096 weights and
+// pass; 28 layers of 6 sequences of 2800 tokens with 4 heads, which fill the device, 19 us.  More workgroups to a head
+// would need four launches, and the move of K and V behind it is the longer one already (110 and 205 us).
+// COLS: a sequence's row of the block table lies in LDS (0: not), as it does up to 8192 columns.  From global memory the
+// long eviction takes 11 us more, those of six sequences the same.
+template <int THREADS, int COLS, int CANDIDATES>
+__global__ __launch_bounds__(THREADS) void evict_select_kernel(const EvictParams p) {
+  constexpr bool TABLE = COLS > 0;
+  constexpr int WAVES = THREADS / 64;
+  __shared__ Digit<THREADS> sh;
+  __shared__ int table[TABLE ? COLS : 1];
+  __shared__ __align__(16) uint32_t keys[CANDIDATES];  // later what stays of a chunk, twice
+  static_assert(CANDIDATES >= 2 * 2 * 4 * THREADS, "two chunks of pairs");
   __shared__ int candidates;
   const int h = blockIdx.x, b = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x;
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -125,12 +132,12 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
   const int64_t head = (int64_t(layer) * p.batch + b) * p.n_kv + h;
   int32_t* kept = p.kept + head * p.max_keep;
   // the second launch's tickets and flags
-  for (int i = tid; i < 2 * (1 + p.move_chunks); i += kSelectThreads) p.marks[head * 2 * (1 + p.move_chunks) + i] = 0;
+  for (int i = tid; i < 2 * (1 + p.move_chunks); i += THREADS) p.marks[head * 2 * (1 + p.move_chunks) + i] = 0;
   const int32_t* bt = p.bt + b * p.bt_stride;
   bool bad = s.bad;
   if (!bad) {
     const int pages = (s.n + (1 << p.log2_page) - 1) >> p.log2_page;
-    for (int c = tid; c < pages; c += kSelectThreads) {
+    for (int c = tid; c < pages; c += THREADS) {
       const int page = bt[c];
       bad |= unsigned(page) >= unsigned(p.num_pages);
       if constexpr (TABLE) table[c] = page;
@@ -139,12 +146,12 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
   if (tid == 0) candidates = 0;
   if (__syncthreads_or(bad)) {
     if (tid == 0) flag_status(p.status, PKV_STATUS_BAD_PAGE);
-    for (int d = tid; d < p.max_keep; d += kSelectThreads) kept[d] = -1;
+    for (int d = tid; d < p.max_keep; d += THREADS) kept[d] = -1;
     return;
   }
-  for (int d = s.keep + tid; d < p.max_keep; d += kSelectThreads) kept[d] = -1;
+  for (int d = s.keep + tid; d < p.max_keep; d += THREADS) kept[d] = -1;
   if (s.keep == s.n) {
-    for (int d = tid; d < s.n; d += kSelectThreads) kept[d] = d;
+    for (int d = tid; d < s.n; d += THREADS) kept[d] = d;
     return;
   }
   float* const w = p.w + layer * p.w_layer + (int64_t(h) << p.log2_page);
@@ -163,7 +170,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
   const bool choose = need > 0;
   // f(four keys, whether all of them count) for every group of four tokens some of whose weights decide, 0 for those that
   // do not; a batch of loads is on its way while the one before it is worked on
-  constexpr int kUnroll = 4, kStride = kSelectThreads * 4;
+  constexpr int kUnroll = 4, kStride = THREADS * 4;
   auto each = [&](auto&& f) {
     f32x4 next[kUnroll];
     auto load = [&](int t0) {
@@ -202,11 +209,11 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
     for (int shift = 32; shift > 0;) {
       const int bits = min(11, shift);
       shift -= bits;
-      for (int i = tid; i < 2048; i += kSelectThreads) sh.hist[i] = 0;
+      for (int i = tid; i < 2048; i += THREADS) sh.hist[i] = 0;
       __syncthreads();
       const uint32_t done = shift + bits == 32 ? 0 : ~0u << (shift + bits), mask = (1u << bits) - 1;
       if (listed) {
-        for (int i = tid; i < n_listed; i += kSelectThreads)
+        for (int i = tid; i < n_listed; i += THREADS)
           if ((keys[i] & done) == threshold) atomicAdd(&sh.hist[(keys[i] >> shift) & mask], 1);
       } else {
         each([&](const uint32_t (&key)[4], bool whole) {
@@ -225,7 +232,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
       threshold |= uint32_t(sh.bin) << shift;
       need -= sh.above;
       n_listed = sh.count;
-      if (!listed && shift > 0 && n_listed <= kCandidates) {
+      if (!listed && shift > 0 && n_listed <= CANDIDATES) {
         listed = true;
         const uint32_t upto = ~0u << shift;
         each([&](const uint32_t (&key)[4], bool whole) {
@@ -275,8 +282,8 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
       int* const sums = sh.chunk_sum[j & 1];  // the other one may still be read
       if (lane == 63) sums[wave] = run;
       __syncthreads();
-      const int waves = wave_running_sum(lane < kSelectWaves ? sums[lane] : 0);  // up to each of them
-      const int all = __builtin_amdgcn_readlane(waves, kSelectWaves - 1);
+      const int waves = wave_running_sum(lane < WAVES ? sums[lane] : 0);  // up to each of them
+      const int all = __builtin_amdgcn_readlane(waves, WAVES - 1);
       const int before = (wave > 0 ? __builtin_amdgcn_readlane(waves, wave - 1) : 0) + run - mine;
       int my_above = above + (before >> 16), my_equal = equal + (before & 0xffff);
       const int start = above + min(equal, need);
@@ -293,7 +300,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
       equal += all & 0xffff;
       const int count = above + min(equal, need) - start;
       __syncthreads();
-      for (int i = tid; i < count; i += kSelectThreads) {
+      for (int i = tid; i < count; i += THREADS) {
         const uint2 it = stage[i];
         const int d = start + i;
         kept[d] = int(it.x);
@@ -302,6 +309,13 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
     }
   }
 }
+
+// Which of them: a workgroup of 1024 threads has its CU to itself (137 KB of LDS), of 256 a CU holds six.  So these take
+// tables of up to 4096 tokens where there are more heads than CUs, and of up to 1024 always.  Evictions as a whole, by
+// 1024 threads and by 256: 4608 heads of 150 tokens 238 and 126 us, of 2000 1083 and 975, 672 heads of 4000 320 and 309,
+// 112 of 4000 62 and 67, 48 of 1000 21 and 20, of 2000 the same.  512 threads are between the two.
+constexpr int kManyTokens = 4096, kFewTokens = 1024, kManyHeads = 256;
+bool short_tables(int64_t tokens, int64_t heads) { return tokens <= (heads > kManyHeads ? kManyTokens : kFewTokens); }
 
 // ---- K and V ----
 // A workgroup takes 32 KB of destination rows of K or of V of one head: it reads their sources, and writes them once the
@@ -450,8 +464,13 @@ extern "C" int pkv_evict(void* k_pool, void* v_pool, int64_t layer_stride, int64
   const hipStream_t s = static_cast<hipStream_t>(stream);
   p.marks = static_cast<int32_t*>(workspace);
   p.move_chunks = move_chunks(max_keep, head_dim);
-  auto* select = max_blocks <= kTableCols ? evict_select_kernel<true> : evict_select_kernel<false>;
-  select<<<dim3(n_kv, batch, layers), kSelectThreads, 0, s>>>(p);
+  const dim3 heads(n_kv, batch, layers);
+  if (short_tables(int64_t(max_blocks) << p.log2_page, int64_t(n_kv) * batch * layers))
+    evict_select_kernel<256, kManyTokens / 16, kManyTokens><<<heads, 256, 0, s>>>(p);
+  else if (max_blocks <= 8192)
+    evict_select_kernel<1024, 8192, 24576><<<heads, 1024, 0, s>>>(p);
+  else
+    evict_select_kernel<1024, 0, 24576><<<heads, 1024, 0, s>>>(p);
   evict_move_kernel<kMoveUnroll><<<dim3(unsigned(wgs), batch, layers), 256, 0, s>>>(p, ilog2(head_dim / 8));
   return check_launch(fn);
 }

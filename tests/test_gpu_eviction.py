@@ -69,6 +69,22 @@ def test_long(gpu, lens, keeps):
     _check(gpu, k, v, w, bt, lens, keeps, 4, 100)
 
 
+@pytest.mark.parametrize("P", [16, 128])
+@pytest.mark.parametrize("L,nk", [(1, 2), (8, 4)])
+def test_short_tables(gpu, L, nk, P):
+    """Up to 1024 tokens, and up to 4096 where the call has more than 256 heads."""
+    for most in (1024, 4096):
+        lens = [0, 1, 63, 64, 700, most, most - 1, most // 2 + 1, most - 130]
+        keeps = [5, 1, 1, 40, 512, most // 2, most - 2, 3, most]
+        k, v, w, bt = _pools(L, lens, P, nk, 64, seed=P + nk)
+        assert bt.shape[1] * P == most
+        w[:, :, 0] = np.round(w[:, :, 0])          # ties in one head of each layer
+        w[:, :, 1, ::7] = -w[:, :, 1, ::7]         # negative ones, zeros of either sign and NaN in another
+        w[:, 0, 1, 3] = np.nan
+        for first, recent in ((4, 64), (0, 0), (3, 100000)):
+            _check(gpu, k, v, w, bt, lens, keeps, first, recent)
+
+
 def test_tables_wider_than_the_kernel_holds(gpu):
     """8200 columns, and a sequence that uses more than 8192 of them."""
     lens, keeps = [131200 - 5, 700], [9000, 300]
