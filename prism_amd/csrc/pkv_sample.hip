@@ -19,7 +19,7 @@
 // The first launch is bound by fp64, an exponential a token: 256 plain fp32 rows of 131072 take 31 us (134 MB, 4.3 TB/s),
 // 32 bf16 rows of 151003 with top-p 13.  The second by the latency of its steps, one workgroup a row: plain rows 13 us,
 // top-p 33 (2 to join the slices' heads, 2 their sums, 5 the classes, 10 to read the row for the cut class, 4 to sort it,
-// 5 to draw), top-k 11 for one row of 32000, 35 for 60 of 128000 with settings of their own.
+// 5 to draw), top-k 11 for one row of 32000, 24 for 60 of 128000 with settings of their own.
 //
 // A decision can fall between tokens 1e-6 of the sum apart, so the weights are taken in fp64 and their sums are fp64 in
 // a fixed order or integers (2^-42 of the largest weight or finer): no order of atomics changes a token.
@@ -1035,16 +1035,40 @@ __device__ __forceinline__ void lists_row(const SampleParams& p, const Rules& ru
       atomicAdd(&hist[bins[j]], 1);
     }
     __syncthreads();
-    int run = hist[tid];
+    // the class that the first `want` end in; `run`: how many up to this thread's
+    int run;
+    auto reach = [&](int want) {
+      run = hist[tid];
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int up = __shfl_up(run, o);
-      if (lane >= o) run += up;
-    }
-    if (lane == 63) lds.left[wave] = uint32_t(run);
+      for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(run, o);
+        if (lane >= o) run += up;
+      }
+      if (lane == 63) lds.left[wave] = uint32_t(run);
+      __syncthreads();
+      for (int i = 0; i < wave; ++i) run += int(lds.left[i]);
+      return __syncthreads_count(run < want);
+    };
+    const int last = reach(rules.top_k);
+    if (tid == last - 1) sh.slice = run;
+    if (tid == last) sh.found_bin = run;
     __syncthreads();
-    for (int i = 0; i < wave; ++i) run += int(lds.left[i]);
-    const int last = __syncthreads_count(run < rules.top_k);  // the class that the first top_k end in
+    if (last > 0 && last < 1023 && sh.found_bin > kRowThreads) {
+      // and of that class by the next ten bits of the distance (60 rows of 128000 with settings of their own: 87 us in
+      // place of 98, as fewer are searched through); classes 0 and 1023 take in what lies behind them, and are not cut
+      const int want = rules.top_k - sh.slice;
+      hist[tid] = 0;
+      __syncthreads();
+      auto finer = [&](uint32_t key) { return int(__float_as_uint(top - value_of(key)) >> 8 & 1023); };
+#pragma unroll
+      for (int j = 0; j < kListMax / kRowThreads; ++j)
+        if (bins[j] == last) atomicAdd(&hist[finer(keys[j])], 1);
+      __syncthreads();
+      const int finer_last = reach(want);
+#pragma unroll
+      for (int j = 0; j < kListMax / kRowThreads; ++j)
+        if (bins[j] == last && finer(keys[j]) > finer_last) bins[j] = 1024;
+    }
 #pragma unroll
     for (int j = 0; j < kListMax / kRowThreads; ++j)
       if (bins[j] <= last && bins[j] < 1024) {
@@ -1376,7 +1400,7 @@ Split split_of(int vocab) {
   const int size = kSlice;
   s.slices = (vocab + 7 + size - 1) / size;
   // a slice lists the first top_k of its own, as far as there is room (with 512 places at most, 115 rows of 6883 tokens
-  // with top-k of up to 1000, more than these places hold, took 84 us, not 65, 17 rows of 1826 67, not 38)
+  // with top-k of up to 1000, more than these places hold, took 84 us, not 52, 17 rows of 1826 67, not 38)
   s.cap = std::min(kSlice, kListMax / s.slices);
   s.part = (std::max<int64_t>(s.cap * sizeof(uint2), kClasses * sizeof(uint64_t)) + 15) / 16 * 16;
   return s;
@@ -1395,7 +1419,7 @@ void launch(const SampleParams& p, const Kinds& k, int rows, hipStream_t stream)
     sample_plain_kernel<T><<<rows, kPlainThreads, 0, stream>>>(p);
   } else {
     sample_slice_kernel<T, 16, false><<<slices, kSliceThreads, 0, stream>>>(p);
-    // two kernels, not one with both: that one would have to spill (60 rows, some of either kind: 35 and 40 us)
+    // two kernels, not one with both: that one would have to spill (60 rows, some of either kind: 24 and 40 us)
     if (k.lists) sample_row_kernel<T, PER, kListRows><<<rows, kRowThreads, 0, stream>>>(p);
     if (k.others) sample_row_kernel<T, PER, kOtherRows><<<rows, kRowThreads, 0, stream>>>(p);
   }

@@ -145,6 +145,18 @@ def test_settings_of_each_row(gpu):
     _draw(x, u, "rows", temperature=0.7, top_k=k, top_p=0.9, min_p=m)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("vocab", [1500, 9000, 40000, 120001])
+def test_hundreds_of_tokens_stay(gpu, dtype, vocab):
+    """top-k whose last token lies in a class of values with many others, equal ones among them."""
+    x, u = _logits(gpu, 6, vocab, dtype, seed=vocab)
+    x[4] = (x[4].float() * 2).round().to(dtype) / 2
+    x[5, 10:] = x[5, 10]
+    for k in (513, 700, 900, 1023, 1024, 1400):
+        _draw(x, u, f"top-k {k} of {vocab}", top_k=k)
+        _draw(x, u, f"top-k {k} of {vocab}, with top-p", top_k=k, top_p=0.97, temperature=1.5)
+
+
 def test_settings_of_rows_that_are_no_number(gpu):
     """NaN: no rule, and the largest logit as a temperature."""
     x, u = _logits(gpu, 4, 9001, torch.float32, seed=17)
