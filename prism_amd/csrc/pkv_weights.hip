@@ -87,8 +87,9 @@ __device__ __forceinline__ float row16_sum(float x) {
 // Decode tokens and verify rows: the reading of K is all there is to do.  The item's query rows lie in LDS, every wave
 // takes a run of 32-key tiles straight into the A operand (16 keys x 32 elements an instruction, a lane's 16 bytes
 // of its key's row), the rows are the columns of the product: C[key, row], a lane has 4 keys of one row.  The next tile
-// is on its way meanwhile.  48 sequences of 2500 keys (4 KV heads of 128, 135 MB): 30 us, 4.5 TB/s; 7 of 50 k keys on one
-// KV head (106 MB): 25 us, 4.2 TB/s.  A copy of this size runs at 4.9.
+// is on its way meanwhile, with its keys' weights so far (read at the end of a tile they cost decode tokens beside chunks
+// 5 us of 75).  48 sequences of 2500 keys (4 KV heads of 128, 135 MB): 30 us
+// where they were read before, 36 from memory, 3.8 TB/s; 7 of 50 k keys on one KV head (106 MB) 25 us, 4.2 TB/s.
 template <int HD>
 struct FewLds {
   u32x4 q[kWeightFewRows * (HD / 8)];
@@ -127,7 +128,8 @@ __device__ __forceinline__ void weigh_few(const WeightParams& p, const WeightIte
   const int in_page = (1 << p.log2_page) - 1;
   const int last_pos = it.pos0 + it.n_tok - 1;
 
-  auto load = [&](int t0, u32x4 (&a)[2][KS]) {
+  // the weights so far come with the keys: lane (quad, i) of the first four of each row of lanes has key quad * 4 + i
+  auto load = [&](int t0, u32x4 (&a)[2][KS], float (&old)[2]) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int page = __builtin_amdgcn_readlane(mine, ((t0 - first) >> 4) + s);
@@ -135,13 +137,18 @@ __device__ __forceinline__ void weigh_few(const WeightParams& p, const WeightIte
       const uint16_t* src = p.k + int64_t(max(page, 0)) * p.page_stride + row * key_st + h * HD + quad * 8;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) a[s][ks] = ld16(src + ks * 32);
+      const int t = t0 + s * 16 + quad * 4 + n16;
+      old[s] = 0.0f;
+      if (n16 < 4 && page >= 0 && t < it.fresh) old[s] = p.w[page * p.w_page + (h << p.log2_page) + (t & in_page)];
     }
   };
   u32x4 a[2][KS];
-  load(first, a);
+  float old[2];
+  load(first, a, old);
   for (int t0 = first; t0 < last; t0 += 32) {
     u32x4 next[2][KS];
-    if (t0 + 32 < last) load(t0 + 32, next);
+    float next_old[2];
+    if (t0 + 32 < last) load(t0 + 32, next, next_old);
     float sum[2][4] = {};
     for (int c0 = 0; c0 < cols; c0 += 16) {
       f32x4 acc[2] = {};
@@ -166,7 +173,6 @@ __device__ __forceinline__ void weigh_few(const WeightParams& p, const WeightIte
     for (int s = 0; s < 2; ++s) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[s][i] = row16_sum(sum[s][i]);
-      // lane (quad, i) of the first four of each row of lanes writes key quad * 4 + i
       const float got = n16 == 0 ? sum[s][0] : n16 == 1 ? sum[s][1] : n16 == 2 ? sum[s][2] : sum[s][3];
       const int group = t0 + s * 16, t = group + quad * 4 + n16;
       const int page = __builtin_amdgcn_readlane(mine, ((t0 - first) >> 4) + s);
@@ -174,14 +180,15 @@ __device__ __forceinline__ void weigh_few(const WeightParams& p, const WeightIte
         if (lane == 0 && group < end && seen(it.pos0, last_pos, p.window, max(group, it.key0), min(group + 16, end)))
           flag_status(p.status, PKV_STATUS_BAD_PAGE);
       } else if (n16 < 4 && t >= it.key0 && t < end) {
-        float* at = p.w + page * p.w_page + (h << p.log2_page) + (t & in_page);
-        *at = t < it.fresh ? *at + got : got;
+        p.w[page * p.w_page + (h << p.log2_page) + (t & in_page)] = t < it.fresh ? old[s] + got : got;
       }
     }
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int s = 0; s < 2; ++s) {
+      old[s] = next_old[s];
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) a[s][ks] = next[s][ks];
+    }
   }
 }
 
