@@ -116,7 +116,7 @@ __device__ __forceinline__ void find_digit(Digit<THREADS>& sh, int bits, int nee
 // pass; 28 layers of 6 sequences of 2800 tokens with 4 heads, which fill the device, 19 us.  More workgroups to a head
 // would need four launches, and the move of K and V behind it is the longer one already (110 and 205 us).
 // COLS: a sequence's row of the block table lies in LDS (0: not), as it does up to 8192 columns.  From global memory the
-// long eviction takes 11 us more, those of six sequences the same.
+// long eviction takes 14 us more, those of six sequences the same.
 template <int THREADS, int COLS, int CANDIDATES>
 __global__ __launch_bounds__(THREADS) void evict_select_kernel(const EvictParams p) {
   constexpr bool TABLE = COLS > 0;
@@ -395,8 +395,8 @@ __global__ __launch_bounds__(256) void evict_move_kernel(const EvictParams p, in
   }
 }
 
-// Rows of 16 bytes a thread: 32 KB a workgroup.  With 16 KB the two evictions above take 256 and 187 us in all, with 32
-// 227 and 172, with 64 231 and 170; a chat's (1700 tokens, 24 layers of two heads of 64) 29, 27 and 30.
+// Rows of 16 bytes a thread: 32 KB a workgroup.  With 16 KB the two evictions above take 240 and 182 us in all, with 32
+// 214 and 167, with 64 222 and 164; a chat's (1700 tokens, 24 layers of two heads of 64) 28, 28 and 30.
 constexpr int kMoveUnroll = 8;
 int move_chunks(int max_keep, int head_dim) {
   const int per = 256 / (head_dim / 8) * kMoveUnroll;

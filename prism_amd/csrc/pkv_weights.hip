@@ -88,8 +88,8 @@ __device__ __forceinline__ float row16_sum(float x) {
 // takes a run of 32-key tiles straight into the A operand (16 keys x 32 elements an instruction, a lane's 16 bytes
 // of its key's row), the rows are the columns of the product: C[key, row], a lane has 4 keys of one row.  The next tile
 // is on its way meanwhile, with its keys' weights so far (read at the end of a tile they cost decode tokens beside chunks
-// 5 us of 75).  48 sequences of 2500 keys (4 KV heads of 128, 135 MB): 30 us
-// where they were read before, 36 from memory, 3.8 TB/s; 7 of 50 k keys on one KV head (106 MB) 25 us, 4.2 TB/s.
+// 5 us of 75).  Memory bounds it: 48 sequences of 2500 keys (4 KV heads of 128, 135 MB) take 37 us, 3.7 TB/s, or 29 where
+// the last-level cache holds some; 7 of 50 k keys on one KV head (106 MB) 25.6, 4.2 TB/s.  A large copy runs at 4.9.
 template <int HD>
 struct FewLds {
   u32x4 q[kWeightFewRows * (HD / 8)];
@@ -198,7 +198,8 @@ __device__ __forceinline__ void weigh_few(const WeightParams& p, const WeightIte
 // row's lse is one value a lane and a key's sum stays in the lane until the end.  Exponentials bound it: of 32 x 32 scores
 // the products take 256 cycles of the matrix pipe, their 16 multiply-adds, exponentials and sums a lane 384 of the vector
 // ALU.  So the products of the second 32 keys are issued between the exponentials of the first, and the other wave of the
-// SIMD fills the rest.  Four prompts of 2600 to 3400 tokens (28 heads of 128 on 4): 184 us, 0.75 PFLOP/s.
+// SIMD fills the rest.  Four prompts of 2600 to 3400 tokens (28 heads of 128 on 4): 175 to 184 us, 0.76 to
+// 0.8 PFLOP/s.
 constexpr int kStepRows = 64;
 template <int HD>
 struct ManyLds {
