@@ -289,6 +289,7 @@ class FlashAttnKVCache:
         fill = [c[2] for c in cow]
         copy_pages(self, self, src, dst, fill)
         copy_key_weights(self, self, src, dst)
+        self._weighed_pages.update(new for old, new, _ in cow if old in self._weighed_pages)
 
     # ------------------------------------------------------------------ block tables
     def block_table_host(self, seq_ids: list[int]) -> tuple[np.ndarray, np.ndarray]:

@@ -181,6 +181,24 @@ def test_sequences_that_share_pages_are_evicted_apart(gpu):
     assert small.seq_pages[1] == small.seq_pages[2] and small.seq_len[1] == 120 and small.pages_free == 1
 
 
+def test_a_copy_of_a_weighed_page_is_one(gpu):
+    """Its weights came along: a prefix on it adds to them, as on the page itself."""
+    kv = prism_amd.FlashAttnKVCache(2, 2, 64, 20, 16, gpu)
+    kv.enable_key_weights()
+    kv.new_sequence(1)
+    kv.prepare_append([1], 64)
+    kv.build_packed_batch([1], 64, 4, weight_rows=None)
+    kv.key_weight_pool.copy_(torch.arange(kv.key_weight_pool.numel(), device=gpu).view(kv.key_weight_pool.shape))
+    kv.update_seqlens([1], 64)
+    kv.fork_sequence(1, 2)
+    old = list(kv.seq_pages[2])
+    kv._copy_on_write([(old[0], new := kv._pop_page(), 16)])
+    assert {new, *old[:4]} <= kv._weighed_pages
+    assert torch.equal(kv.key_weight_pool[:, new], kv.key_weight_pool[:, old[0]])
+    kv.new_sequence(3, prefix_pages=[new, old[1]], prefix_len=32)
+    assert kv._weighed[3] == 32
+
+
 def test_a_captured_decode_step_draws_its_own_tokens(gpu):
     """Attention, weights and the draw in one graph: each replay against the eager calls on the same state."""
     model = Model(gpu, 3)
