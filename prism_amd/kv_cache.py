@@ -269,6 +269,10 @@ class FlashAttnKVCache:
         for sid, n in zip(seq_ids, counts):
             self._plan_growth(sid, self.seq_len[sid] + n, cow)
         self._copy_on_write(cow)
+        if self.key_weight_pool is not None:
+            for sid, n in zip(seq_ids, counts):
+                if n > 0:
+                    self._forget_weights_behind(sid, n)
         return len(cow)
 
     def update_seqlens(self, seq_ids: list[int], num_new_tokens: int | list[int]) -> None:
@@ -289,7 +293,17 @@ class FlashAttnKVCache:
         fill = [c[2] for c in cow]
         copy_pages(self, self, src, dst, fill)
         copy_key_weights(self, self, src, dst)
-        self._weighed_pages.update(new for old, new, _ in cow if old in self._weighed_pages)
+        # (a page copied in part is about to be written to)
+        self._weighed_pages.update(new for old, new, n in cow if n == self.page_size and old in self._weighed_pages)
+
+    def _forget_weights_behind(self, seq_id: int, n: int) -> None:
+        """``n`` keys from seq_len on are to be written: those of before (a prefix taken in part, tokens rolled back,
+        evicted ones) leave their weights in the pool, which are not the new keys'."""
+        start = self.seq_len[seq_id]
+        if self._weighed.get(seq_id, 0) > start:
+            self._weighed[seq_id] = start
+        P = self.page_size
+        self._weighed_pages.difference_update(self.seq_pages[seq_id][start // P:-(-(start + n) // P)])
 
     # ------------------------------------------------------------------ block tables
     def block_table_host(self, seq_ids: list[int]) -> tuple[np.ndarray, np.ndarray]:
@@ -370,6 +384,10 @@ class FlashAttnKVCache:
                 if n > 0:
                     self._weighed[sid] = self.seq_len[sid] + n
                     self._weighed_pages.update(self.seq_pages[sid][had // P:(self.seq_len[sid] + n) // P])
+        elif self.key_weight_pool is not None:
+            for sid, n in zip(seq_ids, counts):
+                if n > 0:
+                    self._forget_weights_behind(sid, n)
         if torch.device(self.device).type == "cuda":
             poll_status(self.device)
         return batch

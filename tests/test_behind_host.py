@@ -340,3 +340,58 @@ def test_a_prefix_whose_keys_were_never_weighed_starts_from_nothing():
         assert weighed_as_prefix(tokens) == (48, want)
         kv.free_sequence(sid)
         pc.evict_lru(3)  # its pages go to the next one
+
+
+def test_keys_written_over_weighed_ones_do_not_count_as_weighed():
+    """Tokens rolled back, or cut away, and written again by steps without weights: the old keys' weights are not theirs."""
+    kv = FlashAttnKVCache(1, 2, 64, 12, 16, "cpu")
+    kv.enable_key_weights()
+
+    def step(sid, n, weights):
+        kv.prepare_append([sid], n)
+        kv.build_packed_batch([sid], n, 4, weight_rows=None if weights else 0)
+        kv.update_seqlens([sid], n)
+
+    def weighed_as_prefix(sid, n):
+        kv.new_sequence(9, prefix_pages=kv.seq_pages[sid][:n // 16], prefix_len=n)
+        got = kv._weighed[9]
+        kv.free_sequence(9)
+        return got
+
+    kv.new_sequence(1)
+    step(1, 48, True)
+    assert (kv._weighed[1], weighed_as_prefix(1, 48)) == (48, 48)
+    kv.seq_len[1] = 20
+    step(1, 28, False)
+    assert (kv._weighed[1], weighed_as_prefix(1, 48)) == (20, 16)
+    kv.seq_len[1] = 20
+    step(1, 28, True)
+    assert (kv._weighed[1], weighed_as_prefix(1, 48)) == (48, 48)
+    # without prepare_append too: the pages are there
+    kv.seq_len[1] = 40
+    kv.build_packed_batch([1], 8, 4)
+    kv.update_seqlens([1], 8)
+    assert (kv._weighed[1], weighed_as_prefix(1, 48)) == (40, 32)
+
+
+def test_a_page_copied_in_part_does_not_count_as_weighed(monkeypatch):
+    """A prefix taken in part: what stands behind it in the copy is written by the sequence that copied it."""
+    monkeypatch.setattr("prism_amd.kv_cache.copy_pages", lambda *a: None)
+    monkeypatch.setattr("prism_amd.kv_cache.copy_key_weights", lambda *a: None)
+    kv = FlashAttnKVCache(1, 2, 64, 12, 16, "cpu")
+    kv.enable_key_weights()
+    kv.new_sequence(1)
+    kv.prepare_append([1], 32)
+    kv.build_packed_batch([1], 32, 4, weight_rows=None)
+    kv.update_seqlens([1], 32)
+    for weights, want in ((0, 16), (None, 32)):
+        kv.new_sequence(2, prefix_pages=kv.seq_pages[1][:2], prefix_len=20)
+        kv.seq_pages[2].pop()  # (its fresh page)
+        assert kv.prepare_append([2], 12) == 1
+        kv.build_packed_batch([2], 12, 4, weight_rows=weights)
+        kv.update_seqlens([2], 12)
+        assert kv.seq_pages[1][1] in kv._weighed_pages
+        kv.new_sequence(3, prefix_pages=kv.seq_pages[2][:2], prefix_len=32)
+        assert kv._weighed[3] == want
+        kv.free_sequence(3)
+        kv.free_sequence(2)
