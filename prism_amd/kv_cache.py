@@ -261,6 +261,8 @@ class FlashAttnKVCache:
         cow: list = []
         self._plan_growth(seq_id, new_total, cow)
         self._copy_on_write(cow)
+        if self.key_weight_pool is not None and new_total > self.seq_len[seq_id]:
+            self._forget_weights_behind(seq_id, new_total - self.seq_len[seq_id])
 
     def prepare_append(self, seq_ids: list[int], num_new_tokens: int | list[int]) -> int:
         """_ensure_capacity for a batch of sequences with one copy-on-write launch; returns #copies."""
@@ -280,7 +282,9 @@ class FlashAttnKVCache:
         counts = [num_new_tokens] * len(seq_ids) if isinstance(num_new_tokens, int) else list(num_new_tokens)
         for sid, n in zip(seq_ids, counts):
             total = self.seq_len[sid] + n
-            self._ensure_capacity(sid, total)
+            cow: list = []
+            self._plan_growth(sid, total, cow)  # (the step's keys are there, and may be weighed)
+            self._copy_on_write(cow)
             self.seq_len[sid] = total
         if torch.device(self.device).type == "cuda":
             poll_status(self.device)

@@ -395,3 +395,18 @@ def test_a_page_copied_in_part_does_not_count_as_weighed(monkeypatch):
         assert kv._weighed[3] == want
         kv.free_sequence(3)
         kv.free_sequence(2)
+
+
+def test_keys_written_without_a_packed_batch_do_not_count_as_weighed():
+    """The growth of one sequence alone says that keys will be written, as prepare_append does."""
+    kv = FlashAttnKVCache(1, 2, 64, 12, 16, "cpu")
+    kv.enable_key_weights()
+    kv.new_sequence(1)
+    kv._ensure_capacity(1, 48)
+    kv.build_packed_batch([1], 48, 4, weight_rows=None)
+    kv.update_seqlens([1], 48)
+    assert kv._weighed[1] == 48 and set(kv.seq_pages[1][:3]) <= kv._weighed_pages
+    kv.seq_len[1] = 20
+    kv._ensure_capacity(1, 48)
+    kv.update_seqlens([1], 28)
+    assert kv._weighed[1] == 20 and kv._weighed_pages == {kv.seq_pages[1][0]}
