@@ -509,6 +509,8 @@ class FlashAttnKVCache:
         if n:
             copy_pages(self, target_kv, src_pages[:n], target_kv.seq_pages[dst_seq_id][:n], None, staged)
             copy_key_weights(self, target_kv, src_pages[:n], target_kv.seq_pages[dst_seq_id][:n])
+            target_kv._weighed_pages.update(new for old, new in zip(src_pages[:n], target_kv.seq_pages[dst_seq_id])
+                                            if old in self._weighed_pages)
         self._copy_eviction_state(seq_id, target_kv, dst_seq_id)
         if target_kv.key_weight_pool is None or self.key_weight_pool is None:
             target_kv._weighed[dst_seq_id] = 0

@@ -410,3 +410,22 @@ def test_keys_written_without_a_packed_batch_do_not_count_as_weighed():
     kv._ensure_capacity(1, 48)
     kv.update_seqlens([1], 28)
     assert kv._weighed[1] == 20 and kv._weighed_pages == {kv.seq_pages[1][0]}
+
+
+@pytest.mark.parametrize("weighing", [True, False])
+def test_a_weighed_page_of_a_transferred_sequence_is_one(monkeypatch, weighing):
+    """A prefix on it adds to its weights, and does not start them anew under the sequence that has them."""
+    monkeypatch.setattr("prism_amd.kv_cache.copy_pages", lambda *a: None)
+    monkeypatch.setattr("prism_amd.kv_cache.copy_key_weights", lambda *a: None)
+    kv, other = (FlashAttnKVCache(1, 2, 64, 12, 16, "cpu") for _ in range(2))
+    kv.enable_key_weights()
+    if weighing:
+        other.enable_key_weights()
+    kv.new_sequence(1)
+    kv.prepare_append([1], 40)
+    kv.build_packed_batch([1], 40, 4, weight_rows=None)
+    kv.update_seqlens([1], 40)
+    assert kv.transfer_sequence(1, other, 7) == 3
+    other.enable_key_weights()
+    other.new_sequence(8, prefix_pages=other.seq_pages[7][:2], prefix_len=32)
+    assert (other._weighed[7], other._weighed[8]) == ((40, 32) if weighing else (0, 0))
