@@ -509,7 +509,7 @@ struct RowShared {
   double wave_d[kRowWaves];
   uint64_t found_before, found_value;
   int found_bin;
-  int n;
+  int n, thinned;  // tokens listed, and those of them that thinning leaves
   double target;
   int slice, token, first;
   uint32_t cut_key, cut_token;
@@ -963,7 +963,7 @@ __device__ __forceinline__ void lists_row(const SampleParams& p, const Rules& ru
     lds.left[wave] = left;
     lds.valid[wave] = valid;
   }
-  if (tid == 0) sh.n = 0;
+  if (tid == 0) sh.n = sh.thinned = 0;
   __syncthreads();
   valid = 0;
 #pragma unroll
@@ -1017,10 +1017,10 @@ __device__ __forceinline__ void lists_row(const SampleParams& p, const Rules& ru
   int n = min(sh.n, kListMax);
   const bool enough = left == 0 || n >= rules.top_k;
   if (n > kRowThreads && enough && rules.top_k < kRowThreads) {
-    // first down to those in the classes of distance that the first top_k reach
+    // first down to those in the classes of distance that the first top_k reach.  They have a count of their own: a wave
+    // may not have read sh.n yet, which decides whether it comes here at all.
     int* const hist = reinterpret_cast<int*>(sh.hist);
     hist[tid] = 0;
-    if (tid == 0) sh.n = 0;
     __syncthreads();
     uint32_t keys[kListMax / kRowThreads], tokens[kListMax / kRowThreads];
     int bins[kListMax / kRowThreads];
@@ -1072,12 +1072,12 @@ __device__ __forceinline__ void lists_row(const SampleParams& p, const Rules& ru
 #pragma unroll
     for (int j = 0; j < kListMax / kRowThreads; ++j)
       if (bins[j] <= last && bins[j] < 1024) {
-        const int at = atomicAdd(&sh.n, 1);
+        const int at = atomicAdd(&sh.thinned, 1);
         lds.list.keys[at] = keys[j];
         lds.list.tokens[at] = tokens[j];
       }
     __syncthreads();
-    n = sh.n;
+    n = sh.thinned;
   }
   if (n <= kRowThreads && enough) {
     // sorted, a token a thread: top-k is the first so many, top-p and min-p a prefix of them

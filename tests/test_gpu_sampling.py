@@ -157,6 +157,20 @@ def test_hundreds_of_tokens_stay(gpu, dtype, vocab):
         _draw(x, u, f"top-k {k} of {vocab}, with top-p", top_k=k, top_p=0.97, temperature=1.5)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("vocab,top_k", [(40009, 300), (60000, 700), (60000, 1000), (128000, 600)])
+def test_long_lists_of_many_rows_are_thinned(gpu, dtype, vocab, top_k):
+    """Rows whose lists hold more than 1024 tokens together, as many at a time as the device runs: every row goes the
+    same way through the lists, whichever of its waves comes late."""
+    x, u = _logits(gpu, 16, vocab, dtype, seed=vocab + top_k)
+    got = _draw(x, u, f"thinned {top_k} of {vocab}", top_k=top_k, temperature=1.3)
+    logs = prism_amd.sample_tokens(x, u, top_k=top_k, temperature=1.3, return_logprobs=True)[1]
+    wide, many = x.repeat(32, 1), u.repeat(32)
+    for _ in range(3):
+        more, more_logs = prism_amd.sample_tokens(wide, many, top_k=top_k, temperature=1.3, return_logprobs=True)
+        assert torch.equal(more, got.repeat(32)) and torch.equal(more_logs, logs.repeat(32))
+
+
 def test_settings_of_rows_that_are_no_number(gpu):
     """NaN: no rule, and the largest logit as a temperature."""
     x, u = _logits(gpu, 4, 9001, torch.float32, seed=17)
