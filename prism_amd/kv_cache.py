@@ -481,6 +481,7 @@ class FlashAttnKVCache:
             del pages[-(-keep // P):]
             self.seq_len[sid] = keep
             self._weighed[sid] = min(self._weighed[sid], n) - (n - keep)
+            self._weighed_pages.difference_update(pages[self._weighed[sid] // P:])  # (keys of before the cut filled them)
             self.seq_evicted[sid] = self.seq_evicted.get(sid, 0) + n - keep
         poll_status(self.device)
         return len(self.free_pages) - free_before

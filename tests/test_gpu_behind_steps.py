@@ -286,3 +286,19 @@ def test_refusals(gpu):
                   ((k, v, wp, bt, i, i, 3), dict(status=i.float()))]:
         with pytest.raises(RuntimeError):
             e(*a, **kw)
+
+
+def test_pages_of_a_cut_sequence_with_keys_never_weighed_do_not_count_as_weighed(gpu):
+    """evict moves the last keys, which need no weights, into pages that were full of weighed ones."""
+    kv = prism_amd.FlashAttnKVCache(1, NK, HD, 20, 16, gpu)
+    kv.enable_key_weights()
+    kv.new_sequence(1)
+    for n, weights in ((64, None), (40, 0)):
+        kv.prepare_append([1], n)
+        kv.build_packed_batch([1], n, NH, weight_rows=weights)
+        kv.update_seqlens([1], n)
+    kv.evict([1], 60, recent=40)
+    assert kv.seq_len[1] == 60 and kv._weighed[1] == 20
+    assert kv._weighed_pages & set(kv.seq_pages[1]) == {kv.seq_pages[1][0]}
+    kv.new_sequence(2, prefix_pages=kv.seq_pages[1][:3], prefix_len=48)
+    assert kv._weighed[2] == 16
