@@ -87,12 +87,14 @@ class FlashAttnKVCache:
         self._holders: dict[int, int] = {}     # page -> number of live sequences listing it
         # tokens that evict() took out of a sequence: its positions go on behind them (sequences without are absent)
         self.seq_evicted: dict[int, int] = {}
-        # per layer, the attention weight of every cached key, fp32 [max_pages, n_kv, page_size] (enable_key_weights);
-        # of a sequence's keys, the first _weighed[seq] have theirs
+        # per layer, the attention weight of every cached key, fp32 [max_pages, n_kv, page_size] (enable_key_weights).
+        # Weights lie in pages, which sequences share: of a page's keys, the first _page_weights[page] have theirs (pages
+        # without are absent).  Of a sequence's keys, the first _weighed[seq] are known to have theirs; others that share
+        # its pages may have weighed more since (_weighed_keys).
         self.key_weight_pool: torch.Tensor | None = None
         self.key_weights: list[torch.Tensor] = []
         self._weighed: dict[int, int] = {}
-        self._weighed_pages: set[int] = set()  # pages all of whose keys have theirs: as a prefix, they count as weighed
+        self._page_weights: dict[int, int] = {}
         self.prefix_cache = None               # set by PrefixCache(kv)
         self._bases: torch.Tensor | None = None
         self.null_page: int | None = None      # reserve_null_page()
@@ -119,7 +121,7 @@ class FlashAttnKVCache:
         if not self.free_pages:
             raise KVCacheOutOfPages(f"Out of KV cache pages ({self.max_pages} total)")
         page = self.free_pages.pop()
-        self._weighed_pages.discard(page)
+        self._page_weights.pop(page, None)
         return page
 
     def _all_pages_free(self) -> list[int]:
@@ -174,7 +176,7 @@ class FlashAttnKVCache:
         self.seq_pages[seq_id] = pages
         self.seq_len[seq_id] = prefix_len if prefix_pages else 0
         self.seq_owner[seq_id] = owner
-        first_without = next((i for i, p in enumerate(pages) if p not in self._weighed_pages), len(pages))
+        first_without = next((i for i, p in enumerate(pages) if self._page_weights.get(p) != self.page_size), len(pages))
         self._weighed[seq_id] = min(self.seq_len[seq_id], first_without * self.page_size)
 
     def fork_sequence(self, src_seq_id: int, dst_seq_id: int, owner: str | None = None) -> None:
@@ -297,17 +299,39 @@ class FlashAttnKVCache:
         fill = [c[2] for c in cow]
         copy_pages(self, self, src, dst, fill)
         copy_key_weights(self, self, src, dst)
-        # (a page copied in part is about to be written to)
-        self._weighed_pages.update(new for old, new, n in cow if n == self.page_size and old in self._weighed_pages)
+        for old, new, n in cow:  # (a page copied in part is about to be written to)
+            self._set_page_weights(new, min(n, self._page_weights.get(old, 0)))
+
+    # ------------------------------------------------------------------ which keys have weights
+    @property
+    def _weighed_pages(self) -> set[int]:
+        """Pages all of whose keys have their weights."""
+        return {page for page, n in self._page_weights.items() if n == self.page_size}
+
+    def _set_page_weights(self, page: int, n: int) -> None:
+        if n > 0:
+            self._page_weights[page] = min(n, self.page_size)
+        else:
+            self._page_weights.pop(page, None)
+
+    def _weighed_keys(self, seq_id: int) -> int:
+        """How many of the sequence's keys, from the first on, have their weights."""
+        had, P = self._weighed.get(seq_id, 0), self.page_size
+        for i, page in enumerate(self.seq_pages[seq_id][had // P:], had // P):
+            n = self._page_weights.get(page, 0)
+            had = max(had, i * P + n)
+            if n < P:
+                break
+        return min(had, self.seq_len[seq_id])
 
     def _forget_weights_behind(self, seq_id: int, n: int) -> None:
         """``n`` keys from seq_len on are to be written: those of before (a prefix taken in part, tokens rolled back,
         evicted ones) leave their weights in the pool, which are not the new keys'."""
-        start = self.seq_len[seq_id]
+        start, P = self.seq_len[seq_id], self.page_size
         if self._weighed.get(seq_id, 0) > start:
             self._weighed[seq_id] = start
-        P = self.page_size
-        self._weighed_pages.difference_update(self.seq_pages[seq_id][start // P:-(-(start + n) // P)])
+        for i, page in enumerate(self.seq_pages[seq_id][start // P:-(-(start + n) // P)], start // P):
+            self._set_page_weights(page, min(start - i * P, self._page_weights.get(page, 0)))
 
     # ------------------------------------------------------------------ block tables
     def block_table_host(self, seq_ids: list[int]) -> tuple[np.ndarray, np.ndarray]:
@@ -359,7 +383,9 @@ class FlashAttnKVCache:
         (prepare_append first: the pages must be there and not shared).  ``windows`` lists the attention windows
         that the model's layers use (None: every key).  With ``weight_rows`` (None: every new token's attention counts;
         n: that of each sequence's last n) the step runs packed_key_weights on ``key_weights`` in every layer, once
-        (enable_key_weights); keys that steps without it appended start from nothing then."""
+        (enable_key_weights); keys that steps without it appended start from nothing then, unless a sequence that
+        shares their pages has weighed them since.  Steps with weights run in the order that their batches are built
+        in."""
         if weight_rows != 0 and self.key_weight_pool is None:
             raise RuntimeError("the cache keeps no key weights: enable_key_weights first")
         counts = [num_new_tokens] * len(seq_ids) if isinstance(num_new_tokens, int) else list(num_new_tokens)
@@ -378,7 +404,7 @@ class FlashAttnKVCache:
             bt, sl = self.block_table_host(seq_ids)
         else:
             bt, sl = np.zeros((0, 1), np.int32), np.zeros(0, np.int32)
-        weighed = [min(self._weighed.get(sid, 0), self.seq_len[sid]) for sid in seq_ids] if weight_rows != 0 else None
+        weighed = [self._weighed_keys(sid) for sid in seq_ids] if weight_rows != 0 else None
         evicted = [self.seq_evicted.get(sid, 0) for sid in seq_ids] if self.seq_evicted else None
         batch = PackedBatch(counts, sl, bt, page_size=P, num_pages=self.max_pages, n_heads=n_heads,
                             n_kv=self.num_kv_heads, head_dim=self.head_dim, windows=windows, weight_rows=weight_rows,
@@ -386,8 +412,9 @@ class FlashAttnKVCache:
         if weight_rows != 0:
             for sid, n, had in zip(seq_ids, counts, weighed):
                 if n > 0:
-                    self._weighed[sid] = self.seq_len[sid] + n
-                    self._weighed_pages.update(self.seq_pages[sid][had // P:(self.seq_len[sid] + n) // P])
+                    total = self._weighed[sid] = self.seq_len[sid] + n
+                    for i, page in enumerate(self.seq_pages[sid][had // P:-(-total // P)], had // P):
+                        self._set_page_weights(page, total - i * P)
         elif self.key_weight_pool is not None:
             for sid, n in zip(seq_ids, counts):
                 if n > 0:
@@ -405,7 +432,7 @@ class FlashAttnKVCache:
             self.key_weight_pool = torch.zeros(shape, dtype=torch.float32, device=self.device)
             self.key_weights = list(self.key_weight_pool.unbind(0))
             self._weighed = dict.fromkeys(self.seq_pages, 0)
-            self._weighed_pages.clear()
+            self._page_weights.clear()
         return self.key_weights
 
     def next_positions(self, seq_ids: list[int]) -> list[int]:
@@ -437,11 +464,12 @@ class FlashAttnKVCache:
             raise ValueError("budgets must be at least 1 token, first and recent not negative")
         P = self.page_size
         todo = [(sid, self.seq_len[sid], b) for sid, b in zip(seq_ids, budgets) if self.seq_len[sid] > b]
+        weighed = {sid: self._weighed_keys(sid) for sid, _, _ in todo}
         for sid, n, keep in todo:
             tail = min(recent, keep - min(first, keep))
-            if min(self._weighed.get(sid, 0), n) < n - tail:
-                raise RuntimeError(f"sequence {sid}: only {min(self._weighed.get(sid, 0), n)} of the {n - tail} tokens before "
-                                   "the recent ones have been weighed (build_packed_batch with weight_rows)")
+            if weighed[sid] < n - tail:
+                raise RuntimeError(f"sequence {sid}: only {weighed[sid]} of the {n - tail} tokens before the recent ones "
+                                   "have been weighed (build_packed_batch with weight_rows)")
         if not todo:
             return 0
         free_before = len(self.free_pages)
@@ -480,8 +508,9 @@ class FlashAttnKVCache:
                 self._release(page)
             del pages[-(-keep // P):]
             self.seq_len[sid] = keep
-            self._weighed[sid] = min(self._weighed[sid], n) - (n - keep)
-            self._weighed_pages.difference_update(pages[self._weighed[sid] // P:])  # (keys of before the cut filled them)
+            self._weighed[sid] = weighed[sid] - (n - keep)
+            for i, page in enumerate(pages):  # (filled with keys of before the cut)
+                self._set_page_weights(page, self._weighed[sid] - i * P)
             self.seq_evicted[sid] = self.seq_evicted.get(sid, 0) + n - keep
         poll_status(self.device)
         return len(self.free_pages) - free_before
@@ -510,11 +539,12 @@ class FlashAttnKVCache:
         if n:
             copy_pages(self, target_kv, src_pages[:n], target_kv.seq_pages[dst_seq_id][:n], None, staged)
             copy_key_weights(self, target_kv, src_pages[:n], target_kv.seq_pages[dst_seq_id][:n])
-            target_kv._weighed_pages.update(new for old, new in zip(src_pages[:n], target_kv.seq_pages[dst_seq_id])
-                                            if old in self._weighed_pages)
         self._copy_eviction_state(seq_id, target_kv, dst_seq_id)
         if target_kv.key_weight_pool is None or self.key_weight_pool is None:
             target_kv._weighed[dst_seq_id] = 0
+        else:
+            for old, new in zip(src_pages[:n], target_kv.seq_pages[dst_seq_id]):
+                target_kv._set_page_weights(new, self._page_weights.get(old, 0))
         return n
 
     def live_pages(self) -> list[int]:
@@ -557,7 +587,7 @@ class FlashAttnKVCache:
             if target.key_weight_pool is None or self.key_weight_pool is None:
                 target._weighed[sid] = 0
         if target.key_weight_pool is not None and self.key_weight_pool is not None:
-            target._weighed_pages.update(remap[p] for p in live if p in self._weighed_pages)
+            target._page_weights.update({remap[p]: self._page_weights[p] for p in live if p in self._page_weights})
         pc = self.prefix_cache
         if pc is not None:
             pc.remap_pages(remap)
@@ -570,7 +600,7 @@ class FlashAttnKVCache:
         self.seq_owner.clear()
         self.seq_evicted.clear()
         self._weighed.clear()
-        self._weighed_pages.clear()
+        self._page_weights.clear()
         self._holders.clear()
         return remap
 
@@ -592,7 +622,7 @@ class FlashAttnKVCache:
         self.free_pages = fresh.free_pages
         self.seq_pages, self.seq_len, self.seq_owner = fresh.seq_pages, fresh.seq_len, fresh.seq_owner
         self._holders = fresh._holders
-        self.seq_evicted, self._weighed, self._weighed_pages = fresh.seq_evicted, fresh._weighed, fresh._weighed_pages
+        self.seq_evicted, self._weighed, self._page_weights = fresh.seq_evicted, fresh._weighed, fresh._page_weights
         self.key_weight_pool = fresh.key_weight_pool
         self.key_weights[:] = fresh.key_weights
         if fresh.prefix_cache is not None:

@@ -429,3 +429,98 @@ def test_a_weighed_page_of_a_transferred_sequence_is_one(monkeypatch, weighing):
     other.enable_key_weights()
     other.new_sequence(8, prefix_pages=other.seq_pages[7][:2], prefix_len=32)
     assert (other._weighed[7], other._weighed[8]) == ((40, 32) if weighing else (0, 0))
+
+
+def _first_keys_without_weights(batch):
+    """Per sequence, the key from which on the batch's packed_key_weights starts from nothing."""
+    _, at, few, many, *_ = batch._weight_plans[None]
+    items = batch._buf[(at - batch._buf.data_ptr()) // 4:][:12 * (few + many)].view(-1, 12)
+    return {int(i[3]): int(i[6]) for i in items}
+
+
+def _weighing_step(kv, sid, n):
+    kv.prepare_append([sid], n)
+    batch = kv.build_packed_batch([sid], n, 4, weight_rows=None)
+    kv.update_seqlens([sid], n)
+    return _first_keys_without_weights(batch)[0]
+
+
+def _plain_step(kv, sid, n):
+    kv.prepare_append([sid], n)
+    kv.build_packed_batch([sid], n, 4)
+    kv.update_seqlens([sid], n)
+
+
+def test_weights_on_shared_pages_are_added_to(monkeypatch):
+    """Sequences on pages that nobody weighed yet: the first one's step starts them, the second one's adds to them."""
+    monkeypatch.setattr("prism_amd.kv_cache.copy_pages", lambda *a: None)
+    monkeypatch.setattr("prism_amd.kv_cache.copy_key_weights", lambda *a: None)
+    for n in (48, 41):  # whole pages, and a last one that each copies for itself
+        kv = FlashAttnKVCache(1, 2, 64, 20, 16, "cpu")
+        kv.enable_key_weights()
+        kv.new_sequence(1)
+        _plain_step(kv, 1, n)
+        kv.fork_sequence(1, 2)
+        kv.fork_sequence(1, 3)
+        assert _weighing_step(kv, 1, 1) == 0
+        # the whole pages are weighed; what lies on a page of its own is not
+        assert _weighing_step(kv, 2, 1) == n // 16 * 16
+        assert _weighing_step(kv, 2, 30) == n + 1
+        assert _weighing_step(kv, 1, 1) == n + 1
+        assert _weighing_step(kv, 3, 20) == n // 16 * 16
+
+
+def test_weights_on_a_prefix_page_weighed_in_part_are_added_to():
+    """A full page whose first keys alone were weighed, then taken as a prefix: what was weighed stays."""
+    kv = FlashAttnKVCache(1, 2, 64, 20, 16, "cpu")
+    kv.enable_key_weights()
+    pc = prism_amd.PrefixCache(kv, 16)
+    kv.new_sequence(1)
+    assert _weighing_step(kv, 1, 40) == 0
+    _plain_step(kv, 1, 8)
+    pc.store(list(range(48)), kv.seq_pages[1], "m")
+    pages, n = pc.lookup(list(range(48)), "m")
+    kv.new_sequence(2, prefix_pages=pages, prefix_len=n)
+    assert _weighing_step(kv, 2, 5) == 40
+    assert _weighing_step(kv, 1, 1) == 48
+    kv.free_sequence(1)
+    kv.new_sequence(3, prefix_pages=pages, prefix_len=n)
+    assert _weighing_step(kv, 3, 5) == 48
+    # stored by steps without weights, weighed by the first that takes it
+    kv.new_sequence(4)
+    _plain_step(kv, 4, 32)
+    pc.store(list(range(100, 132)), kv.seq_pages[4], "m")
+    kv.free_sequence(4)
+    pages, n = pc.lookup(list(range(100, 132)), "m")
+    for sid, start in ((5, 0), (6, 32)):
+        kv.new_sequence(sid, prefix_pages=pages, prefix_len=n)
+        assert _weighing_step(kv, sid, 3) == start
+
+
+def test_weights_of_pages_travel_with_them(monkeypatch):
+    """Copies, transfers and migrations keep what a page weighed in part has; a page given back forgets it."""
+    monkeypatch.setattr("prism_amd.kv_cache.copy_pages", lambda *a: None)
+    monkeypatch.setattr("prism_amd.kv_cache.copy_key_weights", lambda *a: None)
+    kv, other = (FlashAttnKVCache(1, 2, 64, 12, 16, "cpu") for _ in range(2))
+    kv.enable_key_weights()
+    other.enable_key_weights()
+    kv.new_sequence(1)
+    _weighing_step(kv, 1, 40)
+    _plain_step(kv, 1, 8)
+    kv.transfer_sequence(1, other, 1)
+    other.new_sequence(2, prefix_pages=other.seq_pages[1][:3], prefix_len=48)
+    assert _weighing_step(other, 2, 1) == 40
+    target = FlashAttnKVCache(1, 2, 64, 12, 16, "cpu")
+    target.enable_key_weights()
+    kv.migrate_to(target)
+    target.new_sequence(2, prefix_pages=target.seq_pages[1][:3], prefix_len=48)
+    # rolled back into a page that another sequence lists too: its copy has the first keys' weights
+    target.seq_len[1] = 37
+    assert _weighing_step(target, 1, 1) == 37
+    assert _weighing_step(target, 2, 1) == 40
+    pages = list(target.seq_pages[2])
+    target.free_all()
+    target.new_sequence(3)
+    _plain_step(target, 3, 180)
+    assert set(pages) <= set(target.seq_pages[3])
+    assert _weighing_step(target, 3, 1) == 0

@@ -302,3 +302,23 @@ def test_pages_of_a_cut_sequence_with_keys_never_weighed_do_not_count_as_weighed
     assert kv._weighed_pages & set(kv.seq_pages[1]) == {kv.seq_pages[1][0]}
     kv.new_sequence(2, prefix_pages=kv.seq_pages[1][:3], prefix_len=48)
     assert kv._weighed[2] == 16
+
+
+def test_sequences_that_share_pages_weigh_them_in_turn(gpu):
+    """Pages that steps without weights filled: both sequences' attention is in their sums, and decides the eviction."""
+    model = Model(gpu, 4)
+    kv = prism_amd.FlashAttnKVCache(L, NK, HD, 30, 16, gpu)
+    kv.enable_key_weights()
+    kv.new_sequence(1)
+    kv.prepare_append([1], 96)
+    model.step(kv, kv.build_packed_batch([1], 96, NH), torch.arange(96, device=gpu), weigh=False)
+    kv.update_seqlens([1], 96)
+    kv.fork_sequence(1, 2)
+    shared = kv.seq_pages[1][:6]
+    # (each step's weights against fp64: the old ones, zero before the first, and what the step adds)
+    _serve_step(model, kv, [1], torch.arange(7, 20, device=gpu), [13])
+    first = kv.key_weight_pool[:, shared].clone()
+    _serve_step(model, kv, [2], torch.arange(40, 45, device=gpu), [5])
+    assert (kv.key_weight_pool[:, shared] > first).all()
+    _serve_step(model, kv, [1], torch.tensor([5], device=gpu), [1])
+    _evict(kv, [1], 50, recent=16)
