@@ -95,6 +95,8 @@ class FlashAttnKVCache:
         self.key_weights: list[torch.Tensor] = []
         self._weighed: dict[int, int] = {}
         self._page_weights: dict[int, int] = {}
+        # of a sequence whose step with weights is laid out: the first and behind the last of its new keys
+        self._being_weighed: dict[int, tuple[int, int]] = {}
         self.prefix_cache = None               # set by PrefixCache(kv)
         self._bases: torch.Tensor | None = None
         self.null_page: int | None = None      # reserve_null_page()
@@ -207,6 +209,7 @@ class FlashAttnKVCache:
             self.seq_owner.pop(seq_id, None)
             self.seq_evicted.pop(seq_id, None)
             self._weighed.pop(seq_id, None)
+            self._being_weighed.pop(seq_id, None)
 
     def free_model_sequences(self, model_name: str) -> None:
         for sid in [s for s, o in self.seq_owner.items() if o == model_name]:
@@ -219,6 +222,7 @@ class FlashAttnKVCache:
         self.seq_owner.clear()
         self.seq_evicted.clear()
         self._weighed.clear()
+        self._being_weighed.clear()
         self._holders.clear()
         if self.prefix_cache is not None:
             self.prefix_cache.clear()
@@ -285,8 +289,14 @@ class FlashAttnKVCache:
         for sid, n in zip(seq_ids, counts):
             total = self.seq_len[sid] + n
             cow: list = []
-            self._plan_growth(sid, total, cow)  # (the step's keys are there, and may be weighed)
+            self._plan_growth(sid, total, cow)
             self._copy_on_write(cow)
+            if n > 0 and self.key_weight_pool is not None:
+                # the step's keys are there: with weights where a batch was laid out for them, else written over others
+                start, end = self._being_weighed.get(sid, (-1, -1))
+                if start != self.seq_len[sid] or end < total:
+                    self._forget_weights_behind(sid, n)
+                self._being_weighed.pop(sid, None)
             self.seq_len[sid] = total
         if torch.device(self.device).type == "cuda":
             poll_status(self.device)
@@ -328,6 +338,7 @@ class FlashAttnKVCache:
         """``n`` keys from seq_len on are to be written: those of before (a prefix taken in part, tokens rolled back,
         evicted ones) leave their weights in the pool, which are not the new keys'."""
         start, P = self.seq_len[seq_id], self.page_size
+        self._being_weighed.pop(seq_id, None)
         if self._weighed.get(seq_id, 0) > start:
             self._weighed[seq_id] = start
         for i, page in enumerate(self.seq_pages[seq_id][start // P:-(-(start + n) // P)], start // P):
@@ -413,6 +424,7 @@ class FlashAttnKVCache:
             for sid, n, had in zip(seq_ids, counts, weighed):
                 if n > 0:
                     total = self._weighed[sid] = self.seq_len[sid] + n
+                    self._being_weighed[sid] = (self.seq_len[sid], total)
                     for i, page in enumerate(self.seq_pages[sid][had // P:-(-total // P)], had // P):
                         self._set_page_weights(page, total - i * P)
         elif self.key_weight_pool is not None:
@@ -588,6 +600,7 @@ class FlashAttnKVCache:
                 target._weighed[sid] = 0
         if target.key_weight_pool is not None and self.key_weight_pool is not None:
             target._page_weights.update({remap[p]: self._page_weights[p] for p in live if p in self._page_weights})
+            target._being_weighed.update(self._being_weighed)
         pc = self.prefix_cache
         if pc is not None:
             pc.remap_pages(remap)
@@ -600,6 +613,7 @@ class FlashAttnKVCache:
         self.seq_owner.clear()
         self.seq_evicted.clear()
         self._weighed.clear()
+        self._being_weighed.clear()
         self._page_weights.clear()
         self._holders.clear()
         return remap
@@ -623,6 +637,7 @@ class FlashAttnKVCache:
         self.seq_pages, self.seq_len, self.seq_owner = fresh.seq_pages, fresh.seq_len, fresh.seq_owner
         self._holders = fresh._holders
         self.seq_evicted, self._weighed, self._page_weights = fresh.seq_evicted, fresh._weighed, fresh._page_weights
+        self._being_weighed = fresh._being_weighed
         self.key_weight_pool = fresh.key_weight_pool
         self.key_weights[:] = fresh.key_weights
         if fresh.prefix_cache is not None:

@@ -524,3 +524,52 @@ def test_weights_of_pages_travel_with_them(monkeypatch):
     _plain_step(target, 3, 180)
     assert set(pages) <= set(target.seq_pages[3])
     assert _weighing_step(target, 3, 1) == 0
+
+
+def test_keys_counted_by_update_seqlens_alone_do_not_count_as_weighed(monkeypatch):
+    """Tokens rolled back and written again by a step that says so to update_seqlens alone."""
+    monkeypatch.setattr("prism_amd.kv_cache.copy_pages", lambda *a: None)
+    monkeypatch.setattr("prism_amd.kv_cache.copy_key_weights", lambda *a: None)
+    kv = FlashAttnKVCache(1, 2, 64, 12, 16, "cpu")
+    kv.enable_key_weights()
+    kv.new_sequence(1)
+    assert _weighing_step(kv, 1, 48) == 0 and kv._weighed[1] == 48
+    kv.seq_len[1] = 20
+    kv.update_seqlens([1], 28)
+    assert kv._weighed[1] == 20 and kv._weighed_pages == {kv.seq_pages[1][0]}
+    assert _weighing_step(kv, 1, 1) == 20
+    # a step with weights of which the first tokens alone are taken (the others were drafts), then one without
+    kv.prepare_append([1], 6)
+    kv.build_packed_batch([1], 6, 4, weight_rows=None)
+    kv.update_seqlens([1], 4)
+    assert kv._weighed_keys(1) == kv.seq_len[1] == 53
+    kv.update_seqlens([1], 2)
+    assert kv._weighed_keys(1) == 53 and kv.seq_len[1] == 55
+    # a batch that was laid out, then another in its place: the last one counts
+    for rows, want in ((0, 55), (None, 61)):
+        kv.prepare_append([1], 3)
+        kv.build_packed_batch([1], 3, 4, weight_rows=None)
+        kv.build_packed_batch([1], 3, 4, weight_rows=rows)
+        kv.update_seqlens([1], 3)
+        assert kv._weighed_keys(1) == want
+    # a batch that was laid out and given up, the tokens before it rolled back
+    kv.prepare_append([1], 1)
+    kv.build_packed_batch([1], 1, 4, weight_rows=None)
+    kv.seq_len[1] = 57
+    kv.update_seqlens([1], 2)
+    assert kv._weighed_keys(1) == 57
+    # the pages moved in between
+    kv.prepare_append([1], 2)
+    kv.build_packed_batch([1], 2, 4, weight_rows=None)
+    kv.compact()
+    kv.update_seqlens([1], 2)
+    assert kv._weighed_keys(1) == kv.seq_len[1] == 61
+    # of several sequences in one call, each by itself; none new is none written
+    kv.new_sequence(2)
+    kv.prepare_append([1, 2], [1, 9])
+    kv.build_packed_batch([2], 9, 4, weight_rows=None)
+    had = kv._weighed_keys(1)
+    kv.update_seqlens([1, 2], [1, 9])
+    assert (kv._weighed_keys(1), kv._weighed_keys(2)) == (had, 9)
+    kv.update_seqlens([1, 2], 0)
+    assert (kv._weighed_keys(1), kv._weighed_keys(2)) == (had, 9)
