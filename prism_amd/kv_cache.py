@@ -451,9 +451,10 @@ class FlashAttnKVCache:
         """The position of each sequence's next token: its cached tokens and the evicted ones before them."""
         return [self.seq_len[sid] + self.seq_evicted.get(sid, 0) for sid in seq_ids]
 
-    def holds_evicted(self, page: int) -> bool:
-        """Whether a sequence that evict() cut lists the page: what it holds need not be a run of tokens."""
-        return any(page in self.seq_pages[sid] for sid in self.seq_evicted if sid in self.seq_pages)
+    def holds_evicted(self, pages) -> bool:
+        """Whether a sequence that evict() cut lists one of the pages: what it holds need not be a run of tokens."""
+        pages = set(pages)
+        return any(not pages.isdisjoint(self.seq_pages[sid]) for sid in self.seq_evicted if sid in self.seq_pages)
 
     def evict(self, seq_ids: list[int], budget: int | list[int], *, first: int = 4, recent: int = 64) -> int:
         """Cuts each sequence that holds more than ``budget`` tokens down to it (evict_keys, every layer in one call):

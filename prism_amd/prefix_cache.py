@@ -78,7 +78,7 @@ class PrefixCache:
         return pages, n
 
     def store(self, token_ids: list[int], page_ids: list[int], model_name: str) -> None:
-        if getattr(self.kv, "seq_evicted", None) and any(self.kv.holds_evicted(p) for p in page_ids):
+        if getattr(self.kv, "seq_evicted", None) and self.kv.holds_evicted(page_ids):
             raise RuntimeError("pages of a sequence that tokens were evicted from do not hold its prefix any more")
         key = None
         for i, block in enumerate(self._full_blocks(token_ids)):

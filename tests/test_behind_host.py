@@ -573,3 +573,34 @@ def test_keys_counted_by_update_seqlens_alone_do_not_count_as_weighed(monkeypatc
     assert (kv._weighed_keys(1), kv._weighed_keys(2)) == (had, 9)
     kv.update_seqlens([1, 2], 0)
     assert (kv._weighed_keys(1), kv._weighed_keys(2)) == (had, 9)
+
+
+def test_storing_a_prefix_looks_at_each_cut_sequence_once():
+    """However many pages are stored: their owners' pages are gone through once, not for every page."""
+    kv = FlashAttnKVCache(1, 2, 64, 400, 16, "cpu")
+    pc = prism_amd.PrefixCache(kv, 16)
+    looks = []
+
+    class Pages(list):
+        def __iter__(self):
+            looks.append("all")
+            return super().__iter__()
+
+        def __contains__(self, page):
+            looks.append(page)
+            return super().__contains__(page)
+
+    for sid in range(1, 6):
+        kv.new_sequence(sid)
+        kv._ensure_capacity(sid, 640)
+        kv.seq_len[sid] = 640
+    for sid in range(2, 6):
+        kv.seq_evicted[sid] = 10
+        kv.seq_pages[sid] = Pages(kv.seq_pages[sid])
+    pc.store(list(range(640)), kv.seq_pages[1], "m")
+    assert pc.num_cached_pages == 40 and len(looks) <= 4
+    for pages in (kv.seq_pages[5][:1], kv.seq_pages[1][:3] + kv.seq_pages[3][-1:]):
+        with pytest.raises(RuntimeError, match="evicted"):
+            pc.store(list(range(64)), list(pages), "other")
+    assert pc.num_cached_pages == 40
+    pc.store(list(range(64)), [], "other")
