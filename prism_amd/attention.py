@@ -322,6 +322,31 @@ def _check_table(block_table: torch.Tensor, cache_seqlens: torch.Tensor, batch: 
         raise RuntimeError("block_table/cache_seqlens must live on the cache's device")
 
 
+_lengths_of_cut = False   # whether build_block_table has returned lengths of sequences that evict() cut
+
+
+def mark_lengths_of_cut(lengths: torch.Tensor, buffer: torch.Tensor, rows: list[int]) -> None:
+    """Notes that `rows` of `lengths`, just filled in `buffer`, are of sequences that evict() cut."""
+    global _lengths_of_cut
+    _lengths_of_cut |= bool(rows)
+    if _lengths_of_cut:
+        buffer._pkv_cut = lengths._pkv_cut = (lengths._version, rows)
+
+
+def refuse_lengths_of_cut(positions: torch.Tensor, name: str) -> None:
+    """Raises where `positions` are lengths as build_block_table filled them and a row's sequence was cut by evict():
+    its tokens go on behind the evicted ones (FlashAttnKVCache.next_positions).  Lengths written to since are the
+    caller's own."""
+    if not _lengths_of_cut or not isinstance(positions, torch.Tensor):
+        return
+    buffer = positions if positions._base is None else positions._base
+    version, rows = getattr(positions, "_pkv_cut", None) or getattr(buffer, "_pkv_cut", None) or (0, ())
+    at = positions.storage_offset()
+    if any(at <= r < at + positions.numel() for r in rows) and positions._version == version:
+        raise RuntimeError(f"{name} are lengths of a sequence that tokens were evicted from, and not its positions "
+                           "(FlashAttnKVCache.next_positions)")
+
+
 def append_kv(k_cache, v_cache, k, v, cache_seqlens, block_table, *, status=None) -> None:
     """Slot-mapped append only (the append half of flash_attn_with_kvcache)."""
     num_pages, page_size, n_kv, hd = _check_cache(k_cache, v_cache)
@@ -630,6 +655,7 @@ def rope_decode_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     qs, ks, vs = _rows(q, "q", n_heads, hd), _rows(k, "k", n_kv, hd), _rows(v, "v", n_kv, hd)
     device = k_cache.device
     _check_table(block_table, cache_seqlens, batch, device)
+    refuse_lengths_of_cut(cache_seqlens, "cache_seqlens, which the tokens turn by,")
     max_blocks = block_table.shape[1]
     scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(hd)
     if out is None:

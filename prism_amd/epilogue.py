@@ -23,7 +23,7 @@ import math
 import torch
 
 from . import _lib
-from .attention import _BF16, _raw_stream, _require_gpu, _stream_ptr, status_tensor
+from .attention import _BF16, _raw_stream, _require_gpu, _stream_ptr, refuse_lengths_of_cut, status_tensor
 from .packed import _on
 
 
@@ -86,6 +86,7 @@ def rope_qk(qkv: torch.Tensor, positions: torch.Tensor | int, cos: torch.Tensor,
         positions = torch.full((batch,), positions, dtype=torch.int32, device=device)
     if positions.dtype != torch.int32 or positions.device != device or positions.numel() != batch:
         raise RuntimeError("positions must be int32 [B] on the qkv device")
+    refuse_lengths_of_cut(positions, "positions")
     if q_out is None:
         q_out = torch.empty((batch, s_new, n_heads, hd), dtype=_BF16, device=device)
     if k_out is None and return_k:
@@ -261,6 +262,7 @@ def rotate_qk(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, 
     ``-sin`` the rotation turns back, which is also its gradient."""
     dev = q.device
     _require_gpu(q, "q")
+    refuse_lengths_of_cut(positions, "positions")
     with _on(dev):
         return _lib.fast().rotate_qk(q, k, positions, cos, sin, interleaved, q_norm_w, k_norm_w, eps, q_out, k_out,
                                      status if status is not None else status_tensor(dev), _raw_stream(dev.index))

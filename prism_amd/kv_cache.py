@@ -39,7 +39,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .attention import poll_status, status_tensor
+from .attention import mark_lengths_of_cut, poll_status, status_tensor
 from .eviction import evict_keys
 from .packed import PackedBatch
 
@@ -384,6 +384,8 @@ class FlashAttnKVCache:
         shared = shared_prefix_pages(bt_host, sl_host, self.page_size) * self.page_size
         bt._pkv_shared_prefix = (shared, bt._version, sl.data_ptr(), sl._version,
                                  int(sl_host.min()) if batch else 0)
+        # lengths are not positions where tokens were evicted: what would turn tokens by them refuses them
+        mark_lengths_of_cut(sl, self._seqlens_buf, [i for i, sid in enumerate(seq_ids) if sid in self.seq_evicted])
         if pin:
             poll_status(self.device)   # raises PrismKVStatusError for bits an earlier call set
         return bt, sl

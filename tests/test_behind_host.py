@@ -575,6 +575,32 @@ def test_keys_counted_by_update_seqlens_alone_do_not_count_as_weighed(monkeypatc
     assert (kv._weighed_keys(1), kv._weighed_keys(2)) == (had, 9)
 
 
+def test_lengths_of_a_cut_sequence_are_not_taken_for_positions():
+    """As build_block_table returned them, whole or in part; not those of others, nor what was made of them."""
+    from prism_amd.attention import refuse_lengths_of_cut
+    kv = FlashAttnKVCache(1, 2, 64, 12, 16, "cpu")
+    for sid in (1, 2, 3):
+        kv.new_sequence(sid)
+        kv._ensure_capacity(sid, 20)
+        kv.update_seqlens([sid], 20)
+    old = kv.build_block_table([1, 2, 3])[1]
+    kv.seq_evicted[2] = 30
+    refuse_lengths_of_cut(old, "x")
+    _, sl = kv.build_block_table([1, 2, 3])
+    assert sl.tolist() == [20, 20, 20]
+    for bad in (sl, sl[1:], sl[1:2], sl[:2], old):
+        with pytest.raises(RuntimeError, match="next_positions"):
+            refuse_lengths_of_cut(bad, "x")
+    for fine in (sl[:1], sl[2:], sl + 1, sl.clone(), torch.tensor(kv.next_positions([1, 2, 3]))):
+        refuse_lengths_of_cut(fine, "x")
+    sl[1] = 50
+    refuse_lengths_of_cut(sl, "x")
+    _, sl = kv.build_block_table([1, 3])
+    refuse_lengths_of_cut(sl, "x")
+    kv.free_sequence(2)
+    refuse_lengths_of_cut(kv.build_block_table([1, 3])[1], "x")
+
+
 def test_storing_a_prefix_looks_at_each_cut_sequence_once():
     """However many pages are stored: their owners' pages are gone through once, not for every page."""
     kv = FlashAttnKVCache(1, 2, 64, 400, 16, "cpu")

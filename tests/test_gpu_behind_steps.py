@@ -304,6 +304,40 @@ def test_pages_of_a_cut_sequence_with_keys_never_weighed_do_not_count_as_weighed
     assert kv._weighed[2] == 16
 
 
+def test_lengths_of_a_cut_sequence_turn_nothing(gpu):
+    """The decode calls that take cache_seqlens for positions refuse them; attention alone, and rotation by
+    next_positions, go on."""
+    kv = prism_amd.FlashAttnKVCache(1, NK, HD, 8, 256, gpu)
+    kv.enable_key_weights()
+    cos, sin = prism_amd.rope_tables(HD, 512, device=gpu)
+    for sid in (1, 2):
+        kv.new_sequence(sid)
+        kv.prepare_append([sid], 300)
+        kv.build_packed_batch([sid], 300, NH, weight_rows=None)
+        kv.update_seqlens([sid], 300)
+    kv.evict([2], 60)
+    kv.prepare_append([1, 2], 1)
+    bt, sl = kv.build_block_table([1, 2])
+    qkv = torch.randn(2, 1, (NH + 2 * NK) * HD, device=gpu).to(BF16)
+    kc, vc = kv.k_caches[0], kv.v_caches[0]
+    before = kc.clone()
+    append = dict(k_cache=kc, v_cache=vc, block_table=bt, cache_seqlens=sl)
+    fused = lambda rows: prism_amd.rope_decode_attention(qkv[rows], kc, vc, cos, sin, cache_seqlens=sl[rows],
+                                                         block_table=bt[rows], n_heads=NH, n_kv=NK)
+    tables, one = prism_amd.rotary_tables(HD, 512, device=gpu), qkv[:, 0, :NH * HD].unflatten(1, (NH, HD))
+    for call in (lambda: fused(slice(0, 2)), lambda: fused(slice(1, 2)), lambda: prism_amd.rotate_qk(one, None, sl, *tables),
+                 lambda: prism_amd.rope_qk(qkv, sl, cos, sin, NH, NK, **append)):
+        with pytest.raises(RuntimeError, match="next_positions"):
+            call()
+    assert torch.equal(kc, before)
+    fused(slice(0, 1))
+    positions = torch.tensor(kv.next_positions([1, 2]), dtype=torch.int32, device=gpu)
+    q, _ = prism_amd.rope_qk(qkv, positions, cos, sin, NH, NK, **append)
+    prism_amd.rotate_qk(one, None, positions, *tables)
+    out = prism_amd.flash_attn_with_kvcache(q, kc, vc, cache_seqlens=sl + 1, block_table=bt, causal=True)
+    assert out.isfinite().all()
+
+
 def test_sequences_that_share_pages_weigh_them_in_turn(gpu):
     """Pages that steps without weights filled: both sequences' attention is in their sums, and decides the eviction."""
     model = Model(gpu, 4)
