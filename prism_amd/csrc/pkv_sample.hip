@@ -25,7 +25,6 @@
 // a fixed order or integers (2^-42 of the largest weight or finer): no order of atomics changes a token.
 #include <algorithm>
 #include <cmath>
-#include <type_traits>
 
 #include "pkv_common.h"
 
@@ -175,8 +174,6 @@ __device__ __forceinline__ int class_of(double t) { return int(fmin(-t * kPerOct
 template <class T>
 struct Row {
   static constexpr int kVec = 16 / sizeof(T);
-  // lowest bits of the ordered values that are alike for all of one sign
-  static constexpr int kZeros = std::is_same<T, float>::value ? 0 : std::is_same<T, __bf16>::value ? 16 : 13;
   const u32x4* pieces;
   int skip, vocab;
   __device__ __forceinline__ Row(const SampleParams& p, int row) {
@@ -1169,13 +1166,11 @@ __device__ __forceinline__ void classes_row(const SampleParams& p, const Rules& 
   SliceHead head = {};
   if (tid < p.slices) head = p.heads[int64_t(row) * p.slices + tid];
   uint64_t best = wave_max(head.best);
-  uint32_t left = uint32_t(wave_max(uint64_t(head.left)));
   uint32_t valid = head.valid;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) valid += __shfl_xor(valid, o);
   if (lane == 0) {
     lds.best[wave] = best;
-    lds.left[wave] = left;
     lds.valid[wave] = valid;
   }
   if (tid == 0) sh.n = 0;
@@ -1184,7 +1179,6 @@ __device__ __forceinline__ void classes_row(const SampleParams& p, const Rules& 
 #pragma unroll
   for (int i = 0; i < kRowWaves; ++i) {
     best = max(best, lds.best[i]);
-    left = max(left, lds.left[i]);
     valid += lds.valid[i];
   }
   const float top = value_of(uint32_t(best >> 32));
