@@ -72,17 +72,15 @@ def evict_np(k_pool, v_pool, weights, block_table, lens, keeps, first, recent, m
     return k, v, w, kept
 
 
-def sample64(x, u, temperature, top_k, top_p, min_p):
-    """One row: (token, log-probability, how far u lies from the nearest border of a decision, in shares of the sum)."""
+def kept64(x, temperature, top_k, top_p, min_p):
+    """One row: the tokens that stay, ascending, their weights, and how far the nearest border of a rule lies."""
     x = np.asarray(x, np.float64)
     can = ~(np.isnan(x) | np.isneginf(x))
-    if not can.any():
-        return -1, -math.inf, 1.0
     at = np.flatnonzero(can)
     order = at[np.lexsort((at, -x[at]))]
+    if len(order) == 0 or not temperature > 0 or top_p <= 0:
+        return order[:1], np.ones(len(order[:1])), 1.0
     top = x[order[0]]
-    if not temperature > 0 or top_p <= 0:
-        return int(order[0]), 0.0, 1.0
     if 0 < top_k < len(order):
         order = order[:top_k]
     with np.errstate(invalid="ignore"):
@@ -99,7 +97,16 @@ def sample64(x, u, temperature, top_k, top_p, min_p):
         near = min(near, np.abs(w[1:] / min(min_p, 1.0) - 1.0)[w[1:] < 1.0].min(initial=1.0))
         order, w = order[stay], w[stay]
     by = np.argsort(order)
-    order, w = order[by], w[by]
+    return order[by], w[by], near
+
+
+def sample64(x, u, temperature, top_k, top_p, min_p):
+    """One row: (token, log-probability, how far u lies from the nearest border of a decision, in shares of the sum)."""
+    order, w, near = kept64(x, temperature, top_k, top_p, min_p)
+    if len(order) == 0:
+        return -1, -math.inf, 1.0
+    if not temperature > 0 or top_p <= 0:
+        return int(order[0]), 0.0, 1.0
     run = np.cumsum(w)
     near = min(near, np.abs(run[:-1] / run[-1] - u).min(initial=1.0))
     j = int(np.searchsorted(run, min(max(u, 0.0), 1.0) * run[-1], side="right"))

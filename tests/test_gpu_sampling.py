@@ -171,6 +171,45 @@ def test_long_lists_of_many_rows_are_thinned(gpu, dtype, vocab, top_k):
         assert torch.equal(more, got.repeat(32)) and torch.equal(more_logs, logs.repeat(32))
 
 
+def _expect_any(x, t, k, p, m, got, logs, what):
+    """What holds for a row wherever its number lies: the token is one of those that stay, and the logarithm its own
+    share, to _expect's tolerance.  Borders of top-p and min-p that lie nearer than 2^-30 may fall either way: the set
+    and its sum lie between those of rules a little tighter and a little looser."""
+    for i in range(len(got)):
+        row, slack = x[i].double().cpu().numpy(), 2.0 ** -29
+        loose, w, _ = ob.kept64(row, t, k, p * (1 + slack) if 0 < p < 1 else p, m * (1 - slack))
+        _, tight, _ = ob.kept64(row, t, k, p * (1 - slack) if 0 < p < 1 else p, min(m, 1.0) * (1 + slack) if m < 1 else m)
+        if len(loose) == 0:
+            assert got[i] == -1 and logs[i] == -float("inf"), what
+            continue
+        at = np.flatnonzero(loose == int(got[i]))
+        assert len(at) == 1 and w[at[0]] > 0, f"{what} row {i}: {got[i]} does not stay"
+        lo, hi = np.log(w[at[0]] / w.sum()), np.log(w[at[0]] / tight.sum())
+        assert lo - 2.0 ** -29 - 2.0 ** -23 * abs(lo) <= logs[i] <= hi + 2.0 ** -29 + 2.0 ** -23 * abs(hi), f"{what} row {i}"
+
+
+@pytest.mark.parametrize("rules", list(RULES))
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_no_row_goes_unlooked_at(gpu, rules, dtype):
+    """Ordinary rows with ordinary numbers are all far enough from a border to be compared with the oracle's tokens; rows
+    whose numbers lie on borders (equal logits, 0 and 1) still get a token that stays, and its share."""
+    r = dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
+    r.update(RULES[rules])
+    for vocab in (1000, 20000):
+        x, u = _logits(gpu, 12, vocab, dtype, seed=vocab + 1)
+        rule = [float(np.float32(r["temperature"])), r["top_k"], float(np.float32(r["top_p"])), float(np.float32(r["min_p"]))]
+        near = [ob.sample64(x[i].double().cpu().numpy(), float(u[i]), *rule)[2] for i in range(12)]
+        assert min(near) >= 2.0 ** -30, f"{rules} {vocab}: a row of this case decides nothing"
+        ties = x.clone()
+        ties[:4] = 0.5
+        ties[4:8] = (x[4:8].float() / 4).round().to(dtype)
+        ends = torch.tensor([0.0, 0.25, 0.5, 1.0] * 3, device=gpu)
+        for what, a, b in (("rows", x, u), ("ties", ties, u), ("ties and ends", ties, ends), ("ends", x, ends)):
+            got, logs = prism_amd.sample_tokens(a, b, temperature=r["temperature"], top_k=r["top_k"], top_p=r["top_p"],
+                                                min_p=r["min_p"], return_logprobs=True)
+            _expect_any(a, *rule, got.cpu().numpy(), logs.double().cpu().numpy(), f"{rules} {vocab} {what}")
+
+
 def test_settings_of_rows_that_are_no_number(gpu):
     """NaN: no rule, and the largest logit as a temperature."""
     x, u = _logits(gpu, 4, 9001, torch.float32, seed=17)
