@@ -474,7 +474,8 @@ size_t pkv_key_weights_workspace_bytes(int32_t partials, int32_t n_kv);
  * pkv_packed_attn's; the keys are in the cache.  weights is fp32 [num_pages, n_kv, page_size] with a page stride.
  * Keys that the plan lists as not weighed (the new ones) are written, not added to, also where no row sees them.
  * A row of lse -inf or +inf weighs nothing; masked keys take no part, whatever they hold; a NaN in a row, a key or an
- * lse makes NaN of the weights of the keys that the row sees, or of that key.  items (device memory, 16-byte aligned)
+ * lse makes NaN of the weights of the keys that the row sees, or of that key, as an infinite score does in a row of
+ * infinite lse.  items (device memory, 16-byte aligned)
  * and the counts are pkv_key_weights_plan's for the same lengths, heads and window; items that do not fit the call are
  * skipped and flag PKV_STATUS_BAD_PAGE, as is a key that a row sees on a page outside the pool.  Pages of one call
  * must not be shared by its sequences.  bf16 products, fp32 exponentials and sums, in an order that the list fixes.

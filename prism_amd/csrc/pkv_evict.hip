@@ -112,9 +112,10 @@ __device__ __forceinline__ void find_digit(Digit<THREADS>& sh, int bits, int nee
 
 // A workgroup per layer, sequence and head.  Reads the weights three times (first digit; the keys of that digit, which
 // then lie in LDS where CANDIDATES hold them; the kept ones), 16 bytes a lane with the next ones on the way.  What bounds
-// it is a CU's vector ALU: 28 layers' one head of 105 k tokens take 66 us on 28 of 256 CUs, 0.9 us for 4096 weights and
-// pass; 28 layers of 6 sequences of 2800 tokens with 4 heads, which fill the device, 19 us.  More workgroups to a head
-// would need four launches, and the move of K and V behind it is the longer one already (110 and 205 us).
+// it is its one CU, whose vector ALU is busy 63 %, and whose waves wait half of their time: 28 layers' one head of 105 k
+// tokens take 66 us on 28 of 256 CUs, 0.9 us for 4096 weights and pass; 28 layers of 6 sequences of 2800 tokens with 4
+// heads, which fill the device, 19 us.  More workgroups to a head would need four launches, and the move of K and V
+// behind it is the longer one already (110 and 206 us).
 // COLS: a sequence's row of the block table lies in LDS (0: not), as it does up to 8192 columns.  From global memory the
 // long eviction takes 14 us more, those of six sequences the same.
 template <int THREADS, int COLS, int CANDIDATES>

@@ -16,7 +16,7 @@
 // cut lies in none of these (thousands of equal logits, top-k past the lists) are searched through by a radix descent
 // over all their tokens.
 //
-// The first launch is bound by fp64, an exponential a token: 256 plain fp32 rows of 131072 take 31 us (134 MB, 4.3 TB/s),
+// The first launch is bound by fp64, an exponential a token: 256 plain fp32 rows of 131072 take 30 us (134 MB, 4.5 TB/s),
 // 32 bf16 rows of 151003 with top-p 13.  The second by the latency of its steps, one workgroup a row: plain rows 13 us,
 // top-p 33 (2 to join the slices' heads, 2 their sums, 5 the classes, 10 to read the row for the cut class, 4 to sort it,
 // 5 to draw), top-k 11 for one row of 32000, 24 for 60 of 128000 with settings of their own.
@@ -32,7 +32,7 @@ namespace pkv {
 namespace {
 
 constexpr int kSliceThreads = 256;
-// In slices of 8192, 256 plain rows of 131072 take 53 us, not 47, 32 of 151003 with top-p 53, not 49.
+// In slices of 8192, 256 plain rows of 131072 take 54 us, not 46, 32 of 151003 with top-p 52, not 49.
 constexpr int kSlice = 16 * kSliceThreads;
 constexpr int kRowThreads = 1024;
 constexpr int kRowWaves = kRowThreads / 64;
@@ -864,7 +864,7 @@ __device__ int draw_from_slices(Lds& lds, const SampleParams& p, const Row<T>& s
 }
 
 // Rows without a rule: the first wave takes all slices' sums, four a lane, and picks the slice.  256 rows of 131072 take
-// 47 us with both launches, by the kernel of the other rows 51; one row 16 and 17.
+// 46 us with both launches, by the kernel of the other rows 50; one row 16 and 17.
 struct PlainLds {
   struct {
     double wave_d[kRowWaves], target;
@@ -1394,7 +1394,7 @@ Split split_of(int vocab) {
   const int size = kSlice;
   s.slices = (vocab + 7 + size - 1) / size;
   // a slice lists the first top_k of its own, as far as there is room (with 512 places at most, 115 rows of 6883 tokens
-  // with top-k of up to 1000, more than these places hold, took 84 us, not 52, 17 rows of 1826 67, not 38)
+  // with top-k of up to 1000, more than these places hold, took 83 us, not 51, 17 rows of 1826 61, not 40)
   s.cap = std::min(kSlice, kListMax / s.slices);
   s.part = (std::max<int64_t>(s.cap * sizeof(uint2), kClasses * sizeof(uint64_t)) + 15) / 16 * 16;
   return s;

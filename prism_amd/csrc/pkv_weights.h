@@ -7,7 +7,7 @@ namespace pkv {
 
 constexpr int kWeightBlock = 256;    // keys of a block that many query rows go over
 // Sequences with at most so many query rows stream their keys past them.  16 sequences of 4000 keys, 28 heads on 4: 63
-// rows 21 us this way and 25 by blocks of keys, 126 rows 27 and 28; 40 heads on 8: 60 rows 33 and 42, 125 rows 42 and 51.
+// rows 21 us this way and 25 by blocks of keys, 126 rows 26 and 28; 40 heads on 8: 60 rows 33 and 43, 125 rows 41 and 51.
 // More rows would not fit four workgroups' LDS.
 constexpr int kWeightFewRows = 128;
 constexpr int kWeightFewKeys = 3968; // keys of such an item at most: a wave's page ids, one per 16 keys, fit its lanes

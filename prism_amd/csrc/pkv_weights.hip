@@ -46,8 +46,8 @@ __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
 }
 __device__ __forceinline__ bf16x8 frag(u32x4 v) { return __builtin_bit_cast(bf16x8, v); }
 
-// Workgroups of weigh_few_kernel on a CU at once.  48 sequences of 2500 keys, 28 heads on 4: 2 of them 35 us, 4 31, 6 46
-// (too few registers).
+// Workgroups of weigh_few_kernel on a CU at once.  48 sequences of 2500 keys, 28 heads on 4: 2 of them 34 us, 4 30, 6 32
+// (too few registers); 16 of 4000 keys with 20 query rows, 40 heads on 8: 31, 29 and 34.
 constexpr int kFewPerCu = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -194,12 +194,12 @@ __device__ __forceinline__ void weigh_few(const WeightParams& p, const WeightIte
 
 // ---- many query rows: a block of keys stays, the rows go past it ----
 // Prompt chunks: 4 waves hold 64 keys each as the A operand, 64 query rows at a time come through LDS (two buffers, one
-// barrier a step; 32 a step took 10 % longer) as B, 32 a product: C[key, row], a lane has 16 keys of one row twice, so the
+// barrier a step; 32 a step take 4 % longer) as B, 32 a product: C[key, row], a lane has 16 keys of one row twice, so the
 // row's lse is one value a lane and a key's sum stays in the lane until the end.  Exponentials bound it: of 32 x 32 scores
 // the products take 256 cycles of the matrix pipe, their 16 multiply-adds, exponentials and sums a lane 384 of the vector
 // ALU.  So the products of the second 32 keys are issued between the exponentials of the first, and the other wave of the
-// SIMD fills the rest.  Four prompts of 2600 to 3400 tokens (28 heads of 128 on 4): 175 to 184 us, 0.76 to
-// 0.8 PFLOP/s.
+// SIMD fills the rest.  Four prompts of 2600 to 3400 tokens (28 heads of 128 on 4): 175 to
+// 182 us, 0.76 to 0.79 PFLOP/s, or 198 repeated on one state.
 constexpr int kStepRows = 64;
 template <int HD>
 struct ManyLds {
@@ -399,7 +399,8 @@ __global__ __launch_bounds__(256) void weigh_many_kernel(const WeightParams p) {
   __shared__ ManyLds<HD> lds;
   weigh_many<HD>(p, p.items[blockIdx.x / p.n_kv], blockIdx.x % p.n_kv, lds);
 }
-// Both, in turn: the blocks of many rows keep the matrix and vector units busy while the others read.
+// Both, in turn: the blocks of many rows keep the matrix and vector units busy while the others read.  At the registers of
+// the former (250 at head_dim 128) a CU holds two of either, where weigh_few_kernel has four; the list cuts for four.
 template <int HD>
 __global__ __launch_bounds__(256) void weigh_both_kernel(const WeightParams p, int n_few, int n_many) {
   __shared__ union {
@@ -437,10 +438,10 @@ __global__ __launch_bounds__(kWeightBlock) void weigh_merge_kernel(const WeightP
 
 // ---- the host side ----
 // Few rows: pieces of the keys for four workgroups per CU, of 128 keys at least (a tile per wave).
-// Many rows: blocks of 256 keys, their rows in pieces for eight workgroups per CU (four prompts: 4 of them 206 us, 8 197,
-// 16 213), of 12 steps of 32 rows at least, as a partial's way through memory has its price (4 steps: a prompt of 2048
-// tokens 67 us in place of 45, decode tokens beside chunks 91 in place of 68, but one of 512 18 in place of 22; 24 steps:
-// 46, 74 and 35).
+// Many rows: blocks of 256 keys, their rows in pieces for eight workgroups per CU (four prompts: 4 of them 203 us, 8 198,
+// 16 212), of 12 steps of 32 rows at least, as a partial's way through memory has its price (4 steps: a prompt of 2048
+// tokens 65 us in place of 45, decode tokens beside chunks 86 in place of 68, but one of 512 18 in place of 23; 24 steps:
+// 45, 70 and 36).
 constexpr int kManyPerCu = 8;
 constexpr int kMinSteps = 12;
 

@@ -266,7 +266,8 @@ def packed_key_weights(q: torch.Tensor, k_cache: torch.Tensor, lse: torch.Tensor
 
     ``q``, ``window`` and ``softmax_scale`` are packed_attention's, and ``lse`` (fp32 [tokens, n_heads]) what it
     returned with ``return_lse``.  Which tokens count, and which keys start from nothing (this step's own), the batch
-    knows: it was laid out with ``weight_rows``.  A row whose lse is infinite weighs nothing."""
+    knows: it was laid out with ``weight_rows``.  A row whose lse is infinite weighs nothing
+    (its scores being finite)."""
     dev = batch.device
     _require_gpu(q, "q")
     plan = batch._weight_plans.get(window)
